@@ -132,7 +132,8 @@ def _pack(k, v):
     """k, v [tiles..., 16, head_dim] -> bytes [tiles..., 18 * head_dim]. With token t = c + 4 i:
     K codes  [t / 8][c, i % 2][8 dims' group within a block (4)][block] words of 8 codes, lowest bits first
     V codes  [block / 2][4 dims' group within a block (8)][c][block % 2][i / 2][i % 2] 16-bit units of 4 codes
-    scales   [c][block][i] float16, K's then V's"""
+    K scales [c][i % 2][i / 2][block] float16
+    V scales [c][block][i] float16"""
     kc, kd, vc, vd = _codes(k, v)
     lead, nb = k.shape[:-2], k.shape[-1] // 32
     n = math.prod(lead)
@@ -141,7 +142,7 @@ def _pack(k, v):
     kb = (kc[..., 0::2] | kc[..., 1::2] << 4).to(torch.uint8).reshape(n, -1)
     vc = vc.reshape(n, 2, 2, 4, nb // 2, 2, 8, 4).permute(0, 4, 6, 3, 5, 1, 2, 7)  # [block / 2][dims' group][c][block % 2][i / 2][i % 2][4]
     vb = (vc[..., 0::2] | vc[..., 1::2] << 4).to(torch.uint8).reshape(n, -1)
-    sc = [d.reshape(n, 4, 4, nb).permute(0, 2, 3, 1).contiguous().view(torch.uint8).reshape(n, -1) for d in (kd, vd)]
+    sc = [d.contiguous().view(torch.uint8).reshape(n, -1) for d in (kd.reshape(n, 2, 2, 4, nb).permute(0, 3, 2, 1, 4), vd.reshape(n, 4, 4, nb).permute(0, 2, 3, 1))]
     return torch.cat([kb, vb] + sc, 1).reshape(*lead, -1)
 
 
@@ -153,11 +154,9 @@ def _unpack(tiles):
     kb, vb, ks, vs = t.split([8 * hd, 8 * hd, hd, hd], 1)
     kc = torch.stack([kb & 15, kb >> 4], -1).reshape(n, 2, 4, 2, 4, nb, 8).permute(0, 1, 3, 2, 5, 4, 6).reshape(n, 16, nb, 32)
     vc = torch.stack([vb & 15, vb >> 4], -1).reshape(n, nb // 2, 8, 4, 2, 2, 2, 4).permute(0, 5, 6, 3, 1, 4, 2, 7).reshape(n, 16, nb, 32)
-    out = []
-    for c, s in ((kc, ks), (vc, vs)):
-        d = s.contiguous().view(torch.float16).reshape(n, 4, nb, 4).permute(0, 3, 1, 2).reshape(n, 16, nb, 1)
-        out.append(((c.float() - 8) * d.float()).reshape(*lead, 16, hd))
-    return out
+    kd = ks.contiguous().view(torch.float16).reshape(n, 4, 2, 2, nb).permute(0, 3, 2, 1, 4).reshape(n, 16, nb, 1)
+    vd = vs.contiguous().view(torch.float16).reshape(n, 4, nb, 4).permute(0, 3, 1, 2).reshape(n, 16, nb, 1)
+    return [((c.float() - 8) * d.float()).reshape(*lead, 16, hd) for c, d in ((kc, kd), (vc, vd))]
 
 
 def _values(gen, shape, device):
@@ -318,8 +317,8 @@ def _append(s):
     kf[at, :, tile, i // 2, c, i % 2] = lo(kc.unflatten(-1, (nb, 4, 8)).transpose(2, 3))
     vf = pool[..., 8 * hd:16 * hd].unflatten(-1, (nb // 2, 8, 4, 2, 2, 2, 2))
     vf.permute(0, 2, 5, 7, 8, 1, 3, 6, 4, 9)[at, tile, c, i // 2, i % 2] = lo(vc.unflatten(-1, (nb // 2, 2, 8, 4)))
-    for d, begin in ((kd, 16 * hd), (vd, 17 * hd)):
-        pool[..., begin:begin + hd].view(torch.float16).unflatten(-1, (4, nb, 4)).permute(0, 2, 3, 5, 1, 4)[at, tile, c, i] = d
+    pool[..., 16 * hd:17 * hd].view(torch.float16).unflatten(-1, (4, 2, 2, nb)).permute(0, 2, 3, 4, 5, 1, 6)[at, tile, c, i % 2, i // 2] = kd
+    pool[..., 17 * hd:].view(torch.float16).unflatten(-1, (4, nb, 4)).permute(0, 2, 3, 5, 1, 4)[at, tile, c, i] = vd
     k, v = _unpack(pool[at, :, tile])
     r = torch.arange(len(at), device=at.device)
     return k[r, :, t].to(s["k"].dtype), v[r, :, t].to(s["v"].dtype)
@@ -461,9 +460,9 @@ def _exact_tile(raw):
     kbyte, khigh = word * 4 + d % 8 // 2, d % 2
     unit = ((((block // 2) * 8 + d % 32 // 4) * 4 + c) * 2 + block % 2) * 4 + i
     vbyte, vhigh = 8 * hd + unit * 2 + d % 4 // 2, d % 2
-    scale = (c * nb + block) * 4 + i
+    kscale, vscale = ((c * 2 + i % 2) * 2 + i // 2) * nb + block, (c * nb + block) * 4 + i
     out = []
-    for byte, high, begin in ((kbyte, khigh, 16 * hd), (vbyte, vhigh, 17 * hd)):
+    for byte, high, scale, begin in ((kbyte, khigh, kscale, 16 * hd), (vbyte, vhigh, vscale, 17 * hd)):
         b = raw[:, torch.from_numpy(byte).to(raw.device)].int()
         code = torch.where(torch.from_numpy(high).to(raw.device) > 0, b // 16, b % 16)
         f = raw[:, begin:begin + hd].contiguous().view(torch.float16).double()[:, torch.from_numpy(scale).to(raw.device)]
