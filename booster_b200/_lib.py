@@ -26,7 +26,23 @@ B200_SYMBOLS = ["b200_last_error", "b200_device_count", "b200_version", "b200_mo
                 "b200_op_dequantize_row", "b200_op_mul_mat_vec", "b200_op_mul_mat", "b200_op_rms_norm", "b200_op_rope",
                 "b200_op_attention", "b200_op_attention_one_launch", "b200_op_attention_cluster", "b200_set_attention_route", "b200_tokenizer_load", "b200_tokenizer_free", "b200_tokenizer_n_vocab", "b200_tokenize",
                 "b200_token_to_piece", "b200_token_is_eog", "b200_token_nl", "b200_cpt_class", "b200_op_launch_shape", "b200_op_lanes_shape", "b200_op_score_tokens", "b200_op_prompt_kernel",
-                "b200_sampler_new", "b200_sampler_set_standard", "b200_sampler_free", "b200_sampler_reset", "b200_sampler_sample"]
+                "b200_sampler_new", "b200_sampler_set_standard", "b200_sampler_free", "b200_sampler_reset", "b200_sampler_sample",
+                "b200_kv4_append", "b200_kv4_read", "b200_kv4_attention_workspace", "b200_kv4_attention", "b200_pages_workspace", "b200_pages_reserve", "b200_pages_fork",
+                "b200_pages_free", "b200_pages_compact", "b200_pages_copy", "b200_sample"]
+
+
+class Kv4(C.Structure):
+    """struct b200_kv4: one layer of a paged 4-bit cache and a step's rows"""
+    _fields_ = ([(n, C.c_int32) for n in ("device", "n_pages", "page_tokens", "n_head_kv", "head_dim", "n_slots", "max_pages", "n_seq", "n_rows")]
+                + [("stream", C.c_void_p), ("pool", C.c_void_p), ("page_stride", C.c_int64), ("table_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("table", "held", "slots", "first")])
+
+
+class Pages(C.Structure):
+    """struct b200_pages: all layers of a paged cache and its tables"""
+    _fields_ = ([(n, C.c_int32) for n in ("device", "n_pages", "page_tokens", "n_head_kv", "head_dim", "n_slots", "max_pages", "n_layer")]
+                + [("stream", C.c_void_p), ("pool", C.c_void_p), ("layer_stride", C.c_int64), ("page_stride", C.c_int64), ("table_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("table", "held", "refs")])
 
 
 def lib() -> C.CDLL:
@@ -148,6 +164,18 @@ def lib() -> C.CDLL:
     sig("b200_set_prefill_mma", None, [C.c_int])
     sig("b200_set_prefill_attn_batch", None, [C.c_int])
     sig("b200_trace_phases", C.c_int64, [vp, C.c_int32, C.c_int, C.c_int, C.POINTER(C.c_uint64), C.c_int64, i32p, C.c_int64, i32p])
+    kp, pp = C.POINTER(Kv4), C.POINTER(Pages)
+    sig("b200_kv4_append", C.c_int, [kp, C.c_int, vp, C.c_int64, C.c_int64, vp, C.c_int64, C.c_int64])
+    sig("b200_kv4_read", C.c_int, [kp, C.c_int, vp, vp])
+    sig("b200_kv4_attention_workspace", C.c_int64, [kp, C.c_int, C.c_int])
+    sig("b200_kv4_attention", C.c_int, [kp, C.c_int, vp, C.c_int64, C.c_int64, C.c_int, C.c_float, C.c_int, C.c_int, vp, vp, C.c_int64])
+    sig("b200_pages_workspace", C.c_int64, [pp, C.c_int])
+    sig("b200_pages_reserve", C.c_int, [pp, vp, vp, C.c_int, vp])
+    sig("b200_pages_fork", C.c_int, [pp, vp, vp, C.c_int, vp, vp, C.c_int64])
+    sig("b200_pages_free", C.c_int, [pp, vp, C.c_int])
+    sig("b200_pages_compact", C.c_int, [pp, vp, vp, C.c_int64])
+    sig("b200_pages_copy", C.c_int, [pp, vp, vp, C.c_int, vp, vp, C.c_int64])
+    sig("b200_sample", C.c_int, [C.c_int, vp, C.c_int, vp, C.c_int64, C.c_int, C.c_int] + [vp] * 7)
     _lib = L
     return L
 

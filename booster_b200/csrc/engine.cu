@@ -20,6 +20,7 @@
 #include "tokenizer.hpp"
 #include "safetensors.hpp"
 #include "stack.hpp"
+#include "serve.hpp"
 #include "kernels.cuh"
 #ifndef B200_TOKEN_KERNEL
 #define B200_TOKEN_KERNEL 1      // 0: build without the persistent per-token kernel (A/B: code size of the module)
@@ -3098,4 +3099,50 @@ extern "C" int b200_op_attention(const float * q, const uint16_t * k_cache, cons
         CU(cudaStreamSynchronize(st));
         return 0;
     } catch (const std::exception & e) { return set_err(e.what()); }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// device-level operators of many sequences (serve.cu)
+// ------------------------------------------------------------------------------------------------------------
+template <typename F> static int served(const char * name, const void * what, F f) {
+    try {
+        if (!what) throw std::runtime_error("null description");
+        f();
+        return 0;
+    } catch (const std::exception & e) { return set_err(std::string(name) + ": " + e.what()); }
+}
+extern "C" int b200_kv4_append(const b200_kv4 * c, int dtype, const void * k, int64_t k_row, int64_t k_head, const void * v, int64_t v_row, int64_t v_head) {
+    return served("b200_kv4_append", c, [&] { kv4_append(*c, dtype, k, k_row, k_head, v, v_row, v_head); });
+}
+extern "C" int b200_kv4_read(const b200_kv4 * c, int dtype, void * k, void * v) { return served("b200_kv4_read", c, [&] { kv4_read(*c, dtype, k, v); }); }
+extern "C" int64_t b200_kv4_attention_workspace(const b200_kv4 * c, int n_head, int max_rows) {
+    int64_t n = -1;
+    served("b200_kv4_attention_workspace", c, [&] { n = kv4_attention_workspace(*c, n_head, max_rows); });
+    return n;
+}
+extern "C" int b200_kv4_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int max_rows, void * out, void * work,
+                                  int64_t work_bytes) {
+    return served("b200_kv4_attention", c, [&] { kv4_attention(*c, dtype, q, q_row, q_head, n_head, scale, window, max_rows, out, work, work_bytes); });
+}
+extern "C" int64_t b200_pages_workspace(const b200_pages * p, int n) {
+    int64_t bytes = -1;
+    served("b200_pages_workspace", p, [&] { bytes = pages_workspace(*p, n); });
+    return bytes;
+}
+extern "C" int b200_pages_reserve(const b200_pages * p, const int32_t * slots, const int32_t * first, int n, int32_t * status) {
+    return served("b200_pages_reserve", p, [&] { pages_reserve(*p, slots, first, n, status); });
+}
+extern "C" int b200_pages_fork(const b200_pages * p, const int32_t * parents, const int32_t * children, int n, int32_t * status, void * work, int64_t work_bytes) {
+    return served("b200_pages_fork", p, [&] { pages_fork(*p, parents, children, n, status, work, work_bytes); });
+}
+extern "C" int b200_pages_free(const b200_pages * p, const int32_t * slots, int n) { return served("b200_pages_free", p, [&] { pages_free(*p, slots, n); }); }
+extern "C" int b200_pages_compact(const b200_pages * p, int32_t * live, void * work, int64_t work_bytes) {
+    return served("b200_pages_compact", p, [&] { pages_compact(*p, live, work, work_bytes); });
+}
+extern "C" int b200_pages_copy(const b200_pages * p, const int32_t * src, const int32_t * dst, int n, int32_t * status, void * work, int64_t work_bytes) {
+    return served("b200_pages_copy", p, [&] { pages_copy(*p, src, dst, n, status, work, work_bytes); });
+}
+extern "C" int b200_sample(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature,
+                           const int32_t * top_k, const float * top_p, const float * min_p, int32_t * ids, float * logprobs) {
+    return served("b200_sample", "", [&] { sample_rows(device, stream, dtype, logits, row_stride, n_rows, n_vocab, u, temperature, top_k, top_p, min_p, ids, logprobs); });
 }

@@ -338,6 +338,71 @@ int b200_op_attention_cluster(int n_head, int n_head_kv, int n_ctx);
  * exists so that tests cover both routes at every size. */
 void b200_set_attention_route(int route);
 
+/* ---- many sequences at once: device-level operators ------------------------------------------------------
+ * What a server of many sequences runs between its own products: a cache of keys and values in 4 bits whose pages sequences hold and share, attention
+ * over it, and the draw of next tokens. Unlike the rest of this header these take DEVICE pointers of CUDA device `device` and enqueue on `stream`
+ * (a cudaStream_t, NULL: the default stream): nothing is allocated, copied to the host or waited for, and calls can be captured into graphs. Memory
+ * belongs to the caller; a workspace may be used again by the next call on the same stream, and by no other call at the same time. Arguments that the
+ * host can see are checked (non-zero, b200_last_error()). What device tables say is bounded by the kernels: a page or slot that does not exist is
+ * as absent, and never read or written. The caller's current device stays as it is. */
+enum { B200_DTYPE_F32 = 0, B200_DTYPE_BF16 = 1, B200_DTYPE_F16 = 2 };
+
+/* One layer of a paged cache and the rows of a step. The pool holds n_pages pages, page_stride bytes apart, of n_head_kv x page_tokens / 16 tiles of 18 x head_dim
+ * bytes each (booster_b200/csrc/serve_cache.cuh describes a tile); it is zeroed once, before its first use, and written by these calls only. Row s of table
+ * [n_slots][table_stride] names the pages of slot s in order (negative: none) and held[s] its tokens before the step. The step has n_seq sequences: sequence i
+ * is slot slots[i] (slots NULL: slot i) and has the rows first[i] .. first[i + 1] - 1 of the step's n_rows, at positions held, held + 1, ... first ascends; rows behind
+ * the last sequence are left as they are. A slot stands once in a step. head_dim 64 or 128, page_tokens a power of two from 16 to 1024, up to 4096 sequences. */
+typedef struct b200_kv4 {
+    int32_t device, n_pages, page_tokens, n_head_kv, head_dim, n_slots, max_pages, n_seq, n_rows;
+    void * stream;
+    void * pool;
+    int64_t page_stride, table_stride;
+    const int32_t * table, * held, * slots, * first;
+} b200_kv4;
+
+/* keys and values of the step's rows into their pages: k[row * k_row + head * k_head + i] and v likewise (strides in entries), dtype F32, BF16 or F16. A number of a block
+ * of 32 is held as c in 0 .. 15 and stands for (c - 8) d with d = e / -8 (8 significant bits, at most 8160 in magnitude), e the block's entry of largest magnitude (the
+ * negative one of two). A token with an infinity or a NaN in a head is held as such: rows that see it answer NaN for the head. Rows whose page is absent are dropped. */
+int b200_kv4_append(const b200_kv4 * c, int dtype, const void * k, int64_t k_row, int64_t k_head, const void * v, int64_t v_row, int64_t v_head);
+/* the same positions read back: k, v [n_rows][n_head_kv][head_dim] of dtype (rounded once); absent pages read 0 */
+int b200_kv4_read(const b200_kv4 * c, int dtype, void * k, void * v);
+/* attention of the step's rows, after b200_kv4_append of the same step: out[row][head] = sum over the positions j that the row sees of softmax(scale q . k_j) v_j, in
+ * [n_rows][n_head][head_dim]; q[row * q_row + head * q_head + i], dtype BF16 or F16. A row at position p sees j <= p, with window > 0 only j > p - window, and no position
+ * whose page is absent; a row that sees nothing answers 0. n_head is a multiple of n_head_kv. max_rows: no sequence has more rows (it chooses kernels; further rows of a sequence
+ * that has are still computed). work: b200_kv4_attention_workspace() bytes (-1: error) on 16 bytes. */
+int64_t b200_kv4_attention_workspace(const b200_kv4 * c, int n_head, int max_rows);
+int b200_kv4_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int max_rows, void * out, void * work, int64_t work_bytes);
+
+/* The pages' life. refs[n_pages] counts the slots that hold a page (0: free); table and held as above, here [n_slots] of all slots. pool: n_layer layers, layer_stride
+ * bytes apart, as above (not used by b200_pages_reserve and _free). status receives 0, the number of pages that were missing, or -1 for slots, tables or lists that cannot
+ * be; then nothing has changed. Free pages are taken lowest first in the order of the call's list. work: b200_pages_workspace(p, n) bytes (compact: n = n_pages). */
+typedef struct b200_pages {
+    int32_t device, n_pages, page_tokens, n_head_kv, head_dim, n_slots, max_pages, n_layer;
+    void * stream;
+    void * pool;
+    int64_t layer_stride, page_stride, table_stride;
+    int32_t * table, * held, * refs;
+} b200_pages;
+int64_t b200_pages_workspace(const b200_pages * p, int n);
+/* pages for first[i + 1] - first[i] tokens more of slot slots[i] (NULL: slot i), behind its held tokens; held itself is the caller's to advance */
+int b200_pages_reserve(const b200_pages * p, const int32_t * slots, const int32_t * first, int n, int32_t * status);
+/* slot children[i], which is empty, becomes what slot parents[i] is: full pages are shared, the tokens of the last page are copied in every layer when it is part full */
+int b200_pages_fork(const b200_pages * p, const int32_t * parents, const int32_t * children, int n, int32_t * status, void * work, int64_t work_bytes);
+/* the slots give their pages back and are empty */
+int b200_pages_free(const b200_pages * p, const int32_t * slots, int n);
+/* pages in use move to the lowest places, in order (only those behind the number of pages in use do), tables follow; live receives that number */
+int b200_pages_compact(const b200_pages * p, int32_t * live, void * work, int64_t work_bytes);
+/* page dst[i] = page src[i] in every layer; no dst twice, and none that is a src */
+int b200_pages_copy(const b200_pages * p, const int32_t * src, const int32_t * dst, int n, int32_t * status, void * work, int64_t work_bytes);
+
+/* The draw of one token a row from logits[row * row_stride + i], dtype F32, BF16 or F16, n_vocab up to 2^18, in the order of b200_sampler's chain: of the tokens by
+ * descending logit (lower index first among equals) the first top_k[row] (<= 0: all); of those the shortest prefix with at least the share top_p[row] of their weight
+ * exp(logit - largest) (>= 1: all; the first always); of those with a weight of at least min_p[row]; of what is left, token i with the weight exp((logit - largest) / temperature[row]):
+ * ids[row] is the first in order of index at which the sum passes u[row] (0 <= u < 1) of the total. temperature <= 0: the first of the largest. NULL: 1, 0, 1, 0.
+ * logprobs (may be NULL): log of the drawn token's share (0 at temperature <= 0). NaN counts as -infinity; a row of nothing else gives -1 and -infinity. */
+int b200_sample(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature, const int32_t * top_k,
+                const float * top_p, const float * min_p, int32_t * ids, float * logprobs);
+
 #ifdef __cplusplus
 }
 #endif
