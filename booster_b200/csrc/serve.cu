@@ -26,13 +26,17 @@ struct On {
     int was = -1, device;
     int sms = 0;
     explicit On(int d) : device(d) {
-        int n = 0;
-        if (cudaGetDeviceCount(&n) != cudaSuccess) { cudaGetLastError(); n = 0; }
-        need(n > 0, "no CUDA device visible: booster_b200 has no CPU fallback (the CUDA path is the product)");
-        need(d >= 0 && d < n && d < MAX_DEVICES, "no such device: " + std::to_string(d));
+        static std::atomic<int> known[MAX_DEVICES];            // SMs of the devices seen so far
+        if (d < 0 || d >= MAX_DEVICES || !(sms = known[d].load())) {
+            int n = 0;
+            if (cudaGetDeviceCount(&n) != cudaSuccess) { cudaGetLastError(); n = 0; }
+            need(n > 0, "no CUDA device visible: booster_b200 has no CPU fallback (the CUDA path is the product)");
+            need(d >= 0 && d < n && d < MAX_DEVICES, "no such device: " + std::to_string(d));
+            cu(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d), "cudaDeviceGetAttribute");
+            known[d].store(sms);
+        }
         cu(cudaGetDevice(&was), "cudaGetDevice");
         if (was != d) cu(cudaSetDevice(d), "cudaSetDevice");
-        cu(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d), "cudaDeviceGetAttribute");
     }
     ~On() { if (was >= 0 && was != device) cudaSetDevice(was); }
 };
@@ -95,20 +99,22 @@ template <typename T> void read_as(const b200_kv4 & c, const Cache & d, void * k
 
 // attention of few rows: column tiles of 8 (one or two side by side)
 int attend_nt(int group, int max_rows) { return (int64_t) group * max_rows <= 8 ? 1 : 2; }
-int attend_blocks_per_sm() { return 2; }
 size_t attend_before_bytes(int n_seq) { return ((size_t) (n_seq + 2) * 8 + 255) / 256 * 256; }
 size_t attend_bytes(int n_seq, int head_dim, int nt, int sms) {
-    const size_t slots = 2 * (size_t) sms * attend_blocks_per_sm() * AT_WARPS, cols = 8 * (size_t) nt;
+    const size_t slots = 2 * (size_t) sms * at_blocks(nt) * AT_WARPS, cols = 8 * (size_t) nt;
     return attend_before_bytes(n_seq) + slots * cols * (head_dim + 2) * 4;
 }
 template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, int device, int sms, void * stream) {
     static Limits set;
-    const size_t smem = (size_t) (a.c.n_seq + 1) * 8;
+    const size_t smem = at_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8;
     const auto kernel = k_kv4_attend<HD, NT, T>;
     allow_smem(kernel, device, smem, set);
-    launch(kernel, dim3(sms * attend_blocks_per_sm()), AT_WARPS * 32, smem, stream, false, 1, a);
+    launch(kernel, dim3(sms * at_blocks(NT)), AT_WARPS * 32, smem, stream, false, 1, a);
     const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group;
-    launch(k_kv4_join<HD, NT, T>, dim3((unsigned) ((items + 7) / 8)), 256, 0, stream, true, 1, a);
+    // parts a unit has on average, where every sequence has rows: few are one block's four warps' to add, many sixteen's
+    const bool many = (int64_t) sms * at_blocks(NT) * AT_WARPS > 32 * (int64_t) a.c.n_seq * a.c.n_kv;
+    if (many) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, stream, true, 1, a);
+    else launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, stream, true, 1, a);
 }
 template <int HD, typename T> void attend_nt_as(const AttendArgs & a, int nt, int device, int sms, void * stream) {
     nt == 1 ? attend_as<HD, 1, T>(a, device, sms, stream) : attend_as<HD, 2, T>(a, device, sms, stream);
@@ -196,12 +202,13 @@ void kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row,
     On on(c.device);
     if (c.n_seq == 0 || c.n_rows == 0) return;
     a.q = q; a.q_row = q_row; a.q_head = q_head; a.out = out;
+    a.q_whole = aligned(q, 16) && !((q_row | q_head) & 7);
     a.group = n_head / c.n_head_kv;
     a.scale_log2 = scale * 1.44269504088896341f;
     a.window = window;
     const int nt = attend_nt(a.group, max_rows);
     check_work(work, work_bytes, (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms));
-    const size_t slots = 2 * (size_t) on.sms * attend_blocks_per_sm() * AT_WARPS;
+    const size_t slots = 2 * (size_t) on.sms * at_blocks(nt) * AT_WARPS;
     a.before = static_cast<long long *>(work);
     a.ml = reinterpret_cast<float *>(static_cast<uint8_t *>(work) + attend_before_bytes(c.n_seq));
     a.part = a.ml + slots * 8 * nt * 2;

@@ -12,70 +12,110 @@
 namespace b200 {
 namespace srv {
 
+template <typename T> struct alignas(16) Eight { T v[8]; };           // of 16-bit types
 struct AttendArgs {
     Cache c;
     const void * q;
     int64_t q_row, q_head;
+    bool q_whole;                        // eight entries of q stand on 16 bytes
     void * out;                          // [n_rows][n_head][HD]
     int group, col_tiles_max;
     float scale_log2;                    // scale x log2(e)
     int window;                          // 0: all positions
     // workspace
-    long long * before;                  // [n_seq + 1] tiles in front of each sequence; [n_seq + 1]: tiles of a warp
+    long long * before;                  // [n_seq + 1] pairs of tiles in front of each sequence; [n_seq + 1]: pairs of a warp's piece
     float * part, * ml;                  // [2 x warps][8 NT][HD], [2 x warps][8 NT][2]
 };
 
-constexpr int AT_WARPS = 8, AT_MAX_SEQ = 4096;
-
+constexpr int AT_WARPS = 4, AT_MAX_SEQ = 4096, AT_STAGES = 3, AT_OVER = 2;      // AT_OVER: what beginning a unit costs, in pairs of tiles
+__host__ __device__ constexpr int at_blocks(int nt) { return nt == 1 ? 3 : 2; }          // resident on an SM: 168 and 255 registers a thread
+__host__ __device__ constexpr size_t at_ring_bytes(int hd) { return (size_t) AT_WARPS * AT_STAGES * 36 * hd; }
+__device__ __forceinline__ uint32_t smem_at(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
+// 16 bytes from src, or zeros where bytes is 0
+template <int AT> __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t * src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %3], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes), "n"(AT) : "memory");
+}
+// where a lane copies a pair of tiles from: a for what lies in the first one, b in the second (less the first one's length), mid for the 512 bytes that hold the border
+struct PairSrc { const uint8_t * a, * mid, * b; int bytes_a, bytes_mid, bytes_b; };
+template <int HD> __device__ __forceinline__ void copy_pair(uint32_t dst, const PairSrc & s, int lane) {
+    if constexpr (HD == 128) {
+        copy16<0>(dst, s.a, s.bytes_a); copy16<512>(dst, s.a, s.bytes_a); copy16<1024>(dst, s.a, s.bytes_a); copy16<1536>(dst, s.a, s.bytes_a);
+        copy16<2048>(dst, s.mid, s.bytes_mid);
+        copy16<2560>(dst, s.b, s.bytes_b); copy16<3584>(dst, s.b, s.bytes_b); copy16<4096>(dst, s.b, s.bytes_b); copy16<2048 + 1024>(dst, s.b, s.bytes_b);
+    } else {
+        copy16<0>(dst, s.a, s.bytes_a); copy16<512>(dst, s.a, s.bytes_a);
+        copy16<1024>(dst, s.mid, s.bytes_mid);
+        copy16<1536>(dst, s.b, s.bytes_b);
+        if (lane < 16) copy16<2048>(dst, s.b, s.bytes_b);
+    }
+}
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[2]) {       // d = a b + c, c of the two columns
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) { uint32_t r; asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x)); return r; }
 __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
 __device__ __forceinline__ uint32_t as_u(__half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
 __device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-// the eight codes of a word less 8, as pairs (n, n + 4) of nibbles: 1024 + c and 1024 + 16 c are fp16 numbers with the code in their last bits
-__device__ __forceinline__ void codes8(uint32_t w, uint32_t (&p)[4]) {
-    const __half2 eight = as_h2(0xe408e408u), sixteenth = as_h2(0x2c002c00u), seventy_two = as_h2(0xd480d480u);   // -1032, 1 / 16, -72
+// the eight codes of a word as pairs (n, n + 4) of nibbles over the last bits of 1024: 1024 + c for pairs 0 and 2, 1024 + 16 c for 1 and 3
+__device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t over) { uint32_t r; asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(over)); return r; }
+__device__ __forceinline__ void codes8_raw(uint32_t w, uint32_t (&p)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const uint32_t x = i ? w >> 8 : w;
-        p[2 * i] = as_u(__hadd2(as_h2((x & 0x000f000fu) | 0x64006400u), eight));
-        p[2 * i + 1] = as_u(__hfma2(as_h2((x & 0x00f000f0u) | 0x64006400u), sixteenth, seventy_two));
+        p[2 * i] = pick(x, 0x000f000fu, 0x64006400u);
+        p[2 * i + 1] = pick(x, 0x00f000f0u, 0x64006400u);
+    }
+}
+// less 8
+__device__ __forceinline__ void codes8(uint32_t w, uint32_t (&p)[4]) {
+    const __half2 eight = as_h2(0xe408e408u), sixteenth = as_h2(0x2c002c00u), seventy_two = as_h2(0xd480d480u);   // -1032, 1 / 16, -72
+    codes8_raw(w, p);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        p[i] = as_u(__hadd2(as_h2(p[i]), eight));
+        p[i + 1] = as_u(__hfma2(as_h2(p[i + 1]), sixteenth, seventy_two));
     }
 }
 
-// tiles [t_lo, t_lo + n) that the rows a .. b of a sequence see, one at least (it may have nothing to see in it)
+// pairs of tiles [lo, lo + n) that the rows a .. b of a sequence see, one at least (it may have nothing to see in it)
 struct Span { int lo, n; };
 __device__ __forceinline__ Span span_of(const Cache & c, const Seq & q, int window, int a, int b) {
     const int last = min(q.held + b, (c.max_pages << c.page_log2) - 1);
     const int first = window > 0 ? max(0, q.held + a - window + 1) : 0;
     Span s;
-    s.lo = first >> 4;
-    s.n = q.slot < 0 || last < first ? 1 : (last >> 4) - s.lo + 1;
+    s.lo = first >> 5;
+    s.n = q.slot < 0 || last < first ? 1 : (last >> 5) - s.lo + 1;
     return s;
 }
 // a sequence's units: column tiles x KV heads, of which each column tile has a span of its own. Units of a sequence are made equally long: the span of all its rows
 __device__ __forceinline__ int col_tiles(const Seq & q, int group, int cols) { return (q.count * group + cols - 1) / cols; }
 
+__device__ __forceinline__ long long quotient(long long a, int b) { return a >> 31 ? a / b : (long long) ((unsigned) a / (unsigned) b); }
+
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_attend(const AttendArgs a) {
-    constexpr int NB = HD / 32, COLS = 8 * NT, TILE = 18 * HD;
-    extern __shared__ long long before[];                          // [n_seq + 1]
+__global__ void __launch_bounds__(AT_WARPS * 32, at_blocks(NT)) k_kv4_attend(const AttendArgs a) {
+    constexpr int NB = HD / 32, COLS = 8 * NT, TILE = 18 * HD, PAIR = 2 * TILE;
+    constexpr bool FOLD = NT == 1;                                 // the codes' offsets are taken off in the sums, where there are registers for them
+    extern __shared__ __align__(16) uint8_t at_raw[];              // each warp's ring of tiles, then before
+    long long * before = reinterpret_cast<long long *>(at_raw + at_ring_bytes(HD));     // [n_seq + 1]
     __shared__ long long sums[AT_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
     const Cache & c = a.c;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    // tiles in front of each sequence
+    // pairs of tiles in front of each sequence
     {
         const int each = (c.n_seq + AT_WARPS * 32 - 1) / (AT_WARPS * 32), s0 = min(c.n_seq, tid * each), s1 = min(c.n_seq, s0 + each);
         long long mine = 0;
         for (int s = s0; s < s1; s++) {
             const Seq q = seq_at(c, s);
             before[s] = mine;
-            mine += q.count ? (long long) col_tiles(q, a.group, COLS) * c.n_kv * span_of(c, q, a.window, 0, q.count - 1).n : 0;
+            mine += q.count ? (long long) col_tiles(q, a.group, COLS) * c.n_kv * (span_of(c, q, a.window, 0, q.count - 1).n + AT_OVER) : 0;
         }
         long long up = mine;
 #pragma unroll
@@ -90,7 +130,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_attend(const AttendArgs a
     }
     const long long total = before[c.n_seq];
     const int n_warps = (int) gridDim.x * AT_WARPS;
-    const long long per = max(1ll, (total + n_warps - 1) / n_warps);
+    const long long per = max(1ll, quotient(total + n_warps - 1, n_warps));
     if (blockIdx.x == 0) {
         for (int s = tid; s <= c.n_seq; s += AT_WARPS * 32) a.before[s] = before[s];
         if (tid == 0) a.before[c.n_seq + 1] = per;
@@ -102,26 +142,77 @@ __global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_attend(const AttendArgs a
         int s = 0;
         for (int hi = c.n_seq; hi - s > 1;) { const int mid = (s + hi) >> 1; if (before[mid] <= at) s = mid; else hi = mid; }
         const Seq q = seq_at(c, s);
-        const Span sp = span_of(c, q, a.window, 0, q.count - 1);
-        const int x = (int) (at - before[s]), unit = x / sp.n, t0 = x - unit * sp.n, t1 = (int) min((long long) sp.n, t0 + (end - at));
-        const int ct = unit / c.n_kv, head = unit - ct * c.n_kv;
-        at += t1 - t0;
-        // columns: B operand of K Q^T. Lane (g, tq) holds column g's dims 32 b + 8 tq .. + 7 as pairs (n, n + 4)
-        uint32_t qf[NT][NB][4];
-        float factor[NT][2];
-        int p_hi[NT][2];                                           // last position that the lane's two columns of S^T see; -1: no column
+        const Span sp = span_of(c, q, a.window, 0, q.count - 1);               // (in pairs of tiles, like all counts here)
+        const long long x = at - before[s];
+        const int len = sp.n + AT_OVER, unit = (int) quotient(x, len), from = (int) (x - (long long) unit * len), to = (int) min((long long) len, from + (end - at));
+        const int ct = unit / c.n_kv, head = unit - ct * c.n_kv, t0 = max(0, from - AT_OVER), t1 = to - AT_OVER;
+        at += to - from;
+        if (t1 <= 0) continue;
+        // the columns' queries: asked for ahead of the pages
+        Eight<T> raw[NT][NB] = {};
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int col = ct * COLS + 8 * n + g, i = col / a.group, h = head * a.group + col - i * a.group;
-            const bool in = i < q.count;
+            if (i >= q.count) continue;
+            const T * qp = static_cast<const T *>(a.q) + (q.begin + i) * a.q_row + h * a.q_head + 8 * tq;
+            if (a.q_whole) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) raw[n][b] = *reinterpret_cast<const Eight<T> *>(qp + 32 * b);
+            } else {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) raw[n][b].v[j] = qp[32 * b + j];
+            }
+        }
+        // pairs of tiles on their way: AT_STAGES - 1 ahead of the one in hand. A head's tiles of a page are contiguous; lanes hold the next 32 pages of the slot
+        const uint32_t ring = smem_at(at_raw) + (uint32_t) (warp * AT_STAGES * PAIR + 16 * lane);
+        const int tiles_log2 = c.page_log2 - 4, tile_mask = (1 << tiles_log2) - 1;
+        int next = 2 * (sp.lo + t0), pages_from = next >> tiles_log2, my_page = page_at(c, q.slot, (pages_from + lane) << c.page_log2), fill = 0, use = 0;
+        const int end_tile = 2 * (sp.lo + t1);
+        PairSrc src;
+        uint32_t there = 0;                                        // two bits a pair that was asked for: which of its tiles have a page. The newest lowest
+        const auto turn_page = [&]() {
+            const int pi = next >> tiles_log2;
+            if (pi - pages_from >= 31) { pages_from = pi; my_page = page_at(c, q.slot, (pi + lane) << c.page_log2); }
+            const int page_a = __shfl_sync(0xffffffffu, my_page, pi - pages_from);
+            src.bytes_a = page_a >= 0 ? 16 : 0;
+            src.a = c.pool + (page_a >= 0 ? tile_offset(c, page_a, head, next << 4, TILE) : 0) + 16 * lane;
+            if (tile_mask == 0) {                                  // pages of one tile
+                const int page_b = __shfl_sync(0xffffffffu, my_page, pi + 1 - pages_from);
+                src.bytes_b = page_b >= 0 ? 16 : 0;
+                src.b = c.pool + (page_b >= 0 ? tile_offset(c, page_b, head, 0, TILE) - TILE : 0) + 16 * lane;
+                const bool first = lane < TILE % 512 / 16;
+                src.mid = first ? src.a : src.b; src.bytes_mid = first ? src.bytes_a : src.bytes_b;
+            } else { src.mid = src.b = src.a; src.bytes_mid = src.bytes_b = src.bytes_a; }
+        };
+        const auto fetch = [&]() {
+            there <<= 2;
+            if (next < end_tile) {
+                if ((next & tile_mask) == 0) turn_page();
+                copy_pair<HD>(ring + fill, src, lane);
+                there |= (uint32_t) (src.bytes_a >> 4 | src.bytes_b >> 3);
+                src.a += PAIR; src.mid += PAIR; src.b += PAIR;
+                fill = fill == (AT_STAGES - 1) * PAIR ? 0 : fill + PAIR;
+                next += 2;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        __syncwarp();                                              // nobody still reads the ring for the piece before
+        turn_page();
+#pragma unroll
+        for (int i = 0; i < AT_STAGES - 1; i++) fetch();
+        // columns: B operand of K Q^T. Lane (g, tq) holds column g's dims 32 b + 8 tq .. + 7 as pairs (n, n + 4)
+        uint32_t qf[NT][NB][4];
+        float factor[NT][2], offset[NB][2] = {};
+        int p_hi[NT][2];                                           // last position that the lane's two columns of S^T see; -1: no column
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
             float v[NB][8], top = 0.f;
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    v[b][j] = in ? to_f(static_cast<const T *>(a.q)[(q.begin + i) * a.q_row + h * a.q_head + 32 * b + 8 * tq + j]) : 0.f;
-                    top = fmaxf(top, fabsf(v[b][j]));
-                }
+                for (int j = 0; j < 8; j++) { v[b][j] = to_f(raw[n][b].v[j]); top = fmaxf(top, fabsf(v[b][j])); }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // a power of two that brings the column's largest entry to 2^13 .. 2^14
@@ -130,7 +221,25 @@ __global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_attend(const AttendArgs a
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) qf[n][b][j] = as_u(__floats2half2_rn(v[b][j] * up, v[b][j + 4] * up));
+                for (int j = 0; j < 4; j++) {
+                    const float by = FOLD && (j & 1) ? up * 0.0625f : up;      // 16 c is what pairs 1 and 3 of a word give
+                    qf[n][b][j] = as_u(__floats2half2_rn(v[b][j] * by, v[b][j + 4] * by));
+                }
+            if (FOLD) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float2 x = __half22float2(as_h2(qf[n][b][j]));
+                        sum = fmaf(j & 1 ? -1152.f : -1032.f, x.x + x.y, sum);      // 1024 + 8, 1024 + 16 x 8
+                    }
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    offset[b][0] = __shfl_sync(0xffffffffu, sum, 8 * tq);
+                    offset[b][1] = __shfl_sync(0xffffffffu, sum, 8 * tq + 4);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int cc = ct * COLS + 8 * n + 2 * tq + j;
@@ -140,11 +249,11 @@ __global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_attend(const AttendArgs a
         }
         const int row_lo = ct * COLS / a.group, row_hi = min(q.count - 1, (ct * COLS + COLS - 1) / a.group);
         const int all_see_hi = q.held + row_lo, all_see_lo = a.window > 0 ? q.held + row_hi - a.window + 1 : 0;   // positions that every column sees
-        float o[NT][2 * NB][4], m[NT][2], l[NT][2];
+        float o[NT][2 * NB][4], m[NT][2], l[NT][2], base[NT][2], limit[NT][2];       // base: what is taken off scores; limit: where the maximum moves
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) { m[n][j] = -INFINITY; l[n][j] = 0.f; }
+            for (int j = 0; j < 2; j++) { m[n][j] = limit[n][j] = -INFINITY; l[n][j] = base[n][j] = 0.f; }
 #pragma unroll
             for (int k = 0; k < 2 * NB; k++)
 #pragma unroll
@@ -152,98 +261,135 @@ __global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_attend(const AttendArgs a
         }
 #pragma unroll 1
         for (int t = t0; t < t1; t++) {
-            const int pos = (sp.lo + t) << 4, page = page_at(c, q.slot, pos);
-            if (page < 0) continue;
-            const uint8_t * tile = c.pool + tile_offset(c, page, head, pos, TILE);
-            uint32_t kw[2][NB], vw[NB][2];
-            __half ks[2][NB];
-            __half2 vs[NB][2];
+            asm volatile("cp.async.wait_group %0;" :: "n"(AT_STAGES - 2) : "memory");
+            __syncwarp();                                          // all lanes' copies of pair t are there, and all are done with pair t - 1
+            fetch();
+            const uint8_t * pair = at_raw + warp * AT_STAGES * PAIR + use;
+            use = use == (AT_STAGES - 1) * PAIR ? 0 : use + PAIR;
+            const uint32_t both = there >> 2 * (AT_STAGES - 1) & 3;
+            if (both == 0) continue;
+            const int pos = (sp.lo + t) << 5;
+            float st[2][NT][4];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int u = 0; u < 2; u++) {
+                const uint8_t * tile = pair + u * TILE;
+                uint32_t kw[2][NB];
+                __half2 ks[2][NB / 2];
+                if constexpr (NB == 4) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint4 x = reinterpret_cast<const uint4 *>(tile)[j * 32 + lane];
+                        kw[j][0] = x.x; kw[j][1] = x.y; kw[j][2] = x.z; kw[j][3] = x.w;
+                    }
+                    const uint4 x = reinterpret_cast<const uint4 *>(tile + 16 * HD)[g];
+                    ks[0][0] = as_h2(x.x); ks[0][1] = as_h2(x.y); ks[1][0] = as_h2(x.z); ks[1][1] = as_h2(x.w);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint2 x = reinterpret_cast<const uint2 *>(tile)[j * 32 + lane];
+                        kw[j][0] = x.x; kw[j][1] = x.y;
+                    }
+                    const uint2 x = reinterpret_cast<const uint2 *>(tile + 16 * HD)[g];
+                    ks[0][0] = as_h2(x.x); ks[1][0] = as_h2(x.y);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) st[u][n][j] = 0.f;
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    kw[j][b] = reinterpret_cast<const uint32_t *>(tile)[(j * 32 + lane) * NB + b];
-                    vw[b][j] = reinterpret_cast<const uint32_t *>(tile + 8 * HD)[((b >> 1) * 32 + lane) * 4 + (b & 1) * 2 + j];
-                    ks[j][b] = reinterpret_cast<const __half *>(tile + 16 * HD)[(g * 2 + j) * NB + b];
-                    vs[b][j] = reinterpret_cast<const __half2 *>(tile + 17 * HD)[(tq * NB + b) * 2 + j];
-                }
-            float st[NT][4];
+                    uint32_t p0[4], p1[4];
+                    if (FOLD) { codes8_raw(kw[0][b], p0); codes8_raw(kw[1][b], p1); }
+                    else { codes8(kw[0][b], p0); codes8(kw[1][b], p1); }
+                    const float d0 = b & 1 ? __high2float(ks[0][b / 2]) : __low2float(ks[0][b / 2]), d1 = b & 1 ? __high2float(ks[1][b / 2]) : __low2float(ks[1][b / 2]);
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) st[n][j] = 0.f;
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                uint32_t p0[4], p1[4];
-                codes8(kw[0][b], p0);
-                codes8(kw[1][b], p1);
-                const float d0 = __half2float(ks[0][b]), d1 = __half2float(ks[1][b]);
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                    const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
-                    mma_16816(acc, a0, qf[n][b][0], qf[n][b][1]);
-                    mma_16816(acc, a1, qf[n][b][2], qf[n][b][3]);
-                    st[n][0] = fmaf(acc[0], d0, st[n][0]); st[n][1] = fmaf(acc[1], d0, st[n][1]);
-                    st[n][2] = fmaf(acc[2], d1, st[n][2]); st[n][3] = fmaf(acc[3], d1, st[n][3]);
+                    for (int n = 0; n < NT; n++) {
+                        float acc[4];
+                        const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
+                        mma_16816(acc, a0, qf[n][b][0], qf[n][b][1], offset[b]);
+                        mma_16816(acc, a1, qf[n][b][2], qf[n][b][3]);
+                        st[u][n][0] = fmaf(acc[0], d0, st[u][n][0]); st[u][n][1] = fmaf(acc[1], d0, st[u][n][1]);
+                        st[u][n][2] = fmaf(acc[2], d1, st[u][n][2]); st[u][n][3] = fmaf(acc[3], d1, st[u][n][3]);
+                    }
                 }
             }
-            // rows of S^T: tokens c + 4 (2 j + e) with g = 2 c + e
-            const bool edge = pos + 15 > all_see_hi || pos < all_see_lo || row_hi < 0;
-            const int p0 = pos + (g >> 1) + 4 * (g & 1);
             bool more = false;
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    st[n][j] *= factor[n][j & 1];
-                    if (edge) {
-                        const int p = p0 + 8 * (j >> 1), top = p_hi[n][j & 1];
-                        if (p > top || (a.window > 0 && p <= top - a.window)) st[n][j] = -INFINITY;
-                    }
-                    more = more || st[n][j] > m[n][j & 1] + 8.f;
-                }
+                for (int j = 0; j < 4; j++) { st[0][n][j] *= factor[n][j & 1]; st[1][n][j] *= factor[n][j & 1]; }
+            // rows of S^T: tokens c + 4 (2 j + e) with g = 2 c + e
+            if (pos + 31 > all_see_hi || pos < all_see_lo || both != 3) {
+                const int p0 = pos + (g >> 1) + 4 * (g & 1);
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int p = p0 + 16 * u + 8 * (j >> 1), top = p_hi[n][j & 1];
+                            if (p > top || (a.window > 0 && p <= top - a.window) || !(both >> u & 1)) st[u][n][j] = -INFINITY;
+                        }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) more = more || fmaxf(fmaxf(st[0][n][j], st[0][n][j + 2]), fmaxf(st[1][n][j], st[1][n][j + 2])) > limit[n][j];
             // the maximum moves only when a score passes it by 2^8: P stays in fp16's range below that
             if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        float x = fmaxf(st[n][j], st[n][j + 2]);
+                        float x = fmaxf(fmaxf(st[0][n][j], st[0][n][j + 2]), fmaxf(st[1][n][j], st[1][n][j + 2]));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                         const float top = fmaxf(m[n][j], x), down = top > m[n][j] ? exp2_fast(m[n][j] - top) : 1.f;
                         m[n][j] = top;
+                        base[n][j] = top == -INFINITY ? 0.f : top;
+                        limit[n][j] = top + 8.f;
                         l[n][j] *= down;
 #pragma unroll
                         for (int k = 0; k < 2 * NB; k++) { o[n][k][j] *= down; o[n][k][j + 2] *= down; }
                     }
             }
-            uint32_t pb[NT][2];
+            uint32_t pb[2][NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float base = m[n][j & 1] == -INFINITY ? 0.f : m[n][j & 1];
-                    st[n][j] = exp2_fast(st[n][j] - base);
-                    l[n][j & 1] += st[n][j];
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        st[u][n][j] = exp2_fast(st[u][n][j] - base[n][j & 1]);
+                        l[n][j & 1] += st[u][n][j];
+                    }
+                    pb[u][n][0] = transposed(as_u(__floats2half2_rn(st[u][n][0], st[u][n][1])));
+                    pb[u][n][1] = transposed(as_u(__floats2half2_rn(st[u][n][2], st[u][n][3])));
                 }
-                pb[n][0] = transposed(as_u(__floats2half2_rn(st[n][0], st[n][1])));
-                pb[n][1] = transposed(as_u(__floats2half2_rn(st[n][2], st[n][3])));
-            }
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                uint32_t p0[4], p1[4];
-                codes8(vw[b][0], p0);
-                codes8(vw[b][1], p1);
+            for (int u = 0; u < 2; u++) {
+                const uint8_t * tile = pair + u * TILE;
 #pragma unroll
-                for (int i = 0; i < 4; i++) { p0[i] = as_u(__hmul2(as_h2(p0[i]), vs[b][0])); p1[i] = as_u(__hmul2(as_h2(p1[i]), vs[b][1])); }
+                for (int bb = 0; bb < NB / 2; bb++) {
+                    const uint4 y = reinterpret_cast<const uint4 *>(tile + 8 * HD)[bb * 32 + lane], z = reinterpret_cast<const uint4 *>(tile + 17 * HD)[(NB / 2) * tq + bb];
+                    const uint32_t vw[2][2] = {{y.x, y.y}, {y.z, y.w}};
+                    const __half2 vs[2][2] = {{as_h2(z.x), as_h2(z.y)}, {as_h2(z.z), as_h2(z.w)}};
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const uint32_t av[4] = {p0[2 * k], p0[2 * k + 1], p1[2 * k], p1[2 * k + 1]};
+                    for (int e = 0; e < 2; e++) {
+                        const int b = 2 * bb + e;
+                        uint32_t p0[4], p1[4];
+                        codes8(vw[e][0], p0);
+                        codes8(vw[e][1], p1);
 #pragma unroll
-                    for (int n = 0; n < NT; n++) mma_16816(o[n][2 * b + k], av, pb[n][0], pb[n][1]);
+                        for (int i = 0; i < 4; i++) { p0[i] = as_u(__hmul2(as_h2(p0[i]), vs[e][0])); p1[i] = as_u(__hmul2(as_h2(p1[i]), vs[e][1])); }
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const uint32_t av[4] = {p0[2 * k], p0[2 * k + 1], p1[2 * k], p1[2 * k + 1]};
+#pragma unroll
+                            for (int n = 0; n < NT; n++) mma_16816(o[n][2 * b + k], av, pb[u][n][0], pb[u][n][1]);
+                        }
+                    }
                 }
             }
         }
@@ -284,40 +430,75 @@ __global__ void __launch_bounds__(AT_WARPS * 32) k_kv4_attend(const AttendArgs a
     }
 }
 
-// a warp a row and head: adds the partial results of a unit that several warps shared, in their order
-template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(256) k_kv4_join(const AttendArgs a) {
-    constexpr int COLS = 8 * NT, E = HD / 32;
+// a block a row and head: adds the partial results of a unit that several warps shared. A warp takes every AJ_WARPS-th part, eight of them on their way at a time
+template <int HD, int NT, typename T, int AJ_WARPS>
+__global__ void __launch_bounds__(AJ_WARPS * 32) k_kv4_join(const AttendArgs a) {
+    constexpr int COLS = 8 * NT, E = HD / 32, BATCH = 8;
+    __shared__ float sums[AJ_WARPS][HD], ml_s[AJ_WARPS][2];
     const Cache & c = a.c;
-    const int lane = threadIdx.x & 31, n_head = c.n_kv * a.group;
-    const int64_t item = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (item >= (int64_t) c.n_rows * n_head) return;
-    const int row = (int) (item / n_head), h = (int) (item % n_head), s = seq_of_row(c, row);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_head = c.n_kv * a.group, row = blockIdx.x / n_head, h = blockIdx.x % n_head;
+    const int s = seq_of_row(c, row);
     if (s < 0) return;
     const int begin = min(max(c.first[s], 0), c.n_rows), count = min(max(c.first[s + 1], begin), c.n_rows) - begin;
     const int head = h / a.group, col = (row - begin) * a.group + h - head * a.group, ct = col / COLS, in_tile = col - ct * COLS;
-    const long long b0 = a.before[s], per = a.before[c.n_seq + 1];
-    const int n = (int) ((a.before[s + 1] - b0) / ((long long) ((count * a.group + COLS - 1) / COLS) * c.n_kv));
-    const long long u0 = b0 + (long long) (ct * c.n_kv + head) * n, w0 = u0 / per, w1 = (u0 + n - 1) / per;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const long long b0 = a.before[s], b1 = a.before[s + 1];
+    const int per = (int) a.before[c.n_seq + 1], len = (int) quotient(b1 - b0, (count * a.group + COLS - 1) / COLS * c.n_kv);
+    const long long u0 = b0 + (long long) (ct * c.n_kv + head) * len;
+    const int w0 = (int) quotient(u0 + AT_OVER, per), w1 = (int) quotient(u0 + len - 1, per);
     if (w0 == w1) return;
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = 0.f;
-    for (long long w = w0; w <= w1; w++) {
-        const size_t slot = 2 * (size_t) w + (w == w0 ? 1 : 0);
-        const float2 ml = *reinterpret_cast<const float2 *>(a.ml + (slot * COLS + in_tile) * 2);
-        const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top, old = exp2_fast(m - base), now = exp2_fast(ml.x - base);
-        l = l * old + ml.y * now;
-        const float * y = a.part + (slot * COLS + in_tile) * HD + E * lane;
+    for (int w = w0 + warp; w <= w1; w += AJ_WARPS * BATCH) {
+        float2 ml[BATCH];
+        float x[BATCH][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * old + y[e] * now;
+        for (int i = 0; i < BATCH; i++) {
+            const int at = w + i * AJ_WARPS;
+            ml[i] = make_float2(-INFINITY, 0.f);
+            const size_t slot = (2 * (size_t) at + (at == w0 ? 1 : 0)) * COLS + in_tile;
+#pragma unroll
+            for (int e = 0; e < E; e++) x[i][e] = 0.f;
+            if (at <= w1) {
+                ml[i] = *reinterpret_cast<const float2 *>(a.ml + slot * 2);
+                if constexpr (E == 4) { const float4 v = *reinterpret_cast<const float4 *>(a.part + slot * HD + 4 * lane); x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w; }
+                else { const float2 v = *reinterpret_cast<const float2 *>(a.part + slot * HD + 2 * lane); x[i][0] = v.x; x[i][1] = v.y; }
+            }
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) top = fmaxf(top, ml[i].x);
+        const float base = top == -INFINITY ? 0.f : top, old = exp2_fast(m - base);
+        l *= old;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] *= old;
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) {
+            const float by = exp2_fast(ml[i].x - base);
+            l = fmaf(ml[i].y, by, l);
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = fmaf(x[i][e], by, o[e]);
+        }
         m = top;
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    T * y = static_cast<T *>(a.out) + ((size_t) row * n_head + h) * HD + E * lane;
 #pragma unroll
-    for (int e = 0; e < E; e++) y[e] = from_f<T>(o[e] * inv);
+    for (int e = 0; e < E; e++) sums[warp][E * lane + e] = o[e];
+    if (lane == 0) { ml_s[warp][0] = m; ml_s[warp][1] = l; }
+    __syncthreads();
+    if (threadIdx.x < HD) {
+        float top = -INFINITY, total = 0.f, y = 0.f;
+#pragma unroll
+        for (int i = 0; i < AJ_WARPS; i++) top = fmaxf(top, ml_s[i][0]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < AJ_WARPS; i++) {
+            const float by = exp2_fast(ml_s[i][0] - base);
+            total = fmaf(ml_s[i][1], by, total);
+            y = fmaf(sums[i][threadIdx.x], by, y);
+        }
+        static_cast<T *>(a.out)[((size_t) row * n_head + h) * HD + threadIdx.x] = from_f<T>(total != 0.f ? y / total : 0.f);
+    }
 }
 
 }  // namespace srv
