@@ -18,7 +18,7 @@ $(OBJDIR)/stack.o: $(CSRC)/stack.cu $(CSRC)/stack_kernels.cuh $(CSRC)/stack_kern
 	@mkdir -p $(OBJDIR)
 	$(NVCC) $(NVCCFLAGS) -c $< -o $@ 2> $(OBJDIR)/stack.ptxas.log || (cat $(OBJDIR)/stack.ptxas.log; false)
 
-$(OBJDIR)/serve.o: $(CSRC)/serve.cu $(CSRC)/serve.hpp $(CSRC)/serve_cache.cuh $(CSRC)/serve_attn.cuh $(CSRC)/serve_pages.cuh $(CSRC)/serve_sample.cuh include/booster_b200.h
+$(OBJDIR)/serve.o: $(CSRC)/serve.cu $(CSRC)/serve.hpp $(CSRC)/serve_cache.cuh $(CSRC)/serve_attn.cuh $(CSRC)/serve_prompt.cuh $(CSRC)/serve_pages.cuh $(CSRC)/serve_sample.cuh include/booster_b200.h
 	@mkdir -p $(OBJDIR)
 	$(NVCC) $(NVCCFLAGS) -c $< -o $@ 2> $(OBJDIR)/serve.ptxas.log || (cat $(OBJDIR)/serve.ptxas.log; false)
 

@@ -2,12 +2,14 @@
 #include "serve.hpp"
 #include "serve_cache.cuh"
 #include "serve_attn.cuh"
+#include "serve_prompt.cuh"
 #include "serve_pages.cuh"
 #include "serve_sample.cuh"
 
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 
@@ -120,6 +122,48 @@ template <int HD, typename T> void attend_nt_as(const AttendArgs & a, int nt, in
     nt == 1 ? attend_as<HD, 1, T>(a, device, sms, stream) : attend_as<HD, 2, T>(a, device, sms, stream);
 }
 
+// attention of prompts' portions
+int64_t prompt_entries(const b200_kv4 & c, int group) { return (int64_t) c.n_rows * group / PR_COLS + c.n_seq + 1; }
+struct PromptWork { int64_t seq_of, entry_of, n_entries, ml, part, bytes; };       // places in the workspace; `before` is first
+PromptWork prompt_work(const b200_kv4 & c, int group, int sms) {
+    const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    const int64_t n = prompt_entries(c, group), slots = 2 * (int64_t) sms * PR_COLS;
+    PromptWork w;
+    w.seq_of = up((n + 2) * 8);
+    w.entry_of = w.seq_of + up(n * 4);
+    w.n_entries = w.entry_of + up((c.n_seq + 2) * 4);
+    w.ml = w.n_entries + 256;
+    w.part = w.ml + up(slots * 8);
+    w.bytes = w.part + slots * c.head_dim * 4;
+    return w;
+}
+// a word per device that a kernel raises when a bounded wait ran out, in pinned memory, so that the host reads it without waiting. It is looked at by the next call
+int * wait_flag(int device) {
+    static std::mutex lock;
+    static int * words[MAX_DEVICES] = {};
+    std::lock_guard<std::mutex> hold(lock);
+    if (!words[device]) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;         // (this may be the first call inside a capture)
+        cu(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+        void * p = nullptr;
+        const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        cu(e, "cudaHostAlloc");
+        *static_cast<volatile int *>(p) = 0;
+        words[device] = static_cast<int *>(p);
+    }
+    return words[device];
+}
+template <int HD, typename T> void prompt_as(const PromptArgs & p, int device, int sms, void * stream) {
+    static Limits set;
+    const auto kernel = k_kv4_prompt<HD, T>;
+    allow_smem(kernel, device, PromptSmem<HD>::BYTES, set);
+    launch(k_kv4_prompt_plan, dim3(1), 1024, 0, stream, false, 1, p, sms);
+    launch(kernel, dim3(sms), PR_THREADS, PromptSmem<HD>::BYTES, stream, true, 1, p);
+    const int64_t items = (int64_t) p.a.c.n_rows * p.a.c.n_kv * p.a.group;
+    launch(k_kv4_prompt_join<HD, T>, dim3((unsigned) ((items + 7) / 8)), 256, 0, stream, true, 1, p);
+}
+
 Pages checked(const b200_pages & p, bool pool) {
     need(p.page_tokens >= 16 && p.page_tokens <= 1024 && (p.page_tokens & (p.page_tokens - 1)) == 0, "pages: page_tokens is a power of two from 16 to 1024 (got " + std::to_string(p.page_tokens) + ")");
     need(p.n_pages >= 1 && p.n_pages <= PG_MAX_PAGES, "pages: from 1 to 2^20 pages");
@@ -180,14 +224,18 @@ void kv4_read(const b200_kv4 & c, int dtype, void * k, void * v) {
 }
 
 static void check_heads(const b200_kv4 & c, int n_head, int max_rows) {
-    need(n_head >= c.n_head_kv && n_head % std::max(1, c.n_head_kv) == 0 && n_head <= 65536, "kv4_attention: n_head is a multiple of n_head_kv (got " + std::to_string(n_head) + " and " + std::to_string(c.n_head_kv) + ")");
+    need(n_head >= c.n_head_kv && n_head % std::max(1, c.n_head_kv) == 0 && (int64_t) c.n_rows * n_head <= (1 << 30), "kv4_attention: n_head is a multiple of n_head_kv (got " + std::to_string(n_head) + " and " + std::to_string(c.n_head_kv) + "), and rows x heads up to 2^30");
     need(max_rows >= 1 && max_rows <= (1 << 24), "kv4_attention: max_rows is the largest number of rows of a sequence");
 }
+
+// columns of a sequence from which its tiles are worth making fp16 for the tensor cores' larger products
+bool is_prompt(int group, int max_rows) { return (int64_t) group * max_rows > 64; }
 
 int64_t kv4_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
     checked(c, false);
     check_heads(c, n_head, max_rows);
     On on(c.device);
+    if (is_prompt(n_head / c.n_head_kv, max_rows)) return prompt_work(c, n_head / c.n_head_kv, on.sms).bytes;
     return (int64_t) attend_bytes(c.n_seq, c.head_dim, attend_nt(n_head / c.n_head_kv, max_rows), on.sms);
 }
 
@@ -206,11 +254,27 @@ void kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row,
     a.group = n_head / c.n_head_kv;
     a.scale_log2 = scale * 1.44269504088896341f;
     a.window = window;
+    uint8_t * w = static_cast<uint8_t *>(work);
+    if (is_prompt(a.group, max_rows)) {
+        const PromptWork at = prompt_work(c, a.group, on.sms);
+        check_work(work, work_bytes, at.bytes);
+        PromptArgs p = {a, reinterpret_cast<int *>(w + at.seq_of), reinterpret_cast<int *>(w + at.entry_of), reinterpret_cast<int *>(w + at.n_entries), wait_flag(c.device)};
+        if (*static_cast<volatile int *>(p.err)) {
+            *static_cast<volatile int *>(p.err) = 0;
+            throw std::runtime_error("a wait inside an earlier kv4_attention on this device ran out: its results are missing");
+        }
+        p.a.before = reinterpret_cast<long long *>(w);
+        p.a.ml = reinterpret_cast<float *>(w + at.ml);
+        p.a.part = reinterpret_cast<float *>(w + at.part);
+        if (dtype == B200_DTYPE_BF16) c.head_dim == 128 ? prompt_as<128, __nv_bfloat16>(p, c.device, on.sms, c.stream) : prompt_as<64, __nv_bfloat16>(p, c.device, on.sms, c.stream);
+        else c.head_dim == 128 ? prompt_as<128, __half>(p, c.device, on.sms, c.stream) : prompt_as<64, __half>(p, c.device, on.sms, c.stream);
+        return;
+    }
     const int nt = attend_nt(a.group, max_rows);
     check_work(work, work_bytes, (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms));
     const size_t slots = 2 * (size_t) on.sms * at_blocks(nt) * AT_WARPS;
-    a.before = static_cast<long long *>(work);
-    a.ml = reinterpret_cast<float *>(static_cast<uint8_t *>(work) + attend_before_bytes(c.n_seq));
+    a.before = reinterpret_cast<long long *>(w);
+    a.ml = reinterpret_cast<float *>(w + attend_before_bytes(c.n_seq));
     a.part = a.ml + slots * 8 * nt * 2;
     if (dtype == B200_DTYPE_BF16) c.head_dim == 128 ? attend_nt_as<128, __nv_bfloat16>(a, nt, c.device, on.sms, c.stream) : attend_nt_as<64, __nv_bfloat16>(a, nt, c.device, on.sms, c.stream);
     else c.head_dim == 128 ? attend_nt_as<128, __half>(a, nt, c.device, on.sms, c.stream) : attend_nt_as<64, __half>(a, nt, c.device, on.sms, c.stream);

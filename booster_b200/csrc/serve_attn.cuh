@@ -96,6 +96,7 @@ __device__ __forceinline__ Span span_of(const Cache & c, const Seq & q, int wind
 // a sequence's units: column tiles x KV heads, of which each column tile has a span of its own. Units of a sequence are made equally long: the span of all its rows
 __device__ __forceinline__ int col_tiles(const Seq & q, int group, int cols) { return (q.count * group + cols - 1) / cols; }
 
+// (most quotients are of 31 bits)
 __device__ __forceinline__ long long quotient(long long a, int b) { return a >> 31 ? a / b : (long long) ((unsigned) a / (unsigned) b); }
 
 template <int HD, int NT, typename T>

@@ -191,6 +191,28 @@ def test_attention_of_portions(hd, heads, kv, held, counts, window):
     assert_attends(c, c.seen(), q, out, window, 0.2)
 
 
+@pytest.mark.parametrize("hd,heads,kv", [(64, 4, 2), (128, 8, 1)])
+def test_attention_of_many_short_portions(hd, heads, kv):
+    """blocks walk through many pieces of one and of two halves of columns, one after the other"""
+    r = random.Random(hd)
+    n = 260
+    c = Case([r.randrange(0, 300) for _ in range(n)], [r.choice([17, 20, 33, 40, 64]) for _ in range(n)], kv=kv, hd=hd, seed=hd)
+    c.fill()
+    q = c.randn(c.rows, heads, hd).half()
+    out = serve.kv4_attention(q, *c.args(), slots=c.slots, max_rows=64)
+    # the same row by row, by the kernels of single tokens, which the tests above hold to the definition: both round P (2^-11) and the result
+    one = torch.empty_like(out)
+    for i in range(max(c.counts)):
+        sel = [s for s in range(n) if i < c.counts[s]]
+        rows = torch.tensor([c.first_l[s] + i for s in sel], device="cuda")
+        held = c.held.clone()
+        held[c.slots[sel].long()] += i
+        one[rows] = serve.kv4_attention(q[rows], c.pool[0], c.table, held, ints(list(range(len(sel) + 1))), c.slots[sel], max_rows=1)
+    assert torch.isfinite(out).all()
+    big = max(np.abs(v).max() for v in c.v)
+    assert (out.double() - one.double()).abs().max().item() <= big * (2 * 2.0 ** -11 + 2 * 2.0 ** -11 + 2.0 ** -14)
+
+
 @pytest.mark.parametrize("rows,max_rows", [(70, 1), (70, 3), (3, 1000)])
 def test_a_wrong_max_rows_changes_no_result(rows, max_rows):
     c = Case([20, 3], [rows, 2], kv=1, hd=64)
