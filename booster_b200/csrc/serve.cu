@@ -124,15 +124,15 @@ template <int HD, typename T> void attend_nt_as(const AttendArgs & a, int nt, in
 
 // attention of prompts' portions
 int64_t prompt_entries(const b200_kv4 & c, int group) { return (int64_t) c.n_rows * group / PR_COLS + c.n_seq + 1; }
-struct PromptWork { int64_t seq_of, entry_of, n_entries, ml, part, bytes; };       // places in the workspace; `before` is first
+struct PromptWork { int64_t entries, entry_of, first, ml, part, bytes; };       // places in the workspace; `before` is first
 PromptWork prompt_work(const b200_kv4 & c, int group, int sms) {
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     const int64_t n = prompt_entries(c, group), slots = 2 * (int64_t) sms * PR_COLS;
     PromptWork w;
-    w.seq_of = up((n + 2) * 8);
-    w.entry_of = w.seq_of + up(n * 4);
-    w.n_entries = w.entry_of + up((c.n_seq + 2) * 4);
-    w.ml = w.n_entries + 256;
+    w.entries = up((n + 2) * 8);
+    w.entry_of = w.entries + up(n * (int64_t) sizeof(Entry));
+    w.first = w.entry_of + up((c.n_seq + 2) * 4);
+    w.ml = w.first + up((sms + 2) * 4);
     w.part = w.ml + up(slots * 8);
     w.bytes = w.part + slots * c.head_dim * 4;
     return w;
@@ -154,14 +154,13 @@ int * wait_flag(int device) {
     }
     return words[device];
 }
-template <int HD, typename T> void prompt_as(const PromptArgs & p, int device, int sms, void * stream) {
+template <int HD, typename T> void prompt_as(const PromptArgs & p, int64_t entries, int device, int sms, void * stream) {
     static Limits set;
     const auto kernel = k_kv4_prompt<HD, T>;
     allow_smem(kernel, device, PromptSmem<HD>::BYTES, set);
-    launch(k_kv4_prompt_plan, dim3(1), 1024, 0, stream, false, 1, p, sms);
+    launch(k_kv4_prompt_plan, dim3(1), 1024, (size_t) (p.a.c.n_seq + 1) * 4, stream, false, 1, p, sms);
     launch(kernel, dim3(sms), PR_THREADS, PromptSmem<HD>::BYTES, stream, true, 1, p);
-    const int64_t items = (int64_t) p.a.c.n_rows * p.a.c.n_kv * p.a.group;
-    launch(k_kv4_prompt_join<HD, T>, dim3((unsigned) ((items + 7) / 8)), 256, 0, stream, true, 1, p);
+    launch(k_kv4_prompt_join<HD, T>, dim3((unsigned) (entries * (PR_COLS / 32)), (unsigned) p.a.c.n_kv), 256, 0, stream, true, 1, p);
 }
 
 Pages checked(const b200_pages & p, bool pool) {
@@ -258,16 +257,17 @@ void kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row,
     if (is_prompt(a.group, max_rows)) {
         const PromptWork at = prompt_work(c, a.group, on.sms);
         check_work(work, work_bytes, at.bytes);
-        PromptArgs p = {a, reinterpret_cast<int *>(w + at.seq_of), reinterpret_cast<int *>(w + at.entry_of), reinterpret_cast<int *>(w + at.n_entries), wait_flag(c.device)};
+        PromptArgs p = {a, reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.entry_of), reinterpret_cast<int *>(w + at.first), wait_flag(c.device)};
         if (*static_cast<volatile int *>(p.err)) {
             *static_cast<volatile int *>(p.err) = 0;
             throw std::runtime_error("a wait inside an earlier kv4_attention on this device ran out: its results are missing");
         }
+        const int64_t n = prompt_entries(c, a.group);
         p.a.before = reinterpret_cast<long long *>(w);
         p.a.ml = reinterpret_cast<float *>(w + at.ml);
         p.a.part = reinterpret_cast<float *>(w + at.part);
-        if (dtype == B200_DTYPE_BF16) c.head_dim == 128 ? prompt_as<128, __nv_bfloat16>(p, c.device, on.sms, c.stream) : prompt_as<64, __nv_bfloat16>(p, c.device, on.sms, c.stream);
-        else c.head_dim == 128 ? prompt_as<128, __half>(p, c.device, on.sms, c.stream) : prompt_as<64, __half>(p, c.device, on.sms, c.stream);
+        if (dtype == B200_DTYPE_BF16) c.head_dim == 128 ? prompt_as<128, __nv_bfloat16>(p, n, c.device, on.sms, c.stream) : prompt_as<64, __nv_bfloat16>(p, n, c.device, on.sms, c.stream);
+        else c.head_dim == 128 ? prompt_as<128, __half>(p, n, c.device, on.sms, c.stream) : prompt_as<64, __half>(p, n, c.device, on.sms, c.stream);
         return;
     }
     const int nt = attend_nt(a.group, max_rows);

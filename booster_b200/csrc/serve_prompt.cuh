@@ -4,24 +4,27 @@
 // line that is cut evenly, here over one block per SM; k_kv4_prompt_plan lays the line out, k_kv4_prompt_join adds the parts of units that blocks shared.
 //   warps 0-3, 4-7   soft-max of columns 0-127 and 128-255, a thread a column: maximum and exponentials of its row of S, P back into tensor memory in the place of S
 //   warps 8-11       codes of 32 tokens each to fp16 in shared memory (exact: a scale has 8 bits, a code 4), K by rows of tokens, V by rows of dims, both with 128-byte swizzle
-//   warp 12          one thread issues S = Q K^T (128 x 128 x head_dim, twice) and O += P V (P from tensor memory, 128 x head_dim x 128, twice)
+//   warp 12          (of 12-15: registers are shared out by four warps: 128 a thread at launch, then 168, 168, 112 and 64) one thread issues S = Q K^T (128 x 128 x head_dim, twice) and O += P V (P from tensor memory, 128 x head_dim x 128, twice)
 // While one half's soft-max runs, the other half's products do. Tensor memory: S and P [2][128 columns], O [2][head_dim].
 // Tokens of 32 stand as n = 8 c + 4 u + i for token 16 u + c + 4 i in S, P, K and V alike, and dims of 8 as 0 4 1 5 2 6 3 7 in Q and K: the orders in which a word's codes come apart.
 // P is rounded to fp16 (2^-11), q scaled by a power of two into fp16's range; sums are fp32. The maximum moves when a score passes it by 2^8; O is scaled in tensor memory then.
 // Every wait on an mbarrier is bounded: on a timeout the block raises *err, skips what is left and frees its tensor memory.
 #pragma once
 #include "serve_attn.cuh"
+#include <type_traits>
 
 namespace b200 {
 namespace srv {
 
+struct Entry { int slot, begin, count, held, ct, lo, n, pad; };         // a sequence (Seq), its columns' number, their span of tiles
 struct PromptArgs {
     AttendArgs a;                        // a.before: [entries + 1] tiles in front of each entry (a sequence's 256 columns), for all KV heads together
-    int * seq_of, * entry_of, * n_entries;   // [entries], [n_seq + 1], {entries, tiles of a block's piece}
+    Entry * entries;
+    int * entry_of, * first;             // [n_seq + 1] a sequence's first entry; {tiles of a block's piece, total > 0, the entry that each block's piece begins in}
     int * err;
 };
 
-constexpr int PR_COLS = 256, PR_KV = 128, PR_THREADS = 416, PR_OVER = 2;      // PR_OVER: what beginning a unit costs, in tiles
+constexpr int PR_COLS = 256, PR_KV = 128, PR_THREADS = 512, PR_OVER = 2;      // PR_OVER: what beginning a unit costs, in tiles
 constexpr uint64_t PR_DESC = (1ull << 16) | ((uint64_t) (1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);      // K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart
 __host__ __device__ constexpr uint32_t pr_idesc(int n) { return (1u << 4) | ((uint32_t) (n >> 3) << 17) | (8u << 24); }     // D f32, A and B f16, M = 128
 template <int HD> struct PromptSmem {
@@ -41,6 +44,8 @@ __device__ __forceinline__ void pr_arrive(uint32_t bar) { asm volatile("mbarrier
 __device__ __forceinline__ void pr_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory"); }
 __device__ __forceinline__ void pr_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pr_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
 __device__ __forceinline__ bool pr_elect() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
@@ -81,6 +86,11 @@ __device__ __forceinline__ void pr_st_shared(uint32_t at, uint32_t x, uint32_t y
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+__device__ __forceinline__ uint64_t two(float x, float y) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float2 split(uint64_t p) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p)); return r; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
 // tiles of 128 tokens that the columns of an entry see, one at least
 __device__ __forceinline__ Span prompt_span(const Cache & c, const Seq & q, int group, int window, int ct) {
     const int a = ct * PR_COLS / group, b = min(q.count - 1, (ct * PR_COLS + PR_COLS - 1) / group);
@@ -91,58 +101,81 @@ __device__ __forceinline__ Span prompt_span(const Cache & c, const Seq & q, int 
     return s;
 }
 
-// one block: the line of entries
+// sum over the threads in front of this one and of the block, of 1024 threads
+template <typename V> __device__ __forceinline__ V plan_before(V mine, V & all, V * sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    V up = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) { const V x = __shfl_up_sync(0xffffffffu, up, d); if (lane >= d) up += x; }
+    __syncthreads();
+    if (lane == 31) sums[warp] = up;
+    __syncthreads();
+    V part = sums[lane], off = up - mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) { const V x = __shfl_up_sync(0xffffffffu, part, d); if (lane >= d) part += x; }
+    all = __shfl_sync(0xffffffffu, part, 31);
+    const V front = __shfl_sync(0xffffffffu, part, (warp + 31) & 31);
+    return off + (warp ? front : 0);
+}
+
+// one block: the line of entries, a thread an entry
 __global__ void __launch_bounds__(1024) k_kv4_prompt_plan(const PromptArgs p, int n_blocks) {
+    extern __shared__ int entry_of[];                              // [n_seq + 1]
     __shared__ long long sums[32];
     __shared__ int counts[32];
     const Cache & c = p.a.c;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int each = (c.n_seq + 1023) / 1024, s0 = min(c.n_seq, tid * each), s1 = min(c.n_seq, s0 + each);
-    long long tiles = 0;
-    int entries = 0;
-    for (int s = s0; s < s1; s++) {
-        const Seq q = seq_at(c, s);
-        const int n = col_tiles(q, p.a.group, PR_COLS);
-        entries += n;
-        for (int ct = 0; ct < n; ct++) tiles += (long long) c.n_kv * (prompt_span(c, q, p.a.group, p.a.window, ct).n + PR_OVER);
+    int all = 0;
+    for (int s0 = 0; s0 < c.n_seq; s0 += 1024) {
+        const int s = s0 + tid;
+        int some;
+        const int n = s < c.n_seq ? col_tiles(seq_at(c, s), p.a.group, PR_COLS) : 0, at = all + plan_before(n, some, counts);
+        if (s < c.n_seq) { entry_of[s] = at; p.entry_of[s] = at; }
+        all += some;
     }
-    long long up = tiles;
-    int upe = entries;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, up, d);
-        const int y = __shfl_up_sync(0xffffffffu, upe, d);
-        if (lane >= d) { up += x; upe += y; }
-    }
-    if (lane == 31) { sums[warp] = up; counts[warp] = upe; }
+    if (tid == 0) { entry_of[c.n_seq] = all; p.entry_of[c.n_seq] = all; }
     __syncthreads();
-    long long at = up - tiles, total = 0;
-    int e = upe - entries, all = 0;
-    for (int w = 0; w < 32; w++) {
-        if (w < warp) { at += sums[w]; e += counts[w]; }
-        total += sums[w]; all += counts[w];
-    }
-    for (int s = s0; s < s1; s++) {
-        const Seq q = seq_at(c, s);
-        const int n = col_tiles(q, p.a.group, PR_COLS);
-        p.entry_of[s] = e;
-        for (int ct = 0; ct < n; ct++, e++) {
-            p.seq_of[e] = s;
-            p.a.before[e] = at;
-            at += (long long) c.n_kv * (prompt_span(c, q, p.a.group, p.a.window, ct).n + PR_OVER);
+    long long total = 0;
+    for (int e0 = 0; e0 < all; e0 += 1024) {
+        const int e = e0 + tid;
+        long long n = 0, some;
+        if (e < all) {
+            int s = 0;                                             // the last sequence that begins at or before e (those without rows begin where the next one does)
+            for (int hi = c.n_seq; hi - s > 1;) { const int mid = (s + hi) >> 1; if (entry_of[mid] <= e) s = mid; else hi = mid; }
+            const Seq q = seq_at(c, s);
+            const int ct = e - entry_of[s];
+            const Span sp = prompt_span(c, q, p.a.group, p.a.window, ct);
+            p.entries[e] = Entry{q.slot, q.begin, q.count, q.held, ct, sp.lo, sp.n, 0};
+            n = (long long) c.n_kv * (sp.n + PR_OVER);
         }
+        const long long at = total + plan_before(n, some, sums);
+        if (e < all) p.a.before[e] = at;
+        total += some;
     }
-    if (tid == 0) {
-        p.a.before[all] = total;
-        p.entry_of[c.n_seq] = all;
-        p.n_entries[0] = all;
-        p.n_entries[1] = (int) max(1ll, (total + n_blocks - 1) / n_blocks);
+    const int per = (int) max(1ll, quotient(total + n_blocks - 1, n_blocks));
+    if (tid == 0) { p.a.before[all] = total; p.first[0] = per; p.first[1] = all; }
+    __syncthreads();                                               // before[] stands
+    for (int w = tid; w < n_blocks; w += 1024) {                   // the entry that each block's piece begins in
+        const long long at = (long long) w * per;
+        int e = 0;
+        for (int hi = all; hi - e > 1;) { const int mid = (e + hi) >> 1; if (p.a.before[mid] <= at) e = mid; else hi = mid; }
+        p.first[2 + w] = e;
     }
 }
 
+template <typename T> __device__ __noinline__ uint4 eight_apart(const T * src) {         // where they do not stand on 16 bytes
+    const uint16_t * x = reinterpret_cast<const uint16_t *>(src);
+    return make_uint4(x[0] | (uint32_t) x[1] << 16, x[2] | (uint32_t) x[3] << 16, x[4] | (uint32_t) x[5] << 16, x[6] | (uint32_t) x[7] << 16);
+}
+template <typename T> __device__ __forceinline__ float query_entry(const uint4 & f, int j) {    // j: a constant
+    const uint32_t w = j >> 1 == 0 ? f.x : j >> 1 == 1 ? f.y : j >> 1 == 2 ? f.z : f.w;
+    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short) (w >> 16 * (j & 1))));
+    else return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+}
+
 // a piece of one unit
-struct Segment { Seq q; Span sp; int ct, head, t0, t1, halves; bool run; };
+struct Segment { Seq q; Span sp; int ct, head, t0, t1, halves; };
 
 // P's columns hold tokens in this order (of 32)
 __host__ __device__ constexpr int token_of(int col) { return 16 * (col >> 2 & 1) + (col >> 3) + 4 * (col & 3); }
@@ -172,75 +205,84 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
     const uint32_t tmem = tmem_s, t_s = tmem, t_o = tmem + 256;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int entries = p.n_entries[0], per = p.n_entries[1];
+    const int per = p.first[0], entries = p.first[1];
     const long long begin = (long long) blockIdx.x * per, end = min(a.before[entries], begin + per);
-    // the segments of this block's piece, the same for every warp
-    const auto segment = [&](long long & at) {
-        Segment g;
-        int e = 0, n = entries;
-        while (n > 1) {                                            // the last entry that begins at or before `at`, 32 places at a time
-            const int step = (n + 31) >> 5, i = e + lane * step;
-            const unsigned m = __ballot_sync(0xffffffffu, lane * step < n && a.before[min(i, entries - 1)] <= at);
-            const int k = m ? 31 - __clz(m) : 0;
-            e += k * step;
-            n = min(step, n - k * step);
+    // the segments of this block's piece, one after the other and the same for every warp
+    int entry = begin < end ? p.first[2 + blockIdx.x] : 0, head = -1;
+    long long at = begin;
+    const auto segment = [&](Segment & g) {
+        while (at < end) {
+            const Entry e = p.entries[entry];
+            const int len = e.n + PR_OVER;
+            int from = 0;
+            if (head < 0) {                                        // the first one may begin anywhere
+                const long long x = at - a.before[entry];
+                head = (int) quotient(x, len);
+                from = (int) (x - (long long) head * len);
+            }
+            const int to = (int) min((long long) len, from + (end - at));
+            g.q = Seq{e.slot, e.begin, e.count, e.held};
+            g.sp = Span{e.lo, e.n};
+            g.ct = e.ct; g.head = head;
+            g.t0 = max(0, from - PR_OVER);
+            g.t1 = to - PR_OVER;
+            g.halves = e.count * a.group - e.ct * PR_COLS > 128 ? 2 : 1;
+            at += to - from;
+            if (++head == c.n_kv) { head = 0; entry++; }
+            if (g.t1 > 0) return true;
         }
-        const int s = p.seq_of[e];
-        g.q = seq_at(c, s);
-        g.ct = e - p.entry_of[s];
-        g.sp = prompt_span(c, g.q, a.group, a.window, g.ct);
-        const long long x = at - a.before[e];
-        const int len = g.sp.n + PR_OVER, from = (int) (x % len), to = (int) min((long long) len, from + (end - at));
-        g.head = (int) (x / len);
-        g.t0 = max(0, from - PR_OVER);
-        g.t1 = to - PR_OVER;
-        g.run = g.t1 > 0;
-        g.halves = g.q.count * a.group - g.ct * PR_COLS > 128 ? 2 : 1;
-        at += to - from;
-        return g;
+        return false;
     };
     bool dead = false;
     if (warp < 8) {
+        regs_more<168>();
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;          // of the half
         const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, my_s = t_s + lanes + half * 128, my_o = t_o + lanes + half * HD;
         int n_s = 0;                                                       // tiles of this half so far
-        for (long long at = begin; at < end;) {
-            const Segment g = segment(at);
-            if (!g.run) continue;
+        for (Segment g; segment(g);) {
             const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
             const bool in = i < g.q.count;
             if (half >= g.halves) continue;
-            float factor;
+            // the warp's 32 queries, HD / 8 lanes a row: each scaled by a power of two to at most 2^14, dims of eight as 0 4 1 5 2 6 3 7
+            constexpr int LANES = HD / 8, ROWS = 32 / LANES;
+            float factor = 0.f;
             {
-                // the column's query, scaled by a power of two to at most 2^14, dims of eight as 0 4 1 5 2 6 3 7
-                const T * src = static_cast<const T *>(a.q) + (in ? (g.q.begin + i) * a.q_row + h * a.q_head : 0);
-                const auto load = [&](int m) {
-                    Eight<T> f = {};
-                    if (in) {
-                        if (a.q_whole) f = *reinterpret_cast<const Eight<T> *>(src + 8 * m);
-                        else for (int j = 0; j < 8; j++) f.v[j] = src[8 * m + j];
+                const int64_t mine = in ? (g.q.begin + i) * a.q_row + h * a.q_head : -1;
+                const int m = lane % LANES;
+#pragma unroll 1
+                for (int x0 = 0; x0 < 32; x0 += 8 * ROWS) {
+                    uint4 f[8];
+                    int64_t from[8];
+#pragma unroll
+                    for (int x = 0; x < 8; x++) { from[x] = __shfl_sync(0xffffffffu, mine, x0 + x * ROWS + lane / LANES); f[x] = make_uint4(0, 0, 0, 0); }
+                    const T * src = static_cast<const T *>(a.q) + 8 * m;
+                    if (a.q_whole) {
+#pragma unroll
+                        for (int x = 0; x < 8; x++) if (from[x] >= 0) f[x] = *reinterpret_cast<const uint4 *>(src + from[x]);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 8; x++) if (from[x] >= 0) f[x] = eight_apart(src + from[x]);
                     }
-                    return f;
-                };
-                float top = 0.f;
-#pragma unroll 4
-                for (int m = 0; m < HD / 8; m++) {
-                    const Eight<T> f = load(m);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(to_f(f.v[j])));
-                }
-                const int e = min(126, max(-126, 140 - (int) (__float_as_uint(top) >> 23)));
-                float up = top > 0.f && top < INFINITY ? __uint_as_float((uint32_t) (127 + e) << 23) : 1.f;
-                factor = fmaxf(fabsf(a.scale_log2) / up, 1.2e-38f);           // (never 0: it meets the -infinity of what is masked)
-                if (a.scale_log2 < 0.f) up = -up;
-#pragma unroll 4
-                for (int m = 0; m < HD / 8; m++) {
-                    const Eight<T> f = load(m);
-                    uint32_t w[4];
+                    for (int x = 0; x < 8; x++) {
+                        const int r = x0 + x * ROWS + lane / LANES;
+                        float top = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) w[j] = as_u(__floats2half2_rn(to_f(f.v[j]) * up, to_f(f.v[j + 4]) * up));
-                    pr_st_shared(q_s + half * QB + (m >> 3) * SUB + row * 128 + (((m & 7) ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
+                        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(query_entry<T>(f[x], j)));
+#pragma unroll
+                        for (int d = 1; d < LANES; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const int e = min(126, max(-126, 140 - (int) (__float_as_uint(top) >> 23)));
+                        float up = top > 0.f && top < INFINITY ? __uint_as_float((uint32_t) (127 + e) << 23) : 1.f;
+                        const float mine_up = __shfl_sync(0xffffffffu, up, (lane % ROWS) * LANES);
+                        if (lane / ROWS == x0 / ROWS + x) factor = mine_up;
+                        if (a.scale_log2 < 0.f) up = -up;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) w[j] = as_u(__floats2half2_rn(query_entry<T>(f[x], j) * up, query_entry<T>(f[x], j + 4) * up));
+                        pr_st_shared(q_s + half * QB + (m >> 3) * SUB + ((warp & 3) * 32 + r) * 128 + (((m & 7) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+                    }
                 }
+                factor = fmaxf(fabsf(a.scale_log2) / factor, 1.2e-38f);              // (never 0: it meets the -infinity of what is masked)
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -261,24 +303,32 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 const bool edge = !whole || pos + PR_KV - 1 > all_see_hi || pos < all_see_lo;
                 unsigned there = 0xffu;                                    // tiles of 16 tokens that have a page
                 if (!whole) there = __ballot_sync(0xffffffffu, lane < 8 && page_at(c, g.q.slot, pos + 16 * (lane & 7)) >= 0);
-                const auto hide = [&](uint32_t (&r)[32], int ch) {
-                    const int hi = top_pos - pos - 32 * ch, lo = low_pos - pos - 32 * ch;
-#pragma unroll
-                    for (int x = 0; x < 32; x++)
-                        if (token_of(x) > hi || token_of(x) <= lo || !(there >> (2 * ch + (x >> 2 & 1)) & 1)) r[x] = 0xff800000u;
-                };
                 pr_wait(smem_at(&s_full[half]), (uint32_t) (n_s & 1), dead);
                 __syncwarp();
                 pr_fence_after();
+                uint32_t r[2][32];                                         // 32 columns in hand, the next 32 on their way
+                if (edge) {                                                // what a column does not see goes to -infinity, in place
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ch++) {
+                        const int hi = top_pos - pos - 32 * ch, lo = low_pos - pos - 32 * ch;
+                        const unsigned pages = there >> 2 * ch;
+                        pr_ld32(my_s + 32 * ch, r[0]);
+                        pr_ld32_wait(r[0]);
+#pragma unroll
+                        for (int x = 0; x < 32; x++)
+                            if (token_of(x) > hi || token_of(x) <= lo || !(pages >> (x >> 2 & 1) & 1)) r[0][x] = 0xff800000u;
+                        pr_st32(my_s + 32 * ch, r[0]);
+                    }
+                    pr_st_wait();
+                }
                 float x0 = -INFINITY, x1 = -INFINITY;
+                pr_ld32(my_s + 96, r[1]);
 #pragma unroll
-                for (int ch = 0; ch < 4; ch++) {
-                    uint32_t r[32];
-                    pr_ld32(my_s + 32 * ch, r);
-                    pr_ld32_wait(r);
-                    if (edge) hide(r, ch);
+                for (int ch = 3; ch >= 0; ch--) {
+                    pr_ld32_wait(r[ch & 1]);
+                    if (ch) pr_ld32(my_s + 32 * (ch - 1), r[(ch - 1) & 1]);
 #pragma unroll
-                    for (int x = 0; x < 32; x += 2) { x0 = fmaxf(x0, __uint_as_float(r[x])); x1 = fmaxf(x1, __uint_as_float(r[x + 1])); }
+                    for (int x = 0; x < 32; x += 2) { x0 = fmaxf(x0, __uint_as_float(r[ch & 1][x])); x1 = fmaxf(x1, __uint_as_float(r[ch & 1][x + 1])); }
                 }
                 const float high = fmaxf(x0, x1), score = high == -INFINITY ? high : high * factor;
                 if (__any_sync(0xffffffffu, score > limit)) {
@@ -302,22 +352,26 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                     limit = top + 8.f;
                     l *= down;
                 }
-                float l0 = 0.f, l1 = 0.f;
+                const uint64_t by = two(factor, factor), less = two(-base, -base);
+                uint64_t sum = 0;
+                pr_ld32(my_s + 32, r[1]);
 #pragma unroll
-                for (int ch = 0; ch < 4; ch++) {
-                    uint32_t r[32], w[16];
-                    pr_ld32(my_s + 32 * ch, r);
-                    pr_ld32_wait(r);
-                    if (edge) hide(r, ch);
+                for (int ch = 0; ch < 4; ch++) {                           // (the first 32 columns are still there)
+                    uint32_t w[16];
 #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        const float e0 = exp2_fast(fmaf(__uint_as_float(r[x]), factor, -base)), e1 = exp2_fast(fmaf(__uint_as_float(r[x + 1]), factor, -base));
-                        l0 += e0; l1 += e1;
+                        const float2 y = split(fma2(two(__uint_as_float(r[ch & 1][x]), __uint_as_float(r[ch & 1][x + 1])), by, less));
+                        const float e0 = exp2_fast(y.x), e1 = exp2_fast(y.y);
+                        sum = add2(sum, two(e0, e1));
                         w[x / 2] = as_u(__floats2half2_rn(e0, e1));
+                    }
+                    if (ch < 3) {
+                        pr_ld32_wait(r[(ch + 1) & 1]);
+                        if (ch < 2) pr_ld32(my_s + 32 * (ch + 2), r[ch & 1]);
                     }
                     pr_st16(my_s + 16 * ch, w);
                 }
-                l += l0 + l1;
+                l += split(sum).x + split(sum).y;
                 pr_st_wait();
                 pr_fence_before();
                 __syncwarp();
@@ -328,7 +382,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
             pr_fence_after();
             const bool final = g.t0 == 0 && g.t1 == g.sp.n;
             const float inv = l != 0.f ? 1.f / l : 0.f;
-            const size_t slot = (2 * (size_t) blockIdx.x + (g.t0 == 0 ? 1 : 0)) * PR_COLS + half * 128 + row;
+            const size_t part = 2 * (size_t) blockIdx.x + (g.t0 == 0 ? 1 : 0);      // parts are [HD / 4][256 columns][4]: a warp's stores are contiguous
 #pragma unroll
             for (int ch = 0; ch < HD / 32; ch++) {
                 uint32_t r[32];
@@ -345,22 +399,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                             *reinterpret_cast<Eight<T> *>(y + x) = f;
                         }
                     } else {
-                        uint4 * y = reinterpret_cast<uint4 *>(a.part + slot * HD + 32 * ch);
+                        uint4 * y = reinterpret_cast<uint4 *>(a.part + part * PR_COLS * HD) + (size_t) (8 * ch) * PR_COLS + half * 128 + row;
 #pragma unroll
-                        for (int x = 0; x < 8; x++) y[x] = make_uint4(r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]);
+                        for (int x = 0; x < 8; x++) y[x * PR_COLS] = make_uint4(r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]);
                     }
                 }
                 __syncwarp();
             }
-            if (in && !final) *reinterpret_cast<float2 *>(a.ml + slot * 2) = make_float2(m, l);
+            if (in && !final) *reinterpret_cast<float2 *>(a.ml + (part * PR_COLS + half * 128 + row) * 2) = make_float2(m, l);
             pr_fence_before();
         }
     } else if (warp < 12) {
+        regs_less<112>();
         const int w = warp - 8, g8 = lane >> 2, tq = lane & 3, tc = g8 >> 1, te = g8 & 1;
         int n = 0;                                                         // tiles so far
-        for (long long at = begin; at < end;) {
-            const Segment g = segment(at);
-            if (!g.run) continue;
+        for (Segment g; segment(g);) {
             int pages_from = 0, my_page = 0, turned = -1;
             uint4 kr[2][NB / 2], vr[2][NB / 2], ks[2], vs[2][NB / 2];
             const auto place = [&](int t, int u) -> const uint8_t * {      // of 16 tokens
@@ -455,10 +508,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
             }
         }
     } else {
+        regs_less<64>();
         int n = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
-        for (long long at = begin; at < end;) {
-            const Segment g = segment(at);
-            if (!g.run) continue;
+        for (Segment g; warp == 12 && segment(g);) {
             if (pr_elect()) {
                 const int tiles = g.t1 - g.t0;
                 const auto scores = [&](int half, int stage) {             // S = Q K^T of a half
@@ -515,39 +567,49 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
     }
 }
 
-// a warp a row and head: adds the parts of a unit that blocks shared, few as they are
+// a block 32 columns of a unit that blocks shared: adds its parts, few as they are. A lane is a column, a warp has every eighth group of 4 dims
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) k_kv4_prompt_join(const PromptArgs p) {
-    constexpr int E = HD / 32;
+    constexpr int X = HD / 32, PAD = HD + 4;
+    __shared__ __align__(16) float sums[32 * PAD];
     const AttendArgs & a = p.a;
     const Cache & c = a.c;
-    const int lane = threadIdx.x & 31, n_head = c.n_kv * a.group;
-    const int64_t item = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (item >= (int64_t) c.n_rows * n_head) return;
-    const int row = (int) (item / n_head), h = (int) (item % n_head), s = seq_of_row(c, row);
-    if (s < 0) return;
-    const int begin = min(max(c.first[s], 0), c.n_rows), head = h / a.group, col = (row - begin) * a.group + h - head * a.group, ct = col / PR_COLS, in_tile = col - ct * PR_COLS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x / (PR_COLS / 32), c0 = blockIdx.x % (PR_COLS / 32) * 32, head = blockIdx.y;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int e = p.entry_of[s] + ct, per = p.n_entries[1];
-    const long long b0 = a.before[e];
-    const int len = (int) ((a.before[e + 1] - b0) / c.n_kv);
-    const long long u0 = b0 + (long long) head * len;
+    if (e >= p.first[1]) return;
+    const Entry n = p.entries[e];
+    const int len = n.n + PR_OVER, per = p.first[0], cols = min(PR_COLS, n.count * a.group - n.ct * PR_COLS);
+    if (c0 >= cols) return;
+    const long long u0 = a.before[e] + (long long) head * len;
     const int w0 = (int) quotient(u0 + PR_OVER, per), w1 = (int) quotient(u0 + len - 1, per);
     if (w0 == w1) return;
-    float m = -INFINITY, l = 0.f, o[E] = {};
+    float m = -INFINITY, l = 0.f, o[X][4] = {};
     for (int w = w0; w <= w1; w++) {
-        const size_t slot = (2 * (size_t) w + (w == w0 ? 1 : 0)) * PR_COLS + in_tile;
-        const float2 ml = *reinterpret_cast<const float2 *>(a.ml + slot * 2);
+        const size_t part = 2 * (size_t) w + (w == w0 ? 1 : 0);
+        const bool in = c0 + lane < cols;                          // (others were not stored)
+        const float2 ml = in ? *reinterpret_cast<const float2 *>(a.ml + (part * PR_COLS + c0 + lane) * 2) : make_float2(-INFINITY, 0.f);
+        float4 v[X];
+#pragma unroll
+        for (int x = 0; x < X; x++) v[x] = in ? reinterpret_cast<const float4 *>(a.part + part * PR_COLS * HD)[(size_t) (warp + 8 * x) * PR_COLS + c0 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
         const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top, old = exp2_fast(m - base), now = exp2_fast(ml.x - base);
         l = l * old + ml.y * now;
 #pragma unroll
-        for (int x = 0; x < E; x++) o[x] = o[x] * old + a.part[slot * HD + E * lane + x] * now;
+        for (int x = 0; x < X; x++) {
+            o[x][0] = o[x][0] * old + v[x].x * now; o[x][1] = o[x][1] * old + v[x].y * now;
+            o[x][2] = o[x][2] * old + v[x].z * now; o[x][3] = o[x][3] * old + v[x].w * now;
+        }
         m = top;
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
-    T * y = static_cast<T *>(a.out) + ((size_t) row * n_head + h) * HD + E * lane;
 #pragma unroll
-    for (int x = 0; x < E; x++) y[x] = from_f<T>(o[x] * inv);
+    for (int x = 0; x < X; x++) *reinterpret_cast<float4 *>(sums + lane * PAD + 4 * (warp + 8 * x)) = make_float4(o[x][0] * inv, o[x][1] * inv, o[x][2] * inv, o[x][3] * inv);
+    __syncthreads();
+    for (int x = warp; x < 32 && c0 + x < cols; x += 8) {
+        const int col = n.ct * PR_COLS + c0 + x, i = col / a.group, h = head * a.group + col - i * a.group;
+        T * y = static_cast<T *>(a.out) + ((size_t) (n.begin + i) * c.n_kv * a.group + h) * HD + X * lane;
+#pragma unroll
+        for (int j = 0; j < X; j++) y[j] = from_f<T>(sums[x * PAD + X * lane + j]);
+    }
 }
 
 }  // namespace srv
