@@ -164,7 +164,7 @@ def lib() -> C.CDLL:
     sig("b200_set_prefill_mma", None, [C.c_int])
     sig("b200_set_prefill_attn_batch", None, [C.c_int])
     sig("b200_trace_phases", C.c_int64, [vp, C.c_int32, C.c_int, C.c_int, C.POINTER(C.c_uint64), C.c_int64, i32p, C.c_int64, i32p])
-    kp, pp = C.POINTER(Kv4), C.POINTER(Pages)
+    kp = pp = vp          # struct b200_kv4 *, struct b200_pages * (Kv4, Pages, or their bytes)
     sig("b200_kv4_append", C.c_int, [kp, C.c_int, vp, C.c_int64, C.c_int64, vp, C.c_int64, C.c_int64])
     sig("b200_kv4_read", C.c_int, [kp, C.c_int, vp, vp])
     sig("b200_kv4_attention_workspace", C.c_int64, [kp, C.c_int, C.c_int])

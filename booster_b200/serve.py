@@ -16,15 +16,18 @@ slots that a table names but that do not exist count as absent.
 """
 from __future__ import annotations
 
-import ctypes as C
-from typing import Optional, Tuple
+import struct
+from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import Kv4, Pages, check
+from ._lib import check
 
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_KV4, _PAGES = struct.Struct("@9i2P2q4P"), struct.Struct("@8i2P3q3P")      # struct b200_kv4, struct b200_pages
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
+_I32 = torch.int32
 
 
 def kv4_pool(n_pages: int, page_tokens: int, n_head_kv: int, head_dim: int, n_layer: int = 1, device="cuda") -> torch.Tensor:
@@ -39,63 +42,71 @@ def _need(ok, what: str) -> None:
         raise ValueError(what)
 
 
-def _ints(name: str, t: torch.Tensor, device, dims: int, n: Optional[int] = None) -> int:
-    if t.dtype != torch.int32 or t.device != device or t.dim() != dims or (dims == 1 and not t.is_contiguous()) or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} is a contiguous int32 tensor of {dims} dimension(s)" + (f" and {n} entries" if n is not None else "") + f" on {device}")
+def _ints(name: str, t: torch.Tensor, index: int, n: int = -1) -> int:
+    """address of a contiguous int32 vector (of n entries) on device `index`"""
+    if t.dtype is not _I32 or t.get_device() != index or t.dim() != 1 or not t.is_contiguous() or (n >= 0 and t.numel() != n):
+        raise ValueError(f"{name} is a contiguous int32 tensor of 1 dimension" + (f" and {n} entries" if n >= 0 else "") + " on the device of the others")
     return t.data_ptr()
 
 
-def _table(table: torch.Tensor, device) -> int:
-    p = _ints("table", table, device, 2)
-    _need(table.stride(1) == 1 or table.shape[1] == 1, "table's rows are contiguous")
-    return p
+def _table(t: torch.Tensor, index: int) -> Tuple[int, int, int, int]:
+    """address, slots, pages and stride of a slot"""
+    if t.dtype is not _I32 or t.get_device() != index or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1):
+        raise ValueError("table is an int32 tensor [n_slots, max_pages] of contiguous rows on the device of the others")
+    slots, most = t.shape
+    return t.data_ptr(), slots, most, t.stride(0) if slots > 1 else most
 
 
-def _on(device):
-    _need(device.type == "cuda", "tensors are on a CUDA device: booster_b200 has no CPU fallback")
-    return device.index, torch.cuda.current_stream(device).cuda_stream
+def _on(t: torch.Tensor) -> int:
+    index = t.get_device()
+    _need(index >= 0, "tensors are on a CUDA device: booster_b200 has no CPU fallback")
+    return index
 
 
-def _page_stride(pool: torch.Tensor) -> int:
-    _, kv, tiles, size = pool.shape[-4:]
+def _page_stride(pool: torch.Tensor, shape) -> int:
+    kv, tiles, size = shape[-3:]
     st = pool.stride()
-    _need(pool.dtype == torch.uint8 and size % 18 == 0, "pool is a uint8 tensor [..., n_pages, n_head_kv, page_tokens / 16, 18 * head_dim]")
-    _need(st[-1] == 1 and (tiles == 1 or st[-2] == size) and (kv == 1 or st[-3] == tiles * size), "pool's pages are contiguous")
-    return st[-4] if pool.shape[-4] > 1 else max(st[-4], kv * tiles * size)
+    if pool.dtype is not torch.uint8 or size % 18 or st[-1] != 1 or (tiles != 1 and st[-2] != size) or (kv != 1 and st[-3] != tiles * size):
+        raise ValueError("pool is a uint8 tensor [..., n_pages, n_head_kv, page_tokens / 16, 18 * head_dim] of contiguous pages")
+    return st[-4] if shape[-4] > 1 else max(st[-4], kv * tiles * size)
 
 
-def _step(pool, table, held, first, slots, n_rows: int) -> Kv4:
-    device = pool.device
-    index, stream = _on(device)
-    _need(pool.dim() == 4, "pool is one layer's [n_pages, n_head_kv, page_tokens / 16, 18 * head_dim]")
-    stride = _page_stride(pool)
-    pages, kv, tiles, size = pool.shape
-    n_seq = first.shape[0] - 1
+def _step(pool, table, held, first, slots, n_rows: int) -> bytes:
+    """struct b200_kv4 of one layer and a step"""
+    index = _on(pool)
+    shape = pool.shape
+    _need(len(shape) == 4, "pool is one layer's [n_pages, n_head_kv, page_tokens / 16, 18 * head_dim]")
+    pages, kv, tiles, size = shape
+    n_seq = first.numel() - 1
     _need(n_seq >= 0, "first has one entry more than there are sequences")
-    n_slots = table.shape[0]
-    return Kv4(index, pages, 16 * tiles, kv, size // 18, n_slots, table.shape[1], n_seq, n_rows, stream, pool.data_ptr(), stride, table.stride(0) if n_slots > 1 else table.shape[1],
-               _table(table, device), _ints("held", held, device, 1, n_slots), _ints("slots", slots, device, 1, n_seq) if slots is not None else _first_n(n_seq, n_slots),
-               _ints("first", first, device, 1))
+    table_at, n_slots, most, stride = _table(table, index)
+    if slots is None:
+        _need(n_seq <= n_slots, "without slots, sequence i is slot i: more sequences than slots")
+        slots_at = 0
+    else:
+        slots_at = _ints("slots", slots, index, n_seq)
+    return _KV4.pack(index, pages, 16 * tiles, kv, size // 18, n_slots, most, n_seq, n_rows, _stream(index), pool.data_ptr(), _page_stride(pool, shape), stride, table_at,
+                     _ints("held", held, index, n_slots), slots_at, _ints("first", first, index))
 
 
-def _first_n(n_seq: int, n_slots: int) -> None:
-    _need(n_seq <= n_slots, "without slots, sequence i is slot i: more sequences than slots")
-
-
-def _rows(name: str, x: torch.Tensor, pool, heads: Optional[int]) -> None:
-    if x.dim() != 3 or x.device != pool.device or x.shape[2] * 18 != pool.shape[3] or (heads is not None and x.shape[1] != heads):
+def _rows(name: str, x: torch.Tensor, pool, heads: int = -1) -> Tuple[int, int]:
+    """strides of rows and heads"""
+    if x.dim() != 3 or x.get_device() != pool.get_device() or x.shape[2] * 18 != pool.shape[-1] or (heads >= 0 and x.shape[1] != heads):
         raise ValueError(f"{name} is a tensor [rows, heads, head_dim] that fits the pool, on its device")
-    if x.stride(2) != 1:
+    row, head, one = x.stride()
+    if one != 1:
         raise ValueError(f"{name}: the entries of a head are contiguous")
+    return row, head
 
 
 def kv4_append(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: Optional[torch.Tensor] = None) -> None:
     """keys and values [rows, n_head_kv, head_dim] (any strides over rows and heads; float32, bfloat16 or float16) of the step's rows into one layer's pool"""
-    _rows("k", k, pool, pool.shape[1])
-    _rows("v", v, pool, pool.shape[1])
-    _need(k.dtype == v.dtype and k.dtype in _TYPE and k.shape == v.shape, "k and v are float32, bfloat16 or float16, and alike")
-    c = _step(pool, table, held, first, slots, k.shape[0])
-    check(_lib.lib().b200_kv4_append(C.byref(c), _TYPE[k.dtype], k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1)), "kv4_append")
+    kv = pool.shape[1] if pool.dim() == 4 else -1
+    k_row, k_head = _rows("k", k, pool, kv)
+    v_row, v_head = _rows("v", v, pool, kv)
+    dtype = _TYPE.get(k.dtype)
+    _need(dtype is not None and k.dtype is v.dtype and k.shape == v.shape, "k and v are float32, bfloat16 or float16, and alike")
+    check(_lib.lib().b200_kv4_append(_step(pool, table, held, first, slots, k.shape[0]), dtype, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head), "kv4_append")
 
 
 def kv4_read(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first: torch.Tensor, rows: int, dtype: torch.dtype = torch.bfloat16, slots: Optional[torch.Tensor] = None,
@@ -104,10 +115,13 @@ def kv4_read(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first:
     _need(dtype in _TYPE, "dtype is float32, bfloat16 or float16")
     c = _step(pool, table, held, first, slots, rows)
     shape = (rows, pool.shape[1], pool.shape[3] // 18)
-    k, v = out if out is not None else (torch.empty(shape, dtype=dtype, device=pool.device), torch.empty(shape, dtype=dtype, device=pool.device))
-    for x in (k, v):
-        _need(x.shape == shape and x.dtype == dtype and x.device == pool.device and x.is_contiguous(), "out is a pair of contiguous tensors [rows, n_head_kv, head_dim] of dtype")
-    check(_lib.lib().b200_kv4_read(C.byref(c), _TYPE[dtype], k.data_ptr(), v.data_ptr()), "kv4_read")
+    if out is None:
+        k, v = torch.empty(shape, dtype=dtype, device=pool.device), torch.empty(shape, dtype=dtype, device=pool.device)
+    else:
+        k, v = out
+        for x in out:
+            _need(x.shape == shape and x.dtype is dtype and x.device == pool.device and x.is_contiguous(), "out is a pair of contiguous tensors [rows, n_head_kv, head_dim] of dtype")
+    check(_lib.lib().b200_kv4_read(c, _TYPE[dtype], k.data_ptr(), v.data_ptr()), "kv4_read")
     return k, v
 
 
@@ -116,38 +130,53 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, held
     """attention of the step's rows q [rows, n_head, head_dim] (bfloat16 or float16, any strides over rows and heads) over the positions up to their own, kv4_append having put those into
     the pool; window > 0: over the last `window` of them. scale: 1 / sqrt(head_dim). max_rows: the largest number of rows of a sequence, if the program knows it (else: rows).
     Rows of no sequence are left as they are (in `out`)"""
-    _rows("q", q, pool, None)
-    _need(q.dtype in (torch.bfloat16, torch.float16), "q is bfloat16 or float16")
+    row, head = _rows("q", q, pool)
+    dtype = _TYPE.get(q.dtype)
+    _need(dtype, "q is bfloat16 or float16")
     rows, heads, hd = q.shape
     c = _step(pool, table, held, first, slots, rows)
+    device = q.device
     if out is None:
-        out = torch.empty((rows, heads, hd), dtype=q.dtype, device=q.device)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.is_contiguous(), "out is a contiguous tensor like q")
-    most = max(1, rows if max_rows is None else max_rows)
+        out = torch.empty((rows, heads, hd), dtype=q.dtype, device=device)
+    else:
+        _need(out.shape == q.shape and out.dtype is q.dtype and out.device == device and out.is_contiguous(), "out is a contiguous tensor like q")
+    most = rows if max_rows is None else max_rows
+    if most < 1:
+        most = 1
     L = _lib.lib()
-    size = L.b200_kv4_attention_workspace(C.byref(c), heads, most)
-    check(size < 0, "kv4_attention")
-    work = torch.empty(size, dtype=torch.uint8, device=q.device)
-    check(L.b200_kv4_attention(C.byref(c), _TYPE[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), heads, hd ** -0.5 if scale is None else scale, window, most, out.data_ptr(), work.data_ptr(), size),
-          "kv4_attention")
+    shape = (device.index, heads, pool.shape[1], hd, first.numel(), rows, most)
+    size = _work_bytes.get(shape)
+    if size is None:
+        size = L.b200_kv4_attention_workspace(c, heads, most)
+        check(size < 0, "kv4_attention")
+        if len(_work_bytes) > 4096:
+            _work_bytes.clear()
+        _work_bytes[shape] = size
+    work = torch.empty(size, dtype=torch.uint8, device=device)
+    check(L.b200_kv4_attention(c, dtype, q.data_ptr(), row, head, heads, hd ** -0.5 if scale is None else scale, window, most, out.data_ptr(), work.data_ptr(), size), "kv4_attention")
     return out
 
 
-def _pages(table, held, refs, page_tokens: int, pool=None) -> Pages:
-    device = refs.device
-    index, stream = _on(device)
-    n_slots, most = table.shape
-    p = Pages(index, refs.shape[0], page_tokens, 1, 64, n_slots, most, 1, stream, None, 0, 0, table.stride(0) if n_slots > 1 else most, _table(table, device),
-              _ints("held", held, device, 1, n_slots) if held is not None else table.data_ptr(), _ints("refs", refs, device, 1))
-    if pool is not None:
-        _need(pool.dim() == 5 and pool.device == device and pool.shape[1] == refs.shape[0], "pool is [n_layer, n_pages, n_head_kv, page_tokens / 16, 18 * head_dim], refs has an entry a page")
-        p.page_stride = _page_stride(pool)
-        p.pool, p.n_layer, p.layer_stride, p.n_head_kv, p.head_dim = pool.data_ptr(), pool.shape[0], pool.stride(0), pool.shape[2], pool.shape[4] // 18
-    return p
+_work_bytes: Dict[tuple, int] = {}       # sizes of workspaces by the shapes they are for
 
 
-def _work(p: Pages, n: int, device) -> torch.Tensor:
-    size = _lib.lib().b200_pages_workspace(C.byref(p), n)
+def _pages(table, held, refs, page_tokens: int, pool=None) -> bytes:
+    """struct b200_pages"""
+    index = _on(refs)
+    at, n_slots, most, stride = _table(table, index)
+    held_at = _ints("held", held, index, n_slots) if held is not None else at
+    n = refs.numel()
+    if pool is None:
+        return _PAGES.pack(index, n, page_tokens, 1, 64, n_slots, most, 1, _stream(index), 0, 0, 0, stride, at, held_at, _ints("refs", refs, index))
+    shape = pool.shape
+    if len(shape) != 5 or pool.get_device() != index or shape[1] != n:
+        raise ValueError("pool is [n_layer, n_pages, n_head_kv, page_tokens / 16, 18 * head_dim], refs has an entry a page")
+    return _PAGES.pack(index, n, 16 * shape[3], shape[2], shape[4] // 18, n_slots, most, shape[0], _stream(index), pool.data_ptr(), pool.stride(0), _page_stride(pool, shape), stride, at, held_at,
+                       _ints("refs", refs, index))
+
+
+def _work(p: bytes, n: int, device) -> torch.Tensor:
+    size = _lib.lib().b200_pages_workspace(p, n)
     check(size < 0, "pages_workspace")
     return torch.empty(size, dtype=torch.uint8, device=device)
 
@@ -155,45 +184,42 @@ def _work(p: Pages, n: int, device) -> torch.Tensor:
 def pages_reserve(table: torch.Tensor, held: torch.Tensor, refs: torch.Tensor, first: torch.Tensor, page_tokens: int, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     """pages for first[i + 1] - first[i] tokens more of each sequence, the lowest free ones, in order. Returns the status on the device, int32 [1]: 0, the number of pages that were
     missing, or -1 where slots or tables cannot be; then nothing has changed"""
-    n = first.shape[0] - 1
+    n = first.numel() - 1
     _need(n >= 0, "first has one entry more than there are sequences")
-    p = _pages(table, held, refs, page_tokens)
-    status = torch.empty(1, dtype=torch.int32, device=refs.device)
-    s = _ints("slots", slots, refs.device, 1, n) if slots is not None else _first_n(n, table.shape[0])
-    check(_lib.lib().b200_pages_reserve(C.byref(p), s, _ints("first", first, refs.device, 1), n, status.data_ptr()), "pages_reserve")
+    p, index = _pages(table, held, refs, page_tokens), refs.get_device()
+    if slots is None:
+        _need(n <= table.shape[0], "without slots, sequence i is slot i: more sequences than slots")
+    status = torch.empty(1, dtype=_I32, device=refs.device)
+    check(_lib.lib().b200_pages_reserve(p, _ints("slots", slots, index, n) if slots is not None else None, _ints("first", first, index), n, status.data_ptr()), "pages_reserve")
     return status
 
 
 def pages_fork(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, children: torch.Tensor) -> torch.Tensor:
     """slot children[i], which is empty, becomes what slot parents[i] is: full pages are shared, a last page that is part full is copied in every layer. Returns the status, see pages_reserve"""
-    n = parents.shape[0]
-    p = _pages(table, held, refs, 16 * pool.shape[-2], pool)
-    work, status = _work(p, n, refs.device), torch.empty(1, dtype=torch.int32, device=refs.device)
-    check(_lib.lib().b200_pages_fork(C.byref(p), _ints("parents", parents, refs.device, 1), _ints("children", children, refs.device, 1, n), n, status.data_ptr(), work.data_ptr(), work.numel()),
-          "pages_fork")
+    p, n, index = _pages(table, held, refs, 0, pool), parents.numel(), refs.get_device()
+    work, status = _work(p, n, refs.device), torch.empty(1, dtype=_I32, device=refs.device)
+    check(_lib.lib().b200_pages_fork(p, _ints("parents", parents, index), _ints("children", children, index, n), n, status.data_ptr(), work.data_ptr(), work.numel()), "pages_fork")
     return status
 
 
 def pages_free(table: torch.Tensor, held: torch.Tensor, refs: torch.Tensor, slots: torch.Tensor) -> None:
     """the slots give their pages back and are empty"""
-    p = _pages(table, held, refs, 16)
-    check(_lib.lib().b200_pages_free(C.byref(p), _ints("slots", slots, refs.device, 1), slots.shape[0]), "pages_free")
+    check(_lib.lib().b200_pages_free(_pages(table, held, refs, 16), _ints("slots", slots, refs.get_device()), slots.numel()), "pages_free")
 
 
 def pages_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor) -> torch.Tensor:
     """pages in use move to the lowest places and tables follow. Returns how many there are, int32 [1] on the device: no page from that one on is in use"""
-    p = _pages(table, None, refs, 16 * pool.shape[-2], pool)
-    work, live = _work(p, refs.shape[0], refs.device), torch.empty(1, dtype=torch.int32, device=refs.device)
-    check(_lib.lib().b200_pages_compact(C.byref(p), live.data_ptr(), work.data_ptr(), work.numel()), "pages_compact")
+    p = _pages(table, None, refs, 0, pool)
+    work, live = _work(p, refs.numel(), refs.device), torch.empty(1, dtype=_I32, device=refs.device)
+    check(_lib.lib().b200_pages_compact(p, live.data_ptr(), work.data_ptr(), work.numel()), "pages_compact")
     return live
 
 
 def pages_copy(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
     """page dst[i] becomes page src[i] in every layer. Returns the status: -1, and nothing copied, where a page is written twice, or written and read, or does not exist"""
-    n = src.shape[0]
-    p = _pages(table, None, refs, 16 * pool.shape[-2], pool)
-    work, status = _work(p, n, refs.device), torch.empty(1, dtype=torch.int32, device=refs.device)
-    check(_lib.lib().b200_pages_copy(C.byref(p), _ints("src", src, refs.device, 1), _ints("dst", dst, refs.device, 1, n), n, status.data_ptr(), work.data_ptr(), work.numel()), "pages_copy")
+    p, n, index = _pages(table, None, refs, 0, pool), src.numel(), refs.get_device()
+    work, status = _work(p, n, refs.device), torch.empty(1, dtype=_I32, device=refs.device)
+    check(_lib.lib().b200_pages_copy(p, _ints("src", src, index), _ints("dst", dst, index, n), n, status.data_ptr(), work.data_ptr(), work.numel()), "pages_copy")
     return status
 
 
@@ -201,15 +227,23 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
            min_p: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """one token a row of logits [rows, n_vocab] by the row's random number u (0 <= u < 1), temperature, top_k, top_p and min_p (tensors of an entry a row; None: 1, all, 1, 0), the filters in
     that order of b200_sample. Returns ids, int32 [rows], and the log of each drawn token's share of what the filters kept, float32 [rows]"""
+    index = _on(logits)
+    dtype, rows = _TYPE.get(logits.dtype), logits.shape[0]
+    if logits.dim() != 2 or dtype is None or (logits.stride(1) != 1 and logits.shape[1] != 1):
+        raise ValueError("logits is a float32, bfloat16 or float16 tensor [rows, n_vocab] of contiguous rows")
+    vocab = logits.shape[1]
+    f = torch.float32
+    at = (_per_row("u", u, f, rows, index), _per_row("temperature", temperature, f, rows, index), _per_row("top_k", top_k, _I32, rows, index), _per_row("top_p", top_p, f, rows, index),
+          _per_row("min_p", min_p, f, rows, index))
     device = logits.device
-    index, stream = _on(device)
-    _need(logits.dim() == 2 and logits.dtype in _TYPE and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits is a float32, bfloat16 or float16 tensor [rows, n_vocab] of contiguous rows")
-    rows, vocab = logits.shape
-    given = []
-    for name, t, dtype in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if t is not None and (t.dtype != dtype or t.shape != (rows,) or t.device != device or not t.is_contiguous()):
-            raise ValueError(f"{name} is a contiguous {dtype} tensor of {rows} entries on {device}")
-        given.append(t.data_ptr() if t is not None else None)
-    ids, logprobs = torch.empty(rows, dtype=torch.int32, device=device), torch.empty(rows, dtype=torch.float32, device=device)
-    check(_lib.lib().b200_sample(index, stream, _TYPE[logits.dtype], logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, *given, ids.data_ptr(), logprobs.data_ptr()), "sample")
+    ids, logprobs = torch.empty(rows, dtype=_I32, device=device), torch.empty(rows, dtype=f, device=device)
+    check(_lib.lib().b200_sample(index, _stream(index), dtype, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, *at, ids.data_ptr(), logprobs.data_ptr()), "sample")
     return ids, logprobs
+
+
+def _per_row(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != rows or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} is a contiguous {dtype} tensor of {rows} entries on the logits' device")
+    return t.data_ptr()
