@@ -193,7 +193,7 @@ void move_pages(const b200_pages & p, const Pages & d, const int32_t * plan, int
 
 template <typename T> void sample_as(const SampleArgs & a, int cluster, int device, void * stream) {
     static Limits set;
-    const size_t smem = 8 * SA_LIST + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
+    const size_t smem = 8 * SA_LIST + 4 * SA_BINS + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
     allow_smem(k_sample<T>, device, smem, set);
     launch(k_sample<T>, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, false, cluster, a);
 }
@@ -349,7 +349,7 @@ void pages_copy(const b200_pages & p, const int32_t * src, const int32_t * dst, 
 void sample_rows(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature, const int32_t * top_k,
                  const float * top_p, const float * min_p, int32_t * ids, float * logprobs) {
     check_dtype(dtype, true);
-    need(n_vocab >= 1 && n_vocab <= (1 << 18), "sample: from 1 to 2^18 logits a row (got " + std::to_string(n_vocab) + ")");
+    need(n_vocab >= 1 && n_vocab <= SA_MAX_VOCAB, "sample: from 1 to 2^18 logits a row (got " + std::to_string(n_vocab) + ")");
     need(n_rows >= 0 && n_rows <= (1 << 20), "sample: from 0 to 2^20 rows");
     need(row_stride >= n_vocab || n_rows <= 1, "sample: row_stride is n_vocab at least");
     need(n_rows == 0 || (logits && u && ids && aligned(logits, size_of(dtype))), "sample: null pointer");
