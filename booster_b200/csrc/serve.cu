@@ -193,7 +193,7 @@ void move_pages(const b200_pages & p, const Pages & d, const int32_t * plan, int
 
 template <typename T> void sample_as(const SampleArgs & a, int cluster, int device, void * stream) {
     static Limits set;
-    const size_t smem = 8 * SA_LIST + 4 * SA_BINS + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
+    const size_t smem = SA_FIXED + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
     allow_smem(k_sample<T>, device, smem, set);
     launch(k_sample<T>, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, false, cluster, a);
 }

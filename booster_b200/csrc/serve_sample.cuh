@@ -5,10 +5,11 @@
 // first one in order of index at which the sum exceeds u x total. A filter's edge and the draw are decisions on sums, so weights are whole multiples of 2^-40 from 64-bit exponentials and
 // sums of them are exact: no order of summation, and no other split of the row, changes a result.
 //
-// A cluster of blocks takes a row and holds its slice in shared memory: logits cross HBM once. One sweep finds the maximum. A histogram of (largest - logit) by 1 / 32 gives, from counts
-// alone, the bin of the k-th token, and bounds between which the sum for top-p is crossed; only tokens of those bins are sorted (a few hundred of 128 k), exactly as the definition says.
-// With top-k all that can be kept is in that list, and the first block ends the row by itself. Otherwise a last sweep sums what is kept, 128 tokens at a time, and the warp in whose tokens
-// the draw falls looks for it. Rows whose edge lies among more than 2048 candidates (thousands of equal logits, very large k) are bisected over (logit, index) instead.
+// A cluster of blocks takes a row and holds its slice in shared memory: logits cross HBM once. A histogram of floor(32 x logit), against each block's own largest, tells with one meeting
+// of the cluster the row's largest and the bin of the k-th token. Only tokens down to that bin are ordered (a few dozen of 128 k), exactly as the definition says, and the first block
+// ends the row with them. For top-p alone counts bound the bins between which its sum is crossed; one sweep sums all weights, those in front of these bins and, in 1024 finer bins, those
+// between; the tokens of one finer bin are ordered. Then a last sweep sums what is kept, 128 tokens at a time, and the warp in whose tokens the draw falls looks for it. Rows whose edge
+// lies among more than 2048 candidates (thousands of equal logits, very large k) are bisected over (logit, index) instead.
 #pragma once
 #include "serve_cache.cuh"
 #include <cooperative_groups.h>
@@ -18,7 +19,7 @@ namespace srv {
 
 namespace cg = cooperative_groups;
 
-constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 1024, SA_LIST = 2048, SA_MAX_CLUSTER = 8, SA_MAX_VOCAB = 1 << 18, SA_SWEEPS = SA_MAX_VOCAB / SA_MAX_CLUSTER / SA_THREADS / 4;
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 1024, SA_LIST = 2048, SA_SHORT = SA_THREADS, SA_MAX_CLUSTER = 8, SA_MAX_VOCAB = 1 << 18, SA_SWEEPS = SA_MAX_VOCAB / SA_MAX_CLUSTER / SA_THREADS / 4;
 constexpr float SA_PER_NAT = 32.f;
 constexpr double SA_ONE = 1099511627776.0;                               // 2^40
 typedef unsigned long long u64;
@@ -33,29 +34,27 @@ struct SampleArgs {
     float * logprobs;
 };
 
-// 2^40 exp(-x) to the nearest whole number, x >= 0: 2^n times the series of e^f, |f| <= ln 2 / 2, whose first term left out is below 2^-46
-__device__ __forceinline__ u64 fixed_weight(double x) {
-    if (!(x < 30.0)) return 0;
-    const double y = x * -1.4426950408889634, n = rint(y), f = (y - n) * 0.6931471805599453;
-    double p = 1.0 / 479001600.0;
-    p = fma(p, f, 1.0 / 39916800.0);
-    p = fma(p, f, 1.0 / 3628800.0);
-    p = fma(p, f, 1.0 / 362880.0);
-    p = fma(p, f, 1.0 / 40320.0);
-    p = fma(p, f, 1.0 / 5040.0);
-    p = fma(p, f, 1.0 / 720.0);
-    p = fma(p, f, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return (u64) __double2ull_rn(p * __longlong_as_double((long long) (1023 + 40 + (int) n) << 52));
+// 2^40 exp(-x) to the nearest whole number, for x >= 0; 0 from 30 on (also for infinity and NaN). -x log2(e) = n / 16 + f / 16 with |f| <= 1 / 2: a table's 2^(n mod 16 / 16), whose
+// 16 entries are the 32 banks of shared memory, times 2^(n / 16) times the series of exp(f ln 2 / 16), whose first term left out is below 2^-42
+constexpr double SA_LN = 0.69314718055994530942 / 16;
+__constant__ double sa_series[5] = {SA_LN, SA_LN * SA_LN / 2, SA_LN * SA_LN * SA_LN / 6, SA_LN * SA_LN * SA_LN * SA_LN / 24, SA_LN * SA_LN * SA_LN * SA_LN * SA_LN / 120};
+__device__ __forceinline__ u64 fixed_weight(double x, const double * table) {
+    constexpr double WHOLE = 6755399441055744.0;                         // 1.5 x 2^52: added, the last bits are a whole number
+    const double y = x * (-1.0 / SA_LN), t = y + WHOLE, f = y - (t - WHOLE);
+    const int n = __double2loint(t);
+    double p = fma(sa_series[4], f, sa_series[3]);
+    p = fma(p, f, sa_series[2]);
+    p = fma(p, f, sa_series[1]);
+    p = fma(p, f, sa_series[0]);
+    p = fma(p, f, 1.0) * table[n & 15];
+    p = __hiloint2double(__double2hiint(p) + ((40 + (n >> 4)) << 20), __double2loint(p)) + 4503599627370496.0;      // 2^52
+    const u64 w = (u64) __double_as_longlong(p) & 0xfffffffffffffull;
+    return x < 30.0 ? w : 0;
 }
 
 // (logit, index) as one number: larger is earlier in the order
-__device__ __forceinline__ u64 order_key(float v, int i) {
-    const uint32_t b = __float_as_uint(v);
+__device__ __forceinline__ u64 order_key(float v, int i) {                // (-0 as 0, NaN as -infinity)
+    const uint32_t b = __float_as_uint(v == v ? v + 0.f : -INFINITY);
     return (u64) (b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t) ~i;
 }
 __device__ __forceinline__ float key_logit(u64 k) {
@@ -69,12 +68,16 @@ template <typename F> __device__ __forceinline__ u64 warp_reduce(u64 x, F f) {
     for (int d = 16; d; d >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, d));
     return x;
 }
-struct SampleSmem {
-    u64 red[SA_WARPS], each[SA_MAX_CLUSTER], turn[2][SA_MAX_CLUSTER];
-    u64 answer[4], edge;
+struct alignas(128) SampleSmem {
+    double table[16];
+    u64 red[SA_WARPS], each[SA_MAX_CLUSTER], turn[2][SA_MAX_CLUSTER], sums[SA_MAX_CLUSTER][2];
+    u64 answer[4];
     u64 parts[SA_SWEEPS][SA_WARPS];
-    int n_list;
+    float top;                           // the block's largest, and its place among the bins
+    int place, n_list;
 };
+// dynamic shared memory: the list, fine sums, fine counts, bins, the slice
+constexpr int SA_FIXED = 8 * SA_LIST + 8 * SA_BINS + 4 * SA_BINS + 4 * SA_BINS;
 // a number of every thread of the cluster, joined; all threads get it
 template <typename F> __device__ __forceinline__ u64 cluster_join(cg::cluster_group & cl, SampleSmem & sm, u64 x, u64 none, int & turn, F f) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -129,6 +132,11 @@ template <typename T> __device__ __forceinline__ void four_of(const T * vals, in
     for (int e = 0; e < 4; e++) v[e] = to_f(f.v[e]);
 }
 
+// floor(32 x logit), of logits so large that 32 of them are beyond 2^30 the border; a NaN stands with -infinity
+__device__ __forceinline__ int bin_place(float v) { return __float2int_rd(fminf(fmaxf(v * SA_PER_NAT, -1073741824.f), 1073741824.f)); }
+// the smallest float whose place is p or more
+__device__ __forceinline__ float place_from(int p) { return p <= -1073741824 ? -INFINITY : __int2float_ru(p) * (1.f / SA_PER_NAT); }
+
 template <typename T>
 __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t sa_raw[];
@@ -136,46 +144,70 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int) cl.block_rank(), blocks = (int) cl.num_blocks();
     const int row = (int) (blockIdx.x / blocks), base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base)), groups = (n + 3) >> 2;
-    u64 * list = reinterpret_cast<u64 *>(sa_raw);                        // [SA_LIST]; before it is a list, [SA_BINS] fine sums and counts
-    int * bins = reinterpret_cast<int *>(sa_raw + 8 * SA_LIST);          // [SA_BINS]
-    T * vals = reinterpret_cast<T *>(sa_raw + 8 * SA_LIST + 4 * SA_BINS);
-    int turn = 0;
-    // the slice, to whole fours
-    {
-        const T * src = static_cast<const T *>(a.logits) + row * a.row_stride + base;
-        constexpr int E = 16 / sizeof(T);
-        int done = 0;
-        if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-            done = n / E * E;
-            for (int i = tid * E; i < done; i += SA_THREADS * E)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"((uint32_t) __cvta_generic_to_shared(vals + i)), "l"(src + i) : "memory");
-        }
-        for (int i = done + tid; i < 4 * groups; i += SA_THREADS) vals[i] = i < n ? src[i] : from_f<T>(-INFINITY);
-        for (int i = tid; i < SA_BINS; i += SA_THREADS) bins[i] = 0;
-        if (tid == 0) sm.n_list = 0;
-    }
-    const float temperature = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f;
+    u64 * list = reinterpret_cast<u64 *>(sa_raw);                        // [SA_LIST]
+    u64 * fine = list + SA_LIST;                                         // [SA_BINS] sums
+    int * fine_count = reinterpret_cast<int *>(fine + SA_BINS), * bins = fine_count + SA_BINS;
+    T * vals = reinterpret_cast<T *>(bins + SA_BINS);
+    const float temperature = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f, u = a.u[row];
     const int k_all = a.top_k ? a.top_k[row] : 0, k = k_all > 0 && k_all < a.n_vocab ? k_all : 0;
-    const float u = a.u[row];
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
+    const bool by_p = top_p < 1.f, cut = temperature > 0.f && (k > 0 || by_p);
+    int turn = 0;
     const auto add = [](u64 x, u64 y) { return x + y; };
-    // the largest; a NaN becomes -infinity and -0 becomes 0 on the way
-    float top = -INFINITY;
-    for (int g = tid; g < groups; g += SA_THREADS) {
-        float v[4];
-        four_of(vals, g, v);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (v[e] != v[e] || __float_as_uint(v[e]) == 0x80000000u) { v[e] = v[e] == 0.f ? 0.f : -INFINITY; vals[4 * g + e] = from_f<T>(v[e]); }
-            top = fmaxf(top, v[e]);
-        }
-    }
-    top = key_logit(cluster_join(cl, sm, order_key(top, 0), 0ull, turn, [](u64 x, u64 y) { return max(x, y); }));
-    const auto finish = [&](int id, float lp) { a.ids[row] = id; if (a.logprobs) a.logprobs[row] = lp; };
     const auto each = [&](auto f) {                                      // f(four logits, index of the first in the slice)
         for (int g = tid; g < groups; g += SA_THREADS) { float v[4]; four_of(vals, g, v); f(v, 4 * g); }
     };
+    // the slice, to whole fours, and its largest (a NaN is none)
+    float top = -INFINITY;
+    {
+        const T * src = static_cast<const T *>(a.logits) + row * a.row_stride + base;
+        constexpr int E = 16 / sizeof(T);
+        for (int i = tid; i < SA_BINS; i += SA_THREADS) bins[i] = 0;
+        if (tid < 16) sm.table[tid] = exp2((double) tid / 16.0);
+        if (tid == 0) sm.n_list = 0;
+        int done = 0;
+        if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+            done = n / E * E;
+            for (int i0 = tid * E; i0 < done; i0 += 8 * SA_THREADS * E) {
+                uint4 x[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) { const int i = i0 + j * SA_THREADS * E; if (i < done) x[j] = *reinterpret_cast<const uint4 *>(src + i); }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int i = i0 + j * SA_THREADS * E;
+                    if (i < done) {
+                        *reinterpret_cast<uint4 *>(vals + i) = x[j];
+                        const Four<T> * f = reinterpret_cast<const Four<T> *>(&x[j]);
+#pragma unroll
+                        for (int h = 0; h < E / 4; h++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) top = fmaxf(top, to_f(f[h].v[e]));
+                    }
+                }
+            }
+        }
+        for (int i = done + tid; i < 4 * groups; i += SA_THREADS) { const T x = i < n ? src[i] : from_f<T>(-INFINITY); vals[i] = x; top = fmaxf(top, to_f(x)); }
+    }
+    top = key_logit(warp_reduce(order_key(top, 0), [](u64 x, u64 y) { return max(x, y); }));
+    if (lane == 0) sm.red[warp] = __float_as_uint(top);
+    __syncthreads();
+    for (int w = 0; w < SA_WARPS; w++) top = fmaxf(top, __uint_as_float((uint32_t) sm.red[w]));
+    const int place = bin_place(top);
+    if (tid == 0) { sm.top = top; sm.place = place; }
+    if (cut)
+        each([&](const float (&v)[4], int) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) atomicAdd(&bins[min(SA_BINS - 1, place - bin_place(v[e]))], 1);
+        });
+    cl.sync();
+    int places[SA_MAX_CLUSTER], row_place = -1073741824;
+#pragma unroll
+    for (int r = 0; r < SA_MAX_CLUSTER; r++) {
+        const SampleSmem * o = cl.map_shared_rank(&sm, r < blocks ? r : 0);
+        places[r] = o->place;
+        row_place = max(row_place, places[r]);
+        top = fmaxf(top, o->top);
+    }
+    const auto finish = [&](int id, float lp) { a.ids[row] = id; if (a.logprobs) a.logprobs[row] = lp; };
     const auto first_of_largest = [&]() {
         u64 mine = ~0ull;
         each([&](const float (&v)[4], int i) {
@@ -184,22 +216,20 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         });
         return (int) cluster_join(cl, sm, mine, ~0ull, turn, [](u64 x, u64 y) { return min(x, y); });
     };
-    if (top == -INFINITY || !(temperature > 0.f)) {
-        const int i = top == -INFINITY ? -1 : first_of_largest();
-        if (rank == 0 && tid == 0) finish(i, i < 0 ? -INFINITY : 0.f);
-        return;                                                          // (the join was the last that others read here)
+    if (top == -INFINITY || !(temperature > 0.f)) {                      // (behind the join nobody reads here any more)
+        const int i = first_of_largest();
+        if (rank == 0 && tid == 0) finish(top == -INFINITY ? -1 : i, top == -INFINITY ? -INFINITY : 0.f);
+        return;
     }
     const auto below = [&](float v) { return v == top ? 0.f : top - v; };                       // how far a logit is from the largest, to a float
     const auto exactly = [&](float v) { return v == top ? 0.0 : (double) top - (double) v; };
-    const auto weight = [&](float v) { return fixed_weight(exactly(v)); };
-    const auto bin_of = [&](float v) { return (int) fminf(below(v) * SA_PER_NAT, (float) (SA_BINS - 1)); };
+    const auto weight = [&](float v) { return fixed_weight(exactly(v), sm.table); };
     const float far = min_p > 0.f ? 0.01f - logf(min_p) : INFINITY;      // nothing so far below the largest is kept by min-p
     const double cold = 1.0 / (double) temperature;
-    const auto tempered = [&](double x) { return fixed_weight(x == 0.0 ? 0.0 : x * cold); };
+    const auto tempered = [&](double x) { return fixed_weight(x == 0.0 ? 0.0 : x * cold, sm.table); };
     const auto log_share = [&](double x, u64 total) { return (float) (-(x == 0.0 ? 0.0 : x * cold) - log((double) total * (1.0 / SA_ONE))); };
     const auto target_of = [&](u64 total) { const double at = (double) u * (double) total; return at >= (double) total ? total - 1 : at > 0.0 ? (u64) at : 0; };
     u64 edge = 0;                                                        // tokens of keys >= edge are kept by top-k and top-p
-    const bool by_p = top_p < 1.f;
     // the last key of the shortest prefix of the keys >= from that holds `want` tokens, or whose sum of weights reaches `want`
     const auto bisect = [&](u64 from, bool weights, double want) {
         u64 lo = from, hi = order_key(top, 0);                           // the prefix down to lo is enough
@@ -215,85 +245,112 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         }
         return lo;
     };
-    // list of the tokens for which f holds, in the first block of the cluster
-    const auto gather = [&](auto f) {
-        SampleSmem * s0 = cl.map_shared_rank(&sm, 0);
-        u64 * l0 = cl.map_shared_rank(list, 0);
+    // the tokens for which f holds, to the lists of the first `takers` blocks
+    const auto gather = [&](int takers, auto f) {
         each([&](const float (&v)[4], int i) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (f(v[e]) && i + e < n) {
-                    const int at = atomicAdd(&s0->n_list, 1);
-                    if (at < SA_LIST) l0[at] = order_key(v[e], base + i + e);
-                }
+                if (f(v[e]) && i + e < n)
+                    for (int r = 0; r < takers; r++) {
+                        const int at = atomicAdd(&cl.map_shared_rank(&sm, r)->n_list, 1);
+                        if (at < SA_LIST) cl.map_shared_rank(list, r)[at] = order_key(v[e], base + i + e);
+                    }
         });
         cl.sync();
     };
-    const auto sort_padded = [&](int m) {                                // first block: the list in order, padded with zeros
+    const auto sort_padded = [&](int m) {                                // the list in order, padded with zeros
         int pad = 32;
         while (pad < m) pad <<= 1;
         for (int i = m + tid; i < pad; i += SA_THREADS) list[i] = 0;
         __syncthreads();
         sort_list(list, pad);
     };
-    if (k > 0 || by_p) {
-        u64 total = 0, mine = 0;
-        each([&](const float (&v)[4], int i) {
+    if (cut) {
+        // two of the row's bins a thread, over all blocks; what lies behind the last but one is the rest
+        int cnt[2] = {0, 0}, theirs[SA_MAX_CLUSTER][2];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (i + e < n) atomicAdd(&bins[bin_of(v[e])], 1);
-                if (k == 0) mine += weight(v[e]);
-            }
-        });
-        if (k == 0) total = cluster_join(cl, sm, mine, 0ull, turn, add);
-        else cl.sync();
-        // two bins a thread, over all blocks
-        int cnt[2] = {0, 0};
-        for (int r = 0; r < blocks; r++) {
-            const int2 v = reinterpret_cast<const int2 *>(cl.map_shared_rank(bins, r))[tid];
-            cnt[0] += v.x; cnt[1] += v.y;
+        for (int r = 0; r < SA_MAX_CLUSTER; r++) {                       // (a block's places are the row's or lower)
+            const int * o = cl.map_shared_rank(bins, r < blocks ? r : 0);
+            const int at = 2 * tid - (row_place - places[r]);
+            theirs[r][0] = o[max(at, 0)];
+            theirs[r][1] = o[max(at + 1, 0)];
         }
-        u64 dummy;
-        const u64 front = block_before64((u64) (cnt[0] + cnt[1]), dummy, sm.red);
+#pragma unroll
+        for (int r = 0; r < SA_MAX_CLUSTER; r++) {
+            const int at = 2 * tid - (row_place - places[r]);
+            cnt[0] += r < blocks && at >= 0 ? theirs[r][0] : 0;
+            cnt[1] += r < blocks && at >= -1 ? theirs[r][1] : 0;
+        }
+        if (2 * tid + 1 == SA_BINS - 1) cnt[1] = 0;
+        u64 counted;
+        const u64 front = block_before64((u64) (cnt[0] + cnt[1]), counted, sm.red);
+        if (2 * tid + 1 == SA_BINS - 1) cnt[1] = a.n_vocab - (int) counted;
         if (tid == 0) { sm.answer[0] = 0; sm.answer[1] = SA_BINS - 1; sm.answer[2] = sm.answer[3] = 0; }
         __syncthreads();
-        const double want = (double) top_p * (double) total;
         if (k > 0) {
             u64 c = front;
             for (int j = 0; j < 2; j++) {
                 if (c < (u64) k && c + cnt[j] >= (u64) k) { sm.answer[1] = 2 * tid + j; sm.answer[3] = c + cnt[j]; }
                 c += cnt[j];
             }
-        } else {
-            // a bin's sum lies between cnt exp(-(b + 1) / 32) and cnt exp(-b / 32), widened by 1e-4 for the roundings of either side. The sum up to a bin's end is bounded by the bins in
-            // front and, from the exact total, by those behind, which is the sharper of the two near the end
+        } else if (abs(row_place) < (1 << 24)) {
+            // A bin's tokens lie (b - 1) / 32 + s to b / 32 + s below the largest, s what the largest is above its bin's lower end: bounds of each bin's sum, widened by 1e-4 for the
+            // roundings of either side. C, the sum up to a bin's end, has the share p when (1 - p) C >= p (what lies behind)
+            const double s = (double) top - (double) row_place / SA_PER_NAT, p = (double) top_p;
             u64 low = 0, high = 0, l[2], h[2], low_all, high_all;
             for (int j = 0; j < 2; j++) {
-                const double e = exp(-(double) (2 * tid + j) / SA_PER_NAT) * SA_ONE;
-                h[j] = (u64) (cnt[j] * e * 1.0001); l[j] = 2 * tid + j == SA_BINS - 1 ? 0 : (u64) (cnt[j] * e * 0.96923 * 0.9999);
+                const int b = 2 * tid + j;
+                const double e = exp(-(double) b / SA_PER_NAT - s) * SA_ONE * cnt[j];
+                l[j] = b == SA_BINS - 1 ? 0 : (u64) (e * 0.9999);
+                h[j] = (u64) fmin(e * (1.031744 * 1.0001), SA_ONE * cnt[j]) + cnt[j];      // exp(1 / 32); each token's weight is rounded by half a step
                 low += l[j]; high += h[j];
             }
             u64 cl_ = block_before64(low, low_all, sm.red), ch = block_before64(high, high_all, sm.red);
-            const auto least = [&](u64 in_l, u64 in_h) { return fmax((double) in_l, (double) total - (double) (high_all - in_h)); };
-            const auto most = [&](u64 in_l, u64 in_h) { return fmin((double) in_h, (double) total - (double) (low_all - in_l)); };
+            const auto surely = [&](u64 in_l, u64 in_h) { return (1.0 - p) * (double) in_l >= p * (double) (high_all - in_h); };
+            const auto maybe = [&](u64 in_l, u64 in_h) { return (1.0 - p) * (double) in_h * 1.0001 >= p * (double) (low_all - in_l); };
             u64 c = front;
             for (int j = 0; j < 2; j++) {
-                if (most(cl_, ch) < want && most(cl_ + l[j], ch + h[j]) >= want) { sm.answer[0] = 2 * tid + j; sm.answer[2] = c; }
-                if (least(cl_, ch) < want && least(cl_ + l[j], ch + h[j]) >= want) sm.answer[1] = 2 * tid + j;
+                const int b = 2 * tid + j;
+                if (maybe(cl_ + l[j], ch + h[j]) && (b == 0 || !maybe(cl_, ch))) { sm.answer[0] = b; sm.answer[2] = c; }
+                if (surely(cl_ + l[j], ch + h[j]) && (b == 0 || !surely(cl_, ch))) { sm.answer[1] = b; sm.answer[3] = c + cnt[j]; }
                 c += cnt[j]; cl_ += l[j]; ch += h[j];
             }
-            __syncthreads();
-            c = front;
-            for (int j = 0; j < 2; j++) { c += cnt[j]; if (2 * tid + j == (int) sm.answer[1]) sm.answer[3] = c; }
         }
         __syncthreads();
         const int b_lo = (int) sm.answer[0], b_hi = (int) sm.answer[1];
-        int n_between = (int) (sm.answer[3] - sm.answer[2]);
-        if (k > 0 && n_between <= SA_LIST) {
+        const float v_hi = b_lo ? place_from(row_place - b_lo + 1) : INFINITY, v_lo = b_hi == SA_BINS - 1 ? -INFINITY : place_from(row_place - b_hi);      // logits from v_lo to below v_hi
+        if (k > 0 && sm.answer[3] <= SA_LIST) {
             // everything that can be kept: the first block ends the row
-            gather([&](float v) { return bin_of(v) <= b_hi; });
+            gather(1, [&](float v) { return v >= v_lo; });
             if (rank) return;
-            const int m = sm.n_list, per = (m + SA_THREADS - 1) / SA_THREADS, i0 = min(m, tid * per), i1 = min(m, i0 + per);
+            const int m = sm.n_list;
+            if (m <= SA_SHORT) {                                         // a thread a token, which goes through all of them twice
+                u64 * w_of = fine, * t_of = fine + SA_SHORT;
+                const u64 mine = tid < m ? list[tid] : 0, w = tid < m ? weight(key_logit(mine)) : 0;
+                w_of[tid] = w;
+                __syncthreads();
+                int before_me = 0;
+                u64 c = 0;
+                if (tid < m)
+#pragma unroll 4
+                    for (int j = 0; j < m; j++) { const bool first = list[j] > mine; before_me += first; c += first ? w_of[j] : 0; }
+                if (tid < m && before_me == min(k, m) - 1) sm.answer[0] = c + w;
+                __syncthreads();
+                const bool in = tid < m && before_me < k && (before_me == 0 || !by_p || (double) c < (double) top_p * (double) sm.answer[0]) && !((double) w < (double) min_p * SA_ONE);
+                const double x = exactly(key_logit(mine));
+                const u64 t = in ? tempered(x) : 0;
+                t_of[tid] = t;
+                __syncthreads();
+                if (in) {
+                    u64 total = 0, upto = 0;
+#pragma unroll 4
+                    for (int j = 0; j < m; j++) { total += t_of[j]; upto += (uint32_t) list[j] >= (uint32_t) mine ? t_of[j] : 0; }       // (~index)
+                    const u64 target = target_of(total);
+                    if (upto - t <= target && target < upto) finish(key_index(mine), log_share(x, total));
+                }
+                return;
+            }
+            const int per = (m + SA_THREADS - 1) / SA_THREADS, i0 = min(m, tid * per), i1 = min(m, i0 + per);
             sort_padded(m);
             u64 mine_w = 0, all, kept = 0;
             for (int i = i0; i < min(i1, k); i++) mine_w += weight(key_logit(list[i]));
@@ -304,9 +361,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                 kept += (i == 0 || !by_p || (double) c < share) && !((double) w < (double) min_p * SA_ONE);
                 c += w;
             }
-            int n_kept;
             block_before64(kept, all, sm.red);
-            n_kept = (int) all;                                          // a prefix
+            const int n_kept = (int) all;                                // a prefix
             // by index: what is kept, as (~index, logit)
             u64 swapped[SA_LIST / SA_THREADS];
 #pragma unroll
@@ -341,82 +397,110 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                 edge = share > 0.0 ? bisect(edge, true, share) : order_key(top, first_of_largest());
             }
         } else {
-            u64 in_front = 0;                                            // sum of the bins in front of b_lo
-            each([&](const float (&v)[4], int) {
+            // all weights, those in front of the bins, and those in the bins by finer ones
+            const float from = b_lo ? v_hi : top, by = SA_BINS * SA_PER_NAT / (float) (b_hi - b_lo + 1);
+            const auto fine_place = [&](float v) { return fminf((from - v) * by, (float) (SA_BINS - 1)); };       // its whole part is the finer bin
+            const auto between = [&](float v) { return v >= v_lo && v < v_hi; };
+            for (int i = tid; i < SA_BINS; i += SA_THREADS) { fine[i] = 0; fine_count[i] = 0; }
+            __syncthreads();
+            u64 all = 0, in_front = 0;
+            each([&](const float (&v)[4], int i) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) if (bin_of(v[e]) < b_lo) in_front += weight(v[e]);
-            });
-            in_front = cluster_join(cl, sm, in_front, 0ull, turn, add);
-            const float f_lo = (float) b_lo / SA_PER_NAT, f_scale = SA_BINS * SA_PER_NAT / (float) (b_hi - b_lo + 1);
-            const auto fine_bin = [&](float v) { return (int) fminf((below(v) - f_lo) * f_scale, (float) (SA_BINS - 1)); };
-            int f_bin = -1;
-            if (n_between > SA_LIST) {                                   // 1024 finer bins between b_lo and b_hi, their sums exact
-                u64 * fine = list;
-                int * count = reinterpret_cast<int *>(fine + SA_BINS);
-                for (int i = tid; i < SA_BINS; i += SA_THREADS) { fine[i] = 0; count[i] = 0; }
-                __syncthreads();
-                each([&](const float (&v)[4], int i) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int b = bin_of(v[e]);
-                        if (b >= b_lo && b <= b_hi && i + e < n) {
-                            atomicAdd(&fine[fine_bin(v[e])], weight(v[e]));
-                            atomicAdd(&count[fine_bin(v[e])], 1);
-                        }
+                for (int e = 0; e < 4; e++) {
+                    const u64 w = weight(v[e]);
+                    all += w;
+                    in_front += v[e] >= v_hi ? w : 0;
+                    if (between(v[e]) && i + e < n) {
+                        const int b = (int) fine_place(v[e]);
+                        atomicAdd(&fine[b], w);
+                        atomicAdd(&fine_count[b], 1);
                     }
-                });
-                cl.sync();
-                u64 w[2] = {0, 0};
-                int fc[2] = {0, 0};
-                for (int r = 0; r < blocks; r++) {
-                    const u64 * fw = cl.map_shared_rank(fine, r) + 2 * tid;
-                    const int * ff = cl.map_shared_rank(count, r) + 2 * tid;
-                    for (int j = 0; j < 2; j++) { w[j] += fw[j]; fc[j] += ff[j]; }
                 }
-                u64 c = in_front + block_before64(w[0] + w[1], dummy, sm.red);
-                if (tid == 0) sm.answer[0] = SA_BINS;
-                __syncthreads();
-                for (int j = 0; j < 2; j++) {
-                    if ((double) c < want && (double) (c + w[j]) >= want) { sm.answer[0] = 2 * tid + j; sm.answer[1] = c; sm.answer[2] = fc[j]; }
-                    c += w[j];
+            });
+            u64 sums[2];
+            block_before64(all, sums[0], sm.red);
+            block_before64(in_front, sums[1], sm.red);
+            if (tid < blocks) { cl.map_shared_rank(&sm, tid)->sums[rank][0] = sums[0]; cl.map_shared_rank(&sm, tid)->sums[rank][1] = sums[1]; }
+            cl.sync();
+            all = in_front = 0;
+            for (int r = 0; r < blocks; r++) { all += sm.sums[r][0]; in_front += sm.sums[r][1]; }
+            const double want = (double) top_p * (double) all;
+            u64 w[2] = {0, 0};
+            int fc[2] = {0, 0};
+#pragma unroll
+            for (int r0 = 0; r0 < SA_MAX_CLUSTER; r0 += 4) {
+                ulonglong2 x[4];
+                int2 y[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int o = r0 + r < blocks ? r0 + r : 0;
+                    x[r] = reinterpret_cast<const ulonglong2 *>(cl.map_shared_rank(fine, o))[tid];
+                    y[r] = reinterpret_cast<const int2 *>(cl.map_shared_rank(fine_count, o))[tid];
                 }
-                __syncthreads();
-                if (sm.answer[0] < SA_BINS) { f_bin = (int) sm.answer[0]; in_front = sm.answer[1]; n_between = (int) sm.answer[2]; }
-                cl.sync();                                               // the sums have been read: a list may take their place
+#pragma unroll
+                for (int r = 0; r < 4; r++) if (r0 + r < blocks) { w[0] += x[r].x; w[1] += x[r].y; fc[0] += y[r].x; fc[1] += y[r].y; }
             }
-            if (n_between <= SA_LIST) {
-                gather([&](float v) {
-                    const int b = bin_of(v);
-                    return b >= b_lo && b <= b_hi && (f_bin < 0 || fine_bin(v) == f_bin);
-                });
-                if (rank == 0) {
-                    const int m = sm.n_list, per = (m + SA_THREADS - 1) / SA_THREADS, i0 = min(m, tid * per), i1 = min(m, i0 + per);
+            u64 c = in_front + block_before64(w[0] + w[1], counted, sm.red);
+            if (tid == 0) sm.answer[0] = SA_BINS;
+            __syncthreads();
+            for (int j = 0; j < 2; j++) {
+                if ((double) c < want && (double) (c + w[j]) >= want) { sm.answer[0] = 2 * tid + j; sm.answer[1] = c; sm.answer[2] = fc[j]; }
+                c += w[j];
+            }
+            __syncthreads();
+            const int f_bin = (int) sm.answer[0];
+            c = sm.answer[1];
+            if (f_bin < SA_BINS && sm.answer[2] <= SA_LIST) {
+                gather(blocks, [&](float v) { const float at = fine_place(v); return between(v) && at >= (float) f_bin && at < (float) (f_bin + 1); });
+                const int m = sm.n_list;
+                if (m <= SA_SHORT) {
+                    const u64 mine = tid < m ? list[tid] : 0, w_mine = tid < m ? weight(key_logit(mine)) : 0;
+                    if (tid == 0) sm.answer[0] = 0;
+                    fine[tid] = w_mine;                                  // (everybody has read the sums)
+                    __syncthreads();
+                    if (tid < m) {
+#pragma unroll 4
+                        for (int j = 0; j < m; j++) c += list[j] > mine ? fine[j] : 0;
+                        if ((double) c < want && (double) (c + w_mine) >= want) sm.answer[0] = mine;
+                    }
+                } else {
+                    const int per = (m + SA_THREADS - 1) / SA_THREADS, i0 = min(m, tid * per), i1 = min(m, i0 + per);
                     sort_padded(m);
-                    u64 mine_w = 0, all;
+                    u64 mine_w = 0;
                     for (int i = i0; i < i1; i++) mine_w += weight(key_logit(list[i]));
-                    u64 c = in_front + block_before64(mine_w, all, sm.red);
-                    if (tid == 0) sm.answer[0] = m ? list[m - 1] : 0;
+                    c += block_before64(mine_w, counted, sm.red);
+                    if (tid == 0) sm.answer[0] = 0;
                     __syncthreads();
                     for (int i = i0; i < i1; i++) {
-                        const u64 w = weight(key_logit(list[i]));
-                        if ((i == 0 || (double) c < want) && (double) (c + w) >= want) sm.answer[0] = list[i];
-                        c += w;
+                        const u64 w_i = weight(key_logit(list[i]));
+                        if ((double) c < want && (double) (c + w_i) >= want) sm.answer[0] = list[i];
+                        c += w_i;
                     }
-                    __syncthreads();
-                    const u64 e = sm.answer[0];
-                    if (tid < blocks) cl.map_shared_rank(&sm, tid)->edge = e;
                 }
-                cl.sync();
-                edge = sm.edge;
+                __syncthreads();
+                edge = sm.answer[0];
             } else edge = want > 0.0 ? bisect(0, true, want) : order_key(top, first_of_largest());
         }
     }
     // the draw: sums of 128 neighbouring tokens, a warp's at a time, which stand in order of index
-    const auto drawn = [&](float v, int i) -> u64 {
-        if (below(v) > far || v == -INFINITY || (edge && order_key(v, base + i) < edge)) return 0;
-        const double x = exactly(v);
-        if (min_p > 0.f && (double) fixed_weight(x) < (double) min_p * SA_ONE) return 0;
-        return tempered(x);
+    const float edge_logit = edge ? key_logit(edge) : -INFINITY;
+    const int edge_index = edge ? key_index(edge) : 0x7fffffff;
+    const auto drawn = [&](const float (&v)[4], int i, u64 (&w)[4]) {
+        bool in[4], some = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            in[e] = below(v[e]) <= far && (v[e] > edge_logit || (v[e] == edge_logit && base + i + e <= edge_index));
+            some = some || in[e];
+            w[e] = 0;
+        }
+        if (!some) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double x = exactly(v[e]);
+            if (min_p > 0.f) in[e] = in[e] && !((double) fixed_weight(x, sm.table) < (double) min_p * SA_ONE);
+            const u64 t = tempered(x);
+            w[e] = in[e] ? t : 0;
+        }
     };
     const int sweeps = (groups + SA_THREADS - 1) / SA_THREADS;
     for (int s = 0; s < sweeps; s++) {
@@ -424,9 +508,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         u64 sum = 0;
         if (g < groups) {
             float v[4];
+            u64 w[4];
             four_of(vals, g, v);
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += drawn(v[e], 4 * g + e);
+            drawn(v, 4 * g, w);
+            sum = w[0] + w[1] + w[2] + w[3];
         }
         if (__any_sync(0xffffffffu, sum != 0)) sum = warp_reduce(sum, add);
         if (lane == 0) sm.parts[s][warp] = sum;
@@ -448,8 +533,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         if (g < groups) four_of(vals, g, v);
         u64 w[4], sum = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) { w[e] = drawn(v[e], 4 * g + e); sum += w[e]; }
+        drawn(v, 4 * g, w);
+        sum = w[0] + w[1] + w[2] + w[3];
         u64 up = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) { const u64 x = __shfl_up_sync(0xffffffffu, up, d); if (lane >= d) up += x; }
