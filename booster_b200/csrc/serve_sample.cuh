@@ -5,7 +5,7 @@
 // first one in order of index at which the sum exceeds u x total. A filter's edge and the draw are decisions on sums, so weights are whole multiples of 2^-40 from 64-bit exponentials and
 // sums of them are exact: no order of summation, and no other split of the row, changes a result.
 //
-// A cluster of blocks takes a row and holds its slice in shared memory: logits cross HBM once. A histogram of floor(32 x logit), against each block's own largest, tells with one meeting
+// A cluster of blocks takes a row and holds its slice in shared memory: logits cross HBM once. A histogram of floor(16 x logit), against each block's own largest, tells with one meeting
 // of the cluster the row's largest and the bin of the k-th token. Only tokens down to that bin are ordered (a few dozen of 128 k), exactly as the definition says, and the first block
 // ends the row with them. For top-p alone counts bound the bins between which its sum is crossed; one sweep sums all weights, those in front of these bins and, in 1024 finer bins, those
 // between; the tokens of one finer bin are ordered. Then a last sweep sums what is kept, 128 tokens at a time, and the warp in whose tokens the draw falls looks for it. Rows whose edge
@@ -19,8 +19,8 @@ namespace srv {
 
 namespace cg = cooperative_groups;
 
-constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 1024, SA_LIST = 2048, SA_SHORT = SA_THREADS, SA_MAX_CLUSTER = 8, SA_MAX_VOCAB = 1 << 18, SA_SWEEPS = SA_MAX_VOCAB / SA_MAX_CLUSTER / SA_THREADS / 4;
-constexpr float SA_PER_NAT = 32.f;
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 512, SA_FINE = 1024, SA_LIST = 2048, SA_SHORT = SA_THREADS, SA_MAX_CLUSTER = 8, SA_MAX_VOCAB = 1 << 18, SA_SWEEPS = SA_MAX_VOCAB / SA_MAX_CLUSTER / SA_THREADS / 4;
+constexpr float SA_PER_NAT = 16.f;
 constexpr double SA_ONE = 1099511627776.0;                               // 2^40
 typedef unsigned long long u64;
 
@@ -34,13 +34,13 @@ struct SampleArgs {
     float * logprobs;
 };
 
-// 2^40 exp(-x) to the nearest whole number, for x >= 0; 0 from 30 on (also for infinity and NaN). -x log2(e) = n / 16 + f / 16 with |f| <= 1 / 2: a table's 2^(n mod 16 / 16), whose
-// 16 entries are the 32 banks of shared memory, times 2^(n / 16) times the series of exp(f ln 2 / 16), whose first term left out is below 2^-42
+// 2^40 exp(-x), x >= 0, to the nearest whole number, for y = -16 x log2(e) and whether x < 30 (beyond that it is 0): y = n + f with |f| <= 1 / 2: a table's 2^(n mod 16 / 16), whose 16
+// entries are the 32 banks of shared memory, times 2^(n / 16) times the series of exp(f ln 2 / 16), whose first term left out is below 2^-42
 constexpr double SA_LN = 0.69314718055994530942 / 16;
 __constant__ double sa_series[5] = {SA_LN, SA_LN * SA_LN / 2, SA_LN * SA_LN * SA_LN / 6, SA_LN * SA_LN * SA_LN * SA_LN / 24, SA_LN * SA_LN * SA_LN * SA_LN * SA_LN / 120};
-__device__ __forceinline__ u64 fixed_weight(double x, const double * table) {
+__device__ __forceinline__ u64 fixed_weight(double y, bool near, const double * table) {
     constexpr double WHOLE = 6755399441055744.0;                         // 1.5 x 2^52: added, the last bits are a whole number
-    const double y = x * (-1.0 / SA_LN), t = y + WHOLE, f = y - (t - WHOLE);
+    const double t = y + WHOLE, f = y - (t - WHOLE);
     const int n = __double2loint(t);
     double p = fma(sa_series[4], f, sa_series[3]);
     p = fma(p, f, sa_series[2]);
@@ -48,8 +48,7 @@ __device__ __forceinline__ u64 fixed_weight(double x, const double * table) {
     p = fma(p, f, sa_series[0]);
     p = fma(p, f, 1.0) * table[n & 15];
     p = __hiloint2double(__double2hiint(p) + ((40 + (n >> 4)) << 20), __double2loint(p)) + 4503599627370496.0;      // 2^52
-    const u64 w = (u64) __double_as_longlong(p) & 0xfffffffffffffull;
-    return x < 30.0 ? w : 0;
+    return near ? (u64) __double_as_longlong(p) & 0xfffffffffffffull : 0;
 }
 
 // (logit, index) as one number: larger is earlier in the order
@@ -77,7 +76,7 @@ struct alignas(128) SampleSmem {
     int place, n_list;
 };
 // dynamic shared memory: the list, fine sums, fine counts, bins, the slice
-constexpr int SA_FIXED = 8 * SA_LIST + 8 * SA_BINS + 4 * SA_BINS + 4 * SA_BINS;
+constexpr int SA_FIXED = 8 * SA_LIST + 12 * SA_FINE + 4 * SA_BINS;
 // a number of every thread of the cluster, joined; all threads get it
 template <typename F> __device__ __forceinline__ u64 cluster_join(cg::cluster_group & cl, SampleSmem & sm, u64 x, u64 none, int & turn, F f) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -132,10 +131,11 @@ template <typename T> __device__ __forceinline__ void four_of(const T * vals, in
     for (int e = 0; e < 4; e++) v[e] = to_f(f.v[e]);
 }
 
-// floor(32 x logit), of logits so large that 32 of them are beyond 2^30 the border; a NaN stands with -infinity
-__device__ __forceinline__ int bin_place(float v) { return __float2int_rd(fminf(fmaxf(v * SA_PER_NAT, -1073741824.f), 1073741824.f)); }
+// floor(16 x logit), as the last bits of 1.5 x 2^23 + 16 x logit rounded down; logits beyond +-262143 stand with those, a NaN with -infinity
+constexpr float SA_FAR = 262143.f;
+__device__ __forceinline__ int bin_place(float v) { return __float_as_int(__fmaf_rd(fminf(fmaxf(v, -SA_FAR), SA_FAR), SA_PER_NAT, 12582912.f)) - 0x4b400000; }
 // the smallest float whose place is p or more
-__device__ __forceinline__ float place_from(int p) { return p <= -1073741824 ? -INFINITY : __int2float_ru(p) * (1.f / SA_PER_NAT); }
+__device__ __forceinline__ float place_from(int p) { return p <= (int) (-SA_FAR * SA_PER_NAT) ? -INFINITY : (float) p * (1.f / SA_PER_NAT); }
 
 template <typename T>
 __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int) cl.block_rank(), blocks = (int) cl.num_blocks();
     const int row = (int) (blockIdx.x / blocks), base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base)), groups = (n + 3) >> 2;
     u64 * list = reinterpret_cast<u64 *>(sa_raw);                        // [SA_LIST]
-    u64 * fine = list + SA_LIST;                                         // [SA_BINS] sums
-    int * fine_count = reinterpret_cast<int *>(fine + SA_BINS), * bins = fine_count + SA_BINS;
+    u64 * fine = list + SA_LIST;                                         // [SA_FINE] sums
+    int * fine_count = reinterpret_cast<int *>(fine + SA_FINE), * bins = fine_count + SA_FINE;
     T * vals = reinterpret_cast<T *>(bins + SA_BINS);
     const float temperature = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f, u = a.u[row];
     const int k_all = a.top_k ? a.top_k[row] : 0, k = k_all > 0 && k_all < a.n_vocab ? k_all : 0;
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             for (int e = 0; e < 4; e++) atomicAdd(&bins[min(SA_BINS - 1, place - bin_place(v[e]))], 1);
         });
     cl.sync();
-    int places[SA_MAX_CLUSTER], row_place = -1073741824;
+    int places[SA_MAX_CLUSTER], row_place = (int) (-SA_FAR * SA_PER_NAT);
 #pragma unroll
     for (int r = 0; r < SA_MAX_CLUSTER; r++) {
         const SampleSmem * o = cl.map_shared_rank(&sm, r < blocks ? r : 0);
@@ -223,10 +223,19 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     }
     const auto below = [&](float v) { return v == top ? 0.f : top - v; };                       // how far a logit is from the largest, to a float
     const auto exactly = [&](float v) { return v == top ? 0.0 : (double) top - (double) v; };
-    const auto weight = [&](float v) { return fixed_weight(exactly(v), sm.table); };
-    const float far = min_p > 0.f ? 0.01f - logf(min_p) : INFINITY;      // nothing so far below the largest is kept by min-p
-    const double cold = 1.0 / (double) temperature;
-    const auto tempered = [&](double x) { return fixed_weight(x == 0.0 ? 0.0 : x * cold, sm.table); };
+    // y = 16 log2(e) (v - largest), over the temperature or not: by one fma where its rounding, a factor common to all of a row's weights, is small (2^-23 at most), else from the difference
+    const double cold = 1.0 / (double) temperature, steps = 1.0 / SA_LN, steps_cold = steps * cold;
+    const bool direct = fabsf(top) < SA_FAR && fabs((double) top * steps_cold) < 1073741824.0;
+    const double from_top = -(double) top * steps, from_top_cold = -(double) top * steps_cold;
+    const float cold_f = (float) cold;
+    const auto weight = [&](float v) { return fixed_weight(direct ? fma((double) v, steps, from_top) : -exactly(v) * steps, below(v) < 30.f, sm.table); };
+    const auto tempered = [&](float v) {
+        const float d = below(v);
+        return fixed_weight(direct ? fma((double) v, steps_cold, from_top_cold) : d == 0.f ? 0.0 : -exactly(v) * steps_cold, d == 0.f || d * cold_f < 30.f, sm.table);
+    };
+    const double far = min_p > 0.f ? -log((double) min_p) : INFINITY;    // min-p keeps what is at most so far below the largest
+    const float far_f = (float) far * 1.00001f + 1e-30f;
+    const auto near_enough = [&](float v) { return below(v) <= far_f && exactly(v) <= far; };
     const auto log_share = [&](double x, u64 total) { return (float) (-(x == 0.0 ? 0.0 : x * cold) - log((double) total * (1.0 / SA_ONE))); };
     const auto target_of = [&](u64 total) { const double at = (double) u * (double) total; return at >= (double) total ? total - 1 : at > 0.0 ? (u64) at : 0; };
     u64 edge = 0;                                                        // tokens of keys >= edge are kept by top-k and top-p
@@ -266,55 +275,31 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         sort_list(list, pad);
     };
     if (cut) {
-        // two of the row's bins a thread, over all blocks; what lies behind the last but one is the rest
-        int cnt[2] = {0, 0}, theirs[SA_MAX_CLUSTER][2];
+        // a bin of the row's a thread, over all blocks; what lies behind the last but one is the rest
+        int cnt = 0, theirs[SA_MAX_CLUSTER];
 #pragma unroll
-        for (int r = 0; r < SA_MAX_CLUSTER; r++) {                       // (a block's places are the row's or lower)
-            const int * o = cl.map_shared_rank(bins, r < blocks ? r : 0);
-            const int at = 2 * tid - (row_place - places[r]);
-            theirs[r][0] = o[max(at, 0)];
-            theirs[r][1] = o[max(at + 1, 0)];
-        }
+        for (int r = 0; r < SA_MAX_CLUSTER; r++) theirs[r] = cl.map_shared_rank(bins, r < blocks ? r : 0)[max(tid - (row_place - places[r]), 0)];       // (a block's places are the row's or lower)
 #pragma unroll
-        for (int r = 0; r < SA_MAX_CLUSTER; r++) {
-            const int at = 2 * tid - (row_place - places[r]);
-            cnt[0] += r < blocks && at >= 0 ? theirs[r][0] : 0;
-            cnt[1] += r < blocks && at >= -1 ? theirs[r][1] : 0;
-        }
-        if (2 * tid + 1 == SA_BINS - 1) cnt[1] = 0;
+        for (int r = 0; r < SA_MAX_CLUSTER; r++) cnt += r < blocks && tid >= row_place - places[r] ? theirs[r] : 0;
+        if (tid == SA_BINS - 1) cnt = 0;
         u64 counted;
-        const u64 front = block_before64((u64) (cnt[0] + cnt[1]), counted, sm.red);
-        if (2 * tid + 1 == SA_BINS - 1) cnt[1] = a.n_vocab - (int) counted;
+        const u64 front = block_before64((u64) cnt, counted, sm.red);
+        if (tid == SA_BINS - 1) cnt = a.n_vocab - (int) counted;
         if (tid == 0) { sm.answer[0] = 0; sm.answer[1] = SA_BINS - 1; sm.answer[2] = sm.answer[3] = 0; }
         __syncthreads();
         if (k > 0) {
-            u64 c = front;
-            for (int j = 0; j < 2; j++) {
-                if (c < (u64) k && c + cnt[j] >= (u64) k) { sm.answer[1] = 2 * tid + j; sm.answer[3] = c + cnt[j]; }
-                c += cnt[j];
-            }
-        } else if (abs(row_place) < (1 << 24)) {
-            // A bin's tokens lie (b - 1) / 32 + s to b / 32 + s below the largest, s what the largest is above its bin's lower end: bounds of each bin's sum, widened by 1e-4 for the
+            if (front < (u64) k && front + cnt >= (u64) k) { sm.answer[1] = tid; sm.answer[3] = front + cnt; }
+        } else if (fabsf(top) < SA_FAR) {
+            // A bin's tokens lie (b - 1) / 16 + s to b / 16 + s below the largest, s what the largest is above its bin's lower end: bounds of each bin's sum, widened by 1e-4 for the
             // roundings of either side. C, the sum up to a bin's end, has the share p when (1 - p) C >= p (what lies behind)
-            const double s = (double) top - (double) row_place / SA_PER_NAT, p = (double) top_p;
-            u64 low = 0, high = 0, l[2], h[2], low_all, high_all;
-            for (int j = 0; j < 2; j++) {
-                const int b = 2 * tid + j;
-                const double e = exp(-(double) b / SA_PER_NAT - s) * SA_ONE * cnt[j];
-                l[j] = b == SA_BINS - 1 ? 0 : (u64) (e * 0.9999);
-                h[j] = (u64) fmin(e * (1.031744 * 1.0001), SA_ONE * cnt[j]) + cnt[j];      // exp(1 / 32); each token's weight is rounded by half a step
-                low += l[j]; high += h[j];
-            }
-            u64 cl_ = block_before64(low, low_all, sm.red), ch = block_before64(high, high_all, sm.red);
-            const auto surely = [&](u64 in_l, u64 in_h) { return (1.0 - p) * (double) in_l >= p * (double) (high_all - in_h); };
-            const auto maybe = [&](u64 in_l, u64 in_h) { return (1.0 - p) * (double) in_h * 1.0001 >= p * (double) (low_all - in_l); };
-            u64 c = front;
-            for (int j = 0; j < 2; j++) {
-                const int b = 2 * tid + j;
-                if (maybe(cl_ + l[j], ch + h[j]) && (b == 0 || !maybe(cl_, ch))) { sm.answer[0] = b; sm.answer[2] = c; }
-                if (surely(cl_ + l[j], ch + h[j]) && (b == 0 || !surely(cl_, ch))) { sm.answer[1] = b; sm.answer[3] = c + cnt[j]; }
-                c += cnt[j]; cl_ += l[j]; ch += h[j];
-            }
+            const double s = (double) top - (double) row_place / SA_PER_NAT, p = (double) top_p, e = exp(-(double) tid / SA_PER_NAT - s) * SA_ONE * cnt;
+            const u64 l = tid == SA_BINS - 1 ? 0 : (u64) (e * 0.9999), h = (u64) fmin(e * (1.064495 * 1.0001), SA_ONE * cnt) + cnt;      // exp(1 / 16); each token's weight is rounded by half a step
+            u64 low_all, high_all;
+            const u64 in_l = block_before64(l, low_all, sm.red), in_h = block_before64(h, high_all, sm.red);
+            const auto surely = [&](u64 low, u64 high) { return (1.0 - p) * (double) low >= p * (double) (high_all - high); };
+            const auto maybe = [&](u64 low, u64 high) { return (1.0 - p) * (double) high * 1.0001 >= p * (double) (low_all - low); };
+            if (maybe(in_l + l, in_h + h) && (tid == 0 || !maybe(in_l, in_h))) { sm.answer[0] = tid; sm.answer[2] = front; }
+            if (surely(in_l + l, in_h + h) && (tid == 0 || !surely(in_l, in_h))) { sm.answer[1] = tid; sm.answer[3] = front + cnt; }
         }
         __syncthreads();
         const int b_lo = (int) sm.answer[0], b_hi = (int) sm.answer[1];
@@ -336,9 +321,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                     for (int j = 0; j < m; j++) { const bool first = list[j] > mine; before_me += first; c += first ? w_of[j] : 0; }
                 if (tid < m && before_me == min(k, m) - 1) sm.answer[0] = c + w;
                 __syncthreads();
-                const bool in = tid < m && before_me < k && (before_me == 0 || !by_p || (double) c < (double) top_p * (double) sm.answer[0]) && !((double) w < (double) min_p * SA_ONE);
-                const double x = exactly(key_logit(mine));
-                const u64 t = in ? tempered(x) : 0;
+                const bool in = tid < m && before_me < k && (before_me == 0 || !by_p || (double) c < (double) top_p * (double) sm.answer[0]) && near_enough(key_logit(mine));
+                const u64 t = in ? tempered(key_logit(mine)) : 0;
                 t_of[tid] = t;
                 __syncthreads();
                 if (in) {
@@ -346,7 +330,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
 #pragma unroll 4
                     for (int j = 0; j < m; j++) { total += t_of[j]; upto += (uint32_t) list[j] >= (uint32_t) mine ? t_of[j] : 0; }       // (~index)
                     const u64 target = target_of(total);
-                    if (upto - t <= target && target < upto) finish(key_index(mine), log_share(x, total));
+                    if (upto - t <= target && target < upto) finish(key_index(mine), log_share(exactly(key_logit(mine)), total));
                 }
                 return;
             }
@@ -358,7 +342,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             const double share = (double) top_p * (double) all;
             for (int i = i0; i < min(i1, k); i++) {                      // a token is kept while the sum in front of it is short of the share; the first always is
                 const u64 w = weight(key_logit(list[i]));
-                kept += (i == 0 || !by_p || (double) c < share) && !((double) w < (double) min_p * SA_ONE);
+                kept += (i == 0 || !by_p || (double) c < share) && near_enough(key_logit(list[i]));
                 c += w;
             }
             block_before64(kept, all, sm.red);
@@ -373,14 +357,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             sort_padded(n_kept);
             const int d0 = min(n_kept, tid * per), d1 = min(n_kept, d0 + per);
             u64 sum = 0;
-            for (int i = d0; i < d1; i++) sum += tempered(exactly(__uint_as_float((uint32_t) list[i])));
+            for (int i = d0; i < d1; i++) sum += tempered(__uint_as_float((uint32_t) list[i]));
             c = block_before64(sum, all, sm.red);
             const u64 target = target_of(all);
             if (c <= target && target < c + sum) {
                 for (int i = d0; i < d1; i++) {
-                    const double x = exactly(__uint_as_float((uint32_t) list[i]));
-                    c += tempered(x);
-                    if (c > target) { finish((int) ~(uint32_t) (list[i] >> 32), log_share(x, all)); break; }
+                    const float v = __uint_as_float((uint32_t) list[i]);
+                    c += tempered(v);
+                    if (c > target) { finish((int) ~(uint32_t) (list[i] >> 32), log_share(exactly(v), all)); break; }
                 }
             }
             return;
@@ -398,10 +382,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             }
         } else {
             // all weights, those in front of the bins, and those in the bins by finer ones
-            const float from = b_lo ? v_hi : top, by = SA_BINS * SA_PER_NAT / (float) (b_hi - b_lo + 1);
-            const auto fine_place = [&](float v) { return fminf((from - v) * by, (float) (SA_BINS - 1)); };       // its whole part is the finer bin
+            const float from = b_lo ? v_hi : top, by = SA_FINE * SA_PER_NAT / (float) (b_hi - b_lo + 1);
+            const auto fine_place = [&](float v) { return fminf((from - v) * by, (float) (SA_FINE - 1)); };       // its whole part is the finer bin
             const auto between = [&](float v) { return v >= v_lo && v < v_hi; };
-            for (int i = tid; i < SA_BINS; i += SA_THREADS) { fine[i] = 0; fine_count[i] = 0; }
+            for (int i = tid; i < SA_FINE; i += SA_THREADS) { fine[i] = 0; fine_count[i] = 0; }
             __syncthreads();
             u64 all = 0, in_front = 0;
             each([&](const float (&v)[4], int i) {
@@ -441,7 +425,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                 for (int r = 0; r < 4; r++) if (r0 + r < blocks) { w[0] += x[r].x; w[1] += x[r].y; fc[0] += y[r].x; fc[1] += y[r].y; }
             }
             u64 c = in_front + block_before64(w[0] + w[1], counted, sm.red);
-            if (tid == 0) sm.answer[0] = SA_BINS;
+            if (tid == 0) sm.answer[0] = SA_FINE;
             __syncthreads();
             for (int j = 0; j < 2; j++) {
                 if ((double) c < want && (double) (c + w[j]) >= want) { sm.answer[0] = 2 * tid + j; sm.answer[1] = c; sm.answer[2] = fc[j]; }
@@ -450,7 +434,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             __syncthreads();
             const int f_bin = (int) sm.answer[0];
             c = sm.answer[1];
-            if (f_bin < SA_BINS && sm.answer[2] <= SA_LIST) {
+            if (f_bin < SA_FINE && sm.answer[2] <= SA_LIST) {
                 gather(blocks, [&](float v) { const float at = fine_place(v); return between(v) && at >= (float) f_bin && at < (float) (f_bin + 1); });
                 const int m = sm.n_list;
                 if (m <= SA_SHORT) {
@@ -489,16 +473,15 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         bool in[4], some = false;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            in[e] = below(v[e]) <= far && (v[e] > edge_logit || (v[e] == edge_logit && base + i + e <= edge_index));
+            in[e] = below(v[e]) <= far_f && (v[e] > edge_logit || (v[e] == edge_logit && base + i + e <= edge_index));
             some = some || in[e];
             w[e] = 0;
         }
         if (!some) return;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const double x = exactly(v[e]);
-            if (min_p > 0.f) in[e] = in[e] && !((double) fixed_weight(x, sm.table) < (double) min_p * SA_ONE);
-            const u64 t = tempered(x);
+            if (min_p > 0.f) in[e] = in[e] && exactly(v[e]) <= far;
+            const u64 t = tempered(v[e]);
             w[e] = in[e] ? t : 0;
         }
     };
