@@ -87,16 +87,29 @@ void check_dtype(int dtype, bool f32) {
     need(dtype == B200_DTYPE_BF16 || dtype == B200_DTYPE_F16 || (f32 && dtype == B200_DTYPE_F32), f32 ? "dtype is B200_DTYPE_F32, _BF16 or _F16" : "dtype is B200_DTYPE_BF16 or _F16");
 }
 
+// rows by themselves where sequences have few of them, else tile by tile (16 rows a sequence on average: whole tiles begin to be the rule)
+bool by_tiles(const b200_kv4 & c) { return c.n_rows >= 16 * c.n_seq; }
+// heads of a row one after the other in a warp only where there are rows enough to fill the card without (48 rows of 8 heads: one pass 3 us less than four)
+int row_passes(const b200_kv4 & c) { return (int64_t) c.n_rows * c.n_head_kv > 4096 ? 4 : 1; }
+int row_parts(const b200_kv4 & c) { const int per = row_passes(c) * (128 / c.head_dim); return (c.n_head_kv + per - 1) / per; }
+unsigned row_blocks(const b200_kv4 & c) { return (unsigned) (((int64_t) c.n_rows * row_parts(c) + 7) / 8); }
+unsigned tile_blocks(const b200_kv4 & c, int parts) { const int per = 128 / c.head_dim; return (unsigned) (((int64_t) (c.n_rows / 16 + 2 * c.n_seq) * ((c.n_head_kv + per - 1) / per) * parts + 7) / 8); }
+size_t tile_smem(const b200_kv4 & c) { return (size_t) (c.n_seq + 1) * 4; }
 template <typename T> void append_as(const b200_kv4 & c, const Cache & d, const void * k, int64_t kr, int64_t kh, const void * v, int64_t vr, int64_t vh) {
-    const bool whole = aligned(k, 4 * sizeof(T)) && aligned(v, 4 * sizeof(T)) && !((kr | kh | vr | vh) & 3);
-    const int64_t threads = (int64_t) c.n_rows * c.n_head_kv * (c.head_dim / 4);
-    const auto go = [&](auto kernel) { launch(kernel, dim3((unsigned) ((threads + 255) / 256)), 256, 0, c.stream, false, 1, d, static_cast<const T *>(k), kr, kh, static_cast<const T *>(v), vr, vh, whole); };
-    c.head_dim == 128 ? go(k_kv4_append<T, 128>) : go(k_kv4_append<T, 64>);
+    const RowSrc<T> src = {static_cast<const T *>(k), kr, kh, static_cast<const T *>(v), vr, vh, aligned(k, 4 * sizeof(T)) && aligned(v, 4 * sizeof(T)) && !((kr | kh | vr | vh) & 3)};
+    const auto rows = [&](auto kernel) { launch(kernel, dim3(row_blocks(c)), 256, 0, c.stream, false, 1, d, src, row_parts(c)); };
+    const auto tiles = [&](auto kernel) { launch(kernel, dim3(tile_blocks(c, 2)), 256, tile_smem(c), c.stream, false, 1, d, src); };
+    if (by_tiles(c)) c.head_dim == 128 ? tiles(k_kv4_append_tiles<T, 128>) : tiles(k_kv4_append_tiles<T, 64>);
+    else if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv4_append<T, 128, 1>) : rows(k_kv4_append<T, 64, 1>);
+    else c.head_dim == 128 ? rows(k_kv4_append<T, 128, 4>) : rows(k_kv4_append<T, 64, 4>);
 }
 template <typename T> void read_as(const b200_kv4 & c, const Cache & d, void * k, void * v) {
-    const int64_t threads = (int64_t) c.n_rows * c.n_head_kv * (c.head_dim / 4);
-    const auto go = [&](auto kernel) { launch(kernel, dim3((unsigned) ((threads + 255) / 256)), 256, 0, c.stream, false, 1, d, static_cast<T *>(k), static_cast<T *>(v)); };
-    c.head_dim == 128 ? go(k_kv4_read<T, 128>) : go(k_kv4_read<T, 64>);
+    T * ko = static_cast<T *>(k), * vo = static_cast<T *>(v);
+    const auto rows = [&](auto kernel) { launch(kernel, dim3(row_blocks(c)), 256, 0, c.stream, false, 1, d, ko, vo, row_parts(c)); };
+    const auto tiles = [&](auto kernel) { launch(kernel, dim3(tile_blocks(c, 1)), 256, tile_smem(c), c.stream, false, 1, d, ko, vo); };
+    if (by_tiles(c)) c.head_dim == 128 ? tiles(k_kv4_read_tiles<T, 128>) : tiles(k_kv4_read_tiles<T, 64>);
+    else if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv4_read<T, 128, 1>) : rows(k_kv4_read<T, 64, 1>);
+    else c.head_dim == 128 ? rows(k_kv4_read<T, 128, 4>) : rows(k_kv4_read<T, 64, 4>);
 }
 
 // attention of few rows: column tiles of 8 (one or two side by side)

@@ -72,6 +72,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __
 
 // four entries in one access where `whole` says that they stand on their own alignment
 template <typename T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
+template <typename T> struct alignas(2 * sizeof(T)) Two { T v[2]; };
 template <typename T> __device__ __forceinline__ void load4(const T * p, bool whole, float (&x)[4]) {
     if (whole) {
         const Four<T> f = *reinterpret_cast<const Four<T> *>(p);
@@ -83,101 +84,277 @@ template <typename T> __device__ __forceinline__ void load4(const T * p, bool wh
     }
 }
 
-// codes of four entries (lowest bits first) and the scale of their block, which eight neighbouring lanes share
-template <typename T> __device__ __forceinline__ uint32_t quantize4(const float (&x)[4], bool whole, float & scale) {
-    float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+// the larger of each side of a pair of T, a NaN where one is: (-smallest, largest) of a block go through the lanes as one word
+template <typename T> __device__ __forceinline__ uint32_t pair_max(uint32_t x, uint32_t y);
+template <> __device__ __forceinline__ uint32_t pair_max<__half>(uint32_t x, uint32_t y) { uint32_t r; asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y)); return r; }
+template <> __device__ __forceinline__ uint32_t pair_max<__nv_bfloat16>(uint32_t x, uint32_t y) { uint32_t r; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y)); return r; }
+__device__ __forceinline__ float max_nan(float x, float y) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y)); return r; }
+
+// of the block of 32 that eight neighbouring lanes share: whether it is finite, and its scale
+template <typename T> __device__ __forceinline__ bool block_scale(const float (&x)[4], float & d) {
+    float lo = max_nan(max_nan(-x[0], -x[1]), max_nan(-x[2], -x[3])), hi = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));      // lo: turned round
+    if constexpr (sizeof(T) == 2) {
+        Two<T> p = {{from_f<T>(lo), from_f<T>(hi)}};                      // (entries of T: exact)
+        uint32_t w = *reinterpret_cast<uint32_t *>(&p);
 #pragma unroll
-    for (int m = 1; m < 8; m <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+        for (int m = 1; m < 8; m <<= 1) w = pair_max<T>(w, __shfl_xor_sync(0xffffffffu, w, m));
+        p = *reinterpret_cast<Two<T> *>(&w);
+        lo = to_f(p.v[0]); hi = to_f(p.v[1]);
+    } else {
+#pragma unroll
+        for (int m = 1; m < 8; m <<= 1) {
+            lo = max_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+        }
     }
-    float d = (-lo >= hi ? lo : hi) * -0.125f;
+    d = (lo >= hi ? -lo : hi) * -0.125f;
     d = fminf(fmaxf(d, -8160.f), 8160.f);
-    d = __half2float(__float2half_rn(__bfloat162float(__float2bfloat16_rn(d))));
-    if (!whole || d == 0.f) { scale = 0.f; return 0x8888u; }
-    scale = d;
-    uint32_t codes = 0;
+    d = __half2float(__float2half_rn(__bfloat162float(__float2bfloat16_rn(d)))) + 0.f;
+    return lo < INFINITY && hi < INFINITY;
+}
+// codes of four entries of a block of scale d, lowest bits first
+template <typename T> __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float d) {
+    const float by = __fdividef(1.f, d);
+    float c[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float q = __fdiv_rn(x[i], d);
-        float r = rintf(q);
-        // 24-bit entries: a quotient that was rounded to a half lies on one side of it. (n + 1/2) d has 13 bits, so the remainder is exact. Entries of 11 or 8 bits are never that near
-        if (sizeof(T) == 4 && fabsf(q - truncf(q)) == 0.5f) {
-            const float rest = fmaf(-q, d, x[i]);
-            if (rest != 0.f) r = (rest > 0.f) == (d > 0.f) ? ceilf(q) : floorf(q);
+        if constexpr (sizeof(T) == 2) {
+            // rint(x / d): the quotient, put right by its remainder, is exact where x / d is a half, and no other quotient of 11 and 8 bits is as near to one as its rounding
+            const float q = x[i] * by, r = fmaf(fmaf(-q, d, x[i]), by, q);
+            c[i] = fminf(fmaxf(r, -8.f), 7.f) + 12582912.f - 12582912.f;       // 1.5 x 2^23: rounds to a whole number
+        } else {
+            // with 24 bits a quotient may round to a half that it is not. The remainder of the nearest code tells the neighbour: where it is about d / 2 it is exact
+            const float half = 0.5f * fabsf(d), t = fmaf(x[i], by, 12582912.f), rest = fmaf(-(t - 12582912.f), d, x[i]);
+            c[i] = t - 12582912.f;
+            if (fabsf(rest) > half || (fabsf(rest) == half && (__float_as_int(t) & 1))) c[i] += (rest > 0.f) == (d > 0.f) ? 1.f : -1.f;
+            c[i] = fminf(fmaxf(c[i], -8.f), 7.f);
         }
-        codes |= (uint32_t) (__float2int_rn(fminf(fmaxf(r, -8.f), 7.f)) + 8) << (4 * i);
     }
-    return codes;
+    // c0 + 16 c1 + 256 c2 + 4096 c3 + 8 x 0x1111, below 2^16, as last bits
+    const uint32_t w = __float_as_uint(fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0]))) + (8388608.f + 34952.f)) & 0xffffu;
+    return d == 0.f ? 0x8888u : w;
 }
 
-// HD / 4 lanes a row and head, four entries each. Memory bounds it: rows are read once, 4.5 bits a number are written.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_kv4_append(const Cache c, const T * k, int64_t k_row, int64_t k_head, const T * v, int64_t v_row, int64_t v_head, bool whole4) {
-    constexpr int LANES = HD / 4, NB = HD / 32;
-    const int64_t item = ((int64_t) blockIdx.x * blockDim.x + threadIdx.x) / LANES;
-    const int li = threadIdx.x % LANES;
-    const bool in = item < (int64_t) c.n_rows * c.n_kv;
-    const int row = in ? (int) (item / c.n_kv) : 0, head = in ? (int) (item % c.n_kv) : 0;
-    const int s = in ? seq_of_row(c, row) : -1;
-    int page = -1, pos = 0;
-    if (s >= 0) {
-        const Seq q = seq_at(c, s);
-        pos = q.held + row - q.begin;
-        page = page_at(c, q.slot, pos);
+// the sequence of a row, looked for by a whole warp, 32 places at a time; -1: none
+__device__ __forceinline__ int seq_of_row_warp(const Cache & c, int row) {
+    const int lane = threadIdx.x & 31;
+    int s = 0, n = c.n_seq;
+    while (n > 1) {
+        const int step = (n + 31) >> 5, i = s + lane * step;
+        const unsigned m = __ballot_sync(0xffffffffu, lane * step < n && c.first[min(i, c.n_seq)] <= row);
+        const int k = m ? 31 - __clz(m) : 0;
+        s += k * step;
+        n = min(step, n - k * step);
     }
-    float xk[4] = {}, xv[4] = {};
-    if (page >= 0) {
-        load4(k + row * k_row + head * k_head + 4 * li, whole4, xk);
-        load4(v + row * v_row + head * v_head + 4 * li, whole4, xv);
+    return c.first[s] <= row && row < c.first[s + 1] ? s : -1;
+}
+
+// where a lane's four entries of token t stand in a tile: 16-bit units of K and V codes, and the scale of their block
+template <int HD> __device__ __forceinline__ int k_unit(int li, int t) { return 2 * ((((t >> 3) * 8 + 2 * (t & 3) + (t >> 2 & 1)) * 4 + ((li & 7) >> 1)) * (HD / 32) + (li >> 3)) + (li & 1); }
+template <int HD> __device__ __forceinline__ int v_unit(int li, int t) { return ((((li >> 4) * 8 + (li & 7)) * 4 + (t & 3)) * 2 + (li >> 3 & 1)) * 4 + (t >> 2); }
+template <int HD> __device__ __forceinline__ int k_scale_at(int li, int t) { return (((t & 3) * 2 + (t >> 2 & 1)) * 2 + (t >> 3)) * (HD / 32) + (li >> 3); }
+template <int HD> __device__ __forceinline__ int v_scale_at(int li, int t) { return ((t & 3) * (HD / 32) + (li >> 3)) * 4 + (t >> 2); }
+
+template <typename T> struct RowSrc { const T * k; int64_t k_row, k_head; const T * v; int64_t v_row, v_head; bool whole4; };
+// codes and scales of one row and head, HD / 4 lanes of four entries each
+struct Codes { uint32_t k, v; float dk, dv; };
+template <typename T, int HD> __device__ __forceinline__ Codes codes_of(const float (&xk)[4], const float (&xv)[4]) {
+    Codes r;
+    const bool fine_k = block_scale<T>(xk, r.dk), fine_v = block_scale<T>(xv, r.dv);
+    const unsigned mine = HD == 128 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+    const bool fine = (__ballot_sync(0xffffffffu, fine_k && fine_v) & mine) == mine;
+    r.k = fine ? codes4<T>(xk, r.dk) : 0x8888u;
+    r.v = fine ? codes4<T>(xv, r.dv) : 0x8888u;
+    if (!fine) { r.dk = NAN; r.dv = 0.f; }
+    return r;
+}
+template <int HD> __device__ __forceinline__ void put_scales(uint8_t * tile, int li, int t, const Codes & q) {
+    if ((li & 7) == 0) {
+        reinterpret_cast<__half *>(tile + 16 * HD)[k_scale_at<HD>(li, t)] = __float2half_rn(q.dk);
+        reinterpret_cast<__half *>(tile + 17 * HD)[v_scale_at<HD>(li, t)] = __float2half_rn(q.dv);
     }
-    bool fine = true;
+}
+
+// Few rows of each sequence: a warp a row and PASSES passes of its heads (a head at head_dim 128, two at 64), all asked for together. Latency bounds it: row -> sequence -> slot -> page.
+template <typename T, int HD, int PASSES>
+__global__ void __launch_bounds__(256) k_kv4_append(const Cache c, const RowSrc<T> src, int parts) {
+    constexpr int LANES = HD / 4, PER = 32 / LANES;
+    const int64_t item = ((int64_t) blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    const int lane = threadIdx.x & 31, li = lane % LANES, row = (int) (item / parts), h0 = (int) (item % parts) * PASSES * PER + lane / LANES;
+    if (row >= c.n_rows) return;
+    float xk[PASSES][4] = {}, xv[PASSES][4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; i++) fine = fine && isfinite(xk[i]) && isfinite(xv[i]);
-    const unsigned mine = LANES == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
-    fine = (__ballot_sync(0xffffffffu, fine) & mine) == mine;
-    float dk, dv;
-    const uint32_t ck = quantize4<T>(xk, fine, dk), cv = quantize4<T>(xv, fine, dv);
-    if (page < 0) return;
-    const int t = pos & 15, tc = t & 3, ti = t >> 2, b = li >> 3, e = li & 7;
-    uint8_t * tile = c.pool + tile_offset(c, page, head, pos, 18 * HD);
-    reinterpret_cast<uint16_t *>(tile)[2 * ((((ti >> 1) * 8 + 2 * tc + (ti & 1)) * 4 + (e >> 1)) * NB + b) + (e & 1)] = (uint16_t) ck;
-    reinterpret_cast<uint16_t *>(tile + 8 * HD)[((((b >> 1) * 8 + e) * 4 + tc) * 2 + (b & 1)) * 4 + ti] = (uint16_t) cv;
-    if (e == 0) {
-        reinterpret_cast<__half *>(tile + 16 * HD)[((tc * 2 + (ti & 1)) * 2 + (ti >> 1)) * NB + b] = __float2half_rn(fine ? dk : NAN);
-        reinterpret_cast<__half *>(tile + 17 * HD)[(tc * NB + b) * 4 + ti] = __float2half_rn(dv);
+    for (int i = 0; i < PASSES; i++) {
+        const int head = h0 + i * PER;
+        if (head < c.n_kv) {
+            load4(src.k + row * src.k_row + head * src.k_head + 4 * li, src.whole4, xk[i]);
+            load4(src.v + row * src.v_row + head * src.v_head + 4 * li, src.whole4, xv[i]);
+        }
     }
-}
-
-// the rows' positions read back: out [n_rows][n_kv][HD]; a position without a page reads 0
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_kv4_read(const Cache c, T * k, T * v) {
-    constexpr int LANES = HD / 4, NB = HD / 32;
-    const int64_t item = ((int64_t) blockIdx.x * blockDim.x + threadIdx.x) / LANES;
-    if (item >= (int64_t) c.n_rows * c.n_kv) return;
-    const int li = threadIdx.x % LANES, row = (int) (item / c.n_kv), head = (int) (item % c.n_kv), s = seq_of_row(c, row);
+    const int s = seq_of_row_warp(c, row);
     if (s < 0) return;
     const Seq q = seq_at(c, s);
-    const int pos = q.held + row - q.begin, page = page_at(c, q.slot, pos);
-    float dk = 0.f, dv = 0.f;
-    uint32_t ck = 0, cv = 0;
-    if (page >= 0) {
-        const int t = pos & 15, tc = t & 3, ti = t >> 2, b = li >> 3, e = li & 7;
-        const uint8_t * tile = c.pool + tile_offset(c, page, head, pos, 18 * HD);
-        ck = reinterpret_cast<const uint16_t *>(tile)[2 * ((((ti >> 1) * 8 + 2 * tc + (ti & 1)) * 4 + (e >> 1)) * NB + b) + (e & 1)];
-        cv = reinterpret_cast<const uint16_t *>(tile + 8 * HD)[((((b >> 1) * 8 + e) * 4 + tc) * 2 + (b & 1)) * 4 + ti];
-        dk = __half2float(reinterpret_cast<const __half *>(tile + 16 * HD)[((tc * 2 + (ti & 1)) * 2 + (ti >> 1)) * NB + b]);
-        dv = __half2float(reinterpret_cast<const __half *>(tile + 17 * HD)[(tc * NB + b) * 4 + ti]);
-    }
-    Four<T> fk, fv;
+    const int pos = q.held + row - q.begin, page = page_at(c, q.slot, pos), t = pos & 15;
+    if (page < 0) return;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        fk.v[i] = from_f<T>((float) ((int) (ck >> (4 * i) & 15) - 8) * dk);
-        fv.v[i] = from_f<T>((float) ((int) (cv >> (4 * i) & 15) - 8) * dv);
+    for (int i = 0; i < PASSES; i++) {
+        const Codes r = codes_of<T, HD>(xk[i], xv[i]);
+        const int head = h0 + i * PER;
+        if (head < c.n_kv) {
+            uint8_t * tile = c.pool + tile_offset(c, page, head, pos, 18 * HD);
+            reinterpret_cast<uint16_t *>(tile)[k_unit<HD>(li, t)] = (uint16_t) r.k;
+            reinterpret_cast<uint16_t *>(tile + 8 * HD)[v_unit<HD>(li, t)] = (uint16_t) r.v;
+            put_scales<HD>(tile, li, t, r);
+        }
+        __syncwarp();
     }
-    const size_t at = ((size_t) row * c.n_kv + head) * HD + 4 * li;
-    *reinterpret_cast<Four<T> *>(k + at) = fk;
-    *reinterpret_cast<Four<T> *>(v + at) = fv;
+}
+
+// Many rows: a warp half a tile of a head (two at head_dim 64), whose tiles are counted over the sequences by every block. Four tokens are asked for together; a whole half tile's V codes leave
+// as 4 bytes a lane, one that the step fills in part is written entry by entry.
+struct TileItem { int slot, row, pos, lo, hi; };      // rows row + lo .. row + hi - 1 are tokens lo .. hi - 1 of the tile at pos (a multiple of 16)
+__device__ __forceinline__ int tiles_of(const Seq & q) { return q.count ? ((q.held + q.count - 1) >> 4) - (q.held >> 4) + 1 : 0; }
+__device__ __forceinline__ TileItem tile_item(const Cache & c, int item, int * before) {
+    __shared__ int sums[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (c.n_seq + 255) / 256, s0 = min(c.n_seq, tid * each), s1 = min(c.n_seq, s0 + each);
+    int mine = 0;
+    for (int s = s0; s < s1; s++) { before[s] = mine; mine += tiles_of(seq_at(c, s)); }
+    int up = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) { const int x = __shfl_up_sync(0xffffffffu, up, d); if (lane >= d) up += x; }
+    if (lane == 31) sums[warp] = up;
+    __syncthreads();
+    int off = up - mine;
+    for (int w = 0; w < warp; w++) off += sums[w];
+    for (int s = s0; s < s1; s++) before[s] += off;
+    if (tid == 255) before[c.n_seq] = off + mine;
+    __syncthreads();
+    TileItem r = {-1, 0, 0, 0, 0};
+    if (item >= before[c.n_seq]) return r;
+    int s = 0;
+    for (int hi = c.n_seq; hi - s > 1;) { const int mid = (s + hi) >> 1; if (before[mid] <= item) s = mid; else hi = mid; }
+    const Seq q = seq_at(c, s);
+    r.slot = q.slot;
+    r.pos = ((q.held >> 4) + item - before[s]) << 4;
+    r.lo = max(0, q.held - r.pos);
+    r.hi = min(16, q.held + q.count - r.pos);
+    r.row = q.begin + r.pos - q.held;
+    return r;
+}
+template <typename T, int HD>
+__global__ void __launch_bounds__(256, 4) k_kv4_append_tiles(const Cache c, const RowSrc<T> src) {
+    constexpr int LANES = HD / 4, PER = 32 / LANES;
+    extern __shared__ int tile_before[];                           // [n_seq + 1]
+    const int lane = threadIdx.x & 31, li = lane % LANES, groups = (c.n_kv + PER - 1) / PER;
+    const int64_t item = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5);
+    const TileItem r = tile_item(c, (int) (item / (2 * groups)), tile_before);
+    const int t0 = item & 1 ? 8 : 0, lo = max(r.lo, t0), hi = min(r.hi, t0 + 8);
+    if (lo >= hi) return;
+    const int head = (int) (item / 2 % groups) * PER + lane / LANES;
+    const bool in = head < c.n_kv;
+    const int page = page_at(c, r.slot, r.pos);
+    if (page < 0) return;
+    uint8_t * tile = c.pool + tile_offset(c, page, in ? head : 0, r.pos, 18 * HD);
+    const T * k = src.k + (int64_t) (r.row + t0) * src.k_row + head * src.k_head + 4 * li, * v = src.v + (int64_t) (r.row + t0) * src.v_row + head * src.v_head + 4 * li;
+    uint32_t vc[4] = {};                                           // [token % 4] codes of tokens t0 + 0, 4
+#pragma unroll 1
+    for (int b = 0; b < 2; b++) {
+        float xk[4][4] = {}, xv[4][4] = {};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = t0 + 4 * b + i;
+            if (in && t >= lo && t < hi) { load4(k + i * src.k_row, src.whole4, xk[i]); load4(v + i * src.v_row, src.whole4, xv[i]); }
+        }
+        k += 4 * src.k_row; v += 4 * src.v_row;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = t0 + 4 * b + i;
+            const Codes q = codes_of<T, HD>(xk[i], xv[i]);
+            if (in && t >= lo && t < hi) {
+                reinterpret_cast<uint16_t *>(tile)[k_unit<HD>(li, t)] = (uint16_t) q.k;
+                put_scales<HD>(tile, li, t, q);
+                if (hi - lo < 8) reinterpret_cast<uint16_t *>(tile + 8 * HD)[v_unit<HD>(li, t)] = (uint16_t) q.v;
+            }
+            vc[i] |= q.v << (16 * b);
+        }
+    }
+    if (in && hi - lo == 8)
+#pragma unroll
+        for (int i = 0; i < 4; i++) *reinterpret_cast<uint32_t *>(tile + 8 * HD + 2 * v_unit<HD>(li, t0 + i)) = vc[i];
+}
+
+template <typename T> __device__ __forceinline__ Four<T> held_values(uint32_t codes, float d) {
+    Four<T> f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) f.v[i] = from_f<T>((float) ((int) (codes >> (4 * i) & 15) - 8) * d);
+    return f;
+}
+// the rows' positions read back: out [n_rows][n_kv][HD]; a position without a page reads 0. As the two above
+template <typename T, int HD, int PASSES>
+__global__ void __launch_bounds__(256) k_kv4_read(const Cache c, T * k, T * v, int parts) {
+    constexpr int LANES = HD / 4, PER = 32 / LANES;
+    const int64_t item = ((int64_t) blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    const int lane = threadIdx.x & 31, li = lane % LANES, row = (int) (item / parts), h0 = (int) (item % parts) * PASSES * PER + lane / LANES;
+    if (row >= c.n_rows) return;
+    const int s = seq_of_row_warp(c, row);
+    if (s < 0) return;
+    const Seq q = seq_at(c, s);
+    const int pos = q.held + row - q.begin, page = page_at(c, q.slot, pos), t = pos & 15;
+    uint32_t ck[PASSES] = {}, cv[PASSES] = {};
+    float dk[PASSES] = {}, dv[PASSES] = {};
+#pragma unroll
+    for (int i = 0; i < PASSES; i++) {
+        const int head = h0 + i * PER;
+        if (page >= 0 && head < c.n_kv) {
+            const uint8_t * tile = c.pool + tile_offset(c, page, head, pos, 18 * HD);
+            ck[i] = reinterpret_cast<const uint16_t *>(tile)[k_unit<HD>(li, t)];
+            cv[i] = reinterpret_cast<const uint16_t *>(tile + 8 * HD)[v_unit<HD>(li, t)];
+            dk[i] = __half2float(reinterpret_cast<const __half *>(tile + 16 * HD)[k_scale_at<HD>(li, t)]);
+            dv[i] = __half2float(reinterpret_cast<const __half *>(tile + 17 * HD)[v_scale_at<HD>(li, t)]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; i++) {
+        const int head = h0 + i * PER;
+        if (head < c.n_kv) {
+            const size_t at = ((size_t) row * c.n_kv + head) * HD + 4 * li;
+            *reinterpret_cast<Four<T> *>(k + at) = held_values<T>(ck[i], dk[i]);
+            *reinterpret_cast<Four<T> *>(v + at) = held_values<T>(cv[i], dv[i]);
+        }
+    }
+}
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) k_kv4_read_tiles(const Cache c, T * k, T * v) {
+    constexpr int LANES = HD / 4, PER = 32 / LANES;
+    extern __shared__ int tile_before[];
+    const int lane = threadIdx.x & 31, li = lane % LANES, groups = (c.n_kv + PER - 1) / PER;
+    const int64_t item = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5);
+    const TileItem r = tile_item(c, (int) (item / groups), tile_before);
+    const int head = (int) (item % groups) * PER + lane / LANES;
+    if (r.hi == 0 || head >= c.n_kv) return;
+    const int page = page_at(c, r.slot, r.pos);
+    const uint8_t * tile = c.pool + tile_offset(c, max(page, 0), head, r.pos, 18 * HD);
+    uint2 vc[4] = {};
+    uint32_t kc[16] = {};
+    float dk[16] = {}, dv[16] = {};
+    if (page >= 0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) vc[i] = *reinterpret_cast<const uint2 *>(tile + 8 * HD + 2 * v_unit<HD>(li, i));
+#pragma unroll
+        for (int t = 0; t < 16; t++) {
+            kc[t] = reinterpret_cast<const uint16_t *>(tile)[k_unit<HD>(li, t)];
+            dk[t] = __half2float(reinterpret_cast<const __half *>(tile + 16 * HD)[k_scale_at<HD>(li, t)]);
+            dv[t] = __half2float(reinterpret_cast<const __half *>(tile + 17 * HD)[v_scale_at<HD>(li, t)]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 16; t++) {
+        if (t < r.lo || t >= r.hi) continue;
+        const size_t at = ((size_t) (r.row + t) * c.n_kv + head) * HD + 4 * li;
+        const uint32_t w = t >> 3 ? vc[t & 3].y : vc[t & 3].x;
+        *reinterpret_cast<Four<T> *>(k + at) = held_values<T>(kc[t], dk[t]);
+        *reinterpret_cast<Four<T> *>(v + at) = held_values<T>(t >> 2 & 1 ? w >> 16 : w & 0xffffu, dv[t]);
+    }
 }
 
 }  // namespace srv

@@ -86,7 +86,7 @@ def assert_attends(case, seen, q, out, window=0, scale=None):
 # ---- writing and reading -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("page,held,counts", [(16, [0, 3, 15, 16, 40], [1, 1, 1, 1, 1]), (32, [7, 0, 31], [20, 1, 70]), (64, [100, 1], [1, 0]), (16, [2], [16])])
+@pytest.mark.parametrize("page,held,counts", [(16, [0, 3, 15, 16, 40], [1, 1, 1, 1, 1]), (32, [7, 0, 31], [20, 1, 70]), (64, [100, 1], [1, 0]), (16, [2], [16]), (32, [5, 0, 16], [60, 1, 33]), (16, [15, 0], [50, 0])])
 def test_append_writes_the_definition(hd, dtype, page, held, counts):
     c = Case(held, counts, page=page, kv=3, hd=hd, seed=hd + page)
     c.pool.copy_(torch.randint(0, 256, c.pool.shape, generator=c.gen, device="cuda", dtype=torch.uint8))
