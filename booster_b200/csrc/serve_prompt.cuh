@@ -2,10 +2,12 @@
 //
 // A unit of work is 256 columns of a sequence (a column is a row and a query head of one KV head) over the tiles of 128 tokens that they see. As for few rows, all units stand in one
 // line that is cut evenly, here over one block per SM; k_kv4_prompt_plan lays the line out, k_kv4_prompt_join adds the parts of units that blocks shared.
-//   warps 0-3, 4-7   soft-max of columns 0-127 and 128-255, a thread a column: maximum and exponentials of its row of S, P back into tensor memory in the place of S
-//   warps 8-11       codes of 32 tokens each to fp16 in shared memory (exact: a scale has 8 bits, a code 4), K by rows of tokens, V by rows of dims, both with 128-byte swizzle
-//   warp 12          (of 12-15: registers are shared out by four warps: 128 a thread at launch, then 168, 168, 112 and 64) one thread issues S = Q K^T (128 x 128 x head_dim, twice) and O += P V (P from tensor memory, 128 x head_dim x 128, twice)
-// While one half's soft-max runs, the other half's products do. Tensor memory: S and P [2][128 columns], O [2][head_dim].
+//   warps 0-3, 4-7   soft-max of columns 0-127 and 128-255, a thread a column, 64 tokens at a time: its row of S into registers, maximum, exponentials, P back into tensor memory in the
+//                    place of S
+//   warps 8-11       codes of 32 tokens each, copied ahead, to fp16 in shared memory (exact: a scale has 8 bits, a code 4), K by rows of tokens, V by rows of dims, both with 128-byte swizzle
+//   warp 12          (of 12-15: registers are shared out by four warps, 128 a thread at launch, then 168, 168, 112 and 64) one thread issues S = Q K^T (128 x 64 x head_dim) and
+//                    O += P V (P from tensor memory, 128 x head_dim x 64) of both halves
+// Tensor memory: S and P [2 halves][2 turns][64 columns], O [2][head_dim]. Each half has two turns of S, so that the scores of the next 64 tokens are there when those in hand are done with.
 // Tokens of 32 stand as n = 8 c + 4 u + i for token 16 u + c + 4 i in S, P, K and V alike, and dims of 8 as 0 4 1 5 2 6 3 7 in Q and K: the orders in which a word's codes come apart.
 // P is rounded to fp16 (2^-11), q scaled by a power of two into fp16's range; sums are fp32. The maximum moves when a score passes it by 2^8; O is scaled in tensor memory then.
 // Every wait on an mbarrier is bounded: on a timeout the block raises *err, skips what is left and frees its tensor memory.
@@ -29,7 +31,7 @@ constexpr uint64_t PR_DESC = (1ull << 16) | ((uint64_t) (1024u >> 4) << 32) | (1
 __host__ __device__ constexpr uint32_t pr_idesc(int n) { return (1u << 4) | ((uint32_t) (n >> 3) << 17) | (8u << 24); }     // D f32, A and B f16, M = 128
 template <int HD> struct PromptSmem {
     static constexpr int Q = 128 * HD * 2, KV = PR_KV * HD * 2;      // bytes of one half of Q, of a tile's K or V
-    static constexpr int BYTES = 2 * Q + 4 * KV + 1024;              // K and V in two stages each
+    static constexpr int BYTES = 2 * Q + 4 * KV + 4 * 36 * HD + 1024;      // K and V in two stages each, a tile's codes as they come
 };
 
 __device__ __forceinline__ void pr_wait(uint32_t bar, uint32_t parity, bool & dead) {
@@ -57,18 +59,10 @@ __device__ __forceinline__ void pr_mma_ss(uint32_t d, uint64_t da, uint64_t db, 
 __device__ __forceinline__ void pr_mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" :: "r"(d), "r"(a), "l"(db), "r"(idesc), "r"(acc) : "memory");
 }
+// 32 columns of a warp's lanes, there when the statement ends: nothing can be put between the load and the wait for it
 __device__ __forceinline__ void pr_ld32(uint32_t at, uint32_t (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-                   "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-                   "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(at) : "memory");
-}
-// the registers hold what was loaded behind this
-__device__ __forceinline__ void pr_ld32_wait(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
-                   "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
-                   "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(at) : "memory");
 }
 __device__ __forceinline__ void pr_st32(uint32_t at, const uint32_t (&r)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
@@ -76,10 +70,9 @@ __device__ __forceinline__ void pr_st32(uint32_t at, const uint32_t (&r)[32]) {
                     "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
                     "r"(r[30]), "r"(r[31]), "r"(at) : "memory");
 }
-__device__ __forceinline__ void pr_st16(uint32_t at, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
-                 :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-                    "r"(r[15]), "r"(at) : "memory");
+__device__ __forceinline__ void pr_ld64(uint32_t at, uint32_t (&r)[64]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]) : "r"(at) : "memory");
 }
 __device__ __forceinline__ void pr_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pr_st_shared(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -184,7 +177,7 @@ template <int HD, typename T>
 __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p) {
     constexpr int NB = HD / 32, TILE = 18 * HD, QB = PromptSmem<HD>::Q, KVB = PromptSmem<HD>::KV, SUB = 128 * 128;      // SUB: 128 rows of 128 bytes
     extern __shared__ uint8_t pr_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+    __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_full[2][2];      // [half][turn]
     __shared__ uint32_t tmem_s;
     const AttendArgs & a = p.a;
     const Cache & c = a.c;
@@ -192,7 +185,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
     const uint32_t smem = (smem_at(pr_raw) + 1023u) & ~1023u, q_s = smem, k_s = q_s + 2 * QB, v_s = k_s + 2 * KVB;
     if (tid == 0) {
         const auto init = [](uint64_t * b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(smem_at(b)), "r"(n) : "memory"); };
-        for (int i = 0; i < 2; i++) { init(&q_full[i], 4); init(&k_full[i], 4); init(&v_full[i], 4); init(&k_empty[i], 1); init(&v_empty[i], 1); init(&s_full[i], 1); init(&p_full[i], 4); init(&o_full[i], 1); }
+        for (int i = 0; i < 2; i++) { init(&q_full[i], 4); init(&k_full[i], 4); init(&v_full[i], 4); init(&k_empty[i], 1); init(&v_empty[i], 1); for (int b = 0; b < 2; b++) { init(&s_full[i][b], 1); init(&p_full[i][b], 4); init(&o_full[i][b], 1); } }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -238,33 +231,33 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
         regs_more<168>();
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;          // of the half
         const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, my_s = t_s + lanes + half * 128, my_o = t_o + lanes + half * HD;
-        int n_s = 0;                                                       // tiles of this half so far
+        int n_s = 0;                                                       // steps of 64 tokens of this half so far
         for (Segment g; segment(g);) {
             const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
             const bool in = i < g.q.count;
             if (half >= g.halves) continue;
             // the warp's 32 queries, HD / 8 lanes a row: each scaled by a power of two to at most 2^14, dims of eight as 0 4 1 5 2 6 3 7
-            constexpr int LANES = HD / 8, ROWS = 32 / LANES;
+            constexpr int LANES = HD / 8, ROWS = 32 / LANES, X = 8;
             float factor = 0.f;
             {
                 const int64_t mine = in ? (g.q.begin + i) * a.q_row + h * a.q_head : -1;
                 const int m = lane % LANES;
 #pragma unroll 1
-                for (int x0 = 0; x0 < 32; x0 += 8 * ROWS) {
-                    uint4 f[8];
-                    int64_t from[8];
+                for (int x0 = 0; x0 < 32; x0 += X * ROWS) {
+                    uint4 f[X];
+                    int64_t from[X];
 #pragma unroll
-                    for (int x = 0; x < 8; x++) { from[x] = __shfl_sync(0xffffffffu, mine, x0 + x * ROWS + lane / LANES); f[x] = make_uint4(0, 0, 0, 0); }
+                    for (int x = 0; x < X; x++) { from[x] = __shfl_sync(0xffffffffu, mine, x0 + x * ROWS + lane / LANES); f[x] = make_uint4(0, 0, 0, 0); }
                     const T * src = static_cast<const T *>(a.q) + 8 * m;
                     if (a.q_whole) {
 #pragma unroll
-                        for (int x = 0; x < 8; x++) if (from[x] >= 0) f[x] = *reinterpret_cast<const uint4 *>(src + from[x]);
+                        for (int x = 0; x < X; x++) if (from[x] >= 0) f[x] = *reinterpret_cast<const uint4 *>(src + from[x]);
                     } else {
 #pragma unroll
-                        for (int x = 0; x < 8; x++) if (from[x] >= 0) f[x] = eight_apart(src + from[x]);
+                        for (int x = 0; x < X; x++) if (from[x] >= 0) f[x] = eight_apart(src + from[x]);
                     }
 #pragma unroll
-                    for (int x = 0; x < 8; x++) {
+                    for (int x = 0; x < X; x++) {
                         const int r = x0 + x * ROWS + lane / LANES;
                         float top = 0.f;
 #pragma unroll
@@ -298,53 +291,45 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
             const int all_see_hi = g.q.held + row_lo, all_see_lo = a.window > 0 ? g.q.held + row_hi - a.window + 1 : 0;
             const int top_pos = in ? g.q.held + i : -1, low_pos = a.window > 0 ? top_pos - a.window : -1;      // sees low_pos < position <= top_pos
             float m = -INFINITY, l = 0.f, base = 0.f, limit = -INFINITY;
-            for (int t = g.t0; t < g.t1; t++, n_s++) {
-                const int pos = (g.sp.lo + t) * PR_KV;
-                const bool edge = !whole || pos + PR_KV - 1 > all_see_hi || pos < all_see_lo;
-                unsigned there = 0xffu;                                    // tiles of 16 tokens that have a page
-                if (!whole) there = __ballot_sync(0xffffffffu, lane < 8 && page_at(c, g.q.slot, pos + 16 * (lane & 7)) >= 0);
-                pr_wait(smem_at(&s_full[half]), (uint32_t) (n_s & 1), dead);
+            for (int t = 2 * g.t0; t < 2 * g.t1; t++, n_s++) {
+                const int pos = g.sp.lo * PR_KV + 64 * t;
+                const uint32_t at = my_s + 64 * (n_s & 1);
+                const bool edge = !whole || pos + 63 > all_see_hi || pos < all_see_lo;
+                unsigned there = 0xfu;                                     // tiles of 16 tokens that have a page
+                if (!whole) there = __ballot_sync(0xffffffffu, lane < 4 && page_at(c, g.q.slot, pos + 16 * (lane & 3)) >= 0);
+                pr_wait(smem_at(&s_full[half][n_s & 1]), (uint32_t) (n_s >> 1 & 1), dead);
                 __syncwarp();
                 pr_fence_after();
-                uint32_t r[2][32];                                         // 32 columns in hand, the next 32 on their way
-                if (edge) {                                                // what a column does not see goes to -infinity, in place
-#pragma unroll 1
-                    for (int ch = 0; ch < 4; ch++) {
-                        const int hi = top_pos - pos - 32 * ch, lo = low_pos - pos - 32 * ch;
-                        const unsigned pages = there >> 2 * ch;
-                        pr_ld32(my_s + 32 * ch, r[0]);
-                        pr_ld32_wait(r[0]);
+                uint32_t r[64];
+                pr_ld64(at, r);
+                if (edge) {                                                // what a column does not see goes to -infinity
+                    const int hi = top_pos - pos, lo = low_pos - pos;
 #pragma unroll
-                        for (int x = 0; x < 32; x++)
-                            if (token_of(x) > hi || token_of(x) <= lo || !(pages >> (x >> 2 & 1) & 1)) r[0][x] = 0xff800000u;
-                        pr_st32(my_s + 32 * ch, r[0]);
+                    for (int x = 0; x < 64; x++) {
+                        const int token = (x & 32) + token_of(x & 31);
+                        if (token > hi || token <= lo || !(there >> (token >> 4) & 1)) r[x] = 0xff800000u;
                     }
-                    pr_st_wait();
                 }
                 float x0 = -INFINITY, x1 = -INFINITY;
-                pr_ld32(my_s + 96, r[1]);
 #pragma unroll
-                for (int ch = 3; ch >= 0; ch--) {
-                    pr_ld32_wait(r[ch & 1]);
-                    if (ch) pr_ld32(my_s + 32 * (ch - 1), r[(ch - 1) & 1]);
-#pragma unroll
-                    for (int x = 0; x < 32; x += 2) { x0 = fmaxf(x0, __uint_as_float(r[ch & 1][x])); x1 = fmaxf(x1, __uint_as_float(r[ch & 1][x + 1])); }
+                for (int x = 0; x < 64; x += 4) {
+                    x0 = fmaxf(x0, fmaxf(__uint_as_float(r[x]), __uint_as_float(r[x + 1])));
+                    x1 = fmaxf(x1, fmaxf(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3])));
                 }
                 const float high = fmaxf(x0, x1), score = high == -INFINITY ? high : high * factor;
                 if (__any_sync(0xffffffffu, score > limit)) {
                     const float top = fmaxf(m, score), down = top > m ? exp2_fast(m - top) : 1.f;
-                    if (t > g.t0 && __any_sync(0xffffffffu, down != 1.f)) {
-                        pr_wait(smem_at(&o_full[half]), (uint32_t) ((n_s - 1) & 1), dead);
+                    if (t > 2 * g.t0 && __any_sync(0xffffffffu, down != 1.f)) {
+                        pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), dead);
                         __syncwarp();
                         pr_fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (int ch = 0; ch < HD / 32; ch++) {
-                            uint32_t r[32];
-                            pr_ld32(my_o + 32 * ch, r);
-                            pr_ld32_wait(r);
+                            uint32_t y[32];
+                            pr_ld32(my_o + 32 * ch, y);
 #pragma unroll
-                            for (int x = 0; x < 32; x++) r[x] = __float_as_uint(__uint_as_float(r[x]) * down);
-                            pr_st32(my_o + 32 * ch, r);
+                            for (int x = 0; x < 32; x++) y[x] = __float_as_uint(__uint_as_float(y[x]) * down);
+                            pr_st32(my_o + 32 * ch, y);
                         }
                     }
                     m = top;
@@ -354,40 +339,31 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 }
                 const uint64_t by = two(factor, factor), less = two(-base, -base);
                 uint64_t sum = 0;
-                pr_ld32(my_s + 32, r[1]);
+                uint32_t w[32];
 #pragma unroll
-                for (int ch = 0; ch < 4; ch++) {                           // (the first 32 columns are still there)
-                    uint32_t w[16];
-#pragma unroll
-                    for (int x = 0; x < 32; x += 2) {
-                        const float2 y = split(fma2(two(__uint_as_float(r[ch & 1][x]), __uint_as_float(r[ch & 1][x + 1])), by, less));
-                        const float e0 = exp2_fast(y.x), e1 = exp2_fast(y.y);
-                        sum = add2(sum, two(e0, e1));
-                        w[x / 2] = as_u(__floats2half2_rn(e0, e1));
-                    }
-                    if (ch < 3) {
-                        pr_ld32_wait(r[(ch + 1) & 1]);
-                        if (ch < 2) pr_ld32(my_s + 32 * (ch + 2), r[ch & 1]);
-                    }
-                    pr_st16(my_s + 16 * ch, w);
+                for (int x = 0; x < 64; x += 2) {
+                    const float2 y = split(fma2(two(__uint_as_float(r[x]), __uint_as_float(r[x + 1])), by, less));
+                    const float e0 = exp2_fast(y.x), e1 = exp2_fast(y.y);
+                    sum = add2(sum, two(e0, e1));
+                    w[x / 2] = as_u(__floats2half2_rn(e0, e1));
                 }
+                pr_st32(at, w);
                 l += split(sum).x + split(sum).y;
                 pr_st_wait();
                 pr_fence_before();
                 __syncwarp();
-                if (lane == 0) pr_arrive(smem_at(&p_full[half]));
+                if (lane == 0) pr_arrive(smem_at(&p_full[half][n_s & 1]));
             }
-            pr_wait(smem_at(&o_full[half]), (uint32_t) ((n_s - 1) & 1), dead);
+            pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), dead);
             __syncwarp();
             pr_fence_after();
             const bool final = g.t0 == 0 && g.t1 == g.sp.n;
             const float inv = l != 0.f ? 1.f / l : 0.f;
-            const size_t part = 2 * (size_t) blockIdx.x + (g.t0 == 0 ? 1 : 0);      // parts are [HD / 4][256 columns][4]: a warp's stores are contiguous
+            const size_t piece = 2 * (size_t) blockIdx.x + (g.t0 == 0 ? 1 : 0);      // parts are [HD / 4][256 columns][4]: a warp's stores are contiguous
 #pragma unroll
             for (int ch = 0; ch < HD / 32; ch++) {
                 uint32_t r[32];
                 pr_ld32(my_o + 32 * ch, r);
-                pr_ld32_wait(r);
                 if (in && !dead) {
                     if (final) {
                         T * y = static_cast<T *>(a.out) + ((size_t) (g.q.begin + i) * c.n_kv * a.group + h) * HD + 32 * ch;
@@ -399,112 +375,107 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                             *reinterpret_cast<Eight<T> *>(y + x) = f;
                         }
                     } else {
-                        uint4 * y = reinterpret_cast<uint4 *>(a.part + part * PR_COLS * HD) + (size_t) (8 * ch) * PR_COLS + half * 128 + row;
+                        uint4 * y = reinterpret_cast<uint4 *>(a.part + piece * PR_COLS * HD) + (size_t) (8 * ch) * PR_COLS + half * 128 + row;
 #pragma unroll
                         for (int x = 0; x < 8; x++) y[x * PR_COLS] = make_uint4(r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]);
                     }
                 }
                 __syncwarp();
             }
-            if (in && !final) *reinterpret_cast<float2 *>(a.ml + (part * PR_COLS + half * 128 + row) * 2) = make_float2(m, l);
+            if (in && !final) *reinterpret_cast<float2 *>(a.ml + (piece * PR_COLS + half * 128 + row) * 2) = make_float2(m, l);
             pr_fence_before();
         }
     } else if (warp < 12) {
         regs_less<112>();
         const int w = warp - 8, g8 = lane >> 2, tq = lane & 3, tc = g8 >> 1, te = g8 & 1;
         int n = 0;                                                         // tiles so far
+        const uint32_t raw_s = v_s + 2 * KVB + (uint32_t) (w * 2 * TILE);
+        const uint8_t * raw = pr_raw + (raw_s - smem_at(pr_raw));
         for (Segment g; segment(g);) {
-            int pages_from = 0, my_page = 0, turned = -1;
-            uint4 kr[2][NB / 2], vr[2][NB / 2], ks[2], vs[2][NB / 2];
-            const auto place = [&](int t, int u) -> const uint8_t * {      // of 16 tokens
-                const int pos = (g.sp.lo + t) * PR_KV + 32 * w + 16 * u, pi = pos >> c.page_log2;
-                if (turned < 0 || pi - pages_from >= 32) { turned = 0; pages_from = pi; my_page = page_at(c, g.q.slot, (pi + lane) << c.page_log2); }
-                const int page = __shfl_sync(0xffffffffu, my_page, pi - pages_from);
-                return page >= 0 ? c.pool + tile_offset(c, page, g.head, pos, TILE) : nullptr;
+            int pages_from = 0, my_page = 0;
+            bool turned = false;
+            const auto page_of = [&](int pos) {
+                const int pi = pos >> c.page_log2;
+                if (!turned || pi - pages_from >= 32) { turned = true; pages_from = pi; my_page = page_at(c, g.q.slot, (pi + lane) << c.page_log2); }
+                return __shfl_sync(0xffffffffu, my_page, pi - pages_from);
             };
-            const auto ask_k = [&](const uint8_t * const (&src)[2]) {
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const uint4 none = make_uint4(0, 0, 0, 0);
-                    if constexpr (NB == 4) {
-#pragma unroll
-                        for (int j = 0; j < 2; j++) kr[u][j] = src[u] ? reinterpret_cast<const uint4 *>(src[u])[32 * j + lane] : none;
-                        ks[u] = src[u] ? reinterpret_cast<const uint4 *>(src[u] + 16 * HD)[g8] : none;
-                    } else {
-                        const uint2 x = src[u] ? reinterpret_cast<const uint2 *>(src[u])[lane] : make_uint2(0, 0), y = src[u] ? reinterpret_cast<const uint2 *>(src[u])[32 + lane] : make_uint2(0, 0);
-                        kr[u][0] = make_uint4(x.x, x.y, y.x, y.y);
-                        const uint2 z = src[u] ? reinterpret_cast<const uint2 *>(src[u] + 16 * HD)[g8] : make_uint2(0, 0);
-                        ks[u] = make_uint4(z.x, z.y, 0, 0);
-                    }
-                }
+            const auto ask = [&](int t) {                                  // the warp's 32 tokens, zeros where there is no page
+                const int pos = (g.sp.lo + t) * PR_KV + 32 * w, page_a = page_of(pos), page_b = page_of(pos + 16);
+                PairSrc src;
+                src.bytes_a = page_a >= 0 ? 16 : 0;
+                src.bytes_b = page_b >= 0 ? 16 : 0;
+                src.a = c.pool + (page_a >= 0 ? tile_offset(c, page_a, g.head, pos, TILE) : 0) + 16 * lane;
+                src.b = c.pool + (page_b >= 0 ? tile_offset(c, page_b, g.head, pos + 16, TILE) - TILE : 0) + 16 * lane;
+                const bool first = lane < TILE % 512 / 16;
+                src.mid = first ? src.a : src.b; src.bytes_mid = first ? src.bytes_a : src.bytes_b;
+                copy_pair<HD>(raw_s + 16 * lane, src, lane);
             };
-            const auto ask_v = [&](const uint8_t * const (&src)[2]) {
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int j = 0; j < NB / 2; j++) {
-                        const uint4 none = make_uint4(0, 0, 0, 0);
-                        vr[u][j] = src[u] ? reinterpret_cast<const uint4 *>(src[u] + 8 * HD)[32 * j + lane] : none;
-                        vs[u][j] = src[u] ? reinterpret_cast<const uint4 *>(src[u] + 17 * HD)[NB / 2 * tq + j] : none;
-                    }
-            };
-            const uint8_t * src[2] = {place(g.t0, 0), place(g.t0, 1)};
-            ask_k(src);
-            ask_v(src);
+            ask(g.t0);
             for (int t = g.t0; t < g.t1; t++, n++) {
                 const int stage = n & 1;
                 const uint32_t round = (uint32_t) (n >> 1);
-                if (t + 1 < g.t1) { src[0] = place(t + 1, 0); src[1] = place(t + 1, 1); }
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 if (n >= 2) pr_wait(smem_at(&k_empty[stage]), (round - 1) & 1, dead);
                 __syncwarp();
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++) {
+                    const uint8_t * tile = raw + u * TILE;
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         const int row = 32 * w + 8 * tc + 4 * u + 2 * j + te;
+                        uint32_t words[NB], scales[NB / 2];
+                        if constexpr (NB == 4) {
+                            const uint4 x = reinterpret_cast<const uint4 *>(tile)[32 * j + lane];
+                            const uint2 z = reinterpret_cast<const uint2 *>(tile + 16 * HD)[2 * g8 + j];
+                            words[0] = x.x; words[1] = x.y; words[2] = x.z; words[3] = x.w; scales[0] = z.x; scales[1] = z.y;
+                        } else {
+                            const uint2 x = reinterpret_cast<const uint2 *>(tile)[32 * j + lane];
+                            words[0] = x.x; words[1] = x.y; scales[0] = reinterpret_cast<const uint32_t *>(tile + 16 * HD)[2 * g8 + j];
+                        }
 #pragma unroll
                         for (int b = 0; b < NB; b++) {
-                            const uint4 x = NB == 4 ? kr[u][j & (NB / 2 - 1)] : kr[u][0];
-                            const uint32_t word = NB == 4 ? (b == 0 ? x.x : b == 1 ? x.y : b == 2 ? x.z : x.w) : (2 * j + b == 0 ? x.x : 2 * j + b == 1 ? x.y : 2 * j + b == 2 ? x.z : x.w);
-                            const int sw = NB == 4 ? 2 * j + b / 2 : j;
-                            const __half2 sc = as_h2(sw == 0 ? ks[u].x : sw == 1 ? ks[u].y : sw == 2 ? ks[u].z : ks[u].w), d = b & 1 ? __high2half2(sc) : __low2half2(sc);
+                            const __half2 sc = as_h2(scales[b >> 1]), d = b & 1 ? __high2half2(sc) : __low2half2(sc);
                             uint32_t v[4];
-                            codes8(word, v);
+                            codes8(words[b], v);
 #pragma unroll
                             for (int x4 = 0; x4 < 4; x4++) v[x4] = as_u(__hmul2(as_h2(v[x4]), d));
                             pr_st_shared(k_s + stage * KVB + (b >> 1) * SUB + row * 128 + (((4 * (b & 1) + tq) ^ (row & 7)) << 4), v[0], v[1], v[2], v[3]);
                         }
                     }
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) pr_arrive(smem_at(&k_full[stage]));
-                if (t + 1 < g.t1) ask_k(src);
                 if (n >= 2) pr_wait(smem_at(&v_empty[stage]), (round - 1) & 1, dead);
                 __syncwarp();
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    uint32_t v[2][2][4];
+                for (int bb = 0; bb < NB / 2; bb++) {
+                    uint4 y[2], z[2];
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                    for (int u = 0; u < 2; u++) { y[u] = reinterpret_cast<const uint4 *>(raw + u * TILE + 8 * HD)[32 * bb + lane]; z[u] = reinterpret_cast<const uint4 *>(raw + u * TILE + 17 * HD)[NB / 2 * tq + bb]; }
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const uint4 x = vr[u][b >> 1], z = vs[u][b >> 1];
-                            const uint32_t word = b & 1 ? (e ? x.w : x.z) : (e ? x.y : x.x);
-                            const __half2 d = as_h2(b & 1 ? (e ? z.w : z.z) : (e ? z.y : z.x));
-                            codes8(word, v[u][e]);
+                    for (int b = 2 * bb; b < 2 * bb + 2; b++) {
+                        uint32_t v[2][2][4];
 #pragma unroll
-                            for (int x4 = 0; x4 < 4; x4++) v[u][e][x4] = as_u(__hmul2(as_h2(v[u][e][x4]), d));
+                        for (int u = 0; u < 2; u++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                codes8(b & 1 ? (e ? y[u].w : y[u].z) : (e ? y[u].y : y[u].x), v[u][e]);
+                                const __half2 d = as_h2(b & 1 ? (e ? z[u].w : z[u].z) : (e ? z[u].y : z[u].x));
+#pragma unroll
+                                for (int x4 = 0; x4 < 4; x4++) v[u][e][x4] = as_u(__hmul2(as_h2(v[u][e][x4]), d));
+                            }
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            const int row = 32 * b + 4 * g8 + x;
+                            pr_st_shared(v_s + stage * KVB + (w >> 1) * (HD * 128) + row * 128 + (((4 * (w & 1) + tq) ^ (row & 7)) << 4), v[0][0][x], v[0][1][x], v[1][0][x], v[1][1][x]);
                         }
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        const int row = 32 * b + 4 * g8 + x;
-                        pr_st_shared(v_s + stage * KVB + (w >> 1) * (HD * 128) + row * 128 + (((4 * (w & 1) + tq) ^ (row & 7)) << 4), v[0][0][x], v[0][1][x], v[1][0][x], v[1][1][x]);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) pr_arrive(smem_at(&v_full[stage]));
-                if (t + 1 < g.t1) ask_v(src);
+                if (t + 1 < g.t1) ask(t + 1);
             }
         }
     } else {
@@ -512,47 +483,49 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
         int n = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
         for (Segment g; warp == 12 && segment(g);) {
             if (pr_elect()) {
-                const int tiles = g.t1 - g.t0;
-                const auto scores = [&](int half, int stage) {             // S = Q K^T of a half
+                const int steps = 2 * (g.t1 - g.t0);
+                const auto scores = [&](int half, int step) {              // S = Q K^T of a half and 64 tokens
+                    const int turn = step & 1;
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++)
-                        pr_mma_ss(t_s + half * 128, PR_DESC | (uint64_t) ((q_s + half * QB + (k >> 2) * SUB) >> 4) + 2 * (k & 3), PR_DESC | (uint64_t) ((k_s + stage * KVB + (k >> 2) * SUB) >> 4) + 2 * (k & 3),
-                                  pr_idesc(128), k > 0);
-                    pr_commit(smem_at(&s_full[half]));
+                        pr_mma_ss(t_s + half * 128 + 64 * turn, PR_DESC | (uint64_t) ((q_s + half * QB + (k >> 2) * SUB) >> 4) + 2 * (k & 3),
+                                  PR_DESC | (uint64_t) ((k_s + (n + (step >> 1) & 1) * KVB + (k >> 2) * SUB + turn * (SUB / 2)) >> 4) + 2 * (k & 3), pr_idesc(64), k > 0);
+                    pr_commit(smem_at(&s_full[half][turn]));
                 };
                 for (int half = 0; half < g.halves; half++) pr_wait(smem_at(&q_full[half]), (uint32_t) (n_q[half] & 1), dead);
                 pr_wait(smem_at(&k_full[n & 1]), (uint32_t) (n >> 1 & 1), dead);
                 pr_fence_after();
                 if (!dead) {
-                    for (int half = 0; half < g.halves; half++) scores(half, n & 1);
+                    for (int step = 0; step < 2; step++)
+                        for (int half = 0; half < g.halves; half++) scores(half, step);
                     pr_commit(smem_at(&k_empty[n & 1]));
                 }
-                for (int t = 0; t < tiles; t++) {
-                    const int now = n + t, stage = now & 1, after = (now + 1) & 1;
-                    pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), dead);
+                for (int step = 0; step < steps; step++) {
+                    const int turn = step & 1, now = n + (step >> 1), stage = now & 1, after = (now + 1) & 1;
+                    if (turn == 0) pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), dead);
                     for (int half = 0; half < g.halves; half++) {
-                        pr_wait(smem_at(&p_full[half]), (uint32_t) ((n_p[half] + t) & 1), dead);
+                        pr_wait(smem_at(&p_full[half][turn]), (uint32_t) ((n_p[half] + step) >> 1 & 1), dead);
                         pr_fence_after();
                         if (!dead) {
 #pragma unroll
-                            for (int k = 0; k < PR_KV / 16; k++)
-                                pr_mma_ts(t_o + half * HD, t_s + half * 128 + 8 * k, PR_DESC | (uint64_t) ((v_s + stage * KVB + (k >> 2) * (HD * 128)) >> 4) + 2 * (k & 3), pr_idesc(HD), t > 0 || k > 0);
-                            pr_commit(smem_at(&o_full[half]));
+                            for (int k = 0; k < 4; k++)
+                                pr_mma_ts(t_o + half * HD, t_s + half * 128 + 64 * turn + 8 * k, PR_DESC | (uint64_t) ((v_s + stage * KVB + turn * (HD * 128)) >> 4) + 2 * k, pr_idesc(HD), step > 0 || k > 0);
+                            pr_commit(smem_at(&o_full[half][turn]));
                         }
-                        if (t + 1 < tiles) {
-                            if (half == 0) { pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), dead); pr_fence_after(); }
+                        if (step + 2 < steps) {
+                            if (turn == 0 && half == 0) { pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), dead); pr_fence_after(); }
                             if (!dead) {
-                                scores(half, after);
-                                if (half == g.halves - 1) pr_commit(smem_at(&k_empty[after]));
+                                scores(half, step + 2);
+                                if (turn == 1 && half == g.halves - 1) pr_commit(smem_at(&k_empty[after]));
                             }
                         }
                     }
-                    if (!dead) pr_commit(smem_at(&v_empty[stage]));
+                    if (turn == 1 && !dead) pr_commit(smem_at(&v_empty[stage]));
                 }
             }
             __syncwarp();
             n += g.t1 - g.t0;
-            for (int half = 0; half < g.halves; half++) { n_q[half]++; n_p[half] += g.t1 - g.t0; }
+            for (int half = 0; half < g.halves; half++) { n_q[half]++; n_p[half] += 2 * (g.t1 - g.t0); }
         }
     }
     if (dead) {
