@@ -19,7 +19,7 @@ namespace srv {
 
 namespace cg = cooperative_groups;
 
-constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 512, SA_FINE = 1024, SA_LIST = 2048, SA_SHORT = SA_THREADS, SA_MAX_CLUSTER = 8, SA_MAX_VOCAB = 1 << 18, SA_SWEEPS = SA_MAX_VOCAB / SA_MAX_CLUSTER / SA_THREADS / 4;
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 512, SA_FINE = 512, SA_LIST = 2048, SA_SHORT = SA_THREADS, SA_MAX_CLUSTER = 8, SA_MAX_VOCAB = 1 << 18, SA_SWEEPS = SA_MAX_VOCAB / SA_MAX_CLUSTER / SA_THREADS / 4;
 constexpr float SA_PER_NAT = 16.f;
 constexpr double SA_ONE = 1099511627776.0;                               // 2^40
 typedef unsigned long long u64;
@@ -34,21 +34,21 @@ struct SampleArgs {
     float * logprobs;
 };
 
-// 2^40 exp(-x), x >= 0, to the nearest whole number, for y = -16 x log2(e) and whether x < 30 (beyond that it is 0): y = n + f with |f| <= 1 / 2: a table's 2^(n mod 16 / 16), whose 16
-// entries are the 32 banks of shared memory, times 2^(n / 16) times the series of exp(f ln 2 / 16), whose first term left out is below 2^-42
+// 2^40 exp(d steps ln 2 / 16), d <= 0, to the nearest whole number, or 0: y = d steps = n + f with |f| <= 1 / 2, so a table's 2^(n mod 16 / 16), whose 16 entries are the 32 banks of
+// shared memory, times 2^(n / 16) times the series of exp(f ln 2 / 16), whose first term left out is below 2^-42. What is left out has its upper word cleared, which adds nothing to 2^52
 constexpr double SA_LN = 0.69314718055994530942 / 16;
 __constant__ double sa_series[5] = {SA_LN, SA_LN * SA_LN / 2, SA_LN * SA_LN * SA_LN / 6, SA_LN * SA_LN * SA_LN * SA_LN / 24, SA_LN * SA_LN * SA_LN * SA_LN * SA_LN / 120};
-__device__ __forceinline__ u64 fixed_weight(double y, bool near, const double * table) {
-    constexpr double WHOLE = 6755399441055744.0;                         // 1.5 x 2^52: added, the last bits are a whole number
-    const double t = y + WHOLE, f = y - (t - WHOLE);
+__device__ __forceinline__ u64 fixed_weight(double d, double steps, bool in, const double * table) {
+    constexpr double WHOLE = 6755399441055744.0, WIDE = 4503599627370496.0;      // 1.5 x 2^52 and 2^52: added, the last bits are a whole number
+    const double t = fma(d, steps, WHOLE), f = fma(d, steps, WHOLE - t);
     const int n = __double2loint(t);
     double p = fma(sa_series[4], f, sa_series[3]);
     p = fma(p, f, sa_series[2]);
     p = fma(p, f, sa_series[1]);
     p = fma(p, f, sa_series[0]);
     p = fma(p, f, 1.0) * table[n & 15];
-    p = __hiloint2double(__double2hiint(p) + ((40 + (n >> 4)) << 20), __double2loint(p)) + 4503599627370496.0;      // 2^52
-    return near ? (u64) __double_as_longlong(p) & 0xfffffffffffffull : 0;
+    p = __hiloint2double(in ? __double2hiint(p) + ((n & ~15) << 16) + (40 << 20) : 0, __double2loint(p)) + WIDE;
+    return (u64) __double_as_longlong(p) - 0x4330000000000000ull;
 }
 
 // (logit, index) as one number: larger is earlier in the order
@@ -66,6 +66,10 @@ template <typename F> __device__ __forceinline__ u64 warp_reduce(u64 x, F f) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, d));
     return x;
+}
+// sums below 2^54 each, as whole numbers of 27 bits
+__device__ __forceinline__ u64 warp_sum(u64 x) {
+    return (u64) __reduce_add_sync(0xffffffffu, (uint32_t) x & 0x7ffffffu) + ((u64) __reduce_add_sync(0xffffffffu, (uint32_t) (x >> 27)) << 27);
 }
 struct alignas(128) SampleSmem {
     double table[16];
@@ -221,21 +225,21 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         if (rank == 0 && tid == 0) finish(top == -INFINITY ? -1 : i, top == -INFINITY ? -INFINITY : 0.f);
         return;
     }
-    const auto below = [&](float v) { return v == top ? 0.f : top - v; };                       // how far a logit is from the largest, to a float
-    const auto exactly = [&](float v) { return v == top ? 0.0 : (double) top - (double) v; };
-    // y = 16 log2(e) (v - largest), over the temperature or not: by one fma where its rounding, a factor common to all of a row's weights, is small (2^-23 at most), else from the difference
-    const double cold = 1.0 / (double) temperature, steps = 1.0 / SA_LN, steps_cold = steps * cold;
-    const bool direct = fabsf(top) < SA_FAR && fabs((double) top * steps_cold) < 1073741824.0;
-    const double from_top = -(double) top * steps, from_top_cold = -(double) top * steps_cold;
-    const float cold_f = (float) cold;
-    const auto weight = [&](float v) { return fixed_weight(direct ? fma((double) v, steps, from_top) : -exactly(v) * steps, below(v) < 30.f, sm.table); };
-    const auto tempered = [&](float v) {
-        const float d = below(v);
-        return fixed_weight(direct ? fma((double) v, steps_cold, from_top_cold) : d == 0.f ? 0.0 : -exactly(v) * steps_cold, d == 0.f || d * cold_f < 30.f, sm.table);
-    };
-    const double far = min_p > 0.f ? -log((double) min_p) : INFINITY;    // min-p keeps what is at most so far below the largest
-    const float far_f = (float) far * 1.00001f + 1e-30f;
-    const auto near_enough = [&](float v) { return below(v) <= far_f && exactly(v) <= far; };
+    const auto exactly = [&](float v) { return v == top ? 0.0 : (double) top - (double) v; };   // how far a logit is from the largest
+    // Weights are 0 from 28.5 (x temperature) below the largest on, so that the cut at 30, in floats, decides nothing. (An infinity as the largest: only others like it have a weight.)
+    constexpr float MOST = 3.402823466e38f;
+    const double cold = 1.0 / (double) temperature, steps = 1.0 / SA_LN, steps_cold = steps * cold, top_d = (double) fminf(top, MOST);
+    const float from_1 = fmaxf((float) ((double) top - 30.0), -MOST), from_t = fmaxf((float) ((double) top - 30.0 * (double) temperature), -MOST);
+    const auto weight = [&](float v) { return fixed_weight((double) fminf(v, MOST) - top_d, steps, v >= from_1, sm.table); };
+    const auto tempered = [&](float v, bool in) { return fixed_weight((double) fminf(v, MOST) - top_d, steps_cold, in, sm.table); };
+    // min-p keeps the logits from from_p on, the smallest float that is at most -log(min_p) below the largest
+    float from_p = -INFINITY;
+    if (min_p > 0.f) {
+        const double far = -log((double) min_p);
+        from_p = fminf((float) ((double) top - far), top);
+        for (int j = 0; j < 4 && exactly(from_p) > far; j++) from_p = nextafterf(from_p, INFINITY);
+        for (int j = 0; j < 4 && exactly(nextafterf(from_p, -INFINITY)) <= far; j++) from_p = nextafterf(from_p, -INFINITY);
+    }
     const auto log_share = [&](double x, u64 total) { return (float) (-(x == 0.0 ? 0.0 : x * cold) - log((double) total * (1.0 / SA_ONE))); };
     const auto target_of = [&](u64 total) { const double at = (double) u * (double) total; return at >= (double) total ? total - 1 : at > 0.0 ? (u64) at : 0; };
     u64 edge = 0;                                                        // tokens of keys >= edge are kept by top-k and top-p
@@ -257,9 +261,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     // the tokens for which f holds, to the lists of the first `takers` blocks
     const auto gather = [&](int takers, auto f) {
         each([&](const float (&v)[4], int i) {
+            bool in[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) in[e] = f(v[e]) & (i + e < n);
+            if (!(in[0] | in[1] | in[2] | in[3])) return;
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (f(v[e]) && i + e < n)
+                if (in[e])
                     for (int r = 0; r < takers; r++) {
                         const int at = atomicAdd(&cl.map_shared_rank(&sm, r)->n_list, 1);
                         if (at < SA_LIST) cl.map_shared_rank(list, r)[at] = order_key(v[e], base + i + e);
@@ -310,7 +318,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             if (rank) return;
             const int m = sm.n_list;
             if (m <= SA_SHORT) {                                         // a thread a token, which goes through all of them twice
-                u64 * w_of = fine, * t_of = fine + SA_SHORT;
+                u64 * w_of = fine, * t_of = fine + SA_SHORT;                 // (over the counts and the bins, which all blocks have read)
+                static_assert(16 * SA_SHORT <= 12 * SA_FINE + 4 * SA_BINS, "two numbers a token");
                 const u64 mine = tid < m ? list[tid] : 0, w = tid < m ? weight(key_logit(mine)) : 0;
                 w_of[tid] = w;
                 __syncthreads();
@@ -321,8 +330,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                     for (int j = 0; j < m; j++) { const bool first = list[j] > mine; before_me += first; c += first ? w_of[j] : 0; }
                 if (tid < m && before_me == min(k, m) - 1) sm.answer[0] = c + w;
                 __syncthreads();
-                const bool in = tid < m && before_me < k && (before_me == 0 || !by_p || (double) c < (double) top_p * (double) sm.answer[0]) && near_enough(key_logit(mine));
-                const u64 t = in ? tempered(key_logit(mine)) : 0;
+                const bool in = tid < m && before_me < k && (before_me == 0 || !by_p || (double) c < (double) top_p * (double) sm.answer[0]) && key_logit(mine) >= from_p;
+                const u64 t = tempered(key_logit(mine), in && key_logit(mine) >= from_t);
                 t_of[tid] = t;
                 __syncthreads();
                 if (in) {
@@ -342,7 +351,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             const double share = (double) top_p * (double) all;
             for (int i = i0; i < min(i1, k); i++) {                      // a token is kept while the sum in front of it is short of the share; the first always is
                 const u64 w = weight(key_logit(list[i]));
-                kept += (i == 0 || !by_p || (double) c < share) && near_enough(key_logit(list[i]));
+                kept += (i == 0 || !by_p || (double) c < share) && (key_logit(list[i]) >= from_p);
                 c += w;
             }
             block_before64(kept, all, sm.red);
@@ -357,13 +366,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             sort_padded(n_kept);
             const int d0 = min(n_kept, tid * per), d1 = min(n_kept, d0 + per);
             u64 sum = 0;
-            for (int i = d0; i < d1; i++) sum += tempered(__uint_as_float((uint32_t) list[i]));
+            for (int i = d0; i < d1; i++) { const float v = __uint_as_float((uint32_t) list[i]); sum += tempered(v, v >= from_t); }
             c = block_before64(sum, all, sm.red);
             const u64 target = target_of(all);
             if (c <= target && target < c + sum) {
                 for (int i = d0; i < d1; i++) {
                     const float v = __uint_as_float((uint32_t) list[i]);
-                    c += tempered(v);
+                    c += tempered(v, v >= from_t);
                     if (c > target) { finish((int) ~(uint32_t) (list[i] >> 32), log_share(exactly(v), all)); break; }
                 }
             }
@@ -384,19 +393,22 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             // all weights, those in front of the bins, and those in the bins by finer ones
             const float from = b_lo ? v_hi : top, by = SA_FINE * SA_PER_NAT / (float) (b_hi - b_lo + 1);
             const auto fine_place = [&](float v) { return fminf((from - v) * by, (float) (SA_FINE - 1)); };       // its whole part is the finer bin
-            const auto between = [&](float v) { return v >= v_lo && v < v_hi; };
+            const auto between = [&](float v) { return (v >= v_lo) & (v < v_hi); };
             for (int i = tid; i < SA_FINE; i += SA_THREADS) { fine[i] = 0; fine_count[i] = 0; }
             __syncthreads();
             u64 all = 0, in_front = 0;
             each([&](const float (&v)[4], int i) {
+                u64 w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = weight(v[e]);
+                all += w[0] + w[1] + (w[2] + w[3]);
+                if (!((v[0] >= v_lo) | (v[1] >= v_lo) | (v[2] >= v_lo) | (v[3] >= v_lo))) return;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const u64 w = weight(v[e]);
-                    all += w;
-                    in_front += v[e] >= v_hi ? w : 0;
-                    if (between(v[e]) && i + e < n) {
+                    in_front += v[e] >= v_hi ? w[e] : 0;
+                    if (between(v[e]) & (i + e < n)) {
                         const int b = (int) fine_place(v[e]);
-                        atomicAdd(&fine[b], w);
+                        atomicAdd(&fine[b], w[e]);
                         atomicAdd(&fine_count[b], 1);
                     }
                 }
@@ -409,33 +421,21 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             all = in_front = 0;
             for (int r = 0; r < blocks; r++) { all += sm.sums[r][0]; in_front += sm.sums[r][1]; }
             const double want = (double) top_p * (double) all;
-            u64 w[2] = {0, 0};
-            int fc[2] = {0, 0};
+            u64 w = 0, x[SA_MAX_CLUSTER];
+            int fc = 0, y[SA_MAX_CLUSTER];
 #pragma unroll
-            for (int r0 = 0; r0 < SA_MAX_CLUSTER; r0 += 4) {
-                ulonglong2 x[4];
-                int2 y[4];
+            for (int r = 0; r < SA_MAX_CLUSTER; r++) { const int o = r < blocks ? r : 0; x[r] = cl.map_shared_rank(fine, o)[tid]; y[r] = cl.map_shared_rank(fine_count, o)[tid]; }
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int o = r0 + r < blocks ? r0 + r : 0;
-                    x[r] = reinterpret_cast<const ulonglong2 *>(cl.map_shared_rank(fine, o))[tid];
-                    y[r] = reinterpret_cast<const int2 *>(cl.map_shared_rank(fine_count, o))[tid];
-                }
-#pragma unroll
-                for (int r = 0; r < 4; r++) if (r0 + r < blocks) { w[0] += x[r].x; w[1] += x[r].y; fc[0] += y[r].x; fc[1] += y[r].y; }
-            }
-            u64 c = in_front + block_before64(w[0] + w[1], counted, sm.red);
+            for (int r = 0; r < SA_MAX_CLUSTER; r++) if (r < blocks) { w += x[r]; fc += y[r]; }
+            u64 c = in_front + block_before64(w, counted, sm.red);
             if (tid == 0) sm.answer[0] = SA_FINE;
             __syncthreads();
-            for (int j = 0; j < 2; j++) {
-                if ((double) c < want && (double) (c + w[j]) >= want) { sm.answer[0] = 2 * tid + j; sm.answer[1] = c; sm.answer[2] = fc[j]; }
-                c += w[j];
-            }
+            if ((double) c < want && (double) (c + w) >= want) { sm.answer[0] = tid; sm.answer[1] = c; sm.answer[2] = fc; }
             __syncthreads();
             const int f_bin = (int) sm.answer[0];
             c = sm.answer[1];
             if (f_bin < SA_FINE && sm.answer[2] <= SA_LIST) {
-                gather(blocks, [&](float v) { const float at = fine_place(v); return between(v) && at >= (float) f_bin && at < (float) (f_bin + 1); });
+                gather(blocks, [&](float v) { const float at = fine_place(v); return between(v) & (at >= (float) f_bin) & (at < (float) (f_bin + 1)); });
                 const int m = sm.n_list;
                 if (m <= SA_SHORT) {
                     const u64 mine = tid < m ? list[tid] : 0, w_mine = tid < m ? weight(key_logit(mine)) : 0;
@@ -467,23 +467,18 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         }
     }
     // the draw: sums of 128 neighbouring tokens, a warp's at a time, which stand in order of index
-    const float edge_logit = edge ? key_logit(edge) : -INFINITY;
+    const float edge_logit = edge ? key_logit(edge) : -INFINITY, from = fmaxf(fmaxf(from_t, from_p), edge_logit);
     const int edge_index = edge ? key_index(edge) : 0x7fffffff;
     const auto drawn = [&](const float (&v)[4], int i, u64 (&w)[4]) {
-        bool in[4], some = false;
+        bool in[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            in[e] = below(v[e]) <= far_f && (v[e] > edge_logit || (v[e] == edge_logit && base + i + e <= edge_index));
-            some = some || in[e];
-            w[e] = 0;
-        }
-        if (!some) return;
+        for (int e = 0; e < 4; e++) { in[e] = v[e] >= from; w[e] = 0; }
+        if (!(in[0] | in[1] | in[2] | in[3])) return;
+        if ((v[0] == edge_logit) | (v[1] == edge_logit) | (v[2] == edge_logit) | (v[3] == edge_logit))
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (min_p > 0.f) in[e] = in[e] && exactly(v[e]) <= far;
-            const u64 t = tempered(v[e]);
-            w[e] = in[e] ? t : 0;
-        }
+            for (int e = 0; e < 4; e++) in[e] = in[e] & ((v[e] != edge_logit) | (base + i + e <= edge_index));
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = tempered(v[e], in[e]);
     };
     const int sweeps = (groups + SA_THREADS - 1) / SA_THREADS;
     for (int s = 0; s < sweeps; s++) {
@@ -496,7 +491,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             drawn(v, 4 * g, w);
             sum = w[0] + w[1] + w[2] + w[3];
         }
-        if (__any_sync(0xffffffffu, sum != 0)) sum = warp_reduce(sum, add);
+        if (__any_sync(0xffffffffu, sum != 0)) sum = warp_sum(sum);
         if (lane == 0) sm.parts[s][warp] = sum;
     }
     __syncthreads();
