@@ -258,16 +258,16 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         }
         return lo;
     };
-    // the tokens for which f holds, to the lists of the first `takers` blocks
-    const auto gather = [&](int takers, auto f) {
+    // the tokens of logits lo to hi for which f holds, to the lists of the first `takers` blocks
+    const auto gather = [&](int takers, float lo, float hi, auto f) {
         each([&](const float (&v)[4], int i) {
             bool in[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) in[e] = f(v[e]) & (i + e < n);
+            for (int e = 0; e < 4; e++) in[e] = (v[e] >= lo) & (v[e] <= hi);
             if (!(in[0] | in[1] | in[2] | in[3])) return;
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (in[e])
+                if (in[e] && f(v[e]) && i + e < n)
                     for (int r = 0; r < takers; r++) {
                         const int at = atomicAdd(&cl.map_shared_rank(&sm, r)->n_list, 1);
                         if (at < SA_LIST) cl.map_shared_rank(list, r)[at] = order_key(v[e], base + i + e);
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         const float v_hi = b_lo ? place_from(row_place - b_lo + 1) : INFINITY, v_lo = b_hi == SA_BINS - 1 ? -INFINITY : place_from(row_place - b_hi);      // logits from v_lo to below v_hi
         if (k > 0 && sm.answer[3] <= SA_LIST) {
             // everything that can be kept: the first block ends the row
-            gather(1, [&](float v) { return v >= v_lo; });
+            gather(1, v_lo, INFINITY, [](float) { return true; });
             if (rank) return;
             const int m = sm.n_list;
             if (m <= SA_SHORT) {                                         // a thread a token, which goes through all of them twice
@@ -402,16 +402,16 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) w[e] = weight(v[e]);
                 all += w[0] + w[1] + (w[2] + w[3]);
-                if (!((v[0] >= v_lo) | (v[1] >= v_lo) | (v[2] >= v_lo) | (v[3] >= v_lo))) return;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    in_front += v[e] >= v_hi ? w[e] : 0;
+                for (int e = 0; e < 4; e++) in_front += v[e] >= v_hi ? w[e] : 0;
+                if (!(between(v[0]) | between(v[1]) | between(v[2]) | between(v[3]))) return;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
                     if (between(v[e]) & (i + e < n)) {
                         const int b = (int) fine_place(v[e]);
                         atomicAdd(&fine[b], w[e]);
                         atomicAdd(&fine_count[b], 1);
                     }
-                }
             });
             u64 sums[2];
             block_before64(all, sums[0], sm.red);
@@ -435,7 +435,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             const int f_bin = (int) sm.answer[0];
             c = sm.answer[1];
             if (f_bin < SA_FINE && sm.answer[2] <= SA_LIST) {
-                gather(blocks, [&](float v) { const float at = fine_place(v); return between(v) & (at >= (float) f_bin) & (at < (float) (f_bin + 1)); });
+                // bounds of the bin's logits, widened by far more than fine_place rounds, in front of the test itself
+                const float slack = 1e-5f * (fabsf(from) + SA_FINE / by), f_lo = from - (float) (f_bin + 1) / by - slack, f_hi = from - (float) f_bin / by + slack;
+                gather(blocks, f_bin == SA_FINE - 1 ? -INFINITY : f_lo, f_hi, [&](float v) { const float at = fine_place(v); return between(v) & (at >= (float) f_bin) & (at < (float) (f_bin + 1)); });
                 const int m = sm.n_list;
                 if (m <= SA_SHORT) {
                     const u64 mine = tid < m ? list[tid] : 0, w_mine = tid < m ? weight(key_logit(mine)) : 0;
