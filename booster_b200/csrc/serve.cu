@@ -87,28 +87,20 @@ void check_dtype(int dtype, bool f32) {
     need(dtype == B200_DTYPE_BF16 || dtype == B200_DTYPE_F16 || (f32 && dtype == B200_DTYPE_F32), f32 ? "dtype is B200_DTYPE_F32, _BF16 or _F16" : "dtype is B200_DTYPE_BF16 or _F16");
 }
 
-// rows by themselves where sequences have few of them, else tile by tile (16 rows a sequence on average: whole tiles begin to be the rule)
-bool by_tiles(const b200_kv4 & c) { return c.n_rows >= 16 * c.n_seq; }
 // heads of a row one after the other in a warp only where there are rows enough to fill the card without (48 rows of 8 heads: one pass 3 us less than four)
 int row_passes(const b200_kv4 & c) { return (int64_t) c.n_rows * c.n_head_kv > 4096 ? 4 : 1; }
 int row_parts(const b200_kv4 & c) { const int per = row_passes(c) * (128 / c.head_dim); return (c.n_head_kv + per - 1) / per; }
 unsigned row_blocks(const b200_kv4 & c) { return (unsigned) (((int64_t) c.n_rows * row_parts(c) + 7) / 8); }
-unsigned tile_blocks(const b200_kv4 & c, int parts) { const int per = 128 / c.head_dim; return (unsigned) (((int64_t) (c.n_rows / 16 + 2 * c.n_seq) * ((c.n_head_kv + per - 1) / per) * parts + 7) / 8); }
-size_t tile_smem(const b200_kv4 & c) { return (size_t) (c.n_seq + 1) * 4; }
 template <typename T> void append_as(const b200_kv4 & c, const Cache & d, const void * k, int64_t kr, int64_t kh, const void * v, int64_t vr, int64_t vh) {
     const RowSrc<T> src = {static_cast<const T *>(k), kr, kh, static_cast<const T *>(v), vr, vh, aligned(k, 4 * sizeof(T)) && aligned(v, 4 * sizeof(T)) && !((kr | kh | vr | vh) & 3)};
     const auto rows = [&](auto kernel) { launch(kernel, dim3(row_blocks(c)), 256, 0, c.stream, false, 1, d, src, row_parts(c)); };
-    const auto tiles = [&](auto kernel) { launch(kernel, dim3(tile_blocks(c, 2)), 256, tile_smem(c), c.stream, false, 1, d, src); };
-    if (by_tiles(c)) c.head_dim == 128 ? tiles(k_kv4_append_tiles<T, 128>) : tiles(k_kv4_append_tiles<T, 64>);
-    else if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv4_append<T, 128, 1>) : rows(k_kv4_append<T, 64, 1>);
+    if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv4_append<T, 128, 1>) : rows(k_kv4_append<T, 64, 1>);
     else c.head_dim == 128 ? rows(k_kv4_append<T, 128, 4>) : rows(k_kv4_append<T, 64, 4>);
 }
 template <typename T> void read_as(const b200_kv4 & c, const Cache & d, void * k, void * v) {
     T * ko = static_cast<T *>(k), * vo = static_cast<T *>(v);
     const auto rows = [&](auto kernel) { launch(kernel, dim3(row_blocks(c)), 256, 0, c.stream, false, 1, d, ko, vo, row_parts(c)); };
-    const auto tiles = [&](auto kernel) { launch(kernel, dim3(tile_blocks(c, 1)), 256, tile_smem(c), c.stream, false, 1, d, ko, vo); };
-    if (by_tiles(c)) c.head_dim == 128 ? tiles(k_kv4_read_tiles<T, 128>) : tiles(k_kv4_read_tiles<T, 64>);
-    else if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv4_read<T, 128, 1>) : rows(k_kv4_read<T, 64, 1>);
+    if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv4_read<T, 128, 1>) : rows(k_kv4_read<T, 64, 1>);
     else c.head_dim == 128 ? rows(k_kv4_read<T, 128, 4>) : rows(k_kv4_read<T, 64, 4>);
 }
 
@@ -240,14 +232,16 @@ static void check_heads(const b200_kv4 & c, int n_head, int max_rows) {
     need(max_rows >= 1 && max_rows <= (1 << 24), "kv4_attention: max_rows is the largest number of rows of a sequence");
 }
 
-// columns of a sequence from which its tiles are worth making fp16 for the tensor cores' larger products
-bool is_prompt(int group, int max_rows) { return (int64_t) group * max_rows > 64; }
+// Columns of a sequence (rows x query heads of a KV head) from which its tiles are worth making fp16 for the tensor cores' larger products. Where sequences x KV heads give the SMs few units
+// the finer pieces of the form for few rows pay longer. Few rows / many rows, us, 8 KV heads, group 4: one sequence of 8000 positions, 64 columns 25 / 39, 128 38 / 41, 256 64 / 47;
+// 8 of 2000, 32 columns 21 / 30, 64 32 / 31, 96 41 / 32; 48 of 3000, 32 columns 96 / 142, 64 175 / 144, 96 245 / 145
+bool is_prompt(const b200_kv4 & c, int group, int max_rows) { return (int64_t) group * max_rows > ((int64_t) c.n_seq * c.n_head_kv < 64 ? 128 : 48); }
 
 int64_t kv4_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
     checked(c, false);
     check_heads(c, n_head, max_rows);
     On on(c.device);
-    if (is_prompt(n_head / c.n_head_kv, max_rows)) return prompt_work(c, n_head / c.n_head_kv, on.sms).bytes;
+    if (is_prompt(c, n_head / c.n_head_kv, max_rows)) return prompt_work(c, n_head / c.n_head_kv, on.sms).bytes;
     return (int64_t) attend_bytes(c.n_seq, c.head_dim, attend_nt(n_head / c.n_head_kv, max_rows), on.sms);
 }
 
@@ -267,10 +261,10 @@ void kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row,
     a.scale_log2 = scale * 1.44269504088896341f;
     a.window = window;
     uint8_t * w = static_cast<uint8_t *>(work);
-    if (is_prompt(a.group, max_rows)) {
+    if (is_prompt(c, a.group, max_rows)) {
         const PromptWork at = prompt_work(c, a.group, on.sms);
         check_work(work, work_bytes, at.bytes);
-        PromptArgs p = {a, reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.entry_of), reinterpret_cast<int *>(w + at.first), wait_flag(c.device)};
+        PromptArgs p = {a, (int) prompt_entries(c, a.group), reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.entry_of), reinterpret_cast<int *>(w + at.first), wait_flag(c.device)};
         if (*static_cast<volatile int *>(p.err)) {
             *static_cast<volatile int *>(p.err) = 0;
             throw std::runtime_error("a wait inside an earlier kv4_attention on this device ran out: its results are missing");

@@ -175,7 +175,9 @@ template <int HD> __device__ __forceinline__ void put_scales(uint8_t * tile, int
     }
 }
 
-// Few rows of each sequence: a warp a row and PASSES passes of its heads (a head at head_dim 128, two at 64), all asked for together. Latency bounds it: row -> sequence -> slot -> page.
+// A warp a row and PASSES passes of its heads (a head at head_dim 128, two at 64), all asked for together. Latency bounds it: row -> sequence -> slot -> page, then 2 bytes a lane into the
+// two halves of a tile. Warps that took whole tiles of long portions, their V codes as words, were no faster at 8192 rows of 8 heads (26.8 us written and read, 25.4 this way) and slower
+// at 128 sequences of 16 rows (20.1 and 12.3); 4 x 8192 rows 88.6 and 92.8.
 template <typename T, int HD, int PASSES>
 __global__ void __launch_bounds__(256) k_kv4_append(const Cache c, const RowSrc<T> src, int parts) {
     constexpr int LANES = HD / 4, PER = 32 / LANES;
@@ -210,86 +212,13 @@ __global__ void __launch_bounds__(256) k_kv4_append(const Cache c, const RowSrc<
     }
 }
 
-// Many rows: a warp half a tile of a head (two at head_dim 64), whose tiles are counted over the sequences by every block. Four tokens are asked for together; a whole half tile's V codes leave
-// as 4 bytes a lane, one that the step fills in part is written entry by entry.
-struct TileItem { int slot, row, pos, lo, hi; };      // rows row + lo .. row + hi - 1 are tokens lo .. hi - 1 of the tile at pos (a multiple of 16)
-__device__ __forceinline__ int tiles_of(const Seq & q) { return q.count ? ((q.held + q.count - 1) >> 4) - (q.held >> 4) + 1 : 0; }
-__device__ __forceinline__ TileItem tile_item(const Cache & c, int item, int * before) {
-    __shared__ int sums[8];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (c.n_seq + 255) / 256, s0 = min(c.n_seq, tid * each), s1 = min(c.n_seq, s0 + each);
-    int mine = 0;
-    for (int s = s0; s < s1; s++) { before[s] = mine; mine += tiles_of(seq_at(c, s)); }
-    int up = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) { const int x = __shfl_up_sync(0xffffffffu, up, d); if (lane >= d) up += x; }
-    if (lane == 31) sums[warp] = up;
-    __syncthreads();
-    int off = up - mine;
-    for (int w = 0; w < warp; w++) off += sums[w];
-    for (int s = s0; s < s1; s++) before[s] += off;
-    if (tid == 255) before[c.n_seq] = off + mine;
-    __syncthreads();
-    TileItem r = {-1, 0, 0, 0, 0};
-    if (item >= before[c.n_seq]) return r;
-    int s = 0;
-    for (int hi = c.n_seq; hi - s > 1;) { const int mid = (s + hi) >> 1; if (before[mid] <= item) s = mid; else hi = mid; }
-    const Seq q = seq_at(c, s);
-    r.slot = q.slot;
-    r.pos = ((q.held >> 4) + item - before[s]) << 4;
-    r.lo = max(0, q.held - r.pos);
-    r.hi = min(16, q.held + q.count - r.pos);
-    r.row = q.begin + r.pos - q.held;
-    return r;
-}
-template <typename T, int HD>
-__global__ void __launch_bounds__(256, 4) k_kv4_append_tiles(const Cache c, const RowSrc<T> src) {
-    constexpr int LANES = HD / 4, PER = 32 / LANES;
-    extern __shared__ int tile_before[];                           // [n_seq + 1]
-    const int lane = threadIdx.x & 31, li = lane % LANES, groups = (c.n_kv + PER - 1) / PER;
-    const int64_t item = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5);
-    const TileItem r = tile_item(c, (int) (item / (2 * groups)), tile_before);
-    const int t0 = item & 1 ? 8 : 0, lo = max(r.lo, t0), hi = min(r.hi, t0 + 8);
-    if (lo >= hi) return;
-    const int head = (int) (item / 2 % groups) * PER + lane / LANES;
-    const bool in = head < c.n_kv;
-    const int page = page_at(c, r.slot, r.pos);
-    if (page < 0) return;
-    uint8_t * tile = c.pool + tile_offset(c, page, in ? head : 0, r.pos, 18 * HD);
-    const T * k = src.k + (int64_t) (r.row + t0) * src.k_row + head * src.k_head + 4 * li, * v = src.v + (int64_t) (r.row + t0) * src.v_row + head * src.v_head + 4 * li;
-    uint32_t vc[4] = {};                                           // [token % 4] codes of tokens t0 + 0, 4
-#pragma unroll 1
-    for (int b = 0; b < 2; b++) {
-        float xk[4][4] = {}, xv[4][4] = {};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = t0 + 4 * b + i;
-            if (in && t >= lo && t < hi) { load4(k + i * src.k_row, src.whole4, xk[i]); load4(v + i * src.v_row, src.whole4, xv[i]); }
-        }
-        k += 4 * src.k_row; v += 4 * src.v_row;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = t0 + 4 * b + i;
-            const Codes q = codes_of<T, HD>(xk[i], xv[i]);
-            if (in && t >= lo && t < hi) {
-                reinterpret_cast<uint16_t *>(tile)[k_unit<HD>(li, t)] = (uint16_t) q.k;
-                put_scales<HD>(tile, li, t, q);
-                if (hi - lo < 8) reinterpret_cast<uint16_t *>(tile + 8 * HD)[v_unit<HD>(li, t)] = (uint16_t) q.v;
-            }
-            vc[i] |= q.v << (16 * b);
-        }
-    }
-    if (in && hi - lo == 8)
-#pragma unroll
-        for (int i = 0; i < 4; i++) *reinterpret_cast<uint32_t *>(tile + 8 * HD + 2 * v_unit<HD>(li, t0 + i)) = vc[i];
-}
-
 template <typename T> __device__ __forceinline__ Four<T> held_values(uint32_t codes, float d) {
     Four<T> f;
 #pragma unroll
     for (int i = 0; i < 4; i++) f.v[i] = from_f<T>((float) ((int) (codes >> (4 * i) & 15) - 8) * d);
     return f;
 }
-// the rows' positions read back: out [n_rows][n_kv][HD]; a position without a page reads 0. As the two above
+// the rows' positions read back: out [n_rows][n_kv][HD]; a position without a page reads 0. As above
 template <typename T, int HD, int PASSES>
 __global__ void __launch_bounds__(256) k_kv4_read(const Cache c, T * k, T * v, int parts) {
     constexpr int LANES = HD / 4, PER = 32 / LANES;
@@ -323,39 +252,5 @@ __global__ void __launch_bounds__(256) k_kv4_read(const Cache c, T * k, T * v, i
         }
     }
 }
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_kv4_read_tiles(const Cache c, T * k, T * v) {
-    constexpr int LANES = HD / 4, PER = 32 / LANES;
-    extern __shared__ int tile_before[];
-    const int lane = threadIdx.x & 31, li = lane % LANES, groups = (c.n_kv + PER - 1) / PER;
-    const int64_t item = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5);
-    const TileItem r = tile_item(c, (int) (item / groups), tile_before);
-    const int head = (int) (item % groups) * PER + lane / LANES;
-    if (r.hi == 0 || head >= c.n_kv) return;
-    const int page = page_at(c, r.slot, r.pos);
-    const uint8_t * tile = c.pool + tile_offset(c, max(page, 0), head, r.pos, 18 * HD);
-    uint2 vc[4] = {};
-    uint32_t kc[16] = {};
-    float dk[16] = {}, dv[16] = {};
-    if (page >= 0) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) vc[i] = *reinterpret_cast<const uint2 *>(tile + 8 * HD + 2 * v_unit<HD>(li, i));
-#pragma unroll
-        for (int t = 0; t < 16; t++) {
-            kc[t] = reinterpret_cast<const uint16_t *>(tile)[k_unit<HD>(li, t)];
-            dk[t] = __half2float(reinterpret_cast<const __half *>(tile + 16 * HD)[k_scale_at<HD>(li, t)]);
-            dv[t] = __half2float(reinterpret_cast<const __half *>(tile + 17 * HD)[v_scale_at<HD>(li, t)]);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < 16; t++) {
-        if (t < r.lo || t >= r.hi) continue;
-        const size_t at = ((size_t) (r.row + t) * c.n_kv + head) * HD + 4 * li;
-        const uint32_t w = t >> 3 ? vc[t & 3].y : vc[t & 3].x;
-        *reinterpret_cast<Four<T> *>(k + at) = held_values<T>(kc[t], dk[t]);
-        *reinterpret_cast<Four<T> *>(v + at) = held_values<T>(t >> 2 & 1 ? w >> 16 : w & 0xffffu, dv[t]);
-    }
-}
-
 }  // namespace srv
 }  // namespace b200

@@ -21,6 +21,7 @@ namespace srv {
 struct Entry { int slot, begin, count, held, ct, lo, n, pad; };         // a sequence (Seq), its columns' number, their span of tiles
 struct PromptArgs {
     AttendArgs a;                        // a.before: [entries + 1] tiles in front of each entry (a sequence's 256 columns), for all KV heads together
+    int max_entries;                     // as many as rows and sequences can have, where first ascends; no more are looked at
     Entry * entries;
     int * entry_of, * first;             // [n_seq + 1] a sequence's first entry; {tiles of a block's piece, total > 0, the entry that each block's piece begins in}
     int * err;
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(1024) k_kv4_prompt_plan(const PromptArgs p, in
         if (s < c.n_seq) { entry_of[s] = at; p.entry_of[s] = at; }
         all += some;
     }
+    all = min(all, p.max_entries);
     if (tid == 0) { entry_of[c.n_seq] = all; p.entry_of[c.n_seq] = all; }
     __syncthreads();
     long long total = 0;
