@@ -20,25 +20,35 @@ struct Pages {
     int n_layer, n_kv, tile_bytes;
 };
 // what a plan leaves for the kernel behind it: plan[0] copies, plan[1] pages in use before (compaction); then from, to, tiles of each head
-constexpr int PLAN_HEAD = 4, PG_THREADS = 1024, PG_MAX_SLOTS = 1 << 18, PG_MAX_PAGES = 1 << 20, PG_MAX_N = 4096;
+constexpr int PG_CHUNK = 2048, PLAN_HEAD = 4, PG_THREADS = 1024, PG_MAX_SLOTS = 1 << 18, PG_MAX_PAGES = 1 << 20, PG_MAX_N = 4096;
 
-// bits of the pages with refs == 0 (or of the others), 32 a word; the block's threads share the words
+// bits of the pages with refs == 0 (or of the others), 32 a word. A warp reads 1024 neighbouring counts at a time, 16 bytes a lane; eight lanes make a word
 __device__ __forceinline__ void page_bits(const Pages & p, bool free_ones, uint32_t * bits) {
-    const int words = (p.n_pages + 31) >> 5;
-    for (int w = threadIdx.x; w < words; w += blockDim.x) {
-        uint32_t m = 0;
-        const int32_t * r = p.refs + 32 * w;
-        if (32 * w + 32 <= p.n_pages && (reinterpret_cast<uintptr_t>(r) & 15) == 0) {
+    const int words = (p.n_pages + 31) >> 5, lane = threadIdx.x & 31;
+    const bool whole = (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0;
+    for (int r0 = (threadIdx.x >> 5) * 1024; r0 < p.n_pages; r0 += PG_THREADS * 32) {
+        int4 v[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int4 v = reinterpret_cast<const int4 *>(r)[i];
-                m |= ((v.x > 0) | (v.y > 0) << 1 | (v.z > 0) << 2 | (v.w > 0) << 3) << (4 * i);
+        for (int j = 0; j < 8; j++) {
+            const int i = r0 + 128 * j + 4 * lane;
+            v[j] = make_int4(0, 0, 0, 0);
+            if (whole && i + 4 <= p.n_pages) v[j] = *reinterpret_cast<const int4 *>(p.refs + i);
+            else {
+                if (i < p.n_pages) v[j].x = p.refs[i];
+                if (i + 1 < p.n_pages) v[j].y = p.refs[i + 1];
+                if (i + 2 < p.n_pages) v[j].z = p.refs[i + 2];
+                if (i + 3 < p.n_pages) v[j].w = p.refs[i + 3];
             }
-        } else {
-            for (int i = 0; i < 32 && 32 * w + i < p.n_pages; i++) m |= (uint32_t) (r[i] > 0) << i;
         }
-        if (free_ones) m = ~m & (32 * w + 32 <= p.n_pages ? 0xffffffffu : (1u << (p.n_pages & 31)) - 1);
-        bits[w] = m;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            uint32_t m = (uint32_t) ((v[j].x > 0) | (v[j].y > 0) << 1 | (v[j].z > 0) << 2 | (v[j].w > 0) << 3) << (4 * (lane & 7));
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) m |= __shfl_xor_sync(0xffffffffu, m, d);
+            const int w = (r0 >> 5) + 4 * j + (lane >> 3);
+            if (free_ones) m = ~m & (32 * w + 32 <= p.n_pages ? 0xffffffffu : (1u << (p.n_pages & 31)) - 1);
+            if ((lane & 7) == 0 && w < words) bits[w] = m;
+        }
     }
     __syncthreads();
 }
@@ -73,6 +83,7 @@ __device__ __forceinline__ int n_bits(const uint32_t * bits, int words) { return
 __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const Pages p, const int32_t * slots, const int32_t * first, int n, int32_t * status) {
     extern __shared__ uint32_t pg_smem[];
     __shared__ int from[PG_MAX_N], before[PG_MAX_N + 1];           // of each sequence: the first page that is missing, pages missing in front of it
+    __shared__ int chunk[PG_CHUNK];
     __shared__ int bad;
     const int words = (p.n_pages + 31) >> 5, slot_words = (p.n_slots + 31) >> 5;
     uint32_t * free_pages = pg_smem, * seen = pg_smem + words;
@@ -102,12 +113,18 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const Pages p, con
     const int have = n_bits(free_pages, words);
     const bool refused = bad != 0;
     if (!refused && have >= all)
-        each_bit(free_pages, words, all, [&](int k, int page) {
-            int s = 0;
-            for (int hi = n; hi - s > 1;) { const int mid = (s + hi) >> 1; if (before[mid] <= k) s = mid; else hi = mid; }
-            p.table[(int64_t) (slots ? slots[s] : s) * p.table_stride + from[s] + k - before[s]] = page;
-            p.refs[page] = 1;
-        });
+        for (int k0 = 0; k0 < all; k0 += PG_CHUNK) {               // the pages by their bits, then a thread a page
+            each_bit(free_pages, words, min(all, k0 + PG_CHUNK), [&](int k, int page) { if (k >= k0) chunk[k - k0] = page; });
+            __syncthreads();
+            for (int i = threadIdx.x; i < min(PG_CHUNK, all - k0); i += PG_THREADS) {
+                const int k = k0 + i, page = chunk[i];
+                int s = 0;
+                for (int hi = n; hi - s > 1;) { const int mid = (s + hi) >> 1; if (before[mid] <= k) s = mid; else hi = mid; }
+                p.table[(int64_t) (slots ? slots[s] : s) * p.table_stride + from[s] + k - before[s]] = page;
+                p.refs[page] = 1;
+            }
+            __syncthreads();
+        }
     if (threadIdx.x == 0) *status = refused ? -1 : max(0, all - have);
 }
 

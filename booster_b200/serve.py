@@ -128,7 +128,8 @@ def kv4_read(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first:
 def kv4_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first: torch.Tensor, slots: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                   window: int = 0, max_rows: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """attention of the step's rows q [rows, n_head, head_dim] (bfloat16 or float16, any strides over rows and heads) over the positions up to their own, kv4_append having put those into
-    the pool; window > 0: over the last `window` of them. scale: 1 / sqrt(head_dim). max_rows: the largest number of rows of a sequence, if the program knows it (else: rows).
+    the pool; window > 0: over the last `window` of them. scale: 1 / sqrt(head_dim). max_rows: the largest number of rows of a sequence, if the program knows it (it chooses kernels and
+    changes no result; else the mean).
     Rows of no sequence are left as they are (in `out`)"""
     row, head = _rows("q", q, pool)
     dtype = _TYPE.get(q.dtype)
@@ -140,9 +141,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, held
         out = torch.empty((rows, heads, hd), dtype=q.dtype, device=device)
     else:
         _need(out.shape == q.shape and out.dtype is q.dtype and out.device == device and out.is_contiguous(), "out is a contiguous tensor like q")
-    most = rows if max_rows is None else max_rows
-    if most < 1:
-        most = 1
+    most = max(1, -(-rows // max(1, first.numel() - 1)) if max_rows is None else max_rows)
     L = _lib.lib()
     shape = (device.index, heads, pool.shape[1], hd, first.numel(), rows, most)
     size = _work_bytes.get(shape)

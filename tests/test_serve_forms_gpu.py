@@ -111,3 +111,32 @@ def test_rows_that_do_not_ascend_stay_within_bounds(max_rows):
     serve.kv4_attention(q, c.pool[0], c.table, c.held, first, c.slots, max_rows=max_rows, out=out[:rows])
     assert (out[rows:] == 7).all()
     assert torch.equal(right, serve.kv4_attention(q, *c.args(), slots=c.slots, max_rows=max_rows))
+
+
+@pytest.mark.parametrize("n_pages,n_slots,offset", [(1 << 20, 1 << 18, 0), (5003, 40, 1), (70001, 300, 2)])
+def test_reserving_in_large_and_odd_pools(n_pages, n_slots, offset):
+    """thousands of pages by one call, counts on any alignment: the lowest free ones, in the order of the call's sequences"""
+    g = torch.Generator().manual_seed(n_pages)
+    refs_h = (torch.rand(n_pages, generator=g) < 0.3).int() * 3
+    flat = torch.zeros(n_pages + 4, dtype=torch.int32, device="cuda")
+    refs = flat[offset:offset + n_pages]
+    refs.copy_(refs_h)
+    n, width = 33, 120
+    table = torch.full((n_slots, width), -1, dtype=torch.int32, device="cuda")
+    held = torch.zeros(n_slots, dtype=torch.int32, device="cuda")
+    slots = torch.randperm(n_slots, generator=g)[:n]
+    counts = torch.randint(0, width + 1, (n,), generator=g)
+    first = torch.cat([torch.zeros(1, dtype=torch.long), (counts * 16).cumsum(0)])
+    free = (refs_h == 0).nonzero().flatten()
+    assert serve.pages_reserve(table, held, refs, first.int().cuda(), 16, slots.int().cuda()).item() == 0
+    at = 0
+    want = torch.full((n_slots, width), -1, dtype=torch.int32)
+    for s, c in zip(slots.tolist(), counts.tolist()):
+        want[s, :c] = free[at:at + c].int()
+        at += c
+    refs_h[free[:at]] = 1
+    assert at > 1000 and torch.equal(table.cpu(), want) and torch.equal(refs.cpu(), refs_h) and not flat[:offset].any() and not flat[offset + n_pages:].any()
+    # and given back
+    serve.pages_free(table, held, refs, slots.int().cuda())
+    refs_h[free[:at]] = 0
+    assert (table == -1).all() and torch.equal(refs.cpu(), refs_h)
