@@ -27,7 +27,7 @@ struct PromptArgs {
     int * err;
 };
 
-constexpr int PR_COLS = 256, PR_KV = 128, PR_THREADS = 512, PR_OVER = 2;      // PR_OVER: what beginning a unit costs, in tiles
+constexpr int PR_COLS = 256, PR_KV = 128, PR_THREADS = 512, PR_OVER = 4;      // PR_OVER: what beginning a unit costs, in tiles (8192 tokens 780 us with 2, 655, 600, 600, 611 with 3, 4, 5, 8)
 constexpr uint64_t PR_DESC = (1ull << 16) | ((uint64_t) (1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);      // K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart
 __host__ __device__ constexpr uint32_t pr_idesc(int n) { return (1u << 4) | ((uint32_t) (n >> 3) << 17) | (8u << 24); }     // D f32, A and B f16, M = 128
 template <int HD> struct PromptSmem {
@@ -234,11 +234,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;          // of the half
         const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, my_s = t_s + lanes + half * 128, my_o = t_o + lanes + half * HD;
         int n_s = 0;                                                       // steps of 64 tokens of this half so far
-        for (Segment g; segment(g);) {
+        const auto next = [&](Segment & g) {                               // the next segment with columns of this half
+            do { if (!segment(g)) return false; } while (half >= g.halves);
+            return true;
+        };
+        // the warp's 32 queries, HD / 8 lanes a row: each scaled by a power of two to at most 2^14, dims of eight as 0 4 1 5 2 6 3 7. Returns what the column's scores are scaled by
+        const auto queries = [&](const Segment & g) {
             const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
             const bool in = i < g.q.count;
-            if (half >= g.halves) continue;
-            // the warp's 32 queries, HD / 8 lanes a row: each scaled by a power of two to at most 2^14, dims of eight as 0 4 1 5 2 6 3 7
             constexpr int LANES = HD / 8, ROWS = 32 / LANES, X = 8;
             float factor = 0.f;
             {
@@ -282,6 +285,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) pr_arrive(smem_at(&q_full[half]));
+            return factor;
+        };
+        Segment g;
+        bool more = next(g);
+        float factor = more ? queries(g) : 0.f;
+        while (more) {
+            const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
+            const bool in = i < g.q.count;
             // whether every page of the piece is there; where not, each tile's are looked up again
             bool whole = g.q.slot >= 0;
             {
@@ -356,6 +367,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 __syncwarp();
                 if (lane == 0) pr_arrive(smem_at(&p_full[half][n_s & 1]));
             }
+            // the next segment's queries before this one's results: its first scores are made while these are written
+            Segment then;
+            more = next(then);
+            if (more) factor = queries(then);
             pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), dead);
             __syncwarp();
             pr_fence_after();
@@ -386,6 +401,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
             }
             if (in && !final) *reinterpret_cast<float2 *>(a.ml + (piece * PR_COLS + half * 128 + row) * 2) = make_float2(m, l);
             pr_fence_before();
+            g = then;
         }
     } else if (warp < 12) {
         regs_less<112>();
