@@ -5,8 +5,8 @@
 //   warps 0-3, 4-7   soft-max of columns 0-127 and 128-255, a thread a column, 64 tokens at a time: its row of S into registers, maximum, exponentials, P back into tensor memory in the
 //                    place of S
 //   warps 8-11       codes of 32 tokens each, copied ahead, to fp16 in shared memory (exact: a scale has 8 bits, a code 4), K by rows of tokens, V by rows of dims, both with 128-byte swizzle
-//   warp 12          (of 12-15: registers are shared out by four warps, 128 a thread at launch, then 168, 168, 112 and 64) one thread issues S = Q K^T (128 x 64 x head_dim) and
-//                    O += P V (P from tensor memory, 128 x head_dim x 64) of both halves
+//   warps 12, 13     (of 12-15: registers are shared out by four warps, 128 a thread at launch, then 168, 168, 112 and 64) one thread each issues a half's S = Q K^T (128 x 64 x head_dim)
+//                    and O += P V (P from tensor memory, 128 x head_dim x 64): a thread issues a product every 44 clocks or so, 24 of them a half and tile
 // Tensor memory: S and P [2 halves][2 turns][64 columns], O [2][head_dim]. Each half has two turns of S, so that the scores of the next 64 tokens are there when those in hand are done with.
 // Tokens of 32 stand as n = 8 c + 4 u + i for token 16 u + c + 4 i in S, P, K and V alike, and dims of 8 as 0 4 1 5 2 6 3 7 in Q and K: the orders in which a word's codes come apart.
 // P is rounded to fp16 (2^-11), q scaled by a power of two into fp16's range; sums are fp32. The maximum moves when a score passes it by 2^8; O is scaled in tensor memory then.
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
     const uint32_t smem = (smem_at(pr_raw) + 1023u) & ~1023u, q_s = smem, k_s = q_s + 2 * QB, v_s = k_s + 2 * KVB;
     if (tid == 0) {
         const auto init = [](uint64_t * b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(smem_at(b)), "r"(n) : "memory"); };
-        for (int i = 0; i < 2; i++) { init(&q_full[i], 4); init(&k_full[i], 4); init(&v_full[i], 4); init(&k_empty[i], 1); init(&v_empty[i], 1); for (int b = 0; b < 2; b++) { init(&s_full[i][b], 1); init(&p_full[i][b], 4); init(&o_full[i][b], 1); } }
+        for (int i = 0; i < 2; i++) { init(&q_full[i], 4); init(&k_full[i], 4); init(&v_full[i], 4); init(&k_empty[i], 2); init(&v_empty[i], 2); for (int b = 0; b < 2; b++) { init(&s_full[i][b], 1); init(&p_full[i][b], 4); init(&o_full[i][b], 1); } }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -498,52 +498,62 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
         }
     } else {
         regs_less<64>();
-        int n = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
-        for (Segment g; warp == 12 && segment(g);) {
+        const int half = warp - 12;
+        int n = 0, n_q = 0, n_p = 0;                                       // tiles, segments and steps of this half so far
+        for (Segment g; half < 2 && segment(g);) {
+            const int tiles = g.t1 - g.t0, steps = 2 * tiles;
             if (pr_elect()) {
-                const int steps = 2 * (g.t1 - g.t0);
-                const auto scores = [&](int half, int step) {              // S = Q K^T of a half and 64 tokens
-                    const int turn = step & 1;
+                if (half < g.halves) {
+                    const auto scores = [&](int step) {                    // S = Q K^T of 64 tokens
+                        const int turn = step & 1;
 #pragma unroll
-                    for (int k = 0; k < HD / 16; k++)
-                        pr_mma_ss(t_s + half * 128 + 64 * turn, PR_DESC | (uint64_t) ((q_s + half * QB + (k >> 2) * SUB) >> 4) + 2 * (k & 3),
-                                  PR_DESC | (uint64_t) ((k_s + (n + (step >> 1) & 1) * KVB + (k >> 2) * SUB + turn * (SUB / 2)) >> 4) + 2 * (k & 3), pr_idesc(64), k > 0);
-                    pr_commit(smem_at(&s_full[half][turn]));
-                };
-                for (int half = 0; half < g.halves; half++) pr_wait(smem_at(&q_full[half]), (uint32_t) (n_q[half] & 1), dead);
-                pr_wait(smem_at(&k_full[n & 1]), (uint32_t) (n >> 1 & 1), dead);
-                pr_fence_after();
-                if (!dead) {
-                    for (int step = 0; step < 2; step++)
-                        for (int half = 0; half < g.halves; half++) scores(half, step);
-                    pr_commit(smem_at(&k_empty[n & 1]));
-                }
-                for (int step = 0; step < steps; step++) {
-                    const int turn = step & 1, now = n + (step >> 1), stage = now & 1, after = (now + 1) & 1;
-                    if (turn == 0) pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), dead);
-                    for (int half = 0; half < g.halves; half++) {
-                        pr_wait(smem_at(&p_full[half][turn]), (uint32_t) ((n_p[half] + step) >> 1 & 1), dead);
+                        for (int k = 0; k < HD / 16; k++)
+                            pr_mma_ss(t_s + half * 128 + 64 * turn, PR_DESC | (uint64_t) ((q_s + half * QB + (k >> 2) * SUB) >> 4) + 2 * (k & 3),
+                                      PR_DESC | (uint64_t) ((k_s + (n + (step >> 1) & 1) * KVB + (k >> 2) * SUB + turn * (SUB / 2)) >> 4) + 2 * (k & 3), pr_idesc(64), k > 0);
+                        pr_commit(smem_at(&s_full[half][turn]));
+                    };
+                    pr_wait(smem_at(&q_full[half]), (uint32_t) (n_q & 1), dead);
+                    pr_wait(smem_at(&k_full[n & 1]), (uint32_t) (n >> 1 & 1), dead);
+                    pr_fence_after();
+                    if (!dead) {
+                        scores(0);
+                        scores(1);
+                        pr_commit(smem_at(&k_empty[n & 1]));
+                    }
+                    for (int step = 0; step < steps; step++) {
+                        const int turn = step & 1, now = n + (step >> 1), stage = now & 1, after = (now + 1) & 1;
+                        if (turn == 0) pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), dead);
+                        pr_wait(smem_at(&p_full[half][turn]), (uint32_t) ((n_p + step) >> 1 & 1), dead);
                         pr_fence_after();
                         if (!dead) {
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                                 pr_mma_ts(t_o + half * HD, t_s + half * 128 + 64 * turn + 8 * k, PR_DESC | (uint64_t) ((v_s + stage * KVB + turn * (HD * 128)) >> 4) + 2 * k, pr_idesc(HD), step > 0 || k > 0);
                             pr_commit(smem_at(&o_full[half][turn]));
+                            if (turn == 1) pr_commit(smem_at(&v_empty[stage]));
                         }
                         if (step + 2 < steps) {
-                            if (turn == 0 && half == 0) { pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), dead); pr_fence_after(); }
+                            if (turn == 0) { pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), dead); pr_fence_after(); }
                             if (!dead) {
-                                scores(half, step + 2);
-                                if (turn == 1 && half == g.halves - 1) pr_commit(smem_at(&k_empty[after]));
+                                scores(step + 2);
+                                if (turn == 1) pr_commit(smem_at(&k_empty[after]));
                             }
                         }
                     }
-                    if (turn == 1 && !dead) pr_commit(smem_at(&v_empty[stage]));
+                } else {                                                   // no columns here: the tiles are let go as they come
+                    for (int t = 0; t < tiles; t++) {
+                        const int stage = (n + t) & 1;
+                        const uint32_t phase = (uint32_t) ((n + t) >> 1 & 1);
+                        pr_wait(smem_at(&k_full[stage]), phase, dead);
+                        if (!dead) pr_arrive(smem_at(&k_empty[stage]));
+                        pr_wait(smem_at(&v_full[stage]), phase, dead);
+                        if (!dead) pr_arrive(smem_at(&v_empty[stage]));
+                    }
                 }
             }
             __syncwarp();
-            n += g.t1 - g.t0;
-            for (int half = 0; half < g.halves; half++) { n_q[half]++; n_p[half] += 2 * (g.t1 - g.t0); }
+            n += tiles;
+            if (half < g.halves) { n_q++; n_p += steps; }
         }
     }
     if (dead) {
