@@ -7,9 +7,13 @@
 //
 // A cluster of blocks takes a row and holds its slice in shared memory: logits cross HBM once. A histogram of floor(16 x logit), against each block's own largest, tells with one meeting
 // of the cluster the row's largest and the bin of the k-th token. Only tokens down to that bin are ordered (a few dozen of 128 k), exactly as the definition says, and the first block
-// ends the row with them. For top-p alone counts bound the bins between which its sum is crossed; one sweep sums all weights, those in front of these bins and, in 1024 finer bins, those
+// ends the row with them. For top-p alone counts bound the bins between which its sum is crossed; one sweep sums all weights, those in front of these bins and, in 512 finer bins, those
 // between; the tokens of one finer bin are ordered. Then a last sweep sums what is kept, 128 tokens at a time, and the warp in whose tokens the draw falls looks for it. Rows whose edge
 // lies among more than 2048 candidates (thousands of equal logits, very large k) are bisected over (logit, index) instead.
+//
+// Measured with 128 256 logits in fp32, one row / 160 rows (82 MB, 13 us at the copy rate): the largest 6 / 36 us, min-p 8 / 45, top-k 40 10 / 53, no filter 10 / 64, top-p alone 26 / 170.
+// Five waves of clusters, two blocks an SM: a wave loads 3000 clocks, and each meeting of a cluster costs it 1200 to 2500 more; then the 64-bit pipe (11 operations a weight) bounds the
+// sweeps over all weights.
 #pragma once
 #include "serve_cache.cuh"
 #include <cooperative_groups.h>

@@ -362,7 +362,9 @@ typedef struct b200_kv4 {
 
 /* keys and values of the step's rows into their pages: k[row * k_row + head * k_head + i] and v likewise (strides in entries), dtype F32, BF16 or F16. A number of a block
  * of 32 is held as c in 0 .. 15 and stands for (c - 8) d with d = e / -8 (8 significant bits, at most 8160 in magnitude), e the block's entry of largest magnitude (the
- * negative one of two). A token with an infinity or a NaN in a head is held as such: rows that see it answer NaN for the head. Rows whose page is absent are dropped. */
+ * negative one of two). A token with an infinity or a NaN in a head is held as such: rows that see it answer NaN for the head. Rows whose page is absent are dropped. What is written is written
+ * for every slot that holds the page: b200_pages_fork shares full pages only, and rows behind a slot's tokens never meet one; a program that lowers held[s] below a shared
+ * page's end copies the page first. */
 int b200_kv4_append(const b200_kv4 * c, int dtype, const void * k, int64_t k_row, int64_t k_head, const void * v, int64_t v_row, int64_t v_head);
 /* the same positions read back: k, v [n_rows][n_head_kv][head_dim] of dtype (rounded once); absent pages read 0 */
 int b200_kv4_read(const b200_kv4 * c, int dtype, void * k, void * v);
