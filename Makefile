@@ -5,10 +5,12 @@ NVCCFLAGS := $(ARCH) -O3 -std=c++17 -lineinfo -Xcompiler -fPIC,-Wall,-Wno-unused
 CSRC      := booster_b200/csrc
 OBJDIR    := build
 LIB       := booster_b200/libbooster_b200.so
+SERVE     := booster_b200/_serve.so
+PYTHON    ?= python
 
 OBJS := $(OBJDIR)/engine.o $(OBJDIR)/stack.o $(OBJDIR)/serve.o $(OBJDIR)/safetensors.o $(OBJDIR)/gguf.o $(OBJDIR)/bridge.o $(OBJDIR)/tokenizer.o $(OBJDIR)/janus.o
 
-all: $(LIB)
+all: $(LIB) $(SERVE)
 
 $(OBJDIR)/engine.o: $(CSRC)/engine.cu $(CSRC)/kernels.cuh $(CSRC)/token_kernel.cuh $(CSRC)/attn_cluster.cuh $(CSRC)/matvec_q80.cuh $(CSRC)/matvec_kq.cuh $(CSRC)/prefill.cuh $(CSRC)/prefill_mma.cuh $(CSRC)/prefill_umma.cuh $(CSRC)/prefill_umma_q80.cuh $(CSRC)/gguf.hpp $(CSRC)/tokenizer.hpp $(CSRC)/stack.hpp $(CSRC)/serve.hpp $(CSRC)/safetensors.hpp include/booster_b200.h
 	@mkdir -p $(OBJDIR)
@@ -29,10 +31,15 @@ $(OBJDIR)/%.o: $(CSRC)/%.cpp $(CSRC)/gguf.hpp $(CSRC)/tokenizer.hpp $(CSRC)/janu
 $(LIB): $(OBJS)
 	$(NVCC) $(ARCH) -shared -o $@ $^ -ldl
 
+# booster_b200/serve.py's module of torch tensors: the flags are those of the torch that will load it
+$(SERVE): $(CSRC)/serve_torch.cpp include/booster_b200.h
+	flags=$$($(PYTHON) -c 'import os, sysconfig, torch; r = os.path.dirname(torch.__file__); inc = sysconfig.get_path("include"); print(f"-I{r}/include -I{r}/include/torch/csrc/api/include -isystem /usr/local/cuda/include -I{inc} -D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)} -L{r}/lib")') && \
+	$(CXX) -O2 -std=c++17 -fPIC -shared -Wall -Wno-unused-function $< -o $@ $$flags -lc10 -lc10_cuda -ltorch_cpu -ltorch_python
+
 oracle:
 	$(MAKE) -C oracle all
 
 clean:
-	rm -rf $(OBJDIR) $(LIB)
+	rm -rf $(OBJDIR) $(LIB) $(SERVE)
 
 .PHONY: all oracle clean

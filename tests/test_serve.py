@@ -123,3 +123,31 @@ def test_tensors_that_do_not_fit():
         serve.kv4_pool(4, 20, 2, 64, device="cpu")
     with pytest.raises(ValueError):
         serve.kv4_pool(4, 16, 2, 80, device="cpu")
+
+
+def test_what_is_no_tensor_is_refused():
+    pool = serve.kv4_pool(4, 16, 2, 64, device="cpu")
+    x, k = torch.zeros(3, dtype=torch.int32), torch.zeros(2, 2, 64, dtype=torch.half)
+    with pytest.raises(ValueError, match="pool is a tensor"):
+        serve.kv4_append(None, x, x, x, k, k)
+    with pytest.raises(ValueError, match="q is a tensor"):
+        serve.kv4_attention([1.0], pool[0], x, x, x)
+    with pytest.raises(ValueError, match="dtype"):
+        serve.kv4_read(pool[0], x, x, x, 2, "bfloat16")
+    with pytest.raises(ValueError, match="whole number"):
+        serve.kv4_read(pool[0], x, x, x, 1 << 40)
+    with pytest.raises(ValueError, match="refs is a tensor"):
+        serve.pages_free(x, x, 3, x)
+    with pytest.raises(ValueError, match="logits is a tensor"):
+        serve.sample(7, x)
+    with pytest.raises(TypeError):
+        serve.sample(k[0], x, x, x, x, x, x)
+
+
+def test_the_module_calls_the_library_that_is_loaded():
+    """its functions come by address: without them it refuses, and it is the library's own class that its errors have"""
+    module = serve._native()
+    for bad in ((), (_lib.B200Error, 1), (_lib.B200Error,) + (0,) * 12):
+        with pytest.raises((TypeError, ValueError)):
+            module.bind(*bad)
+    assert serve._native() is module
