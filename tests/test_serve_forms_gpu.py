@@ -140,3 +140,58 @@ def test_reserving_in_large_and_odd_pools(n_pages, n_slots, offset):
     serve.pages_free(table, held, refs, slots.int().cuda())
     refs_h[free[:at]] = 0
     assert (table == -1).all() and torch.equal(refs.cpu(), refs_h)
+
+
+@pytest.mark.parametrize("n", [2500, 4096])
+def test_as_many_sequences_as_there_may_be(n):
+    """both forms over thousands of sequences, some without rows, against the form for few rows on 500 of them at a time. All round P and the result to 2^-11"""
+    c = Case([(7 * i) % 40 for i in range(n)], [(1, 1, 2, 0, 1)[i % 5] for i in range(n)], kv=1, hd=64, seed=1)
+    c.fill()
+    q = c.randn(c.rows, 2, 64).half()
+    outs = [serve.kv4_attention(q, *c.args(), slots=c.slots, max_rows=m) for m in (2, MANY)]
+    parts = []
+    for s in range(0, n, 500):
+        e = min(n, s + 500)
+        a, b = c.first_l[s], c.first_l[e]
+        parts.append(serve.kv4_attention(q[a:b], c.pool[0], c.table, c.held, c.first[s:e + 1] - a, c.slots[s:e], max_rows=2))
+    want = torch.cat(parts).double()
+    big = max(np.abs(v).max() for v in c.v if v.size)
+    for out in outs:
+        assert torch.isfinite(out).all() and (out.double() - want).abs().max().item() <= big * (2 * 2.0 ** -11 + 2 * 2.0 ** -11 + 2.0 ** -14)
+    # the cache and the pages take as many: a further token each, reserved, written and read back
+    refs = torch.zeros(c.pages, dtype=torch.int32, device="cuda")
+    used = c.table[c.table >= 0].long()
+    refs[used] = 1
+    extra = serve.kv4_pool(c.pages + n, c.page, 1, 64)
+    refs = torch.cat([refs, torch.zeros(n, dtype=torch.int32, device="cuda")])
+    held = c.held.clone()
+    held[c.slots.long()] += ints(c.counts)
+    one = ints(range(n + 1))
+    assert serve.pages_reserve(c.table, held, refs, one, c.page, c.slots).item() == 0
+    k = c.randn(n, 1, 64).half()
+    serve.kv4_append(extra[0], c.table, held, one, k, -k, c.slots)
+    rk, rv = serve.kv4_read(extra[0], c.table, held, one, n, F16, c.slots)
+    # half a step of a code, an eighth of the block's largest entry, and at the side that has no code 8 a whole one; d itself is rounded to 2^-8
+    step = k.float().view(n, 1, 2, 32).abs().amax(-1, keepdim=True).expand(n, 1, 2, 32).reshape(n, 1, 64) / 8
+    assert ((rk.float() - k.float()).abs() <= 1.05 * step).all() and ((rv.float() + k.float()).abs() <= 1.05 * step).all()
+    assert (refs >= 0).all() and refs.max().item() == 1
+
+
+@pytest.mark.parametrize("max_rows", [1, MANY])
+@pytest.mark.parametrize("page", [128, 1024])
+@pytest.mark.parametrize("window", [0, 33, 70])
+def test_long_pages(max_rows, page, window):
+    """sequences that end and windows that begin anywhere in a page"""
+    c = Case([0, 127, 128, 700, 1023, 1024, 1500], [1, 2, 1, 3, 1, 1, 2], page=page, kv=2, hd=64, seed=page)
+    c.fill()
+    q = c.randn(c.rows, 4, 64).half()
+    assert_attends(c, c.seen(), q, serve.kv4_attention(q, *c.args(), slots=c.slots, window=window, max_rows=max_rows), window)
+
+
+@pytest.mark.parametrize("max_rows", [1, MANY])
+@pytest.mark.parametrize("heads", [71, 128, 300])
+def test_many_heads_on_one(max_rows, heads):
+    c = Case([40, 0, 17], [1, 1, 2], kv=1, hd=64, seed=heads)
+    c.fill()
+    q = c.randn(c.rows, heads, 64).to(BF16)
+    assert_attends(c, c.seen(), q, serve.kv4_attention(q, *c.args(), slots=c.slots, max_rows=max_rows))
