@@ -119,10 +119,12 @@ template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, int d
     allow_smem(kernel, device, smem, set);
     launch(kernel, dim3(sms * at_blocks(NT)), AT_WARPS * 32, smem, stream, false, 1, a);
     const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group;
-    // parts a unit has on average, where every sequence has rows: few are four warps' to add, many sixteen's (one sequence of 20 000: 21 and 16 us; 6 of 4000 16 and 17; 48 of 3000 46 and 56)
-    const bool many = (int64_t) sms * at_blocks(NT) * AT_WARPS > 32 * (int64_t) a.c.n_seq * a.c.n_kv;
-    if (many) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, stream, true, 1, a);
-    else launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, stream, true, 1, a);
+    // parts a unit has on average, where every sequence has rows: few are one warp's to add, many sixteen's. One / four / sixteen warps, us, 8 KV heads: one sequence of 20 000 39 / 22 / 16,
+    // 6 of 4000 20 / 17 / 17, 24 of 4000 33 / 32 / 38, 48 of 3000 43 / 45 / 54, 300 of 100 27 / 38 / 81
+    const int64_t parts = (int64_t) sms * at_blocks(NT) * AT_WARPS / ((int64_t) a.c.n_seq * a.c.n_kv);
+    if (parts > 32) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, stream, true, 1, a);
+    else if (parts > 8) launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, stream, true, 1, a);
+    else launch(k_kv4_join<HD, NT, T, 1>, dim3((unsigned) ((items + 7) / 8)), 256, 0, stream, true, 1, a);
 }
 template <int HD, typename T> void attend_nt_as(const AttendArgs & a, int nt, int device, int sms, void * stream) {
     nt == 1 ? attend_as<HD, 1, T>(a, device, sms, stream) : attend_as<HD, 2, T>(a, device, sms, stream);

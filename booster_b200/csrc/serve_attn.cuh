@@ -6,7 +6,7 @@
 //   S^T = K Q^T: a tile's codes are the A operand of mma.sync (16 tokens x 16 dims), the columns the B operand. A block's 32 products are summed as codes and scaled once.
 //   O^T += V^T P^T: V's codes times their scales (exact in fp16) are the A operand (16 dims x 16 tokens); P^T comes from S^T by movmatrix.
 // Measured with 32 query heads on 8 of 128: HBM bounds long contexts (24 sequences of 12 000 to 32 000 tokens add 85 to 89 % of the copy rate's time), 13 us are the way to the first tile
-// (launch, row, slot, page, codes) and the last parts: 48 sequences of 90 to 4090 tokens (116 MB) 38 us, 3 of 21 000 to 32 700 under 64 heads on 8 (99 MB) 31 us, one of 333 tokens 9.6 us with the join.
+// (launch, row, slot, page, codes) and the last parts: 48 sequences of 90 to 4090 tokens (116 MB) 35 us, 200 of 500 (115 MB) 40 us, 3 of 21 000 to 32 700 under 64 heads on 8 (99 MB) 31 us, one of 333 tokens 9.6 us with the join.
 // P is rounded to fp16 (2^-11), the one rounding beside the output's; q is scaled by a power of two into fp16's range, which keeps its bits. Sums are fp32.
 #pragma once
 #include "serve_cache.cuh"
@@ -29,7 +29,7 @@ struct AttendArgs {
     float * part, * ml;                  // [2 x warps][8 NT][HD], [2 x warps][8 NT][2]
 };
 
-constexpr int AT_WARPS = 4, AT_MAX_SEQ = 4096, AT_STAGES = 3, AT_OVER = 2;      // AT_OVER: what beginning a unit costs, in pairs of tiles
+constexpr int AT_WARPS = 4, AT_MAX_SEQ = 4096, AT_STAGES = 3, AT_OVER = 3;      // AT_OVER: what beginning a unit costs, in pairs of tiles (48 ragged sequences 49, 42, 38, 37, 37 us with 0 to 4)
 __host__ __device__ constexpr int at_blocks(int nt) { return nt == 1 ? 3 : 2; }          // resident on an SM: 168 and 255 registers a thread
 __host__ __device__ constexpr size_t at_ring_bytes(int hd) { return (size_t) AT_WARPS * AT_STAGES * 36 * hd; }
 __device__ __forceinline__ uint32_t smem_at(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
@@ -113,13 +113,20 @@ __global__ void __launch_bounds__(AT_WARPS * 32, at_blocks(NT)) k_kv4_attend(con
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // pairs of tiles in front of each sequence
     {
-        const int each = (c.n_seq + AT_WARPS * 32 - 1) / (AT_WARPS * 32), s0 = min(c.n_seq, tid * each), s1 = min(c.n_seq, s0 + each);
-        long long mine = 0;
-        for (int s = s0; s < s1; s++) {
-            const Seq q = seq_at(c, s);
-            before[s] = mine;
-            mine += q.count ? (long long) col_tiles(q, a.group, COLS) * c.n_kv * (span_of(c, q, a.window, 0, q.count - 1).n + AT_OVER) : 0;
+        constexpr int THREADS = AT_WARPS * 32, BATCH = 4;
+        for (int b0 = tid; b0 < c.n_seq; b0 += THREADS * BATCH) {              // (slot, held, first: dependent reads, of four sequences at a time)
+            Seq q[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) q[i] = seq_at(c, min(b0 + i * THREADS, c.n_seq - 1));
+#pragma unroll
+            for (int i = 0; i < BATCH; i++)
+                if (b0 + i * THREADS < c.n_seq)
+                    before[b0 + i * THREADS] = q[i].count ? (long long) col_tiles(q[i], a.group, COLS) * c.n_kv * (span_of(c, q[i], a.window, 0, q[i].count - 1).n + AT_OVER) : 0;
         }
+        __syncthreads();
+        const int each = (c.n_seq + THREADS - 1) / THREADS, s0 = min(c.n_seq, tid * each), s1 = min(c.n_seq, s0 + each);
+        long long mine = 0;
+        for (int s = s0; s < s1; s++) { const long long n = before[s]; before[s] = mine; mine += n; }
         long long up = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, up, d); if (lane >= d) up += x; }
@@ -433,15 +440,17 @@ __global__ void __launch_bounds__(AT_WARPS * 32, at_blocks(NT)) k_kv4_attend(con
     }
 }
 
-// a block a row and head: adds the partial results of a unit that several warps shared. A warp takes every AJ_WARPS-th part, eight of them on their way at a time. It stands ready behind
+// AJ_WARPS warps a row and head (one: eight of them a block): add the partial results of a unit that several warps shared. A warp takes every AJ_WARPS-th part, eight of them on their way at a
+// time. It stands ready behind
 // the kernel in front (programmatic launch): 3 to 5 us of latency behind that one's end
 template <int HD, int NT, typename T, int AJ_WARPS>
-__global__ void __launch_bounds__(AJ_WARPS * 32) k_kv4_join(const AttendArgs a) {
+__global__ void __launch_bounds__(AJ_WARPS == 1 ? 256 : AJ_WARPS * 32) k_kv4_join(const AttendArgs a) {
     constexpr int COLS = 8 * NT, E = HD / 32, BATCH = 8;
-    __shared__ float sums[AJ_WARPS][HD], ml_s[AJ_WARPS][2];
     const Cache & c = a.c;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_head = c.n_kv * a.group, row = blockIdx.x / n_head, h = blockIdx.x % n_head;
-    const int s = seq_of_row(c, row);
+    const int lane = threadIdx.x & 31, warp = AJ_WARPS == 1 ? 0 : threadIdx.x >> 5, n_head = c.n_kv * a.group, item = AJ_WARPS == 1 ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+    const int row = item / n_head, h = item - row * n_head;
+    if (row >= c.n_rows) return;
+    const int s = seq_of_row_warp(c, row);
     if (s < 0) return;
     const int begin = min(max(c.first[s], 0), c.n_rows), count = min(max(c.first[s + 1], begin), c.n_rows) - begin;
     const int head = h / a.group, col = (row - begin) * a.group + h - head * a.group, ct = col / COLS, in_tile = col - ct * COLS;
@@ -486,22 +495,30 @@ __global__ void __launch_bounds__(AJ_WARPS * 32) k_kv4_join(const AttendArgs a) 
         }
         m = top;
     }
+    if constexpr (AJ_WARPS == 1) {
+        struct alignas(E * sizeof(T)) Dims { T v[E]; } y;
 #pragma unroll
-    for (int e = 0; e < E; e++) sums[warp][E * lane + e] = o[e];
-    if (lane == 0) { ml_s[warp][0] = m; ml_s[warp][1] = l; }
-    __syncthreads();
-    if (threadIdx.x < HD) {
-        float top = -INFINITY, total = 0.f, y = 0.f;
+        for (int e = 0; e < E; e++) y.v[e] = from_f<T>(l != 0.f ? o[e] / l : 0.f);
+        *reinterpret_cast<Dims *>(static_cast<T *>(a.out) + ((size_t) row * n_head + h) * HD + E * lane) = y;
+    } else {
+        __shared__ float sums[AJ_WARPS][HD], ml_s[AJ_WARPS][2];
 #pragma unroll
-        for (int i = 0; i < AJ_WARPS; i++) top = fmaxf(top, ml_s[i][0]);
-        const float base = top == -INFINITY ? 0.f : top;
+        for (int e = 0; e < E; e++) sums[warp][E * lane + e] = o[e];
+        if (lane == 0) { ml_s[warp][0] = m; ml_s[warp][1] = l; }
+        __syncthreads();
+        if (threadIdx.x < HD) {
+            float top = -INFINITY, total = 0.f, y = 0.f;
 #pragma unroll
-        for (int i = 0; i < AJ_WARPS; i++) {
-            const float by = exp2_fast(ml_s[i][0] - base);
-            total = fmaf(ml_s[i][1], by, total);
-            y = fmaf(sums[i][threadIdx.x], by, y);
+            for (int i = 0; i < AJ_WARPS; i++) top = fmaxf(top, ml_s[i][0]);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int i = 0; i < AJ_WARPS; i++) {
+                const float by = exp2_fast(ml_s[i][0] - base);
+                total = fmaf(ml_s[i][1], by, total);
+                y = fmaf(sums[i][threadIdx.x], by, y);
+            }
+            static_cast<T *>(a.out)[((size_t) row * n_head + h) * HD + threadIdx.x] = from_f<T>(total != 0.f ? y / total : 0.f);
         }
-        static_cast<T *>(a.out)[((size_t) row * n_head + h) * HD + threadIdx.x] = from_f<T>(total != 0.f ? y / total : 0.f);
     }
 }
 

@@ -50,12 +50,6 @@ __device__ __forceinline__ int page_at(const Cache & c, int slot, int pos) {
     const int page = c.table[(int64_t) slot * c.table_stride + i];
     return (unsigned) page < (unsigned) c.n_pages ? page : -1;
 }
-// the sequence that a row belongs to: the last one that begins at or before it; -1: none
-__device__ __forceinline__ int seq_of_row(const Cache & c, int row) {
-    int lo = 0, hi = c.n_seq;                                     // first[lo] <= row < first[hi], as far as first ascends
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (c.first[mid] <= row) lo = mid; else hi = mid; }
-    return c.first[lo] <= row && row < c.first[lo + 1] ? lo : -1;
-}
 __device__ __forceinline__ size_t tile_offset(const Cache & c, int page, int head, int pos, int tile_bytes) {
     const int tiles_log2 = c.page_log2 - 4;
     return (size_t) page * c.page_stride + (size_t) ((head << tiles_log2) + ((pos >> 4) & ((1 << tiles_log2) - 1))) * tile_bytes;
@@ -135,7 +129,7 @@ template <typename T> __device__ __forceinline__ uint32_t codes4(const float (&x
     return d == 0.f ? 0x8888u : w;
 }
 
-// the sequence of a row, looked for by a whole warp, 32 places at a time; -1: none
+// the sequence that a row belongs to, the last one that begins at or before it, looked for by a whole warp, 32 places at a time; -1: none
 __device__ __forceinline__ int seq_of_row_warp(const Cache & c, int row) {
     const int lane = threadIdx.x & 31;
     int s = 0, n = c.n_seq;
