@@ -5,7 +5,7 @@
 // with a partial result that k_kv4_join adds. So sequences of any lengths fill the card, and nothing is waited for inside.
 //   S^T = K Q^T: a tile's codes are the A operand of mma.sync (16 tokens x 16 dims), the columns the B operand. A block's 32 products are summed as codes and scaled once.
 //   O^T += V^T P^T: V's codes times their scales (exact in fp16) are the A operand (16 dims x 16 tokens); P^T comes from S^T by movmatrix.
-// Measured with 32 query heads on 8 of 128: HBM bounds long contexts (24 sequences of 12 000 to 32 000 tokens add 85 to 89 % of the copy rate's time), 13 us are the way to the first tile
+// Measured with 32 query heads on 8 of 128: HBM bounds long contexts (24 sequences of 12 000 to 32 000 tokens add 85 to 89 % of the copy rate's time), 10 to 13 us are the way to the first tile
 // (launch, row, slot, page, codes) and the last parts: 48 sequences of 90 to 4090 tokens (116 MB) 35 us, 200 of 500 (115 MB) 40 us, 3 of 21 000 to 32 700 under 64 heads on 8 (99 MB) 31 us, one of 333 tokens 9.6 us with the join.
 // P is rounded to fp16 (2^-11), the one rounding beside the output's; q is scaled by a power of two into fp16's range, which keeps its bits. Sums are fp32.
 #pragma once
