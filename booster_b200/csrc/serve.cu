@@ -236,8 +236,8 @@ static void check_heads(const b200_kv4 & c, int n_head, int max_rows) {
 }
 
 // Columns of a sequence (rows x query heads of a KV head) from which its tiles are worth making fp16 for the tensor cores' larger products. Where sequences x KV heads give the SMs few units
-// the finer pieces of the form for few rows pay longer. Few rows / many rows, us, 8 KV heads, group 4: one sequence of 8000 positions, 64 columns 25 / 39, 128 38 / 41, 256 64 / 47;
-// 8 of 2000, 32 columns 21 / 30, 64 32 / 31, 96 41 / 32; 48 of 3000, 32 columns 96 / 142, 64 175 / 144, 96 245 / 145
+// the finer pieces of the form for few rows pay longer. Few rows / many rows, us, 8 KV heads, group 4: one sequence of 8000 positions, 64 columns 25 / 38, 128 39 / 40, 256 64 / 44;
+// 8 of 2000, 48 columns 27 / 31, 64 32 / 31, 96 40 / 32; 48 of 3000, 48 columns 120 / 143, 64 151 / 144, 96 215 / 144
 bool is_prompt(const b200_kv4 & c, int group, int max_rows) { return (int64_t) group * max_rows > ((int64_t) c.n_seq * c.n_head_kv < 64 ? 128 : 48); }
 
 int64_t kv4_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
