@@ -67,7 +67,7 @@ template <typename K> void allow_smem(K * k, int device, size_t bytes, Limits & 
     set[device].store(bytes);
 }
 
-Cache checked(const b200_kv4 & c, bool writes) {
+Cache checked(const b200_kv4 & c) {
     need(c.head_dim == 64 || c.head_dim == 128, "kv4: head_dim is 64 or 128 (got " + std::to_string(c.head_dim) + ")");
     need(c.page_tokens >= 16 && c.page_tokens <= 1024 && (c.page_tokens & (c.page_tokens - 1)) == 0, "kv4: page_tokens is a power of two from 16 to 1024 (got " + std::to_string(c.page_tokens) + ")");
     need(c.n_head_kv >= 1 && c.n_head_kv <= 1024, "kv4: n_head_kv from 1 to 1024");
@@ -80,7 +80,6 @@ Cache checked(const b200_kv4 & c, bool writes) {
     need(c.pool && c.table && c.held && c.first, "kv4: null pointer");
     need(aligned(c.pool, 16), "kv4: the pool starts on 16 bytes");
     need(aligned(c.table, 4) && aligned(c.held, 4) && aligned(c.first, 4) && aligned(c.slots, 4), "kv4: tables of int32 start on 4 bytes");
-    (void) writes;
     return Cache{static_cast<uint8_t *>(c.pool), c.page_stride, c.n_pages, log2_of(c.page_tokens), c.n_head_kv, c.table, c.table_stride, c.n_slots, c.max_pages, c.held, c.slots, c.first, c.n_seq, c.n_rows};
 }
 void check_dtype(int dtype, bool f32) {
@@ -132,14 +131,13 @@ template <int HD, typename T> void attend_nt_as(const AttendArgs & a, int nt, in
 
 // attention of prompts' portions
 int64_t prompt_entries(const b200_kv4 & c, int group) { return (int64_t) c.n_rows * group / PR_COLS + c.n_seq + 1; }
-struct PromptWork { int64_t entries, entry_of, first, ml, part, bytes; };       // places in the workspace; `before` is first
+struct PromptWork { int64_t entries, first, ml, part, bytes; };       // places in the workspace; `before` is first
 PromptWork prompt_work(const b200_kv4 & c, int group, int sms) {
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     const int64_t n = prompt_entries(c, group), slots = 2 * (int64_t) sms * PR_COLS;
     PromptWork w;
     w.entries = up((n + 2) * 8);
-    w.entry_of = w.entries + up(n * (int64_t) sizeof(Entry));
-    w.first = w.entry_of + up((c.n_seq + 2) * 4);
+    w.first = w.entries + up(n * (int64_t) sizeof(Entry));
     w.ml = w.first + up((sms + 2) * 4);
     w.part = w.ml + up(slots * 8);
     w.bytes = w.part + slots * c.head_dim * 4;
@@ -209,7 +207,7 @@ template <typename T> void sample_as(const SampleArgs & a, int cluster, int devi
 }  // namespace
 
 void kv4_append(const b200_kv4 & c, int dtype, const void * k, int64_t k_row, int64_t k_head, const void * v, int64_t v_row, int64_t v_head) {
-    const Cache d = checked(c, true);
+    const Cache d = checked(c);
     check_dtype(dtype, true);
     need(c.n_rows == 0 || (k && v && aligned(k, size_of(dtype)) && aligned(v, size_of(dtype))), "kv4_append: k and v are pointers to whole entries");
     On on(c.device);
@@ -220,7 +218,7 @@ void kv4_append(const b200_kv4 & c, int dtype, const void * k, int64_t k_row, in
 }
 
 void kv4_read(const b200_kv4 & c, int dtype, void * k, void * v) {
-    const Cache d = checked(c, false);
+    const Cache d = checked(c);
     check_dtype(dtype, true);
     need(c.n_rows == 0 || (k && v && aligned(k, 16) && aligned(v, 16)), "kv4_read: k and v start on 16 bytes");
     On on(c.device);
@@ -241,7 +239,7 @@ static void check_heads(const b200_kv4 & c, int n_head, int max_rows) {
 bool is_prompt(const b200_kv4 & c, int group, int max_rows) { return (int64_t) group * max_rows > ((int64_t) c.n_seq * c.n_head_kv < 64 ? 128 : 48); }
 
 int64_t kv4_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
-    checked(c, false);
+    checked(c);
     check_heads(c, n_head, max_rows);
     On on(c.device);
     if (is_prompt(c, n_head / c.n_head_kv, max_rows)) return prompt_work(c, n_head / c.n_head_kv, on.sms).bytes;
@@ -250,7 +248,7 @@ int64_t kv4_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
 
 void kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int max_rows, void * out, void * work, int64_t work_bytes) {
     AttendArgs a = {};
-    a.c = checked(c, false);
+    a.c = checked(c);
     check_dtype(dtype, false);
     check_heads(c, n_head, max_rows);
     need(c.n_rows == 0 || (q && out && aligned(q, 2) && aligned(out, 16)), "kv4_attention: q points to whole entries, out starts on 16 bytes");
@@ -267,7 +265,7 @@ void kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row,
     if (is_prompt(c, a.group, max_rows)) {
         const PromptWork at = prompt_work(c, a.group, on.sms);
         check_work(work, work_bytes, at.bytes);
-        PromptArgs p = {a, (int) prompt_entries(c, a.group), reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.entry_of), reinterpret_cast<int *>(w + at.first), wait_flag(c.device)};
+        PromptArgs p = {a, (int) prompt_entries(c, a.group), reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.first), wait_flag(c.device)};
         if (*static_cast<volatile int *>(p.err)) {
             *static_cast<volatile int *>(p.err) = 0;
             throw std::runtime_error("a wait inside an earlier kv4_attention on this device ran out: its results are missing");

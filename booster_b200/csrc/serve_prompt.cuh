@@ -26,7 +26,7 @@ struct PromptArgs {
     AttendArgs a;                        // a.before: [entries + 1] tiles in front of each entry (a sequence's 256 columns), for all KV heads together
     int max_entries;                     // as many as rows and sequences can have, where first ascends; no more are looked at
     Entry * entries;
-    int * entry_of, * first;             // [n_seq + 1] a sequence's first entry; {tiles of a block's piece, total > 0, the entry that each block's piece begins in}
+    int * first;                         // tiles of a block's piece, entries, the entry that each block's piece begins in
     int * err;
 };
 
@@ -119,20 +119,18 @@ template <typename V> __device__ __forceinline__ V plan_before(V mine, V & all, 
 __global__ void __launch_bounds__(1024) k_kv4_prompt_plan(const PromptArgs p, int n_blocks) {
     extern __shared__ int entry_of[];                              // [n_seq + 1]
     __shared__ long long sums[32];
-    __shared__ int counts[32];
     const Cache & c = p.a.c;
     const int tid = threadIdx.x;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int all = 0;
     for (int s0 = 0; s0 < c.n_seq; s0 += 1024) {
         const int s = s0 + tid;
-        int some;
-        const int n = s < c.n_seq ? col_tiles(seq_at(c, s), p.a.group, PR_COLS) : 0, at = all + plan_before(n, some, counts);
-        if (s < c.n_seq) { entry_of[s] = at; p.entry_of[s] = at; }
-        all += some;
+        long long some;
+        const long long n = s < c.n_seq ? col_tiles(seq_at(c, s), p.a.group, PR_COLS) : 0, at = all + plan_before(n, some, sums);
+        if (s < c.n_seq) entry_of[s] = (int) min(at, (long long) p.max_entries);
+        all = (int) min(all + some, (long long) p.max_entries);
     }
-    all = min(all, p.max_entries);
-    if (tid == 0) { entry_of[c.n_seq] = all; p.entry_of[c.n_seq] = all; }
+    if (tid == 0) entry_of[c.n_seq] = all;
     __syncthreads();
     long long total = 0;
     for (int e0 = 0; e0 < all; e0 += 1024) {
