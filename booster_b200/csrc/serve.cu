@@ -59,10 +59,10 @@ void launch(void (*k)(P...), dim3 grid, int threads, size_t smem, void * stream,
     cu(cudaLaunchKernelEx(&cfg, k, static_cast<P>(args)...), "launch");
 }
 
-// a kernel's limit of dynamic shared memory, raised once on each device
+// a kernel's limit of dynamic shared memory, raised once on each device. (48 KB need no leave, but what a kernel holds statically counts towards them)
 typedef std::atomic<size_t> Limits[MAX_DEVICES];
 template <typename K> void allow_smem(K * k, int device, size_t bytes, Limits & set) {
-    if (bytes <= 8 * 1024 || set[device].load() >= bytes) return;   // (static shared memory counts towards the 48 KB that need no leave)
+    if (set[device].load() >= bytes) return;
     cu(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes), "cudaFuncSetAttribute");
     set[device].store(bytes);
 }
