@@ -21,7 +21,11 @@ using namespace srv;
 constexpr int MAX_DEVICES = 64;
 
 void need(bool ok, const std::string & what) { if (!ok) throw std::runtime_error(what); }
-void cu(cudaError_t e, const char * what) { if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e)); }
+void cu(cudaError_t e, const char * what) {
+    if (e == cudaSuccess) return;
+    cudaGetLastError();                  // (it is this call's: who asks next, the other operators of this library among them, does not find it)
+    throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+}
 
 // the call's device while it runs, the caller's again behind it
 struct On {

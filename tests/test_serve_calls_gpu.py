@@ -29,3 +29,34 @@ assert serve.pages_reserve(table, held, refs, ints([0, 20]), 16).item() == 0
 assert table[0].tolist() == [3, 4, -1, -1] and refs.sum().item() == 5
 print("done")
 """)
+
+
+def test_a_call_that_failed_leaves_no_error_behind():
+    """a launch that CUDA refuses (the legacy stream, while a stream that waits for it is captured) is that call's error and no other's"""
+    alone("""
+import ctypes as C
+import numpy as np, torch
+from cuda.bindings import runtime as rt
+from booster_b200 import _lib, serve
+L = _lib.lib()
+x = torch.randn(4, 1, 64, device="cuda", dtype=torch.float16)
+pool = serve.kv4_pool(2, 16, 1, 64)[0]
+table, held, first = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([[0, 1]], [0], [0, 4]))
+c = _lib.Kv4(device=0, n_pages=2, page_tokens=16, n_head_kv=1, head_dim=64, n_slots=1, max_pages=2, n_seq=1, n_rows=4, stream=None, pool=pool.data_ptr(), page_stride=18 * 64, table_stride=2,
+             table=table.data_ptr(), held=held.data_ptr(), slots=None, first=first.data_ptr())
+append = lambda: L.b200_kv4_append(C.byref(c), 2, x.data_ptr(), 64, 64, x.data_ptr(), 64, 64)
+assert append() == 0
+torch.cuda.synchronize()
+err, stream = rt.cudaStreamCreate()
+assert int(err) == 0
+assert int(rt.cudaStreamBeginCapture(stream, rt.cudaStreamCaptureMode.cudaStreamCaptureModeGlobal)[0]) == 0
+assert append() != 0 and "launch" in _lib.last_error(), _lib.last_error()
+rt.cudaStreamEndCapture(stream)
+while int(rt.cudaGetLastError()[0]): pass
+y, v = np.zeros(64, np.float32), np.ones(64, np.float32)
+f = C.POINTER(C.c_float)
+rc = L.b200_op_rms_norm(v.ctypes.data_as(f), None, 64, 1e-6, y.ctypes.data_as(f))
+assert rc == 0, _lib.last_error()
+assert append() == 0, _lib.last_error()
+print("done")
+""")
