@@ -449,12 +449,11 @@ __global__ void __launch_bounds__(AJ_WARPS == 1 ? 256 : AJ_WARPS * 32) k_kv4_joi
     const Cache & c = a.c;
     const int lane = threadIdx.x & 31, warp = AJ_WARPS == 1 ? 0 : threadIdx.x >> 5, n_head = c.n_kv * a.group, item = AJ_WARPS == 1 ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
     const int row = item / n_head, h = item - row * n_head;
-    if (row >= c.n_rows) return;
-    const int s = seq_of_row_warp(c, row);
-    if (s < 0) return;
-    const int begin = min(max(c.first[s], 0), c.n_rows), count = min(max(c.first[s + 1], begin), c.n_rows) - begin;
+    const int s = seq_of_row_warp(c, min(row, c.n_rows - 1)), begin = min(max(c.first[max(s, 0)], 0), c.n_rows), count = min(max(c.first[max(s, 0) + 1], begin), c.n_rows) - begin;
     const int head = h / a.group, col = (row - begin) * a.group + h - head * a.group, ct = col / COLS, in_tile = col - ct * COLS;
+    // every block waits, those without work too: this kernel's end is the next one's beginning, and the kernel in front still writes the workspace
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (row >= c.n_rows || s < 0) return;
     const long long b0 = a.before[s], b1 = a.before[s + 1];
     const int per = (int) a.before[c.n_seq + 1], len = (int) quotient(b1 - b0, (count * a.group + COLS - 1) / COLS * c.n_kv);
     const long long u0 = b0 + (long long) (ct * c.n_kv + head) * len;

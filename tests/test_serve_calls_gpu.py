@@ -1,13 +1,19 @@
 """Calls of booster_b200.serve and of its C entry points that a program may make beside those of tests/test_serve_gpu.py."""
+import ctypes as C
 import os
 import subprocess
 import sys
 
 import pytest
+import torch
+
+from booster_b200 import _lib, serve
+from tests.test_serve_gpu import F16, ints
 
 pytestmark = pytest.mark.gpu
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+MANY = 4096                              # rows announced: always the form for many
 
 
 def alone(program):
@@ -60,3 +66,21 @@ assert rc == 0, _lib.last_error()
 assert append() == 0, _lib.last_error()
 print("done")
 """)
+
+
+def test_a_step_whose_rows_belong_to_no_sequence():
+    """a captured step that idles: nothing is computed, but the kernels write their plan into the workspace, which is its owner's again behind the call"""
+    n, rows = 4096, 5
+    L = _lib.lib()
+    pool, table, held, first = serve.kv4_pool(1, 16, 2, 64)[0], ints([[0]] * n), ints([0] * n), ints([0] * (n + 1))
+    out = torch.full((rows, 64, 64), 7.0, dtype=F16, device="cuda")
+    q = torch.randn(rows, 64, 64, device="cuda").half()
+    for heads, max_rows in ((8, 1), (64, 1), (8, MANY)):
+        c = _lib.Kv4(device=0, n_pages=1, page_tokens=16, n_head_kv=2, head_dim=64, n_slots=n, max_pages=1, n_seq=n, n_rows=rows, stream=torch.cuda.current_stream().cuda_stream, pool=pool.data_ptr(),
+                     page_stride=2 * 18 * 64, table_stride=1, table=table.data_ptr(), held=held.data_ptr(), slots=None, first=first.data_ptr())
+        work = torch.empty(L.b200_kv4_attention_workspace(C.byref(c), heads, max_rows), dtype=torch.uint8, device="cuda")
+        for _ in range(50):
+            assert L.b200_kv4_attention(C.byref(c), 2, q.data_ptr(), 64 * 64, 64, heads, 1.0, 0, max_rows, out.data_ptr(), work.data_ptr(), work.numel()) == 0, _lib.last_error()
+            work.fill_(0x55)
+            assert (work == 0x55).all()
+    assert (out == 7).all()
