@@ -63,12 +63,17 @@ void launch(void (*k)(P...), dim3 grid, int threads, size_t smem, void * stream,
     cu(cudaLaunchKernelEx(&cfg, k, static_cast<P>(args)...), "launch");
 }
 
-// a kernel's limit of dynamic shared memory, raised once on each device. (48 KB need no leave, but what a kernel holds statically counts towards them)
-typedef std::atomic<size_t> Limits[MAX_DEVICES];
-template <typename K> void allow_smem(K * k, int device, size_t bytes, Limits & set) {
-    if (set[device].load() >= bytes) return;
-    cu(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes), "cudaFuncSetAttribute");
-    set[device].store(bytes);
+// leave for all the dynamic shared memory that a kernel can have beside what it holds statically, asked for once on each device. Calls of different sizes may come from several host threads:
+// the limit does not depend on the call, so threads that set it together set the same
+typedef std::atomic<bool> Limits[MAX_DEVICES];
+template <typename K> void allow_smem(K * k, int device, Limits & set) {
+    if (set[device].load()) return;
+    cudaFuncAttributes at;
+    int most = 0;
+    cu(cudaFuncGetAttributes(&at, k), "cudaFuncGetAttributes");
+    cu(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device), "cudaDeviceGetAttribute");
+    cu(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int) at.sharedSizeBytes), "cudaFuncSetAttribute");
+    set[device].store(true);
 }
 
 Cache checked(const b200_kv4 & c) {
@@ -119,7 +124,7 @@ template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, int d
     static Limits set;
     const size_t smem = at_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8;
     const auto kernel = k_kv4_attend<HD, NT, T>;
-    allow_smem(kernel, device, smem, set);
+    allow_smem(kernel, device, set);
     launch(kernel, dim3(sms * at_blocks(NT)), AT_WARPS * 32, smem, stream, false, 1, a);
     const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group;
     // parts a unit has on average, where every sequence has rows: few are one warp's to add, many sixteen's. One / four / sixteen warps, us, 8 KV heads: one sequence of 20 000 39 / 22 / 16,
@@ -167,7 +172,7 @@ int * wait_flag(int device) {
 template <int HD, typename T> void prompt_as(const PromptArgs & p, int64_t entries, int device, int sms, void * stream) {
     static Limits set;
     const auto kernel = k_kv4_prompt<HD, T>;
-    allow_smem(kernel, device, PromptSmem<HD>::BYTES, set);
+    allow_smem(kernel, device, set);
     launch(k_kv4_prompt_plan, dim3(1), 1024, (size_t) (p.a.c.n_seq + 1) * 4, stream, false, 1, p, sms);
     launch(kernel, dim3(sms), PR_THREADS, PromptSmem<HD>::BYTES, stream, true, 1, p);
     launch(k_kv4_prompt_join<HD, T>, dim3((unsigned) (entries * (PR_COLS / 32)), (unsigned) p.a.c.n_kv), 256, 0, stream, true, 1, p);
@@ -204,7 +209,7 @@ void move_pages(const b200_pages & p, const Pages & d, const int32_t * plan, int
 template <typename T> void sample_as(const SampleArgs & a, int cluster, int device, void * stream) {
     static Limits set;
     const size_t smem = SA_FIXED + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
-    allow_smem(k_sample<T>, device, smem, set);
+    allow_smem(k_sample<T>, device, set);
     launch(k_sample<T>, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, false, cluster, a);
 }
 
@@ -305,7 +310,7 @@ void pages_reserve(const b200_pages & p, const int32_t * slots, const int32_t * 
     On on(p.device);
     static Limits set;
     const size_t smem = words_bytes(p.n_pages) + words_bytes(p.n_slots);
-    allow_smem(k_pages_reserve, p.device, smem, set);
+    allow_smem(k_pages_reserve, p.device, set);
     launch(k_pages_reserve, dim3(1), PG_THREADS, smem, p.stream, false, 1, d, slots, first, n, status);
 }
 
@@ -317,7 +322,7 @@ void pages_fork(const b200_pages & p, const int32_t * parents, const int32_t * c
     On on(p.device);
     static Limits set;
     const size_t smem = words_bytes(p.n_pages) + words_bytes(p.n_slots);
-    allow_smem(k_pages_fork, p.device, smem, set);
+    allow_smem(k_pages_fork, p.device, set);
     int32_t * plan = static_cast<int32_t *>(work);
     launch(k_pages_fork, dim3(1), PG_THREADS, smem, p.stream, false, 1, d, parents, children, n, status, plan);
     move_pages(p, d, plan, n, true, nullptr, on.sms);
@@ -338,7 +343,7 @@ void pages_compact(const b200_pages & p, int32_t * live, void * work, int64_t wo
     On on(p.device);
     static Limits set;
     const size_t smem = words_bytes(p.n_pages);
-    allow_smem(k_pages_compact, p.device, smem, set);
+    allow_smem(k_pages_compact, p.device, set);
     int32_t * plan = static_cast<int32_t *>(work);
     launch(k_pages_compact, dim3(1), PG_THREADS, smem, p.stream, false, 1, d, live, plan);
     move_pages(p, d, plan, p.n_pages, false, plan + PLAN_HEAD + 2 * (size_t) p.n_pages, on.sms);
@@ -352,7 +357,7 @@ void pages_copy(const b200_pages & p, const int32_t * src, const int32_t * dst, 
     On on(p.device);
     static Limits set;
     const size_t smem = words_bytes(p.n_pages);
-    allow_smem(k_pages_check_copy, p.device, smem, set);
+    allow_smem(k_pages_check_copy, p.device, set);
     int32_t * plan = static_cast<int32_t *>(work);
     launch(k_pages_check_copy, dim3(1), PG_THREADS, smem, p.stream, false, 1, d, src, dst, n, status, plan);
     move_pages(p, d, plan, n, true, nullptr, on.sms);

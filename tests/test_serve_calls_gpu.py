@@ -68,6 +68,46 @@ print("done")
 """)
 
 
+def test_threads_with_calls_of_different_sizes():
+    """two host threads ask for different amounts of shared memory for the same kernels at the same time: each gets its own, and so does every call behind them"""
+    alone("""
+import ctypes as C, threading
+import torch
+from booster_b200 import _lib, serve
+L = _lib.lib()
+N = 4096
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+pool, table, held, first = serve.kv4_pool(1, 16, 1, 64)[0], torch.zeros(N, 1, dtype=torch.int32, device="cuda"), ints([0] * N), ints([0] + [1] * N)
+logits = torch.zeros(1, 1 << 18, device="cuda")
+class Caller:
+    def __init__(self, me):
+        self.stream = torch.cuda.Stream()
+        self.q, self.out = (torch.zeros(1, 1, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+        self.work = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+        self.u, self.ids = torch.zeros(1, device="cuda"), ints([0])
+        self.steps = [_lib.Kv4(device=0, n_pages=1, page_tokens=16, n_head_kv=1, head_dim=64, n_slots=N, max_pages=1, n_seq=2 * i + me, n_rows=1, stream=self.stream.cuda_stream,
+                               pool=pool.data_ptr(), page_stride=18 * 64, table_stride=1, table=table.data_ptr(), held=held.data_ptr(), slots=None, first=first.data_ptr()) for i in range(1, 2000)]
+        # (the addresses are made ready: between two calls stands as little as can be)
+        self.attends = [(C.byref(c), 2, self.q.data_ptr(), 64, 64, 1, 1.0, 0, 1, self.out.data_ptr(), self.work.data_ptr(), self.work.numel()) for c in self.steps]
+        self.samples = [(0, self.stream.cuda_stream, 0, logits.data_ptr(), 1 << 18, 1, 128 * i + 64 * me, self.u.data_ptr(), None, None, None, None, self.ids.data_ptr(), None) for i in range(1, 2000)]
+bad, gate = [], threading.Barrier(2)
+def run(caller, call, all_args):
+    gate.wait()
+    for args in all_args:
+        if call(*args): bad.append((call.__name__, args[6], _lib.last_error()))
+callers = [Caller(0), Caller(1)]
+torch.cuda.synchronize()
+for call, name in ((L.b200_kv4_attention, "attends"), (L.b200_sample, "samples")):
+    threads = [threading.Thread(target=run, args=(c, call, getattr(c, name))) for c in callers]
+    [t.start() for t in threads]; [t.join() for t in threads]
+for args in callers[0].attends[::3]:                                  # and one after the other
+    if L.b200_kv4_attention(*args): bad.append(("later", args[6], _lib.last_error()))
+torch.cuda.synchronize()
+assert not bad, (len(bad), bad[:5])
+print("done")
+""")
+
+
 def test_a_step_whose_rows_belong_to_no_sequence():
     """a captured step that idles: nothing is computed, but the kernels write their plan into the workspace, which is its owner's again behind the call"""
     n, rows = 4096, 5
