@@ -7,7 +7,10 @@
 //   O^T += V^T P^T: V's codes times their scales (exact in fp16) are the A operand (16 dims x 16 tokens); P^T comes from S^T by movmatrix.
 // Measured with 32 query heads on 8 of 128: HBM bounds long contexts (24 sequences of 12 000 to 32 000 tokens add 85 to 89 % of the copy rate's time), 10 to 13 us are the way to the first tile
 // (launch, row, slot, page, codes) and the last parts: 48 sequences of 90 to 4090 tokens (116 MB) 35 us, 200 of 500 (115 MB) 40 us, 3 of 21 000 to 32 700 under 64 heads on 8 (99 MB) 31 us, one of 333 tokens 9.6 us with the join.
-// P is rounded to fp16 (2^-11), the one rounding beside the output's; q is scaled by a power of two into fp16's range, which keeps its bits. Sums are fp32.
+// Roundings: P to fp16 (2^-11, see P_LIFT); sums of scores and values, fp32 as the tensor cores add; the result. q is scaled by a power of two into fp16's range, which keeps its bits. With one
+// column tile the codes' offset is taken off inside the sums of scores (FOLD): their terms are up to 1039 times q's entries, up to 8 times with two tiles and in serve_prompt.cuh. Seen where
+// scores are very large: fp16 results for scores up to 169 are off by 1.80e-4 (rms; 1.65e-4 without, of which 1.59e-4 the result's rounding), up to 21 by 1.42e-4 either way. Without: 48 ragged
+// sequences 35.1 us for 34.9, 3 long 31.2 for 30.7.
 #pragma once
 #include "serve_cache.cuh"
 
@@ -32,6 +35,10 @@ struct AttendArgs {
 constexpr int AT_WARPS = 4, AT_MAX_SEQ = 4096, AT_STAGES = 3, AT_OVER = 3;      // AT_OVER: what beginning a unit costs, in pairs of tiles (48 ragged sequences 49, 42, 38, 37, 37 us with 0 to 4)
 __host__ __device__ constexpr int at_blocks(int nt) { return nt == 1 ? 3 : 2; }          // resident on an SM: 168 and 255 registers a thread
 __host__ __device__ constexpr size_t at_ring_bytes(int hd) { return (size_t) AT_WARPS * AT_STAGES * 36 * hd; }
+// P = 2^(score - base) is rounded to fp16, whose steps below 2^-14 are 2^-24. base is P_LIFT below the largest score, so that weights keep their 11 bits down to 2^-21 of the largest one, and what
+// is left out of any is below 2^-32 of it: over 2^17 tokens behind one that takes most of the weight 2^-15 of the largest value, less than the output's rounding. base moves when a score passes the
+// largest so far by 2^P_PASS; P stays within 2^15 until then. (2^4 and 11: 2^-36, but 48 ragged sequences 35.2 us for 34.9, 512 rows at 6000 74.0 for 70.5, 8192 rows 582 for 557)
+constexpr float P_PASS = 8.f, P_LIFT = 7.f;
 __device__ __forceinline__ uint32_t smem_at(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
 // 16 bytes from src, or zeros where bytes is 0
 template <int AT> __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t * src, int bytes) {
@@ -259,7 +266,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, at_blocks(NT)) k_kv4_attend(con
         }
         const int row_lo = ct * COLS / a.group, row_hi = min(q.count - 1, (ct * COLS + COLS - 1) / a.group);
         const int all_see_hi = q.held + row_lo, all_see_lo = a.window > 0 ? q.held + row_hi - a.window + 1 : 0;   // positions that every column sees
-        float o[NT][2 * NB][4], m[NT][2], l[NT][2], base[NT][2], limit[NT][2];       // base: what is taken off scores; limit: where the maximum moves
+        float o[NT][2 * NB][4], m[NT][2], l[NT][2], base[NT][2], limit[NT][2];       // m: the largest score less P_LIFT; base: what is taken off scores, m or 0; limit: where they move
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, at_blocks(NT)) k_kv4_attend(con
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) more = more || fmaxf(fmaxf(st[0][n][j], st[0][n][j + 2]), fmaxf(st[1][n][j], st[1][n][j + 2])) > limit[n][j];
-            // the maximum moves only when a score passes it by 2^8: P stays in fp16's range below that
+            // base moves when a score passes the largest so far by 2^P_PASS
             if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
@@ -355,10 +362,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32, at_blocks(NT)) k_kv4_attend(con
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        const float top = fmaxf(m[n][j], x), down = top > m[n][j] ? exp2_fast(m[n][j] - top) : 1.f;
+                        const float top = fmaxf(m[n][j], x - P_LIFT), down = top > m[n][j] ? exp2_fast(m[n][j] - top) : 1.f;
                         m[n][j] = top;
                         base[n][j] = top == -INFINITY ? 0.f : top;
-                        limit[n][j] = top + 8.f;
+                        limit[n][j] = top + (P_LIFT + P_PASS);
                         l[n][j] *= down;
 #pragma unroll
                         for (int k = 0; k < 2 * NB; k++) { o[n][k][j] *= down; o[n][k][j + 2] *= down; }

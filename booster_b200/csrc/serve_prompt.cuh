@@ -12,7 +12,8 @@
 // Sixteen soft-max warps, exponentials in part by polynomials, K made a tile ahead of V and other shares of registers were no faster; one issuing thread 595 us, one turn of 128 tokens 4 % more.
 // Tensor memory: S and P [2 halves][2 turns][64 columns], O [2][head_dim]. Each half has two turns of S, so that the scores of the next 64 tokens are there when those in hand are done with.
 // Tokens of 32 stand as n = 8 c + 4 u + i for token 16 u + c + 4 i in S, P, K and V alike, and dims of 8 as 0 4 1 5 2 6 3 7 in Q and K: the orders in which a word's codes come apart.
-// P is rounded to fp16 (2^-11), q scaled by a power of two into fp16's range; sums are fp32. The maximum moves when a score passes it by 2^8; O is scaled in tensor memory then.
+// P is rounded to fp16 (2^-11; P_LIFT and P_PASS in serve_attn.cuh say what that leaves out), q scaled by a power of two into fp16's range; sums are fp32. O is scaled in tensor memory where the
+// base of P moves.
 // Every wait on an mbarrier is bounded: on a timeout the block raises *err, skips what is left and frees its tensor memory.
 #pragma once
 #include "serve_attn.cuh"
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 }
                 const float high = fmaxf(x0, x1), score = high == -INFINITY ? high : high * factor;
                 if (__any_sync(0xffffffffu, score > limit)) {
-                    const float top = fmaxf(m, score), down = top > m ? exp2_fast(m - top) : 1.f;
+                    const float top = fmaxf(m, score - P_LIFT), down = top > m ? exp2_fast(m - top) : 1.f;
                     if (t > 2 * g.t0 && __any_sync(0xffffffffu, down != 1.f)) {
                         pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), dead);
                         __syncwarp();
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                     }
                     m = top;
                     base = top == -INFINITY ? 0.f : top;
-                    limit = top + 8.f;
+                    limit = top + (P_LIFT + P_PASS);
                     l *= down;
                 }
                 const uint64_t by = two(factor, factor), less = two(-base, -base);

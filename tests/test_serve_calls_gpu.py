@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from booster_b200 import _lib, serve
-from tests.test_serve_gpu import F16, ints
+from tests.test_serve_gpu import BF16, F16, F32, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +124,31 @@ def test_a_step_whose_rows_belong_to_no_sequence():
             work.fill_(0x55)
             assert (work == 0x55).all()
     assert (out == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,max_rows", [(4, 1), (64, 1), (4, MANY)])
+def test_weights_far_below_the_largest(heads, max_rows, dtype):
+    """one position stands `above` over all others and has a value of 0, as the first token of a long text does: the result is what the others say, however small their weights. Pieces hold
+    whole sequences here, so that all weights stand against that one. What is left out of P by its rounding is half a step of 2^-24 of weights whose largest is 2^7 or more; a thousand tokens'
+    sums in fp32 add less than 1000 x 2^-23"""
+    n, kv, hd, held = 600, 4, 64, 1999
+    pool = serve.kv4_pool(125, 16, kv, hd)
+    table = ints([list(range(125))]).expand(n, 125).contiguous()
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    k = torch.zeros(held + 1, kv, hd, device="cuda")
+    k[0, :, 0] = 8.0
+    v = 0.25 + torch.rand(held + 1, kv, hd, generator=gen, device="cuda")
+    v[0] = 0
+    serve.kv4_append(pool[0], table, ints([0] * n), ints([0, held + 1]), k, v)
+    k, v = (x.double() for x in serve.kv4_read(pool[0], table, ints([0] * n), ints([0, held + 1]), held + 1, F32))
+    for above in (4.0, 9.0, 13.0, 17.5):
+        q = torch.zeros(n, heads, hd, device="cuda", dtype=dtype)
+        q[:, :, 0] = above / 8
+        assert (q[0, 0, 0].item() * k[0, 0, 0].item()) == above
+        out = serve.kv4_attention(q, pool[0], table, ints([held] * n), ints(list(range(n + 1))), scale=1.0, max_rows=max_rows).double()
+        w = torch.softmax(k[:, 0, 0] * above / 8, 0)
+        want = torch.einsum("t,thd->hd", w, v).repeat_interleave(heads // kv, 0)
+        room = want * (2.0 ** -11 + 2.0 ** -13) + 2.0 ** -32 * v.abs().sum(0).repeat_interleave(heads // kv, 0)
+        room = room + torch.finfo(dtype).eps / 2 * (want + room) + (2.0 ** -25 if dtype == F16 else 0.0)
+        assert ((out - want).abs() <= room).all(), (above, ((out - want).abs() / want).max().item())
