@@ -81,6 +81,12 @@ __device__ __forceinline__ void codes8_raw(uint32_t w, uint32_t (&p)[4]) {
         p[2 * i + 1] = pick(x, 0x00f000f0u, 0x64006400u);
     }
 }
+// what a column's query is multiplied with: a power of two that brings its largest entry to 2^13 .. 2^14 (2^126 at most, of zeros too). An infinity's scores are infinities or NaN, whose
+// soft-max is no number: they all become NaN, since negative ones look like masked ones
+__device__ __forceinline__ float query_scale(float top) {
+    const int e = (int) (__float_as_uint(top) >> 23);
+    return e == 255 ? NAN : __uint_as_float((uint32_t) min(253, max(1, 267 - e)) << 23);
+}
 // less 8
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&p)[4]) {
     const __half2 eight = as_h2(0xe408e408u), sixteenth = as_h2(0x2c002c00u), seventy_two = as_h2(0xd480d480u);   // -1032, 1 / 16, -72
@@ -232,9 +238,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, at_blocks(NT)) k_kv4_attend(con
                 for (int j = 0; j < 8; j++) { v[b][j] = to_f(raw[n][b].v[j]); top = fmaxf(top, fabsf(v[b][j])); }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // a power of two that brings the column's largest entry to 2^13 .. 2^14
-            const int e = min(126, max(-126, 140 - (int) (__float_as_uint(top) >> 23)));
-            const float up = top > 0.f && top < INFINITY ? __uint_as_float((uint32_t) (127 + e) << 23) : 1.f;
+            const float up = top > 0.f ? query_scale(top) : 1.f;           // (a quotient by 2^126 takes the slow way of divisions, and columns without a query would)
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll

@@ -271,8 +271,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                         for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(query_entry<T>(f[x], j)));
 #pragma unroll
                         for (int d = 1; d < LANES; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const int e = min(126, max(-126, 140 - (int) (__float_as_uint(top) >> 23)));
-                        float up = top > 0.f && top < INFINITY ? __uint_as_float((uint32_t) (127 + e) << 23) : 1.f;
+                        float up = query_scale(top);
                         const float mine_up = __shfl_sync(0xffffffffu, up, (lane % ROWS) * LANES);
                         if (lane / ROWS == x0 / ROWS + x) factor = mine_up;
                         if (a.scale_log2 < 0.f) up = -up;

@@ -370,7 +370,7 @@ int b200_kv4_append(const b200_kv4 * c, int dtype, const void * k, int64_t k_row
 int b200_kv4_read(const b200_kv4 * c, int dtype, void * k, void * v);
 /* attention of the step's rows, after b200_kv4_append of the same step: out[row][head] = sum over the positions j that the row sees of softmax(scale q . k_j) v_j, in
  * [n_rows][n_head][head_dim]; q[row * q_row + head * q_head + i], dtype BF16 or F16. A row at position p sees j <= p, with window > 0 only j > p - window, and no position
- * whose page is absent; a row that sees nothing answers 0. n_head is a multiple of n_head_kv. max_rows: no sequence has more rows (it chooses kernels; further rows of a sequence
+ * whose page is absent; a row that sees nothing answers 0, one whose query holds an infinity or a NaN and that sees something NaN. n_head is a multiple of n_head_kv. max_rows: no sequence has more rows (it chooses kernels; further rows of a sequence
  * that has are still computed). work: b200_kv4_attention_workspace() bytes (-1: error) on 16 bytes. */
 int64_t b200_kv4_attention_workspace(const b200_kv4 * c, int n_head, int max_rows);
 int b200_kv4_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int max_rows, void * out, void * work, int64_t work_bytes);

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from booster_b200 import _lib, serve
-from tests.test_serve_gpu import BF16, F16, F32, ints
+from tests.test_serve_gpu import BF16, F16, F32, Case, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +152,26 @@ def test_weights_far_below_the_largest(heads, max_rows, dtype):
         room = want * (2.0 ** -11 + 2.0 ** -13) + 2.0 ** -32 * v.abs().sum(0).repeat_interleave(heads // kv, 0)
         room = room + torch.finfo(dtype).eps / 2 * (want + room) + (2.0 ** -25 if dtype == F16 else 0.0)
         assert ((out - want).abs() <= room).all(), (above, ((out - want).abs() / want).max().item())
+
+
+@pytest.mark.parametrize("heads,max_rows", [(2, 1), (32, 1), (2, MANY)])
+def test_queries_that_are_not_finite(heads, max_rows):
+    """a product with an infinity is an infinity or a NaN, and no soft-max of such scores is a number: the row's head answers NaN, and 0 where it sees nothing. Other rows do not notice"""
+    c = Case([0, 40, 7], [1, 1, 1], kv=2, hd=64)
+    c.fill()
+    k = -torch.ones(c.rows, 2, 64, device="cuda").half()                # the first sequence sees one position; every score with a query of one infinity is an infinity of one sign
+    v = c.randn(c.rows, 2, 64).half()
+    serve.kv4_append(*c.args(), k, v, c.slots)
+    q = c.randn(c.rows, heads, 64).half()
+    right = serve.kv4_attention(q, *c.args(), slots=c.slots, max_rows=max_rows)
+    for x in (float("inf"), -float("inf"), float("nan")):
+        for row in range(c.rows):
+            bad = q.clone()
+            bad[row, 1] = 0
+            bad[row, 1, 9] = x
+            out = serve.kv4_attention(bad, *c.args(), slots=c.slots, max_rows=max_rows)
+            assert torch.isnan(out[row, 1]).all(), (x, row)
+            out[row, 1] = right[row, 1]
+            assert torch.equal(out, right)
+            none = torch.full_like(c.table, -1)
+            assert not serve.kv4_attention(bad, c.pool[0], none, c.held, c.first, c.slots, max_rows=max_rows).any()
