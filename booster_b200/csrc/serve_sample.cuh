@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     u64 * fine = list + SA_LIST;                                         // [SA_FINE] sums
     int * fine_count = reinterpret_cast<int *>(fine + SA_FINE), * bins = fine_count + SA_FINE;
     T * vals = reinterpret_cast<T *>(bins + SA_BINS);
-    const float temperature = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f, u = a.u[row];
+    const float temperature = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, u = a.u[row];
     const int k_all = a.top_k ? a.top_k[row] : 0, k = k_all > 0 && k_all < a.n_vocab ? k_all : 0;
     const bool by_p = top_p < 1.f, cut = temperature > 0.f && (k > 0 || by_p);
     int turn = 0;
@@ -236,10 +236,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     const float from_1 = fmaxf((float) ((double) top - 30.0), -MOST), from_t = fmaxf((float) ((double) top - 30.0 * (double) temperature), -MOST);
     const auto weight = [&](float v) { return fixed_weight((double) fminf(v, MOST) - top_d, steps, v >= from_1, sm.table); };
     const auto tempered = [&](float v, bool in) { return fixed_weight((double) fminf(v, MOST) - top_d, steps_cold, in, sm.table); };
-    // min-p keeps the logits from from_p on, the smallest float that is at most -log(min_p) below the largest
+    // min-p keeps the logits from from_p on, the smallest float that is at most -log(min_p) below the largest (all where min_p is NaN, as top-p does)
     float from_p = -INFINITY;
     if (min_p > 0.f) {
-        const double far = -log((double) min_p);
+        const double far = min_p < 1.f ? -log((double) min_p) : 0.0;
         from_p = fminf((float) ((double) top - far), top);
         for (int j = 0; j < 4 && exactly(from_p) > far; j++) from_p = nextafterf(from_p, INFINITY);
         for (int j = 0; j < 4 && exactly(nextafterf(from_p, -INFINITY)) <= far; j++) from_p = nextafterf(from_p, -INFINITY);

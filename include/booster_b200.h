@@ -400,7 +400,8 @@ int b200_pages_copy(const b200_pages * p, const int32_t * src, const int32_t * d
 /* The draw of one token a row from logits[row * row_stride + i], dtype F32, BF16 or F16, n_vocab up to 2^18, in the order of b200_sampler's chain: of the tokens by
  * descending logit (lower index first among equals) the first top_k[row] (<= 0: all); of those the shortest prefix with at least the share top_p[row] of their weight
  * exp(logit - largest) (>= 1: all; the first always); of those with a weight of at least min_p[row]; of what is left, token i with the weight exp((logit - largest) / temperature[row]):
- * ids[row] is the first in order of index at which the sum passes u[row] (0 <= u < 1) of the total. temperature <= 0: the first of the largest. NULL: 1, 0, 1, 0.
+ * ids[row] is the first in order of index at which the sum passes u[row] (0 <= u < 1) of the total. temperature <= 0: the first of the largest. NULL: 1, 0, 1, 0. A top_p or min_p
+ * that is NaN filters nothing.
  * logprobs (may be NULL): log of the drawn token's share (0 at temperature <= 0). NaN counts as -infinity; a row of nothing else gives -1 and -infinity. */
 int b200_sample(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature, const int32_t * top_k,
                 const float * top_p, const float * min_p, int32_t * ids, float * logprobs);

@@ -1,5 +1,6 @@
 """Calls of booster_b200.serve and of its C entry points that a program may make beside those of tests/test_serve_gpu.py."""
 import ctypes as C
+import math
 import os
 import subprocess
 import sys
@@ -175,3 +176,16 @@ def test_queries_that_are_not_finite(heads, max_rows):
             assert torch.equal(out, right)
             none = torch.full_like(c.table, -1)
             assert not serve.kv4_attention(bad, c.pool[0], none, c.held, c.first, c.slots, max_rows=max_rows).any()
+
+
+def test_a_min_p_that_is_no_number_filters_nothing():
+    """as a top_p that is none does"""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rows, u = torch.randn(64, 1000, generator=gen, device="cuda"), torch.rand(64, generator=gen, device="cuda")
+    nan = torch.full((64,), math.nan, device="cuda")
+    for more in ({}, dict(top_k=ints([30] * 64)), dict(top_p=torch.full((64,), 0.9, device="cuda"))):
+        want = serve.sample(rows, u, **more)
+        for name in ("min_p", "top_p"):
+            if name not in more:
+                got = serve.sample(rows, u, **more, **{name: nan})
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), name
