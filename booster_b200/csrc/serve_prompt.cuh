@@ -497,6 +497,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 if (t + 1 < g.t1) ask(t + 1);
             }
         }
+        for (int i = max(0, n - 2); i < n; i++) {                          // the last tiles are let go: their commits arrive while the block's shared memory is its own
+            pr_wait(smem_at(&k_empty[i & 1]), (uint32_t) (i >> 1 & 1), dead);
+            pr_wait(smem_at(&v_empty[i & 1]), (uint32_t) (i >> 1 & 1), dead);
+        }
     } else {
         regs_less<64>();
         const int half = warp - 12;

@@ -178,6 +178,25 @@ def test_queries_that_are_not_finite(heads, max_rows):
             assert not serve.kv4_attention(bad, c.pool[0], none, c.held, c.first, c.slots, max_rows=max_rows).any()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_calls_one_behind_the_other_repeat_themselves(hd):
+    """blocks of one call begin where those of another have just ended, with barriers and tiles in the same shared memory: every call gives the bits that it gave alone"""
+    cases = [Case([300, 0, 77], [200, 65, 130], page=32, kv=2, hd=hd, seed=1), Case([2000], [40], page=16, kv=4, hd=hd, seed=2), Case([50] * 40, [1] * 40, page=16, kv=2, hd=hd, seed=3)]
+    calls = []
+    for c, most in zip(cases, (MANY, MANY, 1)):
+        c.fill()
+        q = c.randn(c.rows, 8, hd).half()
+        calls.append(lambda c=c, q=q, most=most: serve.kv4_attention(q, *c.args(), slots=c.slots, max_rows=most))
+    alone = []
+    for call in calls:
+        torch.cuda.synchronize()
+        alone.append(call())
+        torch.cuda.synchronize()
+    outs = [[call() for call in calls] for _ in range(100)]
+    for out in outs:
+        assert all(torch.equal(x, y) for x, y in zip(out, alone))
+
+
 def test_a_min_p_that_is_no_number_filters_nothing():
     """as a top_p that is none does"""
     gen = torch.Generator(device="cuda").manual_seed(3)
