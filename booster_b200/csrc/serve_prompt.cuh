@@ -561,12 +561,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
             if (half < g.halves) { n_q++; n_p += steps; }
         }
     }
-    if (dead) {
-        atomicExch_system(p.err, 1);
-        for (int j = 0; j < 1000; j++) __nanosleep(1000);      // products under way end before shared and tensor memory are given back
-    }
+    if (dead) atomicExch_system(p.err, 1);
     pr_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(dead))                                            // nobody issues any more: products under way end before shared and tensor memory are given back
+        for (int j = 0; j < 1000; j++) __nanosleep(1000);
     if (warp == 12) {
         pr_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem));
