@@ -27,7 +27,7 @@ B200_SYMBOLS = ["b200_last_error", "b200_device_count", "b200_version", "b200_mo
                 "b200_op_attention", "b200_op_attention_one_launch", "b200_op_attention_cluster", "b200_set_attention_route", "b200_tokenizer_load", "b200_tokenizer_free", "b200_tokenizer_n_vocab", "b200_tokenize",
                 "b200_token_to_piece", "b200_token_is_eog", "b200_token_nl", "b200_cpt_class", "b200_op_launch_shape", "b200_op_lanes_shape", "b200_op_score_tokens", "b200_op_prompt_kernel",
                 "b200_sampler_new", "b200_sampler_set_standard", "b200_sampler_free", "b200_sampler_reset", "b200_sampler_sample",
-                "b200_kv4_append", "b200_kv4_read", "b200_kv4_attention_workspace", "b200_kv4_attention", "b200_pages_workspace", "b200_pages_reserve", "b200_pages_fork",
+                "b200_kv4_append", "b200_kv4_read", "b200_kv4_attention_workspace", "b200_kv4_attention", "b200_kv4_status", "b200_kv4_drill", "b200_pages_workspace", "b200_pages_reserve", "b200_pages_fork",
                 "b200_pages_free", "b200_pages_compact", "b200_pages_copy", "b200_sample"]
 
 
@@ -169,6 +169,8 @@ def lib() -> C.CDLL:
     sig("b200_kv4_read", C.c_int, [kp, C.c_int, vp, vp])
     sig("b200_kv4_attention_workspace", C.c_int64, [kp, C.c_int, C.c_int])
     sig("b200_kv4_attention", C.c_int, [kp, C.c_int, vp, C.c_int64, C.c_int64, C.c_int, C.c_float, C.c_int, C.c_int, vp, vp, C.c_int64])
+    sig("b200_kv4_status", C.c_int, [C.c_int])
+    sig("b200_kv4_drill", None, [C.c_int])
     sig("b200_pages_workspace", C.c_int64, [pp, C.c_int])
     sig("b200_pages_reserve", C.c_int, [pp, vp, vp, C.c_int, vp])
     sig("b200_pages_fork", C.c_int, [pp, vp, vp, C.c_int, vp, vp, C.c_int64])

@@ -3124,6 +3124,8 @@ extern "C" int b200_kv4_attention(const b200_kv4 * c, int dtype, const void * q,
                                   int64_t work_bytes) {
     return served("b200_kv4_attention", c, [&] { kv4_attention(*c, dtype, q, q_row, q_head, n_head, scale, window, max_rows, out, work, work_bytes); });
 }
+extern "C" int b200_kv4_status(int device) { return served("b200_kv4_status", "", [&] { kv4_status(device); }); }
+extern "C" void b200_kv4_drill(int polls) { kv4_drill(polls); }
 extern "C" int64_t b200_pages_workspace(const b200_pages * p, int n) {
     int64_t bytes = -1;
     served("b200_pages_workspace", p, [&] { bytes = pages_workspace(*p, n); });

@@ -47,6 +47,30 @@ struct On {
     ~On() { if (was >= 0 && was != device) cudaSetDevice(was); }
 };
 
+// A word per device that k_kv4_prompt raises when a bounded wait ran out, in pinned memory, so that the host reads it without waiting. Every call looks at it
+std::atomic<int *> wait_words[MAX_DEVICES];
+std::atomic<int> drill_polls;                                            // b200_kv4_drill
+int * wait_word(int device) {
+    static std::mutex lock;
+    if (int * w = wait_words[device].load()) return w;
+    std::lock_guard<std::mutex> hold(lock);
+    if (int * w = wait_words[device].load()) return w;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;             // (this may be the first call inside a capture)
+    cu(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+    void * p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cu(e, "cudaHostAlloc");
+    *static_cast<volatile int *>(p) = 0;
+    wait_words[device].store(static_cast<int *>(p));
+    return static_cast<int *>(p);
+}
+void heed_waits(int device) {
+    int * w = wait_words[device].load();
+    if (w && *static_cast<volatile int *>(w) && __atomic_exchange_n(w, 0, __ATOMIC_ACQ_REL))
+        throw std::runtime_error("a wait inside an earlier kv4_attention on this device ran out: its results are worthless. This call has done nothing");
+}
+
 bool aligned(const void * p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 int log2_of(int x) { int l = 0; while ((1 << l) < x) l++; return l; }
 int size_of(int dtype) { return dtype == B200_DTYPE_F32 ? 4 : 2; }
@@ -152,23 +176,6 @@ PromptWork prompt_work(const b200_kv4 & c, int group, int sms) {
     w.bytes = w.part + slots * c.head_dim * 4;
     return w;
 }
-// a word per device that a kernel raises when a bounded wait ran out, in pinned memory, so that the host reads it without waiting. It is looked at by the next call
-int * wait_flag(int device) {
-    static std::mutex lock;
-    static int * words[MAX_DEVICES] = {};
-    std::lock_guard<std::mutex> hold(lock);
-    if (!words[device]) {
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;         // (this may be the first call inside a capture)
-        cu(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
-        void * p = nullptr;
-        const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        cu(e, "cudaHostAlloc");
-        *static_cast<volatile int *>(p) = 0;
-        words[device] = static_cast<int *>(p);
-    }
-    return words[device];
-}
 template <int HD, typename T> void prompt_as(const PromptArgs & p, int64_t entries, int device, int sms, void * stream) {
     static Limits set;
     const auto kernel = k_kv4_prompt<HD, T>;
@@ -220,6 +227,7 @@ void kv4_append(const b200_kv4 & c, int dtype, const void * k, int64_t k_row, in
     check_dtype(dtype, true);
     need(c.n_rows == 0 || (k && v && aligned(k, size_of(dtype)) && aligned(v, size_of(dtype))), "kv4_append: k and v are pointers to whole entries");
     On on(c.device);
+    heed_waits(c.device);
     if (c.n_seq == 0 || c.n_rows == 0) return;
     if (dtype == B200_DTYPE_F32) append_as<float>(c, d, k, k_row, k_head, v, v_row, v_head);
     else if (dtype == B200_DTYPE_BF16) append_as<__nv_bfloat16>(c, d, k, k_row, k_head, v, v_row, v_head);
@@ -231,6 +239,7 @@ void kv4_read(const b200_kv4 & c, int dtype, void * k, void * v) {
     check_dtype(dtype, true);
     need(c.n_rows == 0 || (k && v && aligned(k, 16) && aligned(v, 16)), "kv4_read: k and v start on 16 bytes");
     On on(c.device);
+    heed_waits(c.device);
     if (c.n_seq == 0 || c.n_rows == 0) return;
     if (dtype == B200_DTYPE_F32) read_as<float>(c, d, k, v);
     else if (dtype == B200_DTYPE_BF16) read_as<__nv_bfloat16>(c, d, k, v);
@@ -264,6 +273,7 @@ void kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row,
     need(std::isfinite(scale), "kv4_attention: scale is a finite number");
     need(window >= 0, "kv4_attention: window is a number of positions, or 0 for all");
     On on(c.device);
+    heed_waits(c.device);
     if (c.n_seq == 0 || c.n_rows == 0) return;
     a.q = q; a.q_row = q_row; a.q_head = q_head; a.out = out;
     a.q_whole = aligned(q, 16) && !((q_row | q_head) & 7);
@@ -274,11 +284,9 @@ void kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row,
     if (is_prompt(c, a.group, max_rows)) {
         const PromptWork at = prompt_work(c, a.group, on.sms);
         check_work(work, work_bytes, at.bytes);
-        PromptArgs p = {a, (int) prompt_entries(c, a.group), reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.first), wait_flag(c.device)};
-        if (*static_cast<volatile int *>(p.err)) {
-            *static_cast<volatile int *>(p.err) = 0;
-            throw std::runtime_error("a wait inside an earlier kv4_attention on this device ran out: its results are missing");
-        }
+        const int drill = drill_polls.load();
+        PromptArgs p = {a, (int) prompt_entries(c, a.group), reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.first), wait_word(c.device),
+                        drill ? (uint32_t) drill : PR_POLLS, drill ? 1 << 19 : 4};
         const int64_t n = prompt_entries(c, a.group);
         p.a.before = reinterpret_cast<long long *>(w);
         p.a.ml = reinterpret_cast<float *>(w + at.ml);
@@ -308,6 +316,7 @@ void pages_reserve(const b200_pages & p, const int32_t * slots, const int32_t * 
     need(first && status, "pages_reserve: null pointer");
     need(slots || n <= p.n_slots, "pages_reserve: more sequences than slots");
     On on(p.device);
+    heed_waits(p.device);
     static Limits set;
     const size_t smem = words_bytes(p.n_pages) + words_bytes(p.n_slots);
     allow_smem(k_pages_reserve, p.device, set);
@@ -320,6 +329,7 @@ void pages_fork(const b200_pages & p, const int32_t * parents, const int32_t * c
     need(status && ((parents && children) || n == 0), "pages_fork: null pointer");
     check_work(work, work_bytes, pages_workspace(p, n));
     On on(p.device);
+    heed_waits(p.device);
     static Limits set;
     const size_t smem = words_bytes(p.n_pages) + words_bytes(p.n_slots);
     allow_smem(k_pages_fork, p.device, set);
@@ -333,6 +343,7 @@ void pages_free(const b200_pages & p, const int32_t * slots, int n) {
     need(n >= 0 && n <= (1 << 24), "pages_free: from 0 to 2^24 slots");
     need(slots || n == 0, "pages_free: null pointer");
     On on(p.device);
+    heed_waits(p.device);
     if (n) launch(k_pages_free, dim3((n + 7) / 8), 256, 0, p.stream, false, 1, d, slots, n);
 }
 
@@ -341,6 +352,7 @@ void pages_compact(const b200_pages & p, int32_t * live, void * work, int64_t wo
     need(live, "pages_compact: null pointer");
     check_work(work, work_bytes, pages_workspace(p, p.n_pages));
     On on(p.device);
+    heed_waits(p.device);
     static Limits set;
     const size_t smem = words_bytes(p.n_pages);
     allow_smem(k_pages_compact, p.device, set);
@@ -355,6 +367,7 @@ void pages_copy(const b200_pages & p, const int32_t * src, const int32_t * dst, 
     need(status && ((src && dst) || n == 0), "pages_copy: null pointer");
     check_work(work, work_bytes, pages_workspace(p, n));
     On on(p.device);
+    heed_waits(p.device);
     static Limits set;
     const size_t smem = words_bytes(p.n_pages);
     allow_smem(k_pages_check_copy, p.device, set);
@@ -371,6 +384,7 @@ void sample_rows(int device, void * stream, int dtype, const void * logits, int6
     need(row_stride >= n_vocab || n_rows <= 1, "sample: row_stride is n_vocab at least");
     need(n_rows == 0 || (logits && u && ids && aligned(logits, size_of(dtype))), "sample: null pointer");
     On on(device);
+    heed_waits(device);
     if (n_rows == 0) return;
     SampleArgs a = {logits, row_stride, n_rows, n_vocab, 0, u, temperature, top_p, min_p, top_k, ids, logprobs};
     // slices of 64 KB at most, so that two blocks share an SM; smaller ones while rows leave SMs without a block and a slice has work for its threads. Mixed rows, us: 16 of 128 256 logits
@@ -382,5 +396,11 @@ void sample_rows(int device, void * stream, int dtype, const void * logits, int6
     else if (dtype == B200_DTYPE_BF16) sample_as<__nv_bfloat16>(a, cluster, device, stream);
     else sample_as<__half>(a, cluster, device, stream);
 }
+
+void kv4_status(int device) {
+    need(device >= 0 && device < MAX_DEVICES, "no such device: " + std::to_string(device));
+    heed_waits(device);
+}
+void kv4_drill(int polls) { drill_polls.store(std::max(0, polls)); }
 
 }  // namespace b200

@@ -10,6 +10,8 @@ void    kv4_append(const b200_kv4 & c, int dtype, const void * k, int64_t k_row,
 void    kv4_read(const b200_kv4 & c, int dtype, void * k, void * v);
 int64_t kv4_attention_workspace(const b200_kv4 & c, int n_head, int max_rows);
 void    kv4_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int max_rows, void * out, void * work, int64_t work_bytes);
+void    kv4_status(int device);
+void    kv4_drill(int polls);
 
 int64_t pages_workspace(const b200_pages & p, int n);
 void    pages_reserve(const b200_pages & p, const int32_t * slots, const int32_t * first, int n, int32_t * status);

@@ -14,7 +14,7 @@
 // Tokens of 32 stand as n = 8 c + 4 u + i for token 16 u + c + 4 i in S, P, K and V alike, and dims of 8 as 0 4 1 5 2 6 3 7 in Q and K: the orders in which a word's codes come apart.
 // P is rounded to fp16 (2^-11; P_LIFT and P_PASS in serve_attn.cuh say what that leaves out), q scaled by a power of two into fp16's range; sums are fp32. O is scaled in tensor memory where the
 // base of P moves.
-// Every wait on an mbarrier is bounded: on a timeout the block raises *err, skips what is left and frees its tensor memory.
+// Every wait on an mbarrier is bounded: where one runs out the block raises *err, waits for nothing more, lets what is under way end and frees its tensor memory; the call's results are worthless.
 #pragma once
 #include "serve_attn.cuh"
 #include <type_traits>
@@ -29,8 +29,11 @@ struct PromptArgs {
     Entry * entries;
     int * first;                         // tiles of a block's piece, entries, the entry that each block's piece begins in
     int * err;
+    uint32_t polls;                      // of a wait that is given up
+    int queries;                         // arrivals that tell a half's queries there: 4, one from each warp, or more than come (b200_kv4_drill)
 };
 
+constexpr uint32_t PR_POLLS = 1u << 18;       // a poll that finds nothing takes 7800 clocks: a second
 constexpr int PR_COLS = 256, PR_KV = 128, PR_THREADS = 512, PR_OVER = 4;      // PR_OVER: what beginning a unit costs, in tiles (8192 tokens 780 us with 2, 655, 600, 600, 611 with 3, 4, 5, 8)
 constexpr uint64_t PR_DESC = (1ull << 16) | ((uint64_t) (1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);      // K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart
 __host__ __device__ constexpr uint32_t pr_idesc(int n) { return (1u << 4) | ((uint32_t) (n >> 3) << 17) | (8u << 24); }     // D f32, A and B f16, M = 128
@@ -39,12 +42,12 @@ template <int HD> struct PromptSmem {
     static constexpr int BYTES = 2 * Q + 4 * KV + 4 * 36 * HD + 1024;      // K and V in two stages each, a tile's codes as they come
 };
 
-__device__ __forceinline__ void pr_wait(uint32_t bar, uint32_t parity, bool & dead) {
+__device__ __forceinline__ void pr_wait(uint32_t bar, uint32_t parity, uint32_t polls, bool & dead) {
     for (uint32_t spins = 0; !dead; spins++) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) break;
-        if (spins >= (1u << 22)) dead = true;
+        if (spins >= polls) dead = true;
     }
 }
 __device__ __forceinline__ void pr_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
     const uint32_t smem = (smem_at(pr_raw) + 1023u) & ~1023u, q_s = smem, k_s = q_s + 2 * QB, v_s = k_s + 2 * KVB;
     if (tid == 0) {
         const auto init = [](uint64_t * b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(smem_at(b)), "r"(n) : "memory"); };
-        for (int i = 0; i < 2; i++) { init(&q_full[i], 4); init(&k_full[i], 4); init(&v_full[i], 4); init(&k_empty[i], 2); init(&v_empty[i], 2); for (int b = 0; b < 2; b++) { init(&s_full[i][b], 1); init(&p_full[i][b], 4); init(&o_full[i][b], 1); } }
+        for (int i = 0; i < 2; i++) { init(&q_full[i], p.queries); init(&k_full[i], 4); init(&v_full[i], 4); init(&k_empty[i], 2); init(&v_empty[i], 2); for (int b = 0; b < 2; b++) { init(&s_full[i][b], 1); init(&p_full[i][b], 4); init(&o_full[i][b], 1); } }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 const bool edge = !whole || pos + 63 > all_see_hi || pos < all_see_lo;
                 unsigned there = 0xfu;                                     // tiles of 16 tokens that have a page
                 if (!whole) there = __ballot_sync(0xffffffffu, lane < 4 && page_at(c, g.q.slot, pos + 16 * (lane & 3)) >= 0);
-                pr_wait(smem_at(&s_full[half][n_s & 1]), (uint32_t) (n_s >> 1 & 1), dead);
+                pr_wait(smem_at(&s_full[half][n_s & 1]), (uint32_t) (n_s >> 1 & 1), p.polls, dead);
                 __syncwarp();
                 pr_fence_after();
                 uint32_t r[64];
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 if (__any_sync(0xffffffffu, score > limit)) {
                     const float top = fmaxf(m, score - P_LIFT), down = top > m ? exp2_fast(m - top) : 1.f;
                     if (t > 2 * g.t0 && __any_sync(0xffffffffu, down != 1.f)) {
-                        pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), dead);
+                        pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), p.polls, dead);
                         __syncwarp();
                         pr_fence_after();
 #pragma unroll 1
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
             Segment then;
             more = next(then);
             if (more) factor = queries(then);
-            pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), dead);
+            pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), p.polls, dead);
             __syncwarp();
             pr_fence_after();
             const bool final = g.t0 == 0 && g.t1 == g.sp.n;
@@ -434,7 +437,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 const int stage = n & 1;
                 const uint32_t round = (uint32_t) (n >> 1);
                 asm volatile("cp.async.wait_all;" ::: "memory");
-                if (n >= 2) pr_wait(smem_at(&k_empty[stage]), (round - 1) & 1, dead);
+                if (n >= 2) pr_wait(smem_at(&k_empty[stage]), (round - 1) & 1, p.polls, dead);
                 __syncwarp();
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) pr_arrive(smem_at(&k_full[stage]));
-                if (n >= 2) pr_wait(smem_at(&v_empty[stage]), (round - 1) & 1, dead);
+                if (n >= 2) pr_wait(smem_at(&v_empty[stage]), (round - 1) & 1, p.polls, dead);
                 __syncwarp();
 #pragma unroll
                 for (int bb = 0; bb < NB / 2; bb++) {
@@ -498,8 +501,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
             }
         }
         for (int i = max(0, n - 2); i < n; i++) {                          // the last tiles are let go: their commits arrive while the block's shared memory is its own
-            pr_wait(smem_at(&k_empty[i & 1]), (uint32_t) (i >> 1 & 1), dead);
-            pr_wait(smem_at(&v_empty[i & 1]), (uint32_t) (i >> 1 & 1), dead);
+            pr_wait(smem_at(&k_empty[i & 1]), (uint32_t) (i >> 1 & 1), p.polls, dead);
+            pr_wait(smem_at(&v_empty[i & 1]), (uint32_t) (i >> 1 & 1), p.polls, dead);
         }
     } else {
         regs_less<64>();
@@ -517,8 +520,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                                       PR_DESC | (uint64_t) ((k_s + (n + (step >> 1) & 1) * KVB + (k >> 2) * SUB + turn * (SUB / 2)) >> 4) + 2 * (k & 3), pr_idesc(64), k > 0);
                         pr_commit(smem_at(&s_full[half][turn]));
                     };
-                    pr_wait(smem_at(&q_full[half]), (uint32_t) (n_q & 1), dead);
-                    pr_wait(smem_at(&k_full[n & 1]), (uint32_t) (n >> 1 & 1), dead);
+                    pr_wait(smem_at(&q_full[half]), (uint32_t) (n_q & 1), p.polls, dead);
+                    pr_wait(smem_at(&k_full[n & 1]), (uint32_t) (n >> 1 & 1), p.polls, dead);
                     pr_fence_after();
                     if (!dead) {
                         scores(0);
@@ -527,8 +530,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                     }
                     for (int step = 0; step < steps; step++) {
                         const int turn = step & 1, now = n + (step >> 1), stage = now & 1, after = (now + 1) & 1;
-                        if (turn == 0) pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), dead);
-                        pr_wait(smem_at(&p_full[half][turn]), (uint32_t) ((n_p + step) >> 1 & 1), dead);
+                        if (turn == 0) pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), p.polls, dead);
+                        pr_wait(smem_at(&p_full[half][turn]), (uint32_t) ((n_p + step) >> 1 & 1), p.polls, dead);
                         pr_fence_after();
                         if (!dead) {
 #pragma unroll
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                             if (turn == 1) pr_commit(smem_at(&v_empty[stage]));
                         }
                         if (step + 2 < steps) {
-                            if (turn == 0) { pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), dead); pr_fence_after(); }
+                            if (turn == 0) { pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), p.polls, dead); pr_fence_after(); }
                             if (!dead) {
                                 scores(step + 2);
                                 if (turn == 1) pr_commit(smem_at(&k_empty[after]));
@@ -549,9 +552,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_kv4_prompt(const PromptArgs p
                     for (int t = 0; t < tiles; t++) {
                         const int stage = (n + t) & 1;
                         const uint32_t phase = (uint32_t) ((n + t) >> 1 & 1);
-                        pr_wait(smem_at(&k_full[stage]), phase, dead);
+                        pr_wait(smem_at(&k_full[stage]), phase, p.polls, dead);
                         if (!dead) pr_arrive(smem_at(&k_empty[stage]));
-                        pr_wait(smem_at(&v_full[stage]), phase, dead);
+                        pr_wait(smem_at(&v_full[stage]), phase, p.polls, dead);
                         if (!dead) pr_arrive(smem_at(&v_empty[stage]));
                     }
                 }

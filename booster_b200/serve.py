@@ -69,6 +69,12 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, held
     return _native().kv4_attention(q, pool, table, held, first, slots, scale, window, max_rows, out)
 
 
+def kv4_status(device: Optional[int] = None) -> None:
+    """raises B200Error where a bounded wait inside an earlier kv4_attention on the device ran out, so that its results are worthless, and no call has told of it yet. The other calls here look by
+    themselves; a program that replays graphs asks, behind a synchronisation"""
+    _lib.check(_lib.lib().b200_kv4_status(torch.cuda.current_device() if device is None else device), "kv4_status")
+
+
 def pages_reserve(table: torch.Tensor, held: torch.Tensor, refs: torch.Tensor, first: torch.Tensor, page_tokens: int, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     """pages for first[i + 1] - first[i] tokens more of each sequence, the lowest free ones, in order. Returns the status on the device, int32 [1]: 0, the number of pages that were
     missing, or -1 where slots or tables cannot be; then nothing has changed"""

@@ -370,10 +370,19 @@ int b200_kv4_append(const b200_kv4 * c, int dtype, const void * k, int64_t k_row
 int b200_kv4_read(const b200_kv4 * c, int dtype, void * k, void * v);
 /* attention of the step's rows, after b200_kv4_append of the same step: out[row][head] = sum over the positions j that the row sees of softmax(scale q . k_j) v_j, in
  * [n_rows][n_head][head_dim]; q[row * q_row + head * q_head + i], dtype BF16 or F16. A row at position p sees j <= p, with window > 0 only j > p - window, and no position
- * whose page is absent; a row that sees nothing answers 0, one whose query holds an infinity or a NaN and that sees something NaN. n_head is a multiple of n_head_kv. max_rows: no sequence has more rows (it chooses kernels; further rows of a sequence
- * that has are still computed). work: b200_kv4_attention_workspace() bytes (-1: error) on 16 bytes. */
+ * whose page is absent; a row that sees nothing answers 0, one whose query holds an infinity or a NaN and that sees something NaN. n_head is a multiple of n_head_kv. max_rows:
+ * no sequence has more rows (it chooses between kernels, whose results differ by their roundings; further rows of a sequence that has are still computed).
+ * work: b200_kv4_attention_workspace() bytes (-1: error) on 16 bytes. */
 int64_t b200_kv4_attention_workspace(const b200_kv4 * c, int n_head, int max_rows);
 int b200_kv4_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int max_rows, void * out, void * work, int64_t work_bytes);
+
+/* Waits inside b200_kv4_attention's kernels are bounded, to about a second. Should one run out, that call's results are worthless, and the next call of this group on the device that finds it
+ * out fails with a message that says so, has done nothing itself and may be repeated. b200_kv4_status asks without doing anything else: 0, or non-zero where a wait ran out that no call has told
+ * of yet. Work that is still on its way is not waited for, so a program that replays graphs asks behind a synchronisation. */
+int b200_kv4_status(int device);
+/* polls > 0: from now on b200_kv4_attention's kernels of many rows wait for queries that never come, that many polls (of 4 us) long, and give up; 0: as always. Process-wide; exists so that
+ * tests cover waits that run out. */
+void b200_kv4_drill(int polls);
 
 /* The pages' life. refs[n_pages] counts the slots that hold a page (0: free); table and held as above, here [n_slots] of all slots. pool: n_layer layers, layer_stride
  * bytes apart, as above (not used by b200_pages_reserve and _free). status receives 0, the number of pages that were missing, or -1 for slots, tables or lists that cannot

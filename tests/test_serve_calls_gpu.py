@@ -179,6 +179,50 @@ def test_queries_that_are_not_finite(heads, max_rows):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+def test_a_wait_that_runs_out_is_told(hd):
+    """queries that never come: the kernel gives up, frees what it holds and says so, whichever call comes next; that call has done nothing, and after it all is as before"""
+    L = _lib.lib()
+    c = Case([300, 5], [64, 1], kv=2, hd=hd)
+    c.fill()
+    q = c.randn(c.rows, 8, hd).half()
+    attend = lambda most=MANY: serve.kv4_attention(q, *c.args(), slots=c.slots, max_rows=most)
+    right, few = attend(), attend(1)
+    k = c.randn(c.rows, 2, hd).half()
+    refs = torch.ones(c.pages, dtype=torch.int32, device="cuda")
+    pool, one, none = c.pool.clone(), ints([1]), ints([])
+    calls = [lambda: serve.kv4_append(*c.args(), k, k, c.slots), lambda: serve.kv4_read(*c.args(), c.rows, F16, c.slots), lambda: attend(1), attend,
+             lambda: serve.pages_reserve(c.table, c.held, refs, ints([0, 1]), 16, c.slots[:1]), lambda: serve.pages_fork(c.pool, c.table, c.held, refs, none, none),
+             lambda: serve.pages_free(c.table, c.held, refs, c.slots), lambda: serve.pages_compact(c.pool, c.table, refs), lambda: serve.pages_copy(c.pool, c.table, refs, none, none),
+             lambda: serve.sample(torch.zeros(1, 10, device="cuda"), torch.zeros(1, device="cuda")), serve.kv4_status]
+    table, held = c.table.clone(), c.held.clone()
+    try:
+        for call in calls:
+            L.b200_kv4_drill(64)
+            attend()
+            L.b200_kv4_drill(0)
+            torch.cuda.synchronize()
+            with pytest.raises(_lib.B200Error, match="ran out"):
+                call()
+            assert torch.equal(c.pool, pool) and torch.equal(c.table, table) and torch.equal(c.held, held)
+            serve.kv4_status()
+            assert torch.equal(attend(), right) and torch.equal(attend(1), few)
+        # a replayed graph makes no call that could look
+        stream = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        L.b200_kv4_drill(64)
+        with torch.cuda.graph(graph, stream=stream):
+            attend()
+        L.b200_kv4_drill(0)
+        graph.replay()
+        torch.cuda.synchronize()
+        with pytest.raises(_lib.B200Error, match="ran out"):
+            serve.kv4_status(0)
+        assert torch.equal(attend(), right)
+    finally:
+        L.b200_kv4_drill(0)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 def test_calls_one_behind_the_other_repeat_themselves(hd):
     """blocks of one call begin where those of another have just ended, with barriers and tiles in the same shared memory: every call gives the bits that it gave alone"""
     cases = [Case([300, 0, 77], [200, 65, 130], page=32, kv=2, hd=hd, seed=1), Case([2000], [40], page=16, kv=4, hd=hd, seed=2), Case([50] * 40, [1] * 40, page=16, kv=2, hd=hd, seed=3)]
