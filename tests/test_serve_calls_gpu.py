@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from booster_b200 import _lib, serve
-from tests.test_serve_gpu import BF16, F16, F32, Case, ints
+from tests.test_serve_gpu import BF16, F16, F32, Case, check_rows, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -125,6 +125,66 @@ def test_a_step_whose_rows_belong_to_no_sequence():
             work.fill_(0x55)
             assert (work == 0x55).all()
     assert (out == 7).all()
+
+
+def test_first_calls_inside_a_capture():
+    """every operator for the first time in its process while a graph is captured; the graph then gives what calls give"""
+    alone("""
+import torch
+from booster_b200 import serve
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+gen = torch.Generator(device="cuda").manual_seed(0)
+n, page = 3, 16
+table, held, refs, first = torch.full((8, 6), -1, dtype=torch.int32, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda"), torch.zeros(40, dtype=torch.int32, device="cuda"), ints([0, 20, 21, 60])
+advance = torch.zeros(8, dtype=torch.int32, device="cuda")
+advance[:3] = first.diff()
+pool = serve.kv4_pool(40, page, 2, 64, 2)
+k, v, q = (torch.randn(60, h, 64, generator=gen, device="cuda").half() for h in (2, 2, 8))
+logits, u = torch.randn(3, 5000, generator=gen, device="cuda"), torch.rand(3, generator=gen, device="cuda")
+gone, parents, children, src, dst, ks = ints([1]), ints([0, 2]), ints([4, 5]), ints([0]), ints([39]), ints([5, 0, 40])
+def step():
+    out = [serve.pages_reserve(table, held, refs, first, page)]
+    for layer in pool:
+        serve.kv4_append(layer, table, held, first, k, v)
+        out += serve.kv4_read(layer, table, held, first, 60)
+        out += [serve.kv4_attention(q, layer, table, held, first, max_rows=m) for m in (4096, 2, 12)]
+    held.add_(advance)
+    out.append(serve.pages_fork(pool, table, held, refs, parents, children))
+    serve.pages_free(table, held, refs, gone)
+    out.append(serve.pages_compact(pool, table, refs))
+    out.append(serve.pages_copy(pool, table, refs, src, dst))
+    out += serve.sample(logits, u, top_k=ks)
+    return out
+state = (table, held, refs, pool)
+start = [x.clone() for x in state]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = step()
+for x, y in zip(state, start): assert torch.equal(x, y)
+graph.replay()
+torch.cuda.synchronize()
+ends = [x.clone() for x in state]
+for x, y in zip(state, start): x.copy_(y)
+eager = step()
+for x, y in zip(state, ends): assert torch.equal(x, y)
+for x, y in zip(outs, eager): assert torch.equal(x, y)
+assert outs[0].item() == 0 and eager[-5].item() == 0 and outs[-3].item() == 0, [o.tolist() for o in outs[-5:-2]]
+print("done")
+""")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_the_widest_vocabulary(dtype):
+    """2^18 logits: as many parts and as long slices as there are; a row on its own and several"""
+    vocab = 1 << 18
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    rows = (3 * torch.randn(5, vocab, generator=gen, device="cuda")).to(dtype)
+    rows[4, -1] = 40                                                     # the last token
+    u = torch.rand(5, generator=gen, device="cuda")
+    u[3] = 1 - 2.0 ** -24
+    for p in (dict(), dict(top_k=[50] * 5), dict(top_p=[0.9] * 5), dict(top_k=[vocab] * 5, min_p=[0.01] * 5), dict(top_k=[5000] * 5, top_p=[0.99] * 5, temperature=[2.0] * 5)):
+        check_rows(rows, u, **p)
+        check_rows(rows[1:2], u[1:2], **{k: v[:1] for k, v in p.items()})
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])

@@ -40,12 +40,12 @@ def check(q, k, v, present, held, window, scale, form, out):
 
 
 class Long:
-    """sequences of `lengths` positions, rows included, in pages of 16 tokens that stand scattered; some pages are absent"""
+    """sequences of `lengths` positions, rows included, in pages that stand scattered; some pages are absent"""
 
-    def __init__(self, lengths, kv, hd, seed, gone=()):
+    def __init__(self, lengths, kv, hd, seed, gone=(), page=16):
         r = random.Random(seed)
         self.lengths, self.kv, self.hd, n = lengths, kv, hd, len(lengths)
-        need = [-(-t // 16) for t in lengths]
+        need = [-(-t // page) for t in lengths]
         order = list(range(sum(need)))
         r.shuffle(order)
         table = torch.full((n, max(need)), -1, dtype=torch.int32)
@@ -53,7 +53,7 @@ class Long:
         for s, m in enumerate(need):
             table[s, :m] = torch.tensor(order[at:at + m], dtype=torch.int32)
             at += m
-        self.pool, self.table = serve.kv4_pool(sum(need), 16, kv, hd)[0], table.cuda()
+        self.pool, self.table = serve.kv4_pool(sum(need), page, kv, hd)[0], table.cuda()
         first = [0]
         for t in lengths:
             first.append(first[-1] + t)
@@ -63,9 +63,9 @@ class Long:
         serve.kv4_append(self.pool, self.table, ints([0] * n), ints(first), k, v)
         self.k, self.v = (x.double() for x in serve.kv4_read(self.pool, self.table, ints([0] * n), ints(first), first[-1], F32))
         self.first, self.present = first, torch.ones(first[-1], dtype=torch.bool, device="cuda")
-        for s, page in gone:
-            self.table[s, page] = -1
-            self.present[first[s] + 16 * page:first[s] + 16 * page + 16] = False
+        for s, i in gone:
+            self.table[s, i] = -1
+            self.present[first[s] + page * i:first[s] + page * (i + 1)] = False
 
     def attend(self, rows, heads, max_rows, form, window=0, dtype=F16, scale=0.125):
         n = len(self.lengths)
@@ -114,3 +114,19 @@ def test_each_form_within_its_own_roundings(heads, max_rows, form, size, hd):
     all_there = torch.ones(T, dtype=torch.bool, device="cuda")
     for i in range(n):
         check(q[i:i + 1], k, v, all_there, T - 1, 0, 0.0625, form, out[i:i + 1])
+
+
+@pytest.mark.parametrize("kv,heads,rows,max_rows,form,page,hd", [(5, 35, 1, 1, "one", 1024, 64), (5, 35, 2, 2, "two", 512, 128), (5, 35, 7, MANY, "many", 1024, 128), (1, 300, 1, 1, "many", 32, 64),
+                                                                 (1, 300, 3, 3, "many", 256, 128), (1024, 1024, 1, 1, "one", 16, 64), (256, 256, 2, MANY, "many", 16, 64), (3, 3, 300, MANY, "many", 128, 64)])
+def test_odd_heads_and_pages(kv, heads, rows, max_rows, form, page, hd):
+    """groups that do not divide a tile of columns, one head under hundreds, hundreds of heads, the longest pages"""
+    c = Long([rows + x for x in (0, 1, 700, 1500)], kv, hd, heads, page=page)
+    c.attend(rows, heads, max_rows, form, dtype=BF16)
+    c.attend(rows, heads, max_rows, form, window=33)
+
+
+@pytest.mark.parametrize("heads,max_rows,form", [(4, 1, "one"), (32, 1, "two"), (4, MANY, "many")])
+def test_scales_of_any_sign(heads, max_rows, form):
+    c = Long([1, 40, 333], 2, 64, heads)
+    for scale in (-0.25, 0.0, 2.0 ** -60, -2.0 ** -130, 4.0):
+        c.attend(1, heads, max_rows, form, scale=scale)
