@@ -7,7 +7,7 @@
 //   warps 8-11       codes of 32 tokens each, copied ahead, to fp16 in shared memory (exact: a scale has 8 bits, a code 4), K by rows of tokens, V by rows of dims, both with 128-byte swizzle
 //   warps 12, 13     (of 12-15: registers are shared out by four warps, 128 a thread at launch, then 168, 168, 112 and 64) one thread each issues a half's S = Q K^T (128 x 64 x head_dim)
 //                    and O += P V (P from tensor memory, 128 x head_dim x 64): a thread issues a product every 44 clocks or so, 24 of them a half and tile
-// Measured with 32 query heads on 8 of 128: 8192 tokens 572 us (961 TFLOP/s, 57 % of the bf16 rate), 512 rows behind 6000 positions 71 us, of which 5 the plan and 4 the join. What bounds
+// Measured with 32 query heads on 8 of 128: 8192 tokens 552 us (996 TFLOP/s, 59 % of the bf16 rate), 512 rows behind 6000 positions 70 us, of which 5 the plan and 4 the join. What bounds
 // it is the chain from S over the soft-max to P: 1750 clocks for 64 tokens, of which 1024 are exponentials (16 a clock), while products read 128 KB of shared memory and codes write 32.
 // Sixteen soft-max warps, exponentials in part by polynomials, K made a tile ahead of V and other shares of registers were no faster; one issuing thread 595 us, one turn of 128 tokens 4 % more.
 // Tensor memory: S and P [2 halves][2 turns][64 columns], O [2][head_dim]. Each half has two turns of S, so that the scores of the next 64 tokens are there when those in hand are done with.

@@ -63,8 +63,9 @@ def kv4_read(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first:
 def kv4_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first: torch.Tensor, slots: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                   window: int = 0, max_rows: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """attention of the step's rows q [rows, n_head, head_dim] (bfloat16 or float16, any strides over rows and heads) over the positions up to their own, kv4_append having put those into
-    the pool; window > 0: over the last `window` of them. scale: 1 / sqrt(head_dim). max_rows: the largest number of rows of a sequence, if the program knows it (it chooses kernels and
-    changes no result; else the mean).
+    the pool; window > 0: over the last `window` of them. scale: 1 / sqrt(head_dim). max_rows: the largest number of rows of a sequence, if the program knows it. It chooses
+    between kernels, whose results differ by their roundings, and any number is right; without it the mean is taken. Single tokens and a
+    long portion are quickest as two calls (48 tokens at 3000 positions and 512 rows at 6000: 133 us, in one 254 to 395; 200 at 500 and 512 rows at 500: 79, in one 109 to 239).
     Rows of no sequence are left as they are (in `out`)"""
     return _native().kv4_attention(q, pool, table, held, first, slots, scale, window, max_rows, out)
 
