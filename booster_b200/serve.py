@@ -44,7 +44,7 @@ def _native():
 
 def kv4_pool(n_pages: int, page_tokens: int, n_head_kv: int, head_dim: int, n_layer: int = 1, device="cuda") -> torch.Tensor:
     """an empty pool: uint8 [n_layer, n_pages, n_head_kv, page_tokens / 16, 18 * head_dim], 4.5 bits a number"""
-    if page_tokens % 16 or head_dim not in (64, 128):
+    if page_tokens not in (16, 32, 64, 128, 256, 512, 1024) or head_dim not in (64, 128):
         raise ValueError("kv4_pool: page_tokens is a power of two from 16 to 1024, head_dim 64 or 128")
     return torch.zeros(n_layer, n_pages, n_head_kv, page_tokens // 16, 18 * head_dim, dtype=torch.uint8, device=device)
 

@@ -15,3 +15,10 @@ def test_status_without_calls():
         assert L.b200_kv4_status(device) != 0 and re.search("no such device", _lib.last_error())
         with pytest.raises(_lib.B200Error, match="no such device"):
             serve.kv4_status(device)
+
+
+def test_pools_that_no_call_would_take():
+    for page_tokens, head_dim in ((48, 64), (0, 64), (8, 64), (2048, 128), (16, 32), (16, 96)):
+        with pytest.raises(ValueError, match="kv4_pool"):
+            serve.kv4_pool(2, page_tokens, 1, head_dim, device="cpu")
+    assert serve.kv4_pool(2, 1024, 3, 128, device="cpu").shape == (1, 2, 3, 64, 2304)
