@@ -10,7 +10,7 @@ PYTHON    ?= $(shell command -v python3 2>/dev/null || command -v python 2>/dev/
 # the torch that $(PYTHON) would load, with its headers (nothing: none is there, and the library is built without the module of torch tensors)
 TORCH     := $(shell $(PYTHON) -c 'import importlib.metadata as m, importlib.util as u, os, sys; r = os.path.dirname(u.find_spec("torch").origin); os.stat(r + "/include/torch/csrc"); print(m.version("torch") + "-" + sys.implementation.cache_tag)' 2>/dev/null)
 
-OBJS := $(OBJDIR)/engine.o $(OBJDIR)/stack.o $(OBJDIR)/serve.o $(OBJDIR)/safetensors.o $(OBJDIR)/gguf.o $(OBJDIR)/bridge.o $(OBJDIR)/tokenizer.o $(OBJDIR)/janus.o
+OBJS := $(OBJDIR)/engine.o $(OBJDIR)/stack.o $(OBJDIR)/serve.o $(OBJDIR)/serve16.o $(OBJDIR)/safetensors.o $(OBJDIR)/gguf.o $(OBJDIR)/bridge.o $(OBJDIR)/tokenizer.o $(OBJDIR)/janus.o
 
 all: $(LIB) $(if $(TORCH),$(SERVE),no-torch)
 
@@ -22,9 +22,13 @@ $(OBJDIR)/stack.o: $(CSRC)/stack.cu $(CSRC)/stack_kernels.cuh $(CSRC)/stack_kern
 	@mkdir -p $(OBJDIR)
 	$(NVCC) $(NVCCFLAGS) -c $< -o $@ 2> $(OBJDIR)/stack.ptxas.log || (cat $(OBJDIR)/stack.ptxas.log; false)
 
-$(OBJDIR)/serve.o: $(CSRC)/serve.cu $(CSRC)/serve.hpp $(CSRC)/serve_cache.cuh $(CSRC)/serve_attn.cuh $(CSRC)/serve_prompt.cuh $(CSRC)/serve_pages.cuh $(CSRC)/serve_sample.cuh include/booster_b200.h
+$(OBJDIR)/serve.o: $(CSRC)/serve.cu $(CSRC)/serve.hpp $(CSRC)/serve_host.cuh $(CSRC)/serve_cache.cuh $(CSRC)/serve_attn.cuh $(CSRC)/serve_prompt.cuh $(CSRC)/serve_pages.cuh $(CSRC)/serve_sample.cuh include/booster_b200.h
 	@mkdir -p $(OBJDIR)
 	$(NVCC) $(NVCCFLAGS) -c $< -o $@ 2> $(OBJDIR)/serve.ptxas.log || (cat $(OBJDIR)/serve.ptxas.log; false)
+
+$(OBJDIR)/serve16.o: $(CSRC)/serve16.cu $(CSRC)/serve.hpp $(CSRC)/serve_host.cuh $(CSRC)/serve_cache.cuh $(CSRC)/serve_attn.cuh $(CSRC)/serve_prompt.cuh $(CSRC)/serve_tma.cuh $(CSRC)/serve_kv16.cuh $(CSRC)/serve_kv16_prompt.cuh include/booster_b200.h
+	@mkdir -p $(OBJDIR)
+	$(NVCC) $(NVCCFLAGS) -c $< -o $@ 2> $(OBJDIR)/serve16.ptxas.log || (cat $(OBJDIR)/serve16.ptxas.log; false)
 
 $(OBJDIR)/%.o: $(CSRC)/%.cpp $(CSRC)/gguf.hpp $(CSRC)/tokenizer.hpp $(CSRC)/janus.hpp $(CSRC)/unicode_tables.hpp $(CSRC)/safetensors.hpp include/bridge.h include/booster_b200.h
 	@mkdir -p $(OBJDIR)

@@ -3126,6 +3126,18 @@ extern "C" int b200_kv4_attention(const b200_kv4 * c, int dtype, const void * q,
 }
 extern "C" int b200_kv4_status(int device) { return served("b200_kv4_status", "", [&] { kv4_status(device); }); }
 extern "C" void b200_kv4_drill(int polls) { kv4_drill(polls); }
+extern "C" int b200_kv16_append(const b200_kv4 * c, int pool_dtype, int dtype, const void * k, int64_t k_row, int64_t k_head, const void * v, int64_t v_row, int64_t v_head) {
+    return served("b200_kv16_append", c, [&] { kv16_append(*c, pool_dtype, dtype, k, k_row, k_head, v, v_row, v_head); });
+}
+extern "C" int64_t b200_kv16_attention_workspace(const b200_kv4 * c, int n_head, int max_rows) {
+    int64_t n = -1;
+    served("b200_kv16_attention_workspace", c, [&] { n = kv16_attention_workspace(*c, n_head, max_rows); });
+    return n;
+}
+extern "C" int b200_kv16_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int sinks, int max_rows, void * out,
+                                   void * work, int64_t work_bytes) {
+    return served("b200_kv16_attention", c, [&] { kv16_attention(*c, dtype, q, q_row, q_head, n_head, scale, window, sinks, max_rows, out, work, work_bytes); });
+}
 extern "C" int64_t b200_pages_workspace(const b200_pages * p, int n) {
     int64_t bytes = -1;
     served("b200_pages_workspace", p, [&] { bytes = pages_workspace(*p, n); });
@@ -3143,6 +3155,19 @@ extern "C" int b200_pages_compact(const b200_pages * p, int32_t * live, void * w
 }
 extern "C" int b200_pages_copy(const b200_pages * p, const int32_t * src, const int32_t * dst, int n, int32_t * status, void * work, int64_t work_bytes) {
     return served("b200_pages_copy", p, [&] { pages_copy(*p, src, dst, n, status, work, work_bytes); });
+}
+extern "C" int b200_pages_plan(const b200_pages * p, const int32_t * slots, const int32_t * counts, int n, int n_rows, int32_t * first, int32_t * positions, int32_t * places, int32_t * status) {
+    return served("b200_pages_plan", p, [&] { pages_plan(*p, slots, counts, n, n_rows, first, positions, places, status); });
+}
+extern "C" int b200_pages_trim(const b200_pages * p, const int32_t * slots, int n, int window, int sinks) {
+    return served("b200_pages_trim", p, [&] { pages_trim(*p, slots, n, window, sinks); });
+}
+extern "C" int b200_verify(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const int32_t * ids, const int32_t * first, int n_seq,
+                           const float * u, const float * accept, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p, const float * draft_probs,
+                           int64_t draft_stride, int32_t * gained, int32_t * tokens, float * logprobs) {
+    return served("b200_verify", "", [&] {
+        verify_rows(device, stream, dtype, logits, row_stride, n_rows, n_vocab, ids, first, n_seq, u, accept, temperature, top_k, top_p, min_p, draft_probs, draft_stride, gained, tokens, logprobs);
+    });
 }
 extern "C" int b200_sample(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature,
                            const int32_t * top_k, const float * top_p, const float * min_p, int32_t * ids, float * logprobs) {

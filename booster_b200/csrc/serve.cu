@@ -1,123 +1,17 @@
 // serve.cu — host side of the operators of a server that runs many sequences at once (serve.hpp): checks of arguments, launch shapes, launches on the caller's stream.
-#include "serve.hpp"
-#include "serve_cache.cuh"
+#include "serve_host.cuh"
 #include "serve_attn.cuh"
 #include "serve_prompt.cuh"
 #include "serve_pages.cuh"
 #include "serve_sample.cuh"
-
-#include <algorithm>
-#include <atomic>
-#include <cmath>
-#include <mutex>
-#include <stdexcept>
-#include <string>
 
 namespace b200 {
 namespace {
 
 using namespace srv;
 
-constexpr int MAX_DEVICES = 64;
-
-void need(bool ok, const std::string & what) { if (!ok) throw std::runtime_error(what); }
-void cu(cudaError_t e, const char * what) {
-    if (e == cudaSuccess) return;
-    cudaGetLastError();                  // (it is this call's: who asks next, the other operators of this library among them, does not find it)
-    throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
-}
-
-// the call's device while it runs, the caller's again behind it
-struct On {
-    int was = -1, device;
-    int sms = 0;
-    explicit On(int d) : device(d) {
-        static std::atomic<int> known[MAX_DEVICES];            // SMs of the devices seen so far
-        if (d < 0 || d >= MAX_DEVICES || !(sms = known[d].load())) {
-            int n = 0;
-            if (cudaGetDeviceCount(&n) != cudaSuccess) { cudaGetLastError(); n = 0; }
-            need(n > 0, "no CUDA device visible: booster_b200 has no CPU fallback (the CUDA path is the product)");
-            need(d >= 0 && d < n && d < MAX_DEVICES, "no such device: " + std::to_string(d));
-            cu(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d), "cudaDeviceGetAttribute");
-            known[d].store(sms);
-        }
-        cu(cudaGetDevice(&was), "cudaGetDevice");
-        if (was != d) cu(cudaSetDevice(d), "cudaSetDevice");
-    }
-    ~On() { if (was >= 0 && was != device) cudaSetDevice(was); }
-};
-
-// A word per device that k_kv4_prompt raises when a bounded wait ran out, in pinned memory, so that the host reads it without waiting. Every call looks at it
-std::atomic<int *> wait_words[MAX_DEVICES];
-std::atomic<int> drill_polls;                                            // b200_kv4_drill
-int * wait_word(int device) {
-    static std::mutex lock;
-    if (int * w = wait_words[device].load()) return w;
-    std::lock_guard<std::mutex> hold(lock);
-    if (int * w = wait_words[device].load()) return w;
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;             // (this may be the first call inside a capture)
-    cu(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
-    void * p = nullptr;
-    const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    cu(e, "cudaHostAlloc");
-    *static_cast<volatile int *>(p) = 0;
-    wait_words[device].store(static_cast<int *>(p));
-    return static_cast<int *>(p);
-}
-void heed_waits(int device) {
-    int * w = wait_words[device].load();
-    if (w && *static_cast<volatile int *>(w) && __atomic_exchange_n(w, 0, __ATOMIC_ACQ_REL))
-        throw std::runtime_error("a wait inside an earlier kv4_attention on this device ran out: its results are worthless. This call has done nothing");
-}
-
-bool aligned(const void * p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-int log2_of(int x) { int l = 0; while ((1 << l) < x) l++; return l; }
-int size_of(int dtype) { return dtype == B200_DTYPE_F32 ? 4 : 2; }
-
-template <typename... P, typename... A>
-void launch(void (*k)(P...), dim3 grid, int threads, size_t smem, void * stream, bool behind, int cluster, A &&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t) stream;
-    cudaLaunchAttribute at[2];
-    unsigned n = 0;
-    if (behind) { at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[n].val.programmaticStreamSerializationAllowed = 1; n++; }
-    if (cluster > 1) { at[n].id = cudaLaunchAttributeClusterDimension; at[n].val.clusterDim.x = cluster; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1; n++; }
-    cfg.attrs = at; cfg.numAttrs = n;
-    cu(cudaLaunchKernelEx(&cfg, k, static_cast<P>(args)...), "launch");
-}
-
-// leave for all the dynamic shared memory that a kernel can have beside what it holds statically, asked for once on each device. Calls of different sizes may come from several host threads:
-// the limit does not depend on the call, so threads that set it together set the same
-typedef std::atomic<bool> Limits[MAX_DEVICES];
-template <typename K> void allow_smem(K * k, int device, Limits & set) {
-    if (set[device].load()) return;
-    cudaFuncAttributes at;
-    int most = 0;
-    cu(cudaFuncGetAttributes(&at, k), "cudaFuncGetAttributes");
-    cu(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device), "cudaDeviceGetAttribute");
-    cu(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int) at.sharedSizeBytes), "cudaFuncSetAttribute");
-    set[device].store(true);
-}
-
-Cache checked(const b200_kv4 & c) {
-    need(c.head_dim == 64 || c.head_dim == 128, "kv4: head_dim is 64 or 128 (got " + std::to_string(c.head_dim) + ")");
-    need(c.page_tokens >= 16 && c.page_tokens <= 1024 && (c.page_tokens & (c.page_tokens - 1)) == 0, "kv4: page_tokens is a power of two from 16 to 1024 (got " + std::to_string(c.page_tokens) + ")");
-    need(c.n_head_kv >= 1 && c.n_head_kv <= 1024, "kv4: n_head_kv from 1 to 1024");
-    need(c.n_pages >= 1, "kv4: a pool of one page at least");
-    need(c.n_slots >= 1 && c.max_pages >= 1 && (int64_t) c.max_pages * c.page_tokens <= (1 << 30), "kv4: a table of one slot and one page at least, of 2^30 tokens a slot at most");
-    need(c.n_seq >= 0 && c.n_seq <= AT_MAX_SEQ, "kv4: from 0 to " + std::to_string(AT_MAX_SEQ) + " sequences a step");
-    need(c.n_rows >= 0 && c.n_rows <= (1 << 24), "kv4: from 0 to 2^24 rows a step");
-    need(c.page_stride >= (int64_t) c.n_head_kv * c.page_tokens / 16 * 18 * c.head_dim && c.page_stride % 16 == 0, "kv4: page_stride holds a page and is a multiple of 16 bytes");
-    need(c.table_stride >= c.max_pages, "kv4: table_stride is max_pages at least");
-    need(c.pool && c.table && c.held && c.first, "kv4: null pointer");
-    need(aligned(c.pool, 16), "kv4: the pool starts on 16 bytes");
-    need(aligned(c.table, 4) && aligned(c.held, 4) && aligned(c.first, 4) && aligned(c.slots, 4), "kv4: tables of int32 start on 4 bytes");
-    return Cache{static_cast<uint8_t *>(c.pool), c.page_stride, c.n_pages, log2_of(c.page_tokens), c.n_head_kv, c.table, c.table_stride, c.n_slots, c.max_pages, c.held, c.slots, c.first, c.n_seq, c.n_rows};
-}
-void check_dtype(int dtype, bool f32) {
-    need(dtype == B200_DTYPE_BF16 || dtype == B200_DTYPE_F16 || (f32 && dtype == B200_DTYPE_F32), f32 ? "dtype is B200_DTYPE_F32, _BF16 or _F16" : "dtype is B200_DTYPE_BF16 or _F16");
-}
+static_assert(MAX_SEQ == AT_MAX_SEQ, "sequences of a step");
+Cache checked(const b200_kv4 & c) { return checked_cache(c, "kv4", 18 * c.head_dim); }
 
 // heads of a row one after the other in a warp only where there are rows enough to fill the card without. Rows of 8 heads written and read by one pass / by four, us: 48 6.2 / 8.9,
 // 700 9.3 / 11.1, 2100 11.9 / 11.9, 8100 32 / 25
@@ -193,31 +87,42 @@ Pages checked(const b200_pages & p, bool pool) {
     need(p.table_stride >= p.max_pages, "pages: table_stride is max_pages at least");
     need(p.table && p.held && p.refs, "pages: null pointer");
     need(aligned(p.table, 4) && aligned(p.held, 4) && aligned(p.refs, 4), "pages: tables of int32 start on 4 bytes");
+    // a pool in 16 bits: tiles of 16 tokens as well, with as many heads of keys as of values behind them
+    const bool wide = p.head_dim & B200_POOL_16BIT;
+    const int hd = p.head_dim & ~B200_POOL_16BIT, heads = wide ? 2 * p.n_head_kv : p.n_head_kv, tile_bytes = (wide ? 32 : 18) * hd;
     int64_t bytes = 0;
     if (pool) {
-        need(p.head_dim == 64 || p.head_dim == 128, "pages: head_dim is 64 or 128 (got " + std::to_string(p.head_dim) + ")");
+        need(hd == 64 || hd == 128, "pages: head_dim is 64 or 128, with B200_POOL_16BIT of a pool in 16 bits (got " + std::to_string(p.head_dim) + ")");
         need(p.n_head_kv >= 1 && p.n_head_kv <= 1024 && p.n_layer >= 1 && p.n_layer <= 65536, "pages: n_head_kv from 1 to 1024, n_layer from 1 to 65536");
-        bytes = (int64_t) p.n_head_kv * p.page_tokens / 16 * 18 * p.head_dim;
+        bytes = (int64_t) heads * p.page_tokens / 16 * tile_bytes;
         need(p.pool && aligned(p.pool, 16), "pages: the pool starts on 16 bytes");
         need(p.page_stride >= bytes && p.page_stride % 16 == 0 && p.layer_stride % 16 == 0 && (p.n_layer == 1 || p.layer_stride >= bytes), "pages: strides hold a page and are multiples of 16 bytes");
     }
     return Pages{p.table, p.table_stride, p.n_slots, p.max_pages, p.held, p.refs, p.n_pages, log2_of(p.page_tokens), static_cast<uint8_t *>(p.pool), p.layer_stride, p.page_stride,
-                 p.n_layer, p.n_head_kv, 18 * p.head_dim};
+                 p.n_layer, heads, tile_bytes};
 }
 size_t words_bytes(int n) { return (size_t) ((n + 31) / 32) * 4; }
-void check_work(const void * work, int64_t bytes, int64_t wanted) {
-    need(work && aligned(work, 16), "the workspace starts on 16 bytes");
-    need(bytes >= wanted, "the workspace has " + std::to_string(bytes) + " bytes, " + std::to_string(wanted) + " are needed");
-}
 void move_pages(const b200_pages & p, const Pages & d, const int32_t * plan, int n, bool parts, const int32_t * moved_to, int sms) {
     launch(k_pages_move, dim3(sms * 4), 256, 0, p.stream, true, 1, d, plan, n, parts, moved_to);
 }
 
-template <typename T> void sample_as(const SampleArgs & a, int cluster, int device, void * stream) {
+template <typename T, bool VERIFY> void sample_as(const SampleArgs & a, int cluster, int device, void * stream) {
     static Limits set;
     const size_t smem = SA_FIXED + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
-    allow_smem(k_sample<T>, device, set);
-    launch(k_sample<T>, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, false, cluster, a);
+    const auto kernel = k_sample<T, VERIFY>;
+    allow_smem(kernel, device, set);
+    launch(kernel, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, false, cluster, a);
+}
+
+template <bool VERIFY> void sample_all(SampleArgs & a, int dtype, const On & on, void * stream) {
+    // slices of 64 KB at most, so that two blocks share an SM; smaller ones while rows leave SMs without a block and a slice has work for its threads. Mixed rows, us: 16 of 128 256 logits
+    // by 8 blocks 32, by 4 48; 48 of them 45 and 56; 32 of 32 000 by 4 23, by 2 29; one of 4000 by one block 7.3, by two 7.8
+    int cluster = 1;
+    while (cluster < SA_MAX_CLUSTER && ((int64_t) a.n_vocab * size_of(dtype) > 65536ll * cluster || (a.n_rows * cluster < on.sms && a.n_vocab >= 8192 * cluster))) cluster *= 2;
+    a.slice = ((a.n_vocab + cluster - 1) / cluster + 7) / 8 * 8;
+    if (dtype == B200_DTYPE_F32) sample_as<float, VERIFY>(a, cluster, on.device, stream);
+    else if (dtype == B200_DTYPE_BF16) sample_as<__nv_bfloat16, VERIFY>(a, cluster, on.device, stream);
+    else sample_as<__half, VERIFY>(a, cluster, on.device, stream);
 }
 
 }  // namespace
@@ -376,6 +281,32 @@ void pages_copy(const b200_pages & p, const int32_t * src, const int32_t * dst, 
     move_pages(p, d, plan, n, true, nullptr, on.sms);
 }
 
+void pages_plan(const b200_pages & p, const int32_t * slots, const int32_t * counts, int n, int n_rows, int32_t * first, int32_t * positions, int32_t * places, int32_t * status) {
+    const Pages d = checked(p, false);
+    need(n >= 0 && n <= PG_MAX_N, "pages_plan: from 0 to " + std::to_string(PG_MAX_N) + " sequences");
+    need(n_rows >= 0 && n_rows <= (1 << 24), "pages_plan: from 0 to 2^24 rows");
+    need((counts || n == 0) && first && status && ((positions && places) || n_rows == 0), "pages_plan: null pointer");
+    need(slots || n <= p.n_slots, "pages_plan: more sequences than slots");
+    On on(p.device);
+    heed_waits(p.device);
+    static Limits set;
+    const bool apart = n_rows > PLAN_ROWS;
+    const size_t smem = words_bytes(p.n_pages) + words_bytes(p.n_slots) + plan_bytes(n);
+    allow_smem(k_pages_plan, p.device, set);
+    launch(k_pages_plan, dim3(1), PG_THREADS, smem, p.stream, false, 1, d, slots, counts, n, n_rows, first, positions, places, status, !apart);
+    if (apart) launch(k_pages_places, dim3((unsigned) ((n_rows + 1023) / 1024)), 256, 0, p.stream, true, 1, d, slots, first, n, n_rows, positions, places);
+}
+
+void pages_trim(const b200_pages & p, const int32_t * slots, int n, int window, int sinks) {
+    const Pages d = checked(p, false);
+    need(n >= 0 && n <= (1 << 24), "pages_trim: from 0 to 2^24 slots");
+    need(slots || n == 0, "pages_trim: null pointer");
+    need(window >= 0 && sinks >= 0, "pages_trim: window is a number of positions, or 0 for all; sinks is a number of positions");
+    On on(p.device);
+    heed_waits(p.device);
+    if (n) launch(k_pages_trim, dim3((n + 7) / 8), 256, 0, p.stream, false, 1, d, slots, n, window, sinks);
+}
+
 void sample_rows(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature, const int32_t * top_k,
                  const float * top_p, const float * min_p, int32_t * ids, float * logprobs) {
     check_dtype(dtype, true);
@@ -387,14 +318,25 @@ void sample_rows(int device, void * stream, int dtype, const void * logits, int6
     heed_waits(device);
     if (n_rows == 0) return;
     SampleArgs a = {logits, row_stride, n_rows, n_vocab, 0, u, temperature, top_p, min_p, top_k, ids, logprobs};
-    // slices of 64 KB at most, so that two blocks share an SM; smaller ones while rows leave SMs without a block and a slice has work for its threads. Mixed rows, us: 16 of 128 256 logits
-    // by 8 blocks 32, by 4 48; 48 of them 45 and 56; 32 of 32 000 by 4 23, by 2 29; one of 4000 by one block 7.3, by two 7.8
-    int cluster = 1;
-    while (cluster < SA_MAX_CLUSTER && ((int64_t) n_vocab * size_of(dtype) > 65536ll * cluster || (n_rows * cluster < on.sms && n_vocab >= 8192 * cluster))) cluster *= 2;
-    a.slice = ((n_vocab + cluster - 1) / cluster + 7) / 8 * 8;
-    if (dtype == B200_DTYPE_F32) sample_as<float>(a, cluster, device, stream);
-    else if (dtype == B200_DTYPE_BF16) sample_as<__nv_bfloat16>(a, cluster, device, stream);
-    else sample_as<__half>(a, cluster, device, stream);
+    sample_all<false>(a, dtype, on, stream);
+}
+
+void verify_rows(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const int32_t * ids, const int32_t * first, int n_seq, const float * u,
+                 const float * accept, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p, const float * draft_probs, int64_t draft_stride,
+                 int32_t * gained, int32_t * tokens, float * logprobs) {
+    check_dtype(dtype, true);
+    need(n_vocab >= 1 && n_vocab <= SA_MAX_VOCAB, "verify: from 1 to 2^18 logits a row (got " + std::to_string(n_vocab) + ")");
+    need(n_rows >= 0 && n_rows <= (1 << 20), "verify: from 0 to 2^20 rows");
+    need(n_seq >= 0 && n_seq <= MAX_SEQ, "verify: from 0 to 4096 sequences");
+    need(row_stride >= n_vocab || n_rows <= 1, "verify: row_stride is n_vocab at least");
+    need(!draft_probs || draft_stride >= n_vocab || n_rows <= 1, "verify: draft_stride is n_vocab at least");
+    need(first && (gained || n_seq == 0), "verify: null pointer");
+    need(n_rows == 0 || (logits && ids && u && accept && tokens && logprobs && aligned(logits, size_of(dtype))), "verify: null pointer");
+    On on(device);
+    heed_waits(device);
+    SampleArgs a = {logits, row_stride, n_rows, n_vocab, 0, u, temperature, top_p, min_p, top_k, tokens, logprobs, ids, first, n_seq, accept, draft_probs, draft_stride, gained};
+    if (n_rows) sample_all<true>(a, dtype, on, stream);
+    if (n_seq) launch(k_verify_ends<128>, dim3((unsigned) ((n_seq + 3) / 4)), 128, 0, stream, true, 1, a);
 }
 
 void kv4_status(int device) {

@@ -1,0 +1,120 @@
+// serve16.cu — host side of the 16-bit paged cache (serve.hpp): checks of arguments, launch shapes, launches on the caller's stream.
+#include "serve_host.cuh"
+#include "serve_kv16.cuh"
+
+namespace b200 {
+namespace {
+
+using namespace srv;
+
+Cache checked(const b200_kv4 & c) { return checked_cache(c, "kv16", 64 * c.head_dim); }
+
+// boxes of 16 tokens and 64 dims, keys and values of a KV head of a page
+CUtensorMap pool_map(const b200_kv4 & c, bool bf16) {
+    static const auto encode = [] {
+        void * fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) { cudaGetLastError(); fn = nullptr; }
+        return reinterpret_cast<CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill)>(fn);
+    }();
+    need(encode, "the driver has no cuTensorMapEncodeTiled");
+    CUtensorMap m;
+    const cuuint64_t row = (cuuint64_t) c.head_dim * 2, head = row * c.page_tokens, side = head * c.n_head_kv;
+    const cuuint64_t dims[5] = {(cuuint64_t) c.head_dim, (cuuint64_t) c.page_tokens, (cuuint64_t) c.n_head_kv, 2, (cuuint64_t) c.n_pages}, strides[4] = {row, head, side, (cuuint64_t) c.page_stride};
+    const cuuint32_t box[5] = {64, 16, 1, 2, 1}, one[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, c.pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    need(r == CUDA_SUCCESS, r == CUDA_SUCCESS ? std::string() : "cuTensorMapEncodeTiled failed: " + std::to_string((int) r));
+    return m;
+}
+
+// heads of a row one after the other in a warp only where there are rows enough to fill the card without
+int row_passes(const b200_kv4 & c) { return (int64_t) c.n_rows * c.n_head_kv > 16384 ? 4 : 1; }
+template <typename S, typename T> void append_as(const b200_kv4 & c, const Cache & d, const void * k, int64_t kr, int64_t kh, const void * v, int64_t vr, int64_t vh) {
+    const Row16Src<S> src = {static_cast<const S *>(k), kr, kh, static_cast<const S *>(v), vr, vh, aligned(k, 16) && aligned(v, 16) && !((kr | kh | vr | vh) & (16 / (int64_t) sizeof(S) - 1))};
+    const int per = row_passes(c) * (256 / c.head_dim), parts = (c.n_head_kv + per - 1) / per;
+    const auto rows = [&](auto kernel) { launch(kernel, dim3((unsigned) (((int64_t) c.n_rows * parts + 7) / 8)), 256, 0, c.stream, false, 1, d, src, parts); };
+    if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv16_append<S, T, 128, 1>) : rows(k_kv16_append<S, T, 64, 1>);
+    else c.head_dim == 128 ? rows(k_kv16_append<S, T, 128, 4>) : rows(k_kv16_append<S, T, 64, 4>);
+}
+template <typename T> void append_to(const b200_kv4 & c, const Cache & d, int dtype, const void * k, int64_t kr, int64_t kh, const void * v, int64_t vr, int64_t vh) {
+    if (dtype == B200_DTYPE_F32) append_as<float, T>(c, d, k, kr, kh, v, vr, vh);
+    else if (dtype == B200_DTYPE_BF16) append_as<__nv_bfloat16, T>(c, d, k, kr, kh, v, vr, vh);
+    else append_as<__half, T>(c, d, k, kr, kh, v, vr, vh);
+}
+
+int attend_nt(int group, int max_rows) { return (int64_t) group * max_rows <= 8 ? 1 : 2; }
+size_t attend_before_bytes(int n_seq) { return ((size_t) (n_seq + 2) * 8 + 255) / 256 * 256; }
+size_t attend_bytes(int n_seq, int head_dim, int nt, int sms) { return attend_before_bytes(n_seq) + 2 * (size_t) sms * A16_WARPS * 8 * nt * (head_dim + 2) * 4; }
+template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, const CUtensorMap & map, int * err, int device, int sms, void * stream) {
+    static Limits set;
+    const auto kernel = k_kv16_attend<HD, NT, T>;
+    allow_smem(kernel, device, set);
+    launch(kernel, dim3(sms), A16_WARPS * 32, 1024 + a16_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8, stream, false, 1, a, map, err, WAIT_POLLS);
+    const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group, parts = (int64_t) sms * A16_WARPS / ((int64_t) a.c.n_seq * a.c.n_kv);
+    if (parts > 32) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, stream, true, 1, a);
+    else if (parts > 8) launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, stream, true, 1, a);
+    else launch(k_kv4_join<HD, NT, T, 1>, dim3((unsigned) ((items + 7) / 8)), 256, 0, stream, true, 1, a);
+}
+template <typename T> void attend_few(const AttendArgs & a, const CUtensorMap & map, int * err, int head_dim, int nt, int device, int sms, void * stream) {
+    if (head_dim == 128) nt == 1 ? attend_as<128, 1, T>(a, map, err, device, sms, stream) : attend_as<128, 2, T>(a, map, err, device, sms, stream);
+    else nt == 1 ? attend_as<64, 1, T>(a, map, err, device, sms, stream) : attend_as<64, 2, T>(a, map, err, device, sms, stream);
+}
+
+void check_heads(const b200_kv4 & c, int n_head, int max_rows) {
+    need(n_head >= c.n_head_kv && n_head % std::max(1, c.n_head_kv) == 0 && (int64_t) c.n_rows * n_head <= (1 << 30), "n_head is a multiple of n_head_kv, and rows x heads up to 2^30");
+    need(max_rows >= 1 && max_rows <= (1 << 24), "max_rows is the largest number of rows of a sequence");
+}
+
+}  // namespace
+
+void kv16_append(const b200_kv4 & c, int pool_dtype, int dtype, const void * k, int64_t k_row, int64_t k_head, const void * v, int64_t v_row, int64_t v_head) {
+    const Cache d = checked(c);
+    check_dtype(pool_dtype, false);
+    check_dtype(dtype, true);
+    need(c.n_rows == 0 || (k && v && aligned(k, size_of(dtype)) && aligned(v, size_of(dtype))), "k and v are pointers to whole entries");
+    On on(c.device);
+    heed_waits(c.device);
+    if (c.n_seq == 0 || c.n_rows == 0) return;
+    pool_dtype == B200_DTYPE_BF16 ? append_to<__nv_bfloat16>(c, d, dtype, k, k_row, k_head, v, v_row, v_head) : append_to<__half>(c, d, dtype, k, k_row, k_head, v, v_row, v_head);
+}
+
+int64_t kv16_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
+    checked(c);
+    check_heads(c, n_head, max_rows);
+    On on(c.device);
+    return (int64_t) attend_bytes(c.n_seq, c.head_dim, attend_nt(n_head / c.n_head_kv, max_rows), on.sms);
+}
+
+void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int sinks, int max_rows, void * out, void * work,
+                    int64_t work_bytes) {
+    AttendArgs a = {};
+    a.c = checked(c);
+    check_dtype(dtype, false);
+    check_heads(c, n_head, max_rows);
+    need(c.n_rows == 0 || (q && out && aligned(q, 2) && aligned(out, 16)), "q points to whole entries, out starts on 16 bytes");
+    need(std::isfinite(scale), "scale is a finite number");
+    need(window >= 0 && sinks >= 0, "window is a number of positions, or 0 for all; sinks is a number of positions");
+    On on(c.device);
+    heed_waits(c.device);
+    if (c.n_seq == 0 || c.n_rows == 0) return;
+    a.q = q; a.q_row = q_row; a.q_head = q_head; a.out = out;
+    a.q_whole = aligned(q, 16) && !((q_row | q_head) & 7);
+    a.group = n_head / c.n_head_kv;
+    a.scale_log2 = scale * 1.44269504088896341f;
+    a.window = window;
+    a.sinks = window > 0 ? sinks : 0;
+    uint8_t * w = static_cast<uint8_t *>(work);
+    const bool bf16 = dtype == B200_DTYPE_BF16;
+    const CUtensorMap map = pool_map(c, bf16);
+    int * err = wait_word(c.device);
+    const int nt = attend_nt(a.group, max_rows);
+    check_work(work, work_bytes, (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms));
+    a.before = reinterpret_cast<long long *>(w);
+    a.ml = reinterpret_cast<float *>(w + attend_before_bytes(c.n_seq));
+    a.part = a.ml + 2 * (size_t) on.sms * A16_WARPS * 8 * nt * 2;
+    bf16 ? attend_few<__nv_bfloat16>(a, map, err, c.head_dim, nt, c.device, on.sms, c.stream) : attend_few<__half>(a, map, err, c.head_dim, nt, c.device, on.sms, c.stream);
+}
+
+}  // namespace b200

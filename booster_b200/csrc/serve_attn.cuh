@@ -27,6 +27,7 @@ struct AttendArgs {
     int group;
     float scale_log2;                    // scale x log2(e)
     int window;                          // 0: all positions
+    int sinks;                           // first tokens that stay visible under a window (serve_kv16.cuh; the 4-bit cache has none)
     // workspace
     long long * before;                  // [n_seq + 1] pairs of tiles in front of each sequence; [n_seq + 1]: pairs of a warp's piece
     float * part, * ml;                  // [2 x warps][8 NT][HD], [2 x warps][8 NT][2]

@@ -56,16 +56,16 @@ __device__ __forceinline__ void page_bits(const Pages & p, bool free_ones, uint3
     __syncthreads();
 }
 // sum over the threads in front of this one; `all`: of the whole block
-__device__ __forceinline__ int block_before(int mine, int & all) {
-    __shared__ int sums[PG_THREADS / 32];
+template <typename V> __device__ __forceinline__ V block_before(V mine, V & all) {
+    __shared__ V sums[PG_THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int up = mine;
+    V up = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) { const int x = __shfl_up_sync(0xffffffffu, up, d); if (lane >= d) up += x; }
+    for (int d = 1; d < 32; d <<= 1) { const V x = __shfl_up_sync(0xffffffffu, up, d); if (lane >= d) up += x; }
     __syncthreads();
     if (lane == 31) sums[warp] = up;
     __syncthreads();
-    int off = 0, sum = 0;
+    V off = 0, sum = 0;
     for (int w = 0; w < PG_THREADS / 32; w++) { if (w < warp) off += sums[w]; sum += sums[w]; }
     all = sum;
     return off + up - mine;
@@ -129,6 +129,114 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const Pages p, con
             __syncthreads();
         }
     if (threadIdx.x == 0) *status = refused ? -1 : max(0, all - have);
+}
+
+// The tables of a step from its rows' numbers: first, the pages that k_pages_reserve would take, and of each row its position and its place (page x page_tokens + token) in a layer's pool.
+// The one block that hands out pages knows them too: up to PLAN_ROWS rows are its own to write, more are another kernel's
+constexpr int PLAN_ROWS = 4096;
+__host__ __device__ constexpr size_t plan_bytes(int n) { return 4 * ((size_t) 3 * n + 2 + PG_CHUNK); }
+__device__ __forceinline__ void row_place(const Pages & p, const int32_t * slots, const int32_t * first, int n, int r, int32_t * positions, int32_t * places) {
+    int pos = -1, place = -1;
+    if (n > 0 && r < first[n]) {
+        int s = 0;                                                 // the last sequence that begins at or before r
+        for (int hi = n; hi - s > 1;) { const int mid = (s + hi) >> 1; if (first[mid] <= r) s = mid; else hi = mid; }
+        const int slot = slots ? slots[s] : s;
+        if ((unsigned) slot < (unsigned) p.n_slots && p.held[slot] >= 0) {
+            const long long at = (long long) p.held[slot] + r - first[s];
+            pos = (int) min(at, (long long) INT32_MAX);
+            const long long i = at >> p.page_log2;
+            const int page = i < p.max_pages ? p.table[(int64_t) slot * p.table_stride + i] : -1;
+            if ((unsigned) page < (unsigned) p.n_pages) place = (page << p.page_log2) + (pos & ((1 << p.page_log2) - 1));
+        }
+    }
+    positions[r] = pos;
+    places[r] = place;
+}
+static __global__ void __launch_bounds__(PG_THREADS) k_pages_plan(const Pages p, const int32_t * slots, const int32_t * counts, int n, int n_rows, int32_t * first_out, int32_t * positions,
+                                                                  int32_t * places, int32_t * status, bool rows_too) {
+    extern __shared__ uint32_t pg_smem[];
+    __shared__ int bad;
+    const int words = (p.n_pages + 31) >> 5, slot_words = (p.n_slots + 31) >> 5;
+    uint32_t * free_pages = pg_smem, * seen = pg_smem + words;
+    int32_t * first = reinterpret_cast<int32_t *>(seen + slot_words), * from = first + n + 1, * before = from + n, * chunk = before + n + 1;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) bad = 0;
+    for (int i = threadIdx.x; i < slot_words; i += PG_THREADS) seen[i] = 0;
+    page_bits(p, true, free_pages);
+    const int per = (n + PG_THREADS - 1) / PG_THREADS, s0 = min(n, (int) threadIdx.x * per), s1 = min(n, s0 + per);
+    int mine = 0, all;
+    long long rows = 0, all_rows;
+    for (int s = s0; s < s1; s++) {
+        const int slot = slots ? slots[s] : s, more = counts[s];
+        from[s] = 0; before[s] = mine;
+        rows += min(max(more, 0), n_rows + 1);
+        if ((unsigned) slot >= (unsigned) p.n_slots || more < 0) { bad = 1; continue; }
+        if (atomicOr(&seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1) { bad = 1; continue; }
+        const int32_t * row = p.table + (int64_t) slot * p.table_stride;
+        const int64_t need = ((int64_t) p.held[slot] + more + (1 << p.page_log2) - 1) >> p.page_log2;
+        if (p.held[slot] < 0 || need > p.max_pages) { bad = 1; continue; }
+        int f = min(p.held[slot] >> p.page_log2, (int) need);
+        while (f < need && row[f] >= 0) f++;
+        for (int i = f; i < need; i++) if (row[i] >= 0) bad = 1;
+        from[s] = f;
+        mine += (int) need - f;
+    }
+    const int off = block_before(mine, all);
+    long long in_front = block_before(rows, all_rows);
+    for (int s = s0; s < s1; s++) {
+        before[s] += off;
+        first[s] = (int) min(in_front, (long long) n_rows);
+        in_front += min(max(counts[s], 0), n_rows + 1);
+    }
+    if (threadIdx.x == 0) { before[n] = all; first[n] = (int) min(all_rows, (long long) n_rows); if (all_rows > n_rows) bad = 1; }
+    __syncthreads();
+    for (int s = threadIdx.x; s <= n; s += PG_THREADS) first_out[s] = first[s];
+    const int have = n_bits(free_pages, words);
+    const bool refused = bad != 0;
+    if (!refused && have >= all)
+        for (int k0 = 0; k0 < all; k0 += PG_CHUNK) {               // the pages by their bits, then a thread a page
+            each_bit(free_pages, words, min(all, k0 + PG_CHUNK), [&](int k, int page) { if (k >= k0) chunk[k - k0] = page; });
+            __syncthreads();
+            for (int i = threadIdx.x; i < min(PG_CHUNK, all - k0); i += PG_THREADS) {
+                const int k = k0 + i, page = chunk[i];
+                int s = 0;
+                for (int hi = n; hi - s > 1;) { const int mid = (s + hi) >> 1; if (before[mid] <= k) s = mid; else hi = mid; }
+                p.table[(int64_t) (slots ? slots[s] : s) * p.table_stride + from[s] + k - before[s]] = page;
+                p.refs[page] = 1;
+            }
+            __syncthreads();
+        }
+    if (threadIdx.x == 0) *status = refused ? -1 : max(0, all - have);
+    if (rows_too) for (int r = threadIdx.x; r < n_rows; r += PG_THREADS) row_place(p, slots, first, n, r, positions, places);
+}
+static __global__ void __launch_bounds__(256) k_pages_places(const Pages p, const int32_t * slots, const int32_t * first, int n, int n_rows, int32_t * positions, int32_t * places) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const int r = blockIdx.x * 1024 + i * 256 + threadIdx.x; if (r < n_rows) row_place(p, slots, first, n, r, positions, places); }
+}
+
+// Pages that no row to come sees go back: those behind the tokens that are held (rows that were refused), and under a window those that lie whole in front of what the next row sees and behind
+// the first `sinks` tokens. A warp a slot; one that stands twice in the list is looked at twice, its pages go once
+static __global__ void __launch_bounds__(256) k_pages_trim(const Pages p, const int32_t * slots, int n, int window, int sinks) {
+    const int s = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (s >= n) return;
+    const int slot = slots[s];
+    if ((unsigned) slot >= (unsigned) p.n_slots) return;
+    int32_t * row = p.table + (int64_t) slot * p.table_stride;
+    const int P = 1 << p.page_log2, held = max(0, p.held[slot]), seen_from = window > 0 ? held - window + 1 : 0;
+    const int full = (int) (((long long) held + P - 1) >> p.page_log2);                           // pages from this one on hold nothing
+    const int hidden_from = window > 0 ? (int) (((long long) sinks + P - 1) >> p.page_log2) : 0, hidden_to = seen_from > 0 ? seen_from >> p.page_log2 : 0;      // pages of neither
+    for (int i0 = lane; i0 < p.max_pages; i0 += 128) {
+        int page[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) { const int i = i0 + 32 * j; page[j] = i < p.max_pages && (i >= full || (i >= hidden_from && i < hidden_to)) ? row[i] : -1; }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (page[j] >= 0) {
+                const int was = atomicExch(&row[i0 + 32 * j], -1);
+                if ((unsigned) was < (unsigned) p.n_pages) atomicSub(&p.refs[was], 1);
+            }
+    }
 }
 
 // children take their parents' full pages and a copy of the page that is part full

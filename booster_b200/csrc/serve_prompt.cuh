@@ -120,7 +120,7 @@ template <typename V> __device__ __forceinline__ V plan_before(V mine, V & all, 
 }
 
 // one block: the line of entries, a thread an entry. 5 us, its launch and three dependent reads
-__global__ void __launch_bounds__(1024) k_kv4_prompt_plan(const PromptArgs p, int n_blocks) {
+static __global__ void __launch_bounds__(1024) k_kv4_prompt_plan(const PromptArgs p, int n_blocks) {
     extern __shared__ int entry_of[];                              // [n_seq + 1]
     __shared__ long long sums[32];
     const Cache & c = p.a.c;

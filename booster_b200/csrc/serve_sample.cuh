@@ -36,6 +36,12 @@ struct SampleArgs {
     const int32_t * top_k;
     int32_t * ids;
     float * logprobs;
+    // verification of drafted tokens (k_sample<T, true>)
+    const int32_t * step_ids, * first;   // the step's input tokens; sequence i has the rows first[i] .. first[i + 1] - 1
+    int n_seq;
+    const float * accept, * probs;       // probs: what the drafter drew from, [n_rows] rows probs_stride apart, or NULL: it was sure of its token
+    int64_t probs_stride;
+    int32_t * gained;
 };
 
 // 2^40 exp(d steps ln 2 / 16), d <= 0, to the nearest whole number, or 0: y = d steps = n + f with |f| <= 1 / 2, so a table's 2^(n mod 16 / 16), whose 16 entries are the 32 banks of
@@ -66,6 +72,19 @@ __device__ __forceinline__ float key_logit(u64 k) {
 }
 __device__ __forceinline__ int key_index(u64 k) { return (int) ~(uint32_t) k; }
 
+// the last sequence that begins at or before a row, where it holds the row: looked for by a whole warp, 32 places at a time. -1: none
+__device__ __forceinline__ int row_sequence(const int32_t * first, int n_seq, int row) {
+    const int lane = threadIdx.x & 31;
+    int s = 0, n = n_seq;
+    while (n > 1) {
+        const int step = (n + 31) >> 5, i = s + lane * step;
+        const unsigned m = __ballot_sync(0xffffffffu, lane * step < n && first[min(i, n_seq)] <= row);
+        const int k = m ? 31 - __clz(m) : 0;
+        s += k * step;
+        n = min(step, n - k * step);
+    }
+    return n_seq > 0 && first[s] <= row && row < first[s + 1] ? s : -1;
+}
 template <typename F> __device__ __forceinline__ u64 warp_reduce(u64 x, F f) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, d));
@@ -77,7 +96,7 @@ __device__ __forceinline__ u64 warp_sum(u64 x) {
 }
 struct alignas(128) SampleSmem {
     double table[16];
-    u64 red[SA_WARPS], each[SA_MAX_CLUSTER], turn[2][SA_MAX_CLUSTER], sums[SA_MAX_CLUSTER][2];
+    u64 red[SA_WARPS], each[SA_MAX_CLUSTER], rest[SA_MAX_CLUSTER], draft[SA_MAX_CLUSTER], turn[2][SA_MAX_CLUSTER], sums[SA_MAX_CLUSTER][2];
     u64 answer[4];
     u64 parts[SA_SWEEPS][SA_WARPS];
     float top;                           // the block's largest, and its place among the bins
@@ -145,7 +164,10 @@ __device__ __forceinline__ int bin_place(float v) { return __float_as_int(__fmaf
 // the smallest float whose place is p or more
 __device__ __forceinline__ float place_from(int p) { return p <= (int) (-SA_FAR * SA_PER_NAT) ? -INFINITY : (float) p * (1.f / SA_PER_NAT); }
 
-template <typename T>
+// VERIFY: the row's draft is the next row's input token, unless the row is its sequence's last. With p the distribution that the draw is from and q the drafter's, the draft x is taken
+// where accept q(x) < p(x); where it is not, a token is drawn from max(p - q, 0) (p, where that is nothing) by u as always. So what comes out has the distribution p whatever the drafter is.
+// p = t / total and r = max(t - rint(q total), 0) are whole multiples of 2^-40 too. ids[row]: the draft that was taken, or -2 - token of one that was drawn, for k_verify_ends.
+template <typename T, bool VERIFY>
 __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t sa_raw[];
     __shared__ SampleSmem sm;
@@ -159,6 +181,26 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     const float temperature = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, u = a.u[row];
     const int k_all = a.top_k ? a.top_k[row] : 0, k = k_all > 0 && k_all < a.n_vocab ? k_all : 0;
     const bool by_p = top_p < 1.f, cut = temperature > 0.f && (k > 0 || by_p);
+    int draft = -1;                                                      // -1: none is checked here
+    if constexpr (VERIFY) {
+        const int s = row_sequence(a.first, a.n_seq, row);
+        if (s < 0) {
+            if (rank == 0 && tid == 0) { a.ids[row] = -1; a.logprobs[row] = 0.f; }
+            return;
+        }
+        if (row + 1 < min(a.first[s + 1], a.n_rows)) { draft = a.step_ids[row + 1]; if ((unsigned) draft >= (unsigned) a.n_vocab) draft = -2; }
+    }
+    const float * q_row = VERIFY && a.probs && draft != -1 ? a.probs + row * a.probs_stride : nullptr;
+    const auto q_at = [&](int i) { const float q = q_row[i]; return q > 0.f ? (double) q : 0.0; };
+    // whether the draft, of weight t, is taken; what is left of a weight for the draw where it is not
+    const auto takes = [&](u64 t, u64 total) { return draft >= 0 && (double) a.accept[row] * (q_row ? q_at(draft) : 1.0) * (double) total < (double) t; };
+    const auto rest_of = [&](u64 t, int i, u64 total) {
+        if (t == 0) return t;
+        if (!q_row) return i == draft ? 0ull : t;
+        const double x = q_at(i) * (double) total;
+        const u64 less = x < 9e18 ? __double2ull_rn(x) : ~0ull;
+        return t > less ? t - less : 0ull;
+    };
     int turn = 0;
     const auto add = [](u64 x, u64 y) { return x + y; };
     const auto each = [&](auto f) {                                      // f(four logits, index of the first in the slice)
@@ -215,7 +257,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         row_place = max(row_place, places[r]);
         top = fmaxf(top, o->top);
     }
-    const auto finish = [&](int id, float lp) { a.ids[row] = id; if (a.logprobs) a.logprobs[row] = lp; };
+    const auto finish = [&](int id, float lp, bool taken = false) { a.ids[row] = VERIFY && !taken ? -2 - id : id; if (a.logprobs) a.logprobs[row] = lp; };
     const auto first_of_largest = [&]() {
         u64 mine = ~0ull;
         each([&](const float (&v)[4], int i) {
@@ -226,7 +268,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     };
     if (top == -INFINITY || !(temperature > 0.f)) {                      // (behind the join nobody reads here any more)
         const int i = first_of_largest();
-        if (rank == 0 && tid == 0) finish(top == -INFINITY ? -1 : i, top == -INFINITY ? -INFINITY : 0.f);
+        if (rank == 0 && tid == 0) finish(top == -INFINITY ? -1 : i, top == -INFINITY ? -INFINITY : 0.f, VERIFY && draft >= 0 && draft == i && top != -INFINITY);
         return;
     }
     const auto exactly = [&](float v) { return v == top ? 0.0 : (double) top - (double) v; };   // how far a logit is from the largest
@@ -337,6 +379,36 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                 const bool in = tid < m && before_me < k && (before_me == 0 || !by_p || (double) c < (double) top_p * (double) sm.answer[0]) && key_logit(mine) >= from_p;
                 const u64 t = tempered(key_logit(mine), in && key_logit(mine) >= from_t);
                 t_of[tid] = t;
+                if constexpr (VERIFY) {
+                    if (tid == 0) sm.answer[1] = 0;
+                    __syncthreads();
+                    const bool is_draft = tid < m && key_index(mine) == draft;
+                    if (is_draft) sm.answer[1] = t;
+                    u64 total = 0;
+#pragma unroll 4
+                    for (int j = 0; j < m; j++) total += t_of[j];
+                    __syncthreads();
+                    if (takes(sm.answer[1], total)) {
+                        if (is_draft) finish(draft, log_share(exactly(key_logit(mine)), total), true);
+                        return;
+                    }
+                    const u64 r = draft == -1 ? t : rest_of(t, key_index(mine), total);
+                    w_of[tid] = r;                                       // (the sums in order are done with)
+                    if (tid == 0) sm.answer[2] = 0;
+                    __syncthreads();
+                    if (r) sm.answer[2] = 1;
+                    __syncthreads();
+                    const u64 * of = sm.answer[2] ? w_of : t_of;
+                    const u64 own = of[tid];
+                    if (own) {
+                        u64 all = 0, upto = 0;
+#pragma unroll 4
+                        for (int j = 0; j < m; j++) { all += of[j]; upto += (uint32_t) list[j] >= (uint32_t) mine ? of[j] : 0; }
+                        const u64 target = target_of(all);
+                        if (upto - own <= target && target < upto) finish(key_index(mine), log_share(exactly(key_logit(mine)), total));
+                    }
+                    return;
+                }
                 __syncthreads();
                 if (in) {
                     u64 total = 0, upto = 0;
@@ -372,6 +444,39 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
             u64 sum = 0;
             for (int i = d0; i < d1; i++) { const float v = __uint_as_float((uint32_t) list[i]); sum += tempered(v, v >= from_t); }
             c = block_before64(sum, all, sm.red);
+            if constexpr (VERIFY) {
+                const u64 total = all;
+                if (tid == 0) sm.answer[1] = 0;
+                __syncthreads();
+                float v_draft = 0.f;
+                bool is_draft = false;
+                for (int i = d0; i < d1; i++)
+                    if ((int) ~(uint32_t) (list[i] >> 32) == draft) { is_draft = true; v_draft = __uint_as_float((uint32_t) list[i]); sm.answer[1] = tempered(v_draft, v_draft >= from_t); }
+                __syncthreads();
+                if (takes(sm.answer[1], total)) {
+                    if (is_draft) finish(draft, log_share(exactly(v_draft), total), true);
+                    return;
+                }
+                const auto rest = [&](int i) {
+                    const float v = __uint_as_float((uint32_t) list[i]);
+                    const u64 t = tempered(v, v >= from_t);
+                    return draft == -1 ? t : rest_of(t, (int) ~(uint32_t) (list[i] >> 32), total);
+                };
+                u64 rest_sum = 0, rest_all;
+                for (int i = d0; i < d1; i++) rest_sum += rest(i);
+                const u64 rest_c = block_before64(rest_sum, rest_all, sm.red);
+                if (rest_all) {
+                    const u64 target = target_of(rest_all);
+                    if (rest_c <= target && target < rest_c + rest_sum) {
+                        c = rest_c;
+                        for (int i = d0; i < d1; i++) {
+                            c += rest(i);
+                            if (c > target) { finish((int) ~(uint32_t) (list[i] >> 32), log_share(exactly(__uint_as_float((uint32_t) list[i])), total)); break; }
+                        }
+                    }
+                    return;
+                }
+            }
             const u64 target = target_of(all);
             if (c <= target && target < c + sum) {
                 for (int i = d0; i < d1; i++) {
@@ -487,26 +592,73 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         for (int e = 0; e < 4; e++) w[e] = tempered(v[e], in[e]);
     };
     const int sweeps = (groups + SA_THREADS - 1) / SA_THREADS;
-    for (int s = 0; s < sweeps; s++) {
-        const int g = s * SA_THREADS + tid;
-        u64 sum = 0;
-        if (g < groups) {
-            float v[4];
-            u64 w[4];
-            four_of(vals, g, v);
-            drawn(v, 4 * g, w);
-            sum = w[0] + w[1] + w[2] + w[3];
+    const auto sum_parts = [&](auto weigh) {                             // the block's weights, a part a warp and sweep
+        for (int s = 0; s < sweeps; s++) {
+            const int g = s * SA_THREADS + tid;
+            u64 sum = 0;
+            if (g < groups) {
+                float v[4];
+                u64 w[4];
+                four_of(vals, g, v);
+                weigh(v, 4 * g, w);
+                sum = w[0] + w[1] + w[2] + w[3];
+            }
+            if (__any_sync(0xffffffffu, sum != 0)) sum = warp_sum(sum);
+            if (lane == 0) sm.parts[s][warp] = sum;
         }
-        if (__any_sync(0xffffffffu, sum != 0)) sum = warp_sum(sum);
-        if (lane == 0) sm.parts[s][warp] = sum;
-    }
-    __syncthreads();
+        __syncthreads();
+    };
+    sum_parts(drawn);
     u64 mine = tid < sweeps * SA_WARPS ? sm.parts[tid / SA_WARPS][tid % SA_WARPS] : 0, block_sum;      // (256 parts at most)
     const u64 in_block = block_before64(mine, block_sum, sm.red);
     if (tid < blocks) cl.map_shared_rank(&sm, tid)->each[rank] = block_sum;
+    float v_draft = 0.f;
+    u64 t_draft = 0;
+    const bool draft_here = VERIFY && draft >= base && draft - base < n;
+    if constexpr (VERIFY) {
+        if (tid < blocks) {
+            if (draft_here) {
+                float v[4];
+                u64 w[4];
+                four_of(vals, (draft - base) >> 2, v);
+                drawn(v, (draft - base) & ~3, w);
+#pragma unroll
+                for (int e = 0; e < 4; e++) if (((draft - base) & 3) == e) { v_draft = v[e]; t_draft = w[e]; }
+            }
+            cl.map_shared_rank(&sm, tid)->draft[rank] = t_draft;
+        }
+    }
     cl.sync();
     u64 total = 0, front = in_block;
     for (int r = 0; r < blocks; r++) { if (r < rank) front += sm.each[r]; total += sm.each[r]; }
+    const u64 whole = total;
+    bool by_rest = false;
+    if constexpr (VERIFY) {
+        if (draft != -1) {
+            u64 t = 0;
+            for (int r = 0; r < blocks; r++) t += sm.draft[r];
+            if (takes(t, whole)) {
+                if (draft_here && tid == 0) finish(draft, log_share(exactly(v_draft), whole), true);
+                return;
+            }
+            // the same of what is left of each weight; without the drafter's distribution only the draft's own goes
+            if (q_row) sum_parts([&](const float (&v)[4], int i, u64 (&w)[4]) {
+                drawn(v, i, w);
+#pragma unroll
+                for (int e = 0; e < 4; e++) if (w[e]) w[e] = rest_of(w[e], base + i + e, whole);
+            });
+            else {
+                if (draft_here && tid == 0) { const int g = (draft - base) >> 2; sm.parts[g / SA_THREADS][g % SA_THREADS / 32] -= t_draft; }
+                __syncthreads();
+            }
+            const u64 mine_r = tid < sweeps * SA_WARPS ? sm.parts[tid / SA_WARPS][tid % SA_WARPS] : 0, in_block_r = block_before64(mine_r, block_sum, sm.red);
+            if (tid < blocks) cl.map_shared_rank(&sm, tid)->rest[rank] = block_sum;
+            cl.sync();
+            u64 total_r = 0, front_r = in_block_r;
+            for (int r = 0; r < blocks; r++) { if (r < rank) front_r += sm.rest[r]; total_r += sm.rest[r]; }
+            if (total_r) { by_rest = true; total = total_r; front = front_r; mine = mine_r; }
+        }
+    }
     const u64 target = target_of(total);
     if (tid == 0) sm.answer[3] = ~0ull;
     __syncthreads();
@@ -518,6 +670,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         if (g < groups) four_of(vals, g, v);
         u64 w[4], sum = 0;
         drawn(v, 4 * g, w);
+        if (VERIFY && by_rest)
+#pragma unroll
+            for (int e = 0; e < 4; e++) if (w[e]) w[e] = rest_of(w[e], base + 4 * g + e, whole);
         sum = w[0] + w[1] + w[2] + w[3];
         u64 up = sum;
 #pragma unroll
@@ -526,9 +681,31 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
         if (c <= target && target < c + sum)
             for (int e = 0; e < 4; e++) {
                 c += w[e];
-                if (c > target) { finish(base + 4 * g + e, log_share(exactly(v[e]), total)); break; }
+                if (c > target) { finish(base + 4 * g + e, log_share(exactly(v[e]), whole)); break; }
             }
     }
+}
+
+// a warp a sequence: its rows up to the first whose draft was not taken gain a token each; what stands behind goes to -1 and 0
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) k_verify_ends(const SampleArgs a) {
+    const int s = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (s >= a.n_seq) return;
+    const int begin = min(max(a.first[s], 0), a.n_rows), end = min(max(a.first[s + 1], begin), a.n_rows);
+    int stop = end;                                                      // the row that the sequence ends with
+    for (int r0 = begin; r0 < end; r0 += 32) {
+        const int r = r0 + lane, id = r < end ? a.ids[r] : 0;
+        if (stop == end) {
+            const unsigned drawn = __ballot_sync(0xffffffffu, id < 0);
+            if (drawn) stop = r0 + __ffs(drawn) - 1;
+        }
+        if (r < end && r >= stop) {
+            a.ids[r] = r == stop ? -2 - id : -1;
+            if (r > stop) a.logprobs[r] = 0.f;
+        }
+    }
+    if (lane == 0) a.gained[s] = min(stop + 1, end) - begin;
 }
 
 }  // namespace srv

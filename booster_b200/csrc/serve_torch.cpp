@@ -34,6 +34,12 @@ struct Api {
     decltype(&b200_pages_compact) pages_compact;
     decltype(&b200_pages_copy) pages_copy;
     decltype(&b200_sample) sample;
+    decltype(&b200_kv16_append) kv16_append;
+    decltype(&b200_kv16_attention_workspace) kv16_attention_workspace;
+    decltype(&b200_kv16_attention) kv16_attention;
+    decltype(&b200_pages_plan) pages_plan;
+    decltype(&b200_pages_trim) pages_trim;
+    decltype(&b200_verify) verify;
 } api;
 PyObject * library_error;
 
@@ -88,20 +94,29 @@ int64_t page_stride(const at::Tensor & pool) {
          "pool is a uint8 tensor [..., n_pages, n_head_kv, page_tokens / 16, 18 * head_dim] of contiguous pages");
     return pool.size(d - 4) > 1 ? pool.stride(d - 4) : std::max(pool.stride(d - 4), kv * tiles * size);
 }
-// one layer's cache and a step
-b200_kv4 step_of(const at::Tensor & pool, PyObject * table, PyObject * held, PyObject * first, PyObject * slots, int64_t n_rows) {
+// the same in bytes of a pool in 16 bits, [..., n_pages, 2, n_head_kv, page_tokens, head_dim]
+int64_t page_stride16(const at::Tensor & pool) {
+    const int64_t d = pool.dim(), hd = pool.size(d - 1), tokens = pool.size(d - 2), kv = pool.size(d - 3), page = 2 * kv * tokens * hd;
+    need((pool.scalar_type() == at::kBFloat16 || pool.scalar_type() == at::kHalf) && pool.size(d - 4) == 2 && (pool.stride(d - 1) == 1 || hd == 1) && (tokens == 1 || pool.stride(d - 2) == hd) &&
+             (kv == 1 || pool.stride(d - 3) == tokens * hd) && pool.stride(d - 4) == kv * tokens * hd,
+         "pool is a bfloat16 or float16 tensor [..., n_pages, 2, n_head_kv, page_tokens, head_dim] of contiguous pages");
+    return 2 * (pool.size(d - 5) > 1 ? pool.stride(d - 5) : std::max(pool.stride(d - 5), page));
+}
+// one layer's cache, of 4 or 16 bits, and a step
+template <bool WIDE = false> b200_kv4 step_of(const at::Tensor & pool, PyObject * table, PyObject * held, PyObject * first, PyObject * slots, int64_t n_rows) {
     const int index = on(pool);
-    need(pool.dim() == 4, "pool is one layer's [n_pages, n_head_kv, page_tokens / 16, 18 * head_dim]");
+    if (WIDE) need(pool.dim() == 5, "pool is one layer's [n_pages, 2, n_head_kv, page_tokens, head_dim]");
+    else need(pool.dim() == 4, "pool is one layer's [n_pages, n_head_kv, page_tokens / 16, 18 * head_dim]");
     const int64_t n_seq = tensor(first, "first").numel() - 1;
     need(n_seq >= 0, "first has one entry more than there are sequences");
     const Table t = table_of(table, index);
     b200_kv4 c;
     c.device = index;
-    c.page_stride = page_stride(pool);
+    c.page_stride = WIDE ? page_stride16(pool) : page_stride(pool);
     c.n_pages = small(pool.size(0), "pool: too many pages");
-    c.n_head_kv = small(pool.size(1), "pool: too many heads");
-    c.page_tokens = small(16 * pool.size(2), "pool: pages too long");
-    c.head_dim = small(pool.size(3) / 18, "pool: heads too wide");
+    c.n_head_kv = small(pool.size(WIDE ? 2 : 1), "pool: too many heads");
+    c.page_tokens = small(WIDE ? pool.size(3) : 16 * pool.size(2), "pool: pages too long");
+    c.head_dim = small(WIDE ? pool.size(4) : pool.size(3) / 18, "pool: heads too wide");
     c.n_slots = t.slots; c.max_pages = t.most;
     c.n_seq = small(n_seq, "first: too many sequences");
     c.n_rows = small(n_rows, "too many rows");
@@ -190,6 +205,47 @@ PyObject * kv4_attention(PyObject * const * a) {                         // q, p
     return THPVariable_Wrap(out);
 }
 
+Rows rows16_of(const char * name, const at::Tensor & x, const at::Tensor & pool, int64_t heads = -1) {
+    if (x.dim() != 3 || x.device() != pool.device() || pool.dim() != 5 || x.size(2) != pool.size(4) || (heads >= 0 && x.size(1) != heads))
+        throw Refused(std::string(name) + " is a tensor [rows, heads, head_dim] that fits one layer's pool, on its device");
+    if (x.stride(2) != 1) throw Refused(std::string(name) + ": the entries of a head are contiguous");
+    return {x.stride(0), x.stride(1)};
+}
+PyObject * kv16_append(PyObject * const * a) {                           // pool, table, held, first, k, v, slots
+    const at::Tensor & pool = tensor(a[0], "pool"), & k = tensor(a[4], "k"), & v = tensor(a[5], "v");
+    const Rows rk = rows16_of("k", k, pool, pool.dim() == 5 ? pool.size(2) : -1), rv = rows16_of("v", v, pool);
+    const int type = type_of(k);
+    need(type >= 0 && k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes(), "k and v are float32, bfloat16 or float16, and alike");
+    const b200_kv4 c = step_of<true>(pool, a[1], a[2], a[3], a[6], k.size(0));
+    done(api.kv16_append(&c, type_of(pool), type, k.data_ptr(), rk.row, rk.head, v.data_ptr(), rv.row, rv.head) == 0, "kv16_append");
+    Py_RETURN_NONE;
+}
+PyObject * kv16_attention(PyObject * const * a) {                        // q, pool, table, held, first, slots, scale, window, sinks, max_rows, out
+    const at::Tensor & q = tensor(a[0], "q"), & pool = tensor(a[1], "pool");
+    const Rows r = rows16_of("q", q, pool);
+    need(q.scalar_type() == pool.scalar_type(), "q has the pool's type");
+    const int64_t rows = q.size(0);
+    const b200_kv4 c = step_of<true>(pool, a[2], a[3], a[4], a[5], rows);
+    const int heads = small(q.size(1), "q: too many heads"), window = number(a[7], "window"), sinks = number(a[8], "sinks");
+    double scale = 1.0 / std::sqrt((double) c.head_dim);
+    if (a[6] != Py_None) {
+        scale = PyFloat_AsDouble(a[6]);
+        if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); throw Refused("scale is a number"); }
+    }
+    const int most = a[9] != Py_None ? std::max(1, number(a[9], "max_rows")) : std::max<int>(1, (int) ((rows + c.n_seq - 1) / std::max(1, c.n_seq)));
+    at::Tensor out;
+    if (a[10] == Py_None) out = at::empty(q.sizes(), q.options());
+    else {
+        out = tensor(a[10], "out");
+        need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.is_contiguous(), "out is a contiguous tensor like q");
+    }
+    const int64_t size = api.kv16_attention_workspace(&c, heads, most);
+    done(size >= 0, "kv16_attention");
+    const at::Tensor work = at::empty({size}, pool.options().dtype(at::kByte));
+    done(api.kv16_attention(&c, type_of(q), q.data_ptr(), r.row, r.head, heads, (float) scale, window, sinks, most, out.data_ptr(), work.data_ptr(), size) == 0, "kv16_attention");
+    return THPVariable_Wrap(out);
+}
+
 b200_pages pages_of(PyObject * table, PyObject * held, PyObject * refs_o, int page_tokens, PyObject * pool_o) {
     const at::Tensor & refs = tensor(refs_o, "refs");
     const int index = on(refs);
@@ -209,14 +265,18 @@ b200_pages pages_of(PyObject * table, PyObject * held, PyObject * refs_o, int pa
     p.refs = ints("refs", refs_o, index);
     if (pool_o) {
         const at::Tensor & pool = tensor(pool_o, "pool");
-        need(pool.dim() == 5 && there(pool, index) && pool.size(1) == p.n_pages, "pool is [n_layer, n_pages, n_head_kv, page_tokens / 16, 18 * head_dim], refs has an entry a page");
-        p.page_stride = page_stride(pool);
+        const bool wide = pool.dim() == 6;
+        need((pool.dim() == 5 || wide) && there(pool, index) && pool.size(1) == p.n_pages,
+             "pool is [n_layer, n_pages, n_head_kv, page_tokens / 16, 18 * head_dim] or [n_layer, n_pages, 2, n_head_kv, page_tokens, head_dim], refs has an entry a page");
+        p.page_stride = wide ? page_stride16(pool) : page_stride(pool);
         p.n_layer = small(pool.size(0), "pool: too many layers");
-        p.n_head_kv = small(pool.size(2), "pool: too many heads");
-        p.page_tokens = small(16 * pool.size(3), "pool: pages too long");
-        p.head_dim = small(pool.size(4) / 18, "pool: heads too wide");
+        p.n_head_kv = small(pool.size(wide ? 3 : 2), "pool: too many heads");
+        p.page_tokens = small(wide ? pool.size(4) : 16 * pool.size(3), "pool: pages too long");
+        const int64_t width = wide ? pool.size(5) : pool.size(4) / 18;
+        need(width < B200_POOL_16BIT, "pool: heads too wide");
+        p.head_dim = (int) width | (wide ? B200_POOL_16BIT : 0);
         p.pool = pool.data_ptr();
-        p.layer_stride = pool.stride(0);
+        p.layer_stride = pool.stride(0) * (wide ? 2 : 1);
     }
     return p;
 }
@@ -266,6 +326,27 @@ PyObject * pages_copy(PyObject * const * a) {                            // pool
     done(api.pages_copy(&p, src, dst, n, static_cast<int32_t *>(status.data_ptr()), work.data_ptr(), work.numel()) == 0, "pages_copy");
     return THPVariable_Wrap(status);
 }
+PyObject * pages_plan(PyObject * const * a) {                            // table, held, refs, counts, page_tokens, rows, slots
+    const int64_t n64 = tensor(a[3], "counts").numel();
+    const int n = small(n64, "counts: too many sequences"), rows = number(a[5], "rows");
+    need(rows >= 0, "rows is the number of rows of the step");
+    const b200_pages p = pages_of(a[0], a[1], a[2], number(a[4], "page_tokens"), nullptr);
+    need(a[6] != Py_None || n <= p.n_slots, "without slots, sequence i is slot i: more sequences than slots");
+    const int32_t * slots = a[6] != Py_None ? ints("slots", a[6], p.device, n) : nullptr, * counts = ints("counts", a[3], p.device);
+    const at::TensorOptions like = THPVariable_Unpack(a[2]).options();
+    at::Tensor out[4] = {at::empty({n + 1}, like), at::empty({rows}, like), at::empty({rows}, like), at::empty({1}, like)};
+    done(api.pages_plan(&p, slots, counts, n, rows, static_cast<int32_t *>(out[0].data_ptr()), static_cast<int32_t *>(out[1].data_ptr()), static_cast<int32_t *>(out[2].data_ptr()),
+                        static_cast<int32_t *>(out[3].data_ptr())) == 0, "pages_plan");
+    PyObject * r = PyTuple_New(4);
+    for (int i = 0; r && i < 4; i++) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(out[i]));
+    return r;
+}
+PyObject * pages_trim(PyObject * const * a) {                            // table, held, refs, page_tokens, slots, window, sinks
+    const b200_pages p = pages_of(a[0], a[1], a[2], number(a[3], "page_tokens"), nullptr);
+    const int32_t * slots = ints("slots", a[4], p.device);
+    done(api.pages_trim(&p, slots, small(THPVariable_Unpack(a[4]).numel(), "slots: too many"), number(a[5], "window"), number(a[6], "sinks")) == 0, "pages_trim");
+    Py_RETURN_NONE;
+}
 const void * per_row(const char * name, PyObject * o, at::ScalarType type, int64_t rows, int index) {
     if (o == Py_None) return nullptr;
     const at::Tensor & t = tensor(o, name);
@@ -286,6 +367,40 @@ PyObject * sample(PyObject * const * a) {                                // logi
                     static_cast<int32_t *>(ids.data_ptr()), static_cast<float *>(logprobs.data_ptr())) == 0, "sample");
     PyObject * pi = THPVariable_Wrap(ids), * pl = THPVariable_Wrap(logprobs), * r = pi && pl ? PyTuple_Pack(2, pi, pl) : nullptr;
     Py_XDECREF(pi); Py_XDECREF(pl);
+    return r;
+}
+
+PyObject * verify(PyObject * const * a) {                                // logits, ids, first, u, accept, temperature, top_k, top_p, min_p, draft_probs
+    const at::Tensor & logits = tensor(a[0], "logits");
+    const int index = on(logits), type = type_of(logits);
+    need(logits.dim() == 2 && type >= 0 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits is a float32, bfloat16 or float16 tensor [rows, n_vocab] of contiguous rows");
+    const int rows = small(logits.size(0), "logits: too many rows"), vocab = small(logits.size(1), "logits: too many a row");
+    const int64_t n64 = tensor(a[2], "first").numel() - 1;
+    need(n64 >= 0, "first has one entry more than there are sequences");
+    const int n = small(n64, "first: too many sequences");
+    const int32_t * ids = ints("ids", a[1], index, rows), * first = ints("first", a[2], index);
+    const float * in[2];
+    for (int i = 0; i < 2; i++) {
+        need(a[3 + i] != Py_None, "u and accept are float32 tensors of an entry a row");
+        in[i] = static_cast<const float *>(per_row(i ? "accept" : "u", a[3 + i], at::kFloat, rows, index));
+    }
+    const float * temperature = static_cast<const float *>(per_row("temperature", a[5], at::kFloat, rows, index));
+    const int32_t * top_k = static_cast<const int32_t *>(per_row("top_k", a[6], at::kInt, rows, index));
+    const float * top_p = static_cast<const float *>(per_row("top_p", a[7], at::kFloat, rows, index)), * min_p = static_cast<const float *>(per_row("min_p", a[8], at::kFloat, rows, index));
+    const float * probs = nullptr;
+    int64_t probs_stride = 0;
+    if (a[9] != Py_None) {
+        const at::Tensor & q = tensor(a[9], "draft_probs");
+        need(q.scalar_type() == at::kFloat && there(q, index) && q.sizes() == logits.sizes() && (q.stride(1) == 1 || q.size(1) == 1), "draft_probs is a float32 tensor like logits, of contiguous rows");
+        probs = static_cast<const float *>(q.data_ptr());
+        probs_stride = rows > 1 ? q.stride(0) : vocab;
+    }
+    const at::TensorOptions whole = logits.options().dtype(at::kInt);
+    at::Tensor out[3] = {at::empty({n}, whole), at::empty({rows}, whole), at::empty({rows}, logits.options().dtype(at::kFloat))};
+    done(api.verify(index, stream_of(index), type, logits.data_ptr(), rows > 1 ? logits.stride(0) : vocab, rows, vocab, ids, first, n, in[0], in[1], temperature, top_k, top_p, min_p, probs,
+                    probs_stride, static_cast<int32_t *>(out[0].data_ptr()), static_cast<int32_t *>(out[1].data_ptr()), static_cast<float *>(out[2].data_ptr())) == 0, "verify");
+    PyObject * r = PyTuple_New(3);
+    for (int i = 0; r && i < 3; i++) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(out[i]));
     return r;
 }
 
@@ -317,6 +432,7 @@ PyObject * bind(PyObject *, PyObject * const * args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&bind)), METH_FASTCALL, nullptr},
     FAST(kv4_append, 7), FAST(kv4_read, 8), FAST(kv4_attention, 10), FAST(pages_reserve, 6), FAST(pages_fork, 6), FAST(pages_free, 4), FAST(pages_compact, 3), FAST(pages_copy, 5), FAST(sample, 6),
+    FAST(kv16_append, 7), FAST(kv16_attention, 11), FAST(pages_plan, 7), FAST(pages_trim, 7), FAST(verify, 10),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serve", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

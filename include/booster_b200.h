@@ -346,6 +346,7 @@ void b200_set_attention_route(int route);
  * host can see are checked (non-zero, b200_last_error()). What device tables say is bounded by the kernels: a page or slot that does not exist is
  * as absent, and never read or written. The caller's current device stays as it is. */
 enum { B200_DTYPE_F32 = 0, B200_DTYPE_BF16 = 1, B200_DTYPE_F16 = 2 };
+enum { B200_POOL_16BIT = 0x10000 };          /* beside head_dim in struct b200_pages: the pool is one of b200_kv16_* */
 
 /* One layer of a paged cache and the rows of a step. The pool holds n_pages pages, page_stride bytes apart, of n_head_kv x page_tokens / 16 tiles of 18 x head_dim
  * bytes each (booster_b200/csrc/serve_cache.cuh describes a tile); it is zeroed once, before its first use, and written by these calls only. Row s of table
@@ -376,7 +377,19 @@ int b200_kv4_read(const b200_kv4 * c, int dtype, void * k, void * v);
 int64_t b200_kv4_attention_workspace(const b200_kv4 * c, int n_head, int max_rows);
 int b200_kv4_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int max_rows, void * out, void * work, int64_t work_bytes);
 
-/* Waits inside b200_kv4_attention's kernels are bounded, to about a second. Should one run out, that call's results are worthless, and the next call of this group on the device that finds it
+/* The same cache in 16 bits: struct b200_kv4 with another pool, of pages [2][n_head_kv][page_tokens][head_dim] of the type pool_dtype (BF16 or F16), keys and then values. It is zeroed once, before
+ * its first use, and written by these calls only (b200_pages_fork, _compact and _copy take it with B200_POOL_16BIT).
+ * b200_kv16_append: k and v (strides in entries, dtype F32, BF16 or F16) are rounded once. A token with an infinity or a NaN in a head's key or value, or a number that the pool's type cannot
+ * hold, stands as a key of NaN and a value of 0: rows that see it answer NaN for the head. Rows whose page is absent are dropped. */
+int b200_kv16_append(const b200_kv4 * c, int pool_dtype, int dtype, const void * k, int64_t k_row, int64_t k_head, const void * v, int64_t v_row, int64_t v_head);
+/* attention as b200_kv4_attention has it, q and out of the pool's dtype. With window > 0 a row at position p sees, of the positions j <= p that have a page, those with j > p - window or
+ * j < sinks (the first ones stay visible); window 0: all, whatever sinks is. A row that sees nothing answers 0, one whose query holds an infinity or a NaN and that sees something NaN; scores beyond
+ * fp32's range are infinities. work: b200_kv16_attention_workspace() bytes (-1: error) on 16 bytes. */
+int64_t b200_kv16_attention_workspace(const b200_kv4 * c, int n_head, int max_rows);
+int b200_kv16_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int sinks, int max_rows, void * out, void * work,
+                        int64_t work_bytes);
+
+/* Waits inside the kernels of b200_kv4_attention and b200_kv16_attention are bounded, to about a second. Should one run out, that call's results are worthless, and the next call of this group on the device that finds it
  * out fails with a message that says so, has done nothing itself and may be repeated. b200_kv4_status asks without doing anything else: 0, or non-zero where a wait ran out that no call has told
  * of yet. Work that is still on its way is not waited for, so a program that replays graphs asks behind a synchronisation. */
 int b200_kv4_status(int device);
@@ -397,6 +410,14 @@ typedef struct b200_pages {
 int64_t b200_pages_workspace(const b200_pages * p, int n);
 /* pages for first[i + 1] - first[i] tokens more of slot slots[i] (NULL: slot i), behind its held tokens; held itself is the caller's to advance */
 int b200_pages_reserve(const b200_pages * p, const int32_t * slots, const int32_t * first, int n, int32_t * status);
+/* The tables of a step from counts[i] new rows of slot slots[i] (NULL: slot i): first[n + 1], their sums from 0; the pages that b200_pages_reserve would take with it; and of each of n_rows rows
+ * its position in its sequence and its place in a layer's pool, page x page_tokens + token (what keys, values or anything else that stands by tokens is written to). Rows of no sequence have -1 and
+ * -1, so a step may be padded; a place without a page is -1. status: as above, -1 for negative counts or more than n_rows too; first, positions and places (of the pages that are there) are
+ * written in any case, first n_rows at most. */
+int b200_pages_plan(const b200_pages * p, const int32_t * slots, const int32_t * counts, int n, int n_rows, int32_t * first, int32_t * positions, int32_t * places, int32_t * status);
+/* pages of the slots that no row to come sees go back: those behind the held tokens (the program has lowered held behind rows that were refused) and, with window > 0, those whose tokens all stand
+ * in front of the last window - 1 of the held ones and behind the first sinks. A slot without its first pages cannot be forked */
+int b200_pages_trim(const b200_pages * p, const int32_t * slots, int n, int window, int sinks);
 /* slot children[i], which is empty, becomes what slot parents[i] is: full pages are shared, the tokens of the last page are copied in every layer when it is part full */
 int b200_pages_fork(const b200_pages * p, const int32_t * parents, const int32_t * children, int n, int32_t * status, void * work, int64_t work_bytes);
 /* the slots give their pages back and are empty */
@@ -414,6 +435,18 @@ int b200_pages_copy(const b200_pages * p, const int32_t * src, const int32_t * d
  * logprobs (may be NULL): log of the drawn token's share (0 at temperature <= 0). NaN counts as -infinity; a row of nothing else gives -1 and -infinity. */
 int b200_sample(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature, const int32_t * top_k,
                 const float * top_p, const float * min_p, int32_t * ids, float * logprobs);
+
+/* Verification of drafted tokens. A step's rows are its input tokens ids[n_rows]; sequence i has the rows first[i] .. first[i + 1] - 1 (first[n_seq + 1] ascends), a token that is certain and
+ * then its drafts, and logits[row] are the target's for what follows the row. With p the distribution that b200_sample draws from (temperature, top_k, top_p, min_p by row; temperature <= 0:
+ * all on the first of the largest) and q = draft_probs[row * draft_stride + i] (F32) what the drafter drew the row's draft ids[row + 1] from (NULL: it was sure, 1 at the draft), the draft is taken if
+ * accept[row] q(draft) < p(draft). Where it is not, the sequence ends with a token drawn by u[row] as b200_sample draws, from max(p - q, 0) instead of p (p where that is nothing); where all are
+ * taken, with one drawn from p at its last row. So the tokens have the target's distribution, and a sequence of one row gets b200_sample's token. A draft outside 0 .. n_vocab - 1 is never taken and
+ * takes nothing off p; entries of q that are negative or NaN count as 0.
+ * gained[n_seq]: how many tokens sequence i has gained (drafts taken and one drawn; 0 without rows), which is what its held tokens grow by; tokens[n_rows]: what follows each row up to there, -1
+ * behind and for rows of no sequence; logprobs[n_rows]: log p of those (0 at temperature <= 0), 0 where tokens has -1. A row of no finite logit ends its sequence with -1 and -infinity. */
+int b200_verify(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const int32_t * ids, const int32_t * first, int n_seq, const float * u,
+                const float * accept, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p, const float * draft_probs, int64_t draft_stride, int32_t * gained,
+                int32_t * tokens, float * logprobs);
 
 #ifdef __cplusplus
 }
