@@ -57,19 +57,6 @@ template <int HD, typename T> void attend_nt_as(const AttendArgs & a, int nt, in
 }
 
 // attention of prompts' portions
-int64_t prompt_entries(const b200_kv4 & c, int group) { return (int64_t) c.n_rows * group / PR_COLS + c.n_seq + 1; }
-struct PromptWork { int64_t entries, first, ml, part, bytes; };       // places in the workspace; `before` is first
-PromptWork prompt_work(const b200_kv4 & c, int group, int sms) {
-    const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    const int64_t n = prompt_entries(c, group), slots = 2 * (int64_t) sms * PR_COLS;
-    PromptWork w;
-    w.entries = up((n + 2) * 8);
-    w.first = w.entries + up(n * (int64_t) sizeof(Entry));
-    w.ml = w.first + up((sms + 2) * 4);
-    w.part = w.ml + up(slots * 8);
-    w.bytes = w.part + slots * c.head_dim * 4;
-    return w;
-}
 template <int HD, typename T> void prompt_as(const PromptArgs & p, int64_t entries, int device, int sms, void * stream) {
     static Limits set;
     const auto kernel = k_kv4_prompt<HD, T>;

@@ -1,6 +1,6 @@
 // serve16.cu — host side of the 16-bit paged cache (serve.hpp): checks of arguments, launch shapes, launches on the caller's stream.
 #include "serve_host.cuh"
-#include "serve_kv16.cuh"
+#include "serve_kv16_prompt.cuh"
 
 namespace b200 {
 namespace {
@@ -9,8 +9,8 @@ using namespace srv;
 
 Cache checked(const b200_kv4 & c) { return checked_cache(c, "kv16", 64 * c.head_dim); }
 
-// boxes of 16 tokens and 64 dims, keys and values of a KV head of a page
-CUtensorMap pool_map(const b200_kv4 & c, bool bf16) {
+// boxes of `tokens` tokens and 64 dims of a KV head of a page, of keys and values at once or of one of them
+CUtensorMap pool_map(const b200_kv4 & c, bool bf16, int tokens, int sides) {
     static const auto encode = [] {
         void * fn = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -22,7 +22,7 @@ CUtensorMap pool_map(const b200_kv4 & c, bool bf16) {
     CUtensorMap m;
     const cuuint64_t row = (cuuint64_t) c.head_dim * 2, head = row * c.page_tokens, side = head * c.n_head_kv;
     const cuuint64_t dims[5] = {(cuuint64_t) c.head_dim, (cuuint64_t) c.page_tokens, (cuuint64_t) c.n_head_kv, 2, (cuuint64_t) c.n_pages}, strides[4] = {row, head, side, (cuuint64_t) c.page_stride};
-    const cuuint32_t box[5] = {64, 16, 1, 2, 1}, one[5] = {1, 1, 1, 1, 1};
+    const cuuint32_t box[5] = {64, (cuuint32_t) tokens, 1, (cuuint32_t) sides, 1}, one[5] = {1, 1, 1, 1, 1};
     const CUresult r = encode(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, c.pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     need(r == CUDA_SUCCESS, r == CUDA_SUCCESS ? std::string() : "cuTensorMapEncodeTiled failed: " + std::to_string((int) r));
@@ -62,6 +62,18 @@ template <typename T> void attend_few(const AttendArgs & a, const CUtensorMap & 
     else nt == 1 ? attend_as<64, 1, T>(a, map, err, device, sms, stream) : attend_as<64, 2, T>(a, map, err, device, sms, stream);
 }
 
+template <int HD, typename T> void prompt_as(const PromptArgs & p, const CUtensorMap & map, int64_t entries, int device, int sms, void * stream) {
+    static Limits set;
+    const auto kernel = k_kv16_prompt<HD, T>;
+    allow_smem(kernel, device, set);
+    launch(k_kv16_plan, dim3(1), 1024, (size_t) (p.a.c.n_seq + 1) * 4, stream, false, 1, p, sms);
+    launch(kernel, dim3(sms), P16_THREADS, Prompt16Smem<HD>::BYTES, stream, true, 1, p, map);
+    launch(k_kv4_prompt_join<HD, T>, dim3((unsigned) (entries * (PR_COLS / 32)), (unsigned) p.a.c.n_kv), 256, 0, stream, true, 1, p);
+}
+
+// columns of a sequence (rows x query heads of a KV head) from which tcgen05 is worth a plan and a join of its own
+bool is_prompt(int group, int max_rows) { return (int64_t) group * max_rows > 16; }
+
 void check_heads(const b200_kv4 & c, int n_head, int max_rows) {
     need(n_head >= c.n_head_kv && n_head % std::max(1, c.n_head_kv) == 0 && (int64_t) c.n_rows * n_head <= (1 << 30), "n_head is a multiple of n_head_kv, and rows x heads up to 2^30");
     need(max_rows >= 1 && max_rows <= (1 << 24), "max_rows is the largest number of rows of a sequence");
@@ -84,6 +96,7 @@ int64_t kv16_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
     checked(c);
     check_heads(c, n_head, max_rows);
     On on(c.device);
+    if (is_prompt(n_head / c.n_head_kv, max_rows)) return prompt_work(c, n_head / c.n_head_kv, on.sms).bytes;
     return (int64_t) attend_bytes(c.n_seq, c.head_dim, attend_nt(n_head / c.n_head_kv, max_rows), on.sms);
 }
 
@@ -107,8 +120,22 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
     a.sinks = window > 0 ? sinks : 0;
     uint8_t * w = static_cast<uint8_t *>(work);
     const bool bf16 = dtype == B200_DTYPE_BF16;
-    const CUtensorMap map = pool_map(c, bf16);
     int * err = wait_word(c.device);
+    if (is_prompt(a.group, max_rows)) {
+        const PromptWork at = prompt_work(c, a.group, on.sms);
+        check_work(work, work_bytes, at.bytes);
+        const int drill = drill_polls.load();
+        const int64_t n = prompt_entries(c, a.group);
+        PromptArgs p = {a, (int) n, reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.first), err, drill ? (uint32_t) drill : WAIT_POLLS, drill ? 1 << 19 : 4};
+        p.a.before = reinterpret_cast<long long *>(w);
+        p.a.ml = reinterpret_cast<float *>(w + at.ml);
+        p.a.part = reinterpret_cast<float *>(w + at.part);
+        const CUtensorMap map = pool_map(c, bf16, std::min(c.page_tokens, PR_KV), 1);
+        if (bf16) c.head_dim == 128 ? prompt_as<128, __nv_bfloat16>(p, map, n, c.device, on.sms, c.stream) : prompt_as<64, __nv_bfloat16>(p, map, n, c.device, on.sms, c.stream);
+        else c.head_dim == 128 ? prompt_as<128, __half>(p, map, n, c.device, on.sms, c.stream) : prompt_as<64, __half>(p, map, n, c.device, on.sms, c.stream);
+        return;
+    }
+    const CUtensorMap map = pool_map(c, bf16, 16, 2);
     const int nt = attend_nt(a.group, max_rows);
     check_work(work, work_bytes, (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms));
     a.before = reinterpret_cast<long long *>(w);

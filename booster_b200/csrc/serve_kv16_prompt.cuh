@@ -1,0 +1,411 @@
+// serve_kv16_prompt.cuh — attention of many rows of a sequence over the 16-bit cache (sm_100a, tcgen05): prompts' portions, and the drafts of sequences whose heads share keys.
+//
+// As over the 4-bit cache (serve_prompt.cuh): a unit of work is 256 columns of a sequence (a column is a row and a query head of one KV head) over the tiles of 128 tokens that they see; all units
+// stand in one line that is cut evenly over one block per SM, k_kv16_plan lays it out and k_kv4_prompt_join adds the parts of units that blocks shared. Under a window a unit's tiles are those of
+// the first tokens and those of the window.
+//   warps 0-3, 4-7   soft-max of columns 0-127 and 128-255, a thread a column, 64 tokens at a time: its row of S into registers, maximum, exponentials, P back into tensor memory in the
+//                    place of S
+//   warp 8           tiles by TMA, a lane a page: K as rows of tokens, V as it stands too, since the second product takes its B operand with the dims contiguous (MN-major)
+//   warps 9, 10      (of 8-11: registers are shared out by four warps, 168 a thread at launch, then 216, 216 and 72) one thread each issues a half's S = Q K^T (128 x 64 x head_dim) and
+//                    O += P V (P from tensor memory, 128 x head_dim x 64)
+// Tensor memory: S and P [2 halves][2 turns][64 columns], O [2][head_dim]. Each half has two turns of S, so that the scores of the next 64 tokens are there when those in hand are done with.
+// P is rounded to the type once, with P_LIFT and P_PASS of serve_attn.cuh; the sum of weights is that of the rounded ones, so that a weight's rounding moves a result towards or from that
+// token's value and not its size. O is scaled in tensor memory where the base of P moves.
+// Every wait on an mbarrier is bounded: where one runs out the block raises *err, waits for nothing more, lets what is under way end and frees its tensor memory; the call's results are worthless.
+#pragma once
+#include "serve_kv16.cuh"
+#include "serve_prompt.cuh"
+
+namespace b200 {
+namespace srv {
+
+constexpr int P16_THREADS = 384;
+template <typename T> __host__ __device__ constexpr uint32_t p16_idesc(int n, bool b_by_dims) {      // D f32, A and B of T, M = 128
+    const uint32_t t = std::is_same<T, __half>::value ? 0u : 1u;
+    return (1u << 4) | (t << 7) | (t << 10) | (b_by_dims ? 1u << 16 : 0u) | ((uint32_t) (n >> 3) << 17) | (8u << 24);
+}
+// V as [64 dims' half][128 tokens][64 dims]: blocks of 64 dims 16384 bytes apart, groups of 8 tokens 1024
+constexpr uint64_t P16_V_DESC = ((uint64_t) (16384u >> 4) << 16) | ((uint64_t) (1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+template <int HD> struct Prompt16Smem {
+    static constexpr int Q = 128 * HD * 2, KV = PR_KV * HD * 2;      // bytes of one half of Q, of a tile's K or V
+    static constexpr int BYTES = 2 * Q + 4 * KV + 1024;              // K and V in two stages each
+};
+// the box's tokens of 64 dims of a KV head of a page, keys (side 0) or values
+__device__ __forceinline__ void tma_side(uint32_t dst, const CUtensorMap * map, uint32_t bar, int dim, int token, int head, int side, int page) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                 :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(dim), "r"(token), "r"(head), "r"(side), "r"(page) : "memory");
+}
+
+// one block: the line of entries, a thread an entry
+static __global__ void __launch_bounds__(1024) k_kv16_plan(const PromptArgs p, int n_blocks) {
+    extern __shared__ int entry_of[];                              // [n_seq + 1]
+    __shared__ long long sums[32];
+    const Cache & c = p.a.c;
+    const int tid = threadIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    int all = 0;
+    for (int s0 = 0; s0 < c.n_seq; s0 += 1024) {
+        const int s = s0 + tid;
+        long long some;
+        const long long n = s < c.n_seq ? col_tiles(seq_at(c, s), p.a.group, PR_COLS) : 0, at = all + plan_before(n, some, sums);
+        if (s < c.n_seq) entry_of[s] = (int) min(at, (long long) p.max_entries);
+        all = (int) min(all + some, (long long) p.max_entries);
+    }
+    if (tid == 0) entry_of[c.n_seq] = all;
+    __syncthreads();
+    long long total = 0;
+    for (int e0 = 0; e0 < all; e0 += 1024) {
+        const int e = e0 + tid;
+        long long n = 0, some;
+        if (e < all) {
+            int s = 0;                                             // the last sequence that begins at or before e (those without rows begin where the next one does)
+            for (int hi = c.n_seq; hi - s > 1;) { const int mid = (s + hi) >> 1; if (entry_of[mid] <= e) s = mid; else hi = mid; }
+            const Seq q = seq_at(c, s);
+            const int ct = e - entry_of[s], a = ct * PR_COLS / p.a.group, b = min(q.count - 1, (ct * PR_COLS + PR_COLS - 1) / p.a.group);
+            const Steps sp = steps_of(c, q, p.a.window, p.a.sinks, a, b, 7);
+            p.entries[e] = Entry{q.slot, q.begin, q.count, q.held, ct, sp.lo, sp.n, sp.head};
+            n = (long long) c.n_kv * (sp.n + PR_OVER);
+        }
+        const long long at = total + plan_before(n, some, sums);
+        if (e < all) p.a.before[e] = at;
+        total += some;
+    }
+    const int per = (int) max(1ll, quotient(total + n_blocks - 1, n_blocks));
+    if (tid == 0) { p.a.before[all] = total; p.first[0] = per; p.first[1] = all; }
+    __syncthreads();                                               // before[] stands
+    for (int w = tid; w < n_blocks; w += 1024) {                   // the entry that each block's piece begins in
+        const long long at = (long long) w * per;
+        int e = 0;
+        for (int hi = all; hi - e > 1;) { const int mid = (e + hi) >> 1; if (p.a.before[mid] <= at) e = mid; else hi = mid; }
+        p.first[2 + w] = e;
+    }
+}
+
+struct Segment16 { Seq q; Steps sp; int ct, head, t0, t1, halves; };
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs p, const __grid_constant__ CUtensorMap map) {
+    constexpr int QB = Prompt16Smem<HD>::Q, KVB = Prompt16Smem<HD>::KV, SUB = 128 * 128;      // SUB: 128 rows of 128 bytes
+    extern __shared__ uint8_t pr_raw[];
+    __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_full[2][2];      // [half][turn]
+    __shared__ uint32_t tmem_s;
+    const AttendArgs & a = p.a;
+    const Cache & c = a.c;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t smem = (smem_at(pr_raw) + 1023u) & ~1023u, q_s = smem, k_s = q_s + 2 * QB, v_s = k_s + 2 * KVB;
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_at(&q_full[i]), p.queries);
+            mbar_init(smem_at(&k_full[i]), 1); mbar_init(smem_at(&v_full[i]), 1);
+            mbar_init(smem_at(&k_empty[i]), 2); mbar_init(smem_at(&v_empty[i]), 2);
+            for (int b = 0; b < 2; b++) { mbar_init(smem_at(&s_full[i][b]), 1); mbar_init(smem_at(&p_full[i][b]), 4); mbar_init(smem_at(&o_full[i][b]), 1); }
+        }
+        mbar_init_done();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_at(&tmem_s)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pr_fence_before();
+    __syncthreads();
+    pr_fence_after();
+    const uint32_t tmem = tmem_s, t_s = tmem, t_o = tmem + 256;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int per = p.first[0], entries = p.first[1];
+    const long long begin = (long long) blockIdx.x * per, end = min(a.before[entries], begin + per);
+    // the segments of this block's piece, one after the other and the same for every warp
+    int entry = begin < end ? p.first[2 + blockIdx.x] : 0, head = -1;
+    long long at = begin;
+    const auto segment = [&](Segment16 & g) {
+        while (at < end) {
+            const Entry e = p.entries[entry];
+            const int len = e.n + PR_OVER;
+            int from = 0;
+            if (head < 0) {                                        // the first one may begin anywhere
+                const long long x = at - a.before[entry];
+                head = (int) quotient(x, len);
+                from = (int) (x - (long long) head * len);
+            }
+            const int to = (int) min((long long) len, from + (end - at));
+            g.q = Seq{e.slot, e.begin, e.count, e.held};
+            g.sp = Steps{e.head, e.lo, e.n};
+            g.ct = e.ct; g.head = head;
+            g.t0 = max(0, from - PR_OVER);
+            g.t1 = to - PR_OVER;
+            g.halves = e.count * a.group - e.ct * PR_COLS > 128 ? 2 : 1;
+            at += to - from;
+            if (++head == c.n_kv) { head = 0; entry++; }
+            if (g.t1 > 0) return true;
+        }
+        return false;
+    };
+    bool dead = false;
+    if (warp < 8) {
+        regs_more<216>();
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane;          // of the half
+        const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, my_s = t_s + lanes + half * 128, my_o = t_o + lanes + half * HD;
+        const float factor = fmaxf(fabsf(a.scale_log2), 1.2e-38f);         // (never 0: it meets the -infinity of what is masked)
+        const uint32_t turn_round = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+        int n_s = 0;                                                       // steps of 64 tokens of this half so far
+        const auto next = [&](Segment16 & g) {                             // the next segment with columns of this half
+            do { if (!segment(g)) return false; } while (half >= g.halves);
+            return true;
+        };
+        // the warp's 32 queries, HD / 8 lanes a row. One with an infinity or a NaN becomes NaN, since its negative scores would look like masked ones
+        const auto queries = [&](const Segment16 & g) {
+            const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
+            constexpr int LANES = HD / 8, ROWS = 32 / LANES, X = 8;
+            const int64_t mine = i < g.q.count ? (g.q.begin + i) * a.q_row + h * a.q_head : -1;
+            const int m = lane % LANES;
+            const unsigned group = (LANES == 16 ? 0xffffu : 0xffu) << (lane / LANES * LANES);
+#pragma unroll 1
+            for (int x0 = 0; x0 < 32; x0 += X * ROWS) {
+                uint4 f[X];
+                int64_t from[X];
+#pragma unroll
+                for (int x = 0; x < X; x++) { from[x] = __shfl_sync(0xffffffffu, mine, x0 + x * ROWS + lane / LANES); f[x] = make_uint4(0, 0, 0, 0); }
+                const T * src = static_cast<const T *>(a.q) + 8 * m;
+                if (a.q_whole) {
+#pragma unroll
+                    for (int x = 0; x < X; x++) if (from[x] >= 0) f[x] = *reinterpret_cast<const uint4 *>(src + from[x]);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < X; x++) if (from[x] >= 0) f[x] = eight_apart(src + from[x]);
+                }
+#pragma unroll
+                for (int x = 0; x < X; x++) {
+                    const int r = x0 + x * ROWS + lane / LANES;
+                    const bool bad = wild<T>(f[x].x) || wild<T>(f[x].y) || wild<T>(f[x].z) || wild<T>(f[x].w);
+                    if (__ballot_sync(0xffffffffu, bad) & group) f[x] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+                    pr_st_shared(q_s + half * QB + (m >> 3) * SUB + ((warp & 3) * 32 + r) * 128 + (((m & 7) ^ (r & 7)) << 4), f[x].x ^ turn_round, f[x].y ^ turn_round, f[x].z ^ turn_round,
+                                 f[x].w ^ turn_round);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) pr_arrive(smem_at(&q_full[half]));
+        };
+        Segment16 g;
+        bool more = next(g);
+        if (more) queries(g);
+        while (more) {
+            const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
+            const bool in = i < g.q.count;
+            // whether every page of the piece is there; where not, each tile's are looked up again
+            bool whole = g.q.slot >= 0;
+            {
+                const int last = g.q.held + g.q.count - 1, log2 = min(c.page_log2, 7), more_log2 = 7 - log2;       // a page of a tile a lane
+                for (int x = (g.t0 << more_log2) + lane; x < g.t1 << more_log2; x += 32) {
+                    const int pos = step_at(g.sp, x >> more_log2) * PR_KV + ((x & ((1 << more_log2) - 1)) << log2);
+                    if (pos <= last) whole = whole && page_at(c, g.q.slot, pos) >= 0;
+                }
+                whole = __all_sync(0xffffffffu, whole);
+            }
+            const int row_lo = g.ct * PR_COLS / a.group, row_hi = min(g.q.count - 1, (g.ct * PR_COLS + PR_COLS - 1) / a.group);
+            const int all_see_hi = g.q.held + row_lo, all_see_lo = a.window > 0 ? g.q.held + row_hi - a.window + 1 : 0;
+            const int top_pos = in ? g.q.held + i : -1, low_pos = a.window > 0 ? top_pos - a.window : -1;      // sees low_pos < position <= top_pos, and what is below sinks
+            float m = -INFINITY, l = 0.f, base = 0.f, limit = -INFINITY;
+            for (int t = 2 * g.t0; t < 2 * g.t1; t++, n_s++) {
+                const int pos = step_at(g.sp, t >> 1) * PR_KV + 64 * (t & 1);
+                const uint32_t at = my_s + 64 * (n_s & 1);
+                const bool edge = !whole || pos + 63 > all_see_hi || (pos < all_see_lo && pos + 63 >= a.sinks);
+                unsigned there = 0xfu;                                     // tiles of 16 tokens that have a page
+                if (!whole) there = __ballot_sync(0xffffffffu, lane < 4 && page_at(c, g.q.slot, pos + 16 * (lane & 3)) >= 0);
+                pr_wait(smem_at(&s_full[half][n_s & 1]), (uint32_t) (n_s >> 1 & 1), p.polls, dead);
+                __syncwarp();
+                pr_fence_after();
+                uint32_t r[64];
+                pr_ld64(at, r);
+                if (edge) {                                                // what a column does not see goes to -infinity
+                    const int hi = top_pos - pos, lo = low_pos - pos, sinks = a.sinks - pos;
+#pragma unroll
+                    for (int x = 0; x < 64; x++)
+                        if (x > hi || (x <= lo && x >= sinks) || !(there >> (x >> 4) & 1)) r[x] = 0xff800000u;
+                }
+                float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 64; x += 4) {
+                    x0 = fmaxf(x0, fmaxf(__uint_as_float(r[x]), __uint_as_float(r[x + 1])));
+                    x1 = fmaxf(x1, fmaxf(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3])));
+                }
+                const float high = fmaxf(x0, x1), score = high == -INFINITY ? high : high * factor;
+                if (__any_sync(0xffffffffu, score > limit)) {
+                    const float top = fmaxf(m, score - P_LIFT), down = top > m ? exp2_fast(m - top) : 1.f;
+                    if (t > 2 * g.t0 && __any_sync(0xffffffffu, down != 1.f)) {
+                        pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), p.polls, dead);
+                        __syncwarp();
+                        pr_fence_after();
+#pragma unroll 1
+                        for (int ch = 0; ch < HD / 32; ch++) {
+                            uint32_t y[32];
+                            pr_ld32(my_o + 32 * ch, y);
+#pragma unroll
+                            for (int x = 0; x < 32; x++) y[x] = __float_as_uint(__uint_as_float(y[x]) * down);
+                            pr_st32(my_o + 32 * ch, y);
+                        }
+                    }
+                    m = top;
+                    base = top == -INFINITY ? 0.f : top;
+                    limit = top + (P_LIFT + P_PASS);
+                    l *= down;
+                }
+                const uint64_t by = two(factor, factor), less = two(-base, -base);
+                uint64_t sum = 0;
+                uint32_t w[32];
+#pragma unroll
+                for (int x = 0; x < 64; x += 2) {
+                    const float2 y = split(fma2(two(__uint_as_float(r[x]), __uint_as_float(r[x + 1])), by, less));
+                    w[x / 2] = pair_of<T>(exp2_fast(y.x), exp2_fast(y.y));
+                    const float2 e = floats_of<T>(w[x / 2]);
+                    sum = add2(sum, two(e.x, e.y));
+                }
+                pr_st32(at, w);
+                l += split(sum).x + split(sum).y;
+                pr_st_wait();
+                pr_fence_before();
+                __syncwarp();
+                if (lane == 0) pr_arrive(smem_at(&p_full[half][n_s & 1]));
+            }
+            // the next segment's queries before this one's results: its first scores are made while these are written
+            Segment16 then;
+            more = next(then);
+            if (more) queries(then);
+            pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), p.polls, dead);
+            __syncwarp();
+            pr_fence_after();
+            const bool final = g.t0 == 0 && g.t1 == g.sp.n;
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+            const size_t piece = 2 * (size_t) blockIdx.x + (g.t0 == 0 ? 1 : 0);      // parts are [HD / 4][256 columns][4]: a warp's stores are contiguous
+#pragma unroll
+            for (int ch = 0; ch < HD / 32; ch++) {
+                uint32_t r[32];
+                pr_ld32(my_o + 32 * ch, r);
+                if (in && !dead) {
+                    if (final) {
+                        T * y = static_cast<T *>(a.out) + ((size_t) (g.q.begin + i) * c.n_kv * a.group + h) * HD + 32 * ch;
+#pragma unroll
+                        for (int x = 0; x < 32; x += 8) {
+                            Eight<T> f;
+#pragma unroll
+                            for (int j = 0; j < 8; j++) f.v[j] = from_f<T>(__uint_as_float(r[x + j]) * inv);
+                            *reinterpret_cast<Eight<T> *>(y + x) = f;
+                        }
+                    } else {
+                        uint4 * y = reinterpret_cast<uint4 *>(a.part + piece * PR_COLS * HD) + (size_t) (8 * ch) * PR_COLS + half * 128 + row;
+#pragma unroll
+                        for (int x = 0; x < 8; x++) y[x * PR_COLS] = make_uint4(r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]);
+                    }
+                }
+                __syncwarp();
+            }
+            if (in && !final) *reinterpret_cast<float2 *>(a.ml + (piece * PR_COLS + half * 128 + row) * 2) = make_float2(m, l);
+            pr_fence_before();
+            g = then;
+        }
+    } else {
+        regs_less<72>();
+        if (warp == 8) {
+            // a lane brings its tokens of a tile: a page's, or 128 of a longer page's
+            const int log2 = min(c.page_log2, 7), pieces = PR_KV >> log2;
+            int n = 0;                                                     // tiles so far
+            for (Segment16 g; segment(g);) {
+                const auto page_of = [&](int t) { return lane < pieces && t < g.t1 ? page_at(c, g.q.slot, min(step_at(g.sp, t) * PR_KV + (lane << log2), c.max_pages << c.page_log2)) : -1; };
+                int page = page_of(g.t0);
+                for (int t = g.t0; t < g.t1; t++, n++) {
+                    const int stage = n & 1, then = page_of(t + 1);
+                    const uint32_t round = (uint32_t) (n >> 1);
+                    const int token = (step_at(g.sp, t) * PR_KV + (lane << log2)) & ((1 << c.page_log2) - 1), z = page >= 0 ? page : c.n_pages;
+#pragma unroll
+                    for (int side = 0; side < 2; side++) {
+                        const uint32_t full = smem_at(side ? &v_full[stage] : &k_full[stage]), dst = (side ? v_s : k_s) + stage * KVB + (uint32_t) (lane << log2) * 128;
+                        if (n >= 2) pr_wait(smem_at(side ? &v_empty[stage] : &k_empty[stage]), (round - 1) & 1, p.polls, dead);
+                        dead = __any_sync(0xffffffffu, dead);
+                        if (!dead) {
+                            if (lane == 0) mbar_expect(full, KVB);
+                            __syncwarp();
+                            if (lane < pieces)
+#pragma unroll
+                                for (int d = 0; d < HD / 64; d++) tma_side(dst + d * SUB, &map, full, 64 * d, token, g.head, side, z);
+                        }
+                    }
+                    page = then;
+                }
+            }
+            for (int i = max(0, n - 2); i < n; i++) {                      // the last tiles are let go: their commits arrive while the block's shared memory is its own
+                pr_wait(smem_at(&k_empty[i & 1]), (uint32_t) (i >> 1 & 1), p.polls, dead);
+                pr_wait(smem_at(&v_empty[i & 1]), (uint32_t) (i >> 1 & 1), p.polls, dead);
+            }
+        } else {
+            const int half = warp - 9;
+            int n = 0, n_q = 0, n_p = 0;                                   // tiles, segments and steps of this half so far
+            for (Segment16 g; half < 2 && segment(g);) {
+                const int tiles = g.t1 - g.t0, steps = 2 * tiles;
+                if (pr_elect()) {
+                    if (half < g.halves) {
+                        const auto scores = [&](int step) {                // S = Q K^T of 64 tokens
+                            const int turn = step & 1;
+#pragma unroll
+                            for (int k = 0; k < HD / 16; k++)
+                                pr_mma_ss(t_s + half * 128 + 64 * turn, PR_DESC | (uint64_t) ((q_s + half * QB + (k >> 2) * SUB) >> 4) + 2 * (k & 3),
+                                          PR_DESC | (uint64_t) ((k_s + (n + (step >> 1) & 1) * KVB + (k >> 2) * SUB + turn * (SUB / 2)) >> 4) + 2 * (k & 3), p16_idesc<T>(64, false), k > 0);
+                            pr_commit(smem_at(&s_full[half][turn]));
+                        };
+                        pr_wait(smem_at(&q_full[half]), (uint32_t) (n_q & 1), p.polls, dead);
+                        pr_wait(smem_at(&k_full[n & 1]), (uint32_t) (n >> 1 & 1), p.polls, dead);
+                        pr_fence_after();
+                        if (!dead) {
+                            scores(0);
+                            scores(1);
+                            pr_commit(smem_at(&k_empty[n & 1]));
+                        }
+                        for (int step = 0; step < steps; step++) {
+                            const int turn = step & 1, now = n + (step >> 1), stage = now & 1, after = (now + 1) & 1;
+                            if (turn == 0) pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), p.polls, dead);
+                            pr_wait(smem_at(&p_full[half][turn]), (uint32_t) ((n_p + step) >> 1 & 1), p.polls, dead);
+                            pr_fence_after();
+                            if (!dead) {
+#pragma unroll
+                                for (int k = 0; k < 4; k++)
+                                    pr_mma_ts(t_o + half * HD, t_s + half * 128 + 64 * turn + 8 * k, P16_V_DESC | (uint64_t) ((v_s + stage * KVB + turn * (SUB / 2) + k * 2048) >> 4), p16_idesc<T>(HD, true),
+                                              step > 0 || k > 0);
+                                pr_commit(smem_at(&o_full[half][turn]));
+                                if (turn == 1) pr_commit(smem_at(&v_empty[stage]));
+                            }
+                            if (step + 2 < steps) {
+                                if (turn == 0) { pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), p.polls, dead); pr_fence_after(); }
+                                if (!dead) {
+                                    scores(step + 2);
+                                    if (turn == 1) pr_commit(smem_at(&k_empty[after]));
+                                }
+                            }
+                        }
+                    } else {                                               // no columns here: the tiles are let go as they come
+                        for (int t = 0; t < tiles; t++) {
+                            const int stage = (n + t) & 1;
+                            const uint32_t phase = (uint32_t) ((n + t) >> 1 & 1);
+                            pr_wait(smem_at(&k_full[stage]), phase, p.polls, dead);
+                            if (!dead) pr_arrive(smem_at(&k_empty[stage]));
+                            pr_wait(smem_at(&v_full[stage]), phase, p.polls, dead);
+                            if (!dead) pr_arrive(smem_at(&v_empty[stage]));
+                        }
+                    }
+                }
+                __syncwarp();
+                n += tiles;
+                if (half < g.halves) { n_q++; n_p += steps; }
+            }
+        }
+    }
+    if (dead) atomicExch_system(p.err, 1);
+    pr_fence_before();
+    if (__syncthreads_or(dead))                                            // nobody issues any more: products and copies under way end before shared and tensor memory are given back
+        for (int j = 0; j < 1000; j++) __nanosleep(1000);
+    if (warp == 8) {
+        pr_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem));
+    }
+}
+
+}  // namespace srv
+}  // namespace b200

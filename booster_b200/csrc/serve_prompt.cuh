@@ -17,12 +17,13 @@
 // Every wait on an mbarrier is bounded: where one runs out the block raises *err, waits for nothing more, lets what is under way end and frees its tensor memory; the call's results are worthless.
 #pragma once
 #include "serve_attn.cuh"
+#include "../../include/booster_b200.h"
 #include <type_traits>
 
 namespace b200 {
 namespace srv {
 
-struct Entry { int slot, begin, count, held, ct, lo, n, pad; };         // a sequence (Seq), its columns' number, their span of tiles
+struct Entry { int slot, begin, count, held, ct, lo, n, head; };        // a sequence (Seq), its columns' number, their span of tiles (head: serve_kv16.cuh)
 struct PromptArgs {
     AttendArgs a;                        // a.before: [entries + 1] tiles in front of each entry (a sequence's 256 columns), for all KV heads together
     int max_entries;                     // as many as rows and sequences can have, where first ascends; no more are looked at
@@ -617,6 +618,21 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_join(const PromptArgs p) {
 #pragma unroll
         for (int j = 0; j < X; j++) y[j] = from_f<T>(sums[x * PAD + X * lane + j]);
     }
+}
+
+// ---- host: the workspace of a step ----
+inline int64_t prompt_entries(const b200_kv4 & c, int group) { return (int64_t) c.n_rows * group / PR_COLS + c.n_seq + 1; }
+struct PromptWork { int64_t entries, first, ml, part, bytes; };       // places in the workspace; `before` is first
+inline PromptWork prompt_work(const b200_kv4 & c, int group, int sms) {
+    const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    const int64_t n = prompt_entries(c, group), slots = 2 * (int64_t) sms * PR_COLS;
+    PromptWork w;
+    w.entries = up((n + 2) * 8);
+    w.first = w.entries + up(n * (int64_t) sizeof(Entry));
+    w.ml = w.first + up((sms + 2) * 4);
+    w.part = w.ml + up(slots * 8);
+    w.bytes = w.part + slots * c.head_dim * 4;
+    return w;
 }
 
 }  // namespace srv
