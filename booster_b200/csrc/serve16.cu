@@ -9,24 +9,29 @@ using namespace srv;
 
 Cache checked(const b200_kv4 & c) { return checked_cache(c, "kv16", 64 * c.head_dim); }
 
-// boxes of `tokens` tokens and 64 dims of a KV head of a page, of keys and values at once or of one of them
-CUtensorMap pool_map(const b200_kv4 & c, bool bf16, int tokens, int sides) {
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+CUtensorMap map_of(bool bf16, int n, const void * base, const cuuint64_t * dims, const cuuint64_t * strides, const cuuint32_t * box) {
     static const auto encode = [] {
         void * fn = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) { cudaGetLastError(); fn = nullptr; }
-        return reinterpret_cast<CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
-                                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill)>(fn);
+        return reinterpret_cast<EncodeTiled>(fn);
     }();
     need(encode, "the driver has no cuTensorMapEncodeTiled");
     CUtensorMap m;
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, n, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string((int) r));
+    return m;
+}
+// boxes of `tokens` tokens and 64 dims of a KV head of a page, of keys and values at once or of one of them
+CUtensorMap pool_map(const b200_kv4 & c, bool bf16, int tokens, int sides) {
     const cuuint64_t row = (cuuint64_t) c.head_dim * 2, head = row * c.page_tokens, side = head * c.n_head_kv;
     const cuuint64_t dims[5] = {(cuuint64_t) c.head_dim, (cuuint64_t) c.page_tokens, (cuuint64_t) c.n_head_kv, 2, (cuuint64_t) c.n_pages}, strides[4] = {row, head, side, (cuuint64_t) c.page_stride};
-    const cuuint32_t box[5] = {64, (cuuint32_t) tokens, 1, (cuuint32_t) sides, 1}, one[5] = {1, 1, 1, 1, 1};
-    const CUresult r = encode(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, c.pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    need(r == CUDA_SUCCESS, r == CUDA_SUCCESS ? std::string() : "cuTensorMapEncodeTiled failed: " + std::to_string((int) r));
-    return m;
+    const cuuint32_t box[5] = {64, (cuuint32_t) tokens, 1, (cuuint32_t) sides, 1};
+    return map_of(bf16, 5, c.pool, dims, strides, box);
 }
 
 // heads of a row one after the other in a warp only where there are rows enough to fill the card without
@@ -62,13 +67,13 @@ template <typename T> void attend_few(const AttendArgs & a, const CUtensorMap & 
     else nt == 1 ? attend_as<64, 1, T>(a, map, err, device, sms, stream) : attend_as<64, 2, T>(a, map, err, device, sms, stream);
 }
 
-template <int HD, typename T> void prompt_as(const PromptArgs & p, const CUtensorMap & map, int64_t entries, int device, int sms, void * stream) {
+template <int HD, typename T> void prompt_as(const PromptArgs & p, const CUtensorMap & map, const CUtensorMap & q_map, bool by_box, int64_t entries, int device, int sms, void * stream) {
     static Limits set;
     const auto kernel = k_kv16_prompt<HD, T>;
     allow_smem(kernel, device, set);
     launch(k_kv16_plan, dim3(1), 1024, (size_t) (p.a.c.n_seq + 1) * 4, stream, false, 1, p, sms);
-    launch(kernel, dim3(sms), P16_THREADS, Prompt16Smem<HD>::BYTES, stream, true, 1, p, map);
-    launch(k_kv4_prompt_join<HD, T>, dim3((unsigned) (entries * (PR_COLS / 32)), (unsigned) p.a.c.n_kv), 256, 0, stream, true, 1, p);
+    launch(kernel, dim3(sms), P16_THREADS, Prompt16Smem<HD>::BYTES, stream, true, 1, p, map, q_map, by_box);
+    launch(k_kv16_prompt_join<HD, T>, dim3((unsigned) (entries * (PR_COLS / 32)), (unsigned) p.a.c.n_kv), 256, 0, stream, true, 1, p);
 }
 
 // columns of a sequence (rows x query heads of a KV head) from which tcgen05 is worth a plan and a join of its own
@@ -126,13 +131,22 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
         check_work(work, work_bytes, at.bytes);
         const int drill = drill_polls.load();
         const int64_t n = prompt_entries(c, a.group);
-        PromptArgs p = {a, (int) n, reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.first), err, drill ? (uint32_t) drill : WAIT_POLLS, drill ? 1 << 19 : 4};
+        // 128 columns as one box: whole rows of a group, rows and heads at distances that a tensor map can have
+        const bool by_box = a.q_whole && 128 % a.group == 0 && q_head > 0 && (q_row > 0 || c.n_rows == 1) && q_row < (1ll << 38) && q_head < (1ll << 38);
+        PromptArgs p = {a, (int) n, reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.first), err, drill ? (uint32_t) drill : WAIT_POLLS, drill ? 1 << 19 : by_box ? 1 : 4};
         p.a.before = reinterpret_cast<long long *>(w);
         p.a.ml = reinterpret_cast<float *>(w + at.ml);
         p.a.part = reinterpret_cast<float *>(w + at.part);
         const CUtensorMap map = pool_map(c, bf16, std::min(c.page_tokens, PR_KV), 1);
-        if (bf16) c.head_dim == 128 ? prompt_as<128, __nv_bfloat16>(p, map, n, c.device, on.sms, c.stream) : prompt_as<64, __nv_bfloat16>(p, map, n, c.device, on.sms, c.stream);
-        else c.head_dim == 128 ? prompt_as<128, __half>(p, map, n, c.device, on.sms, c.stream) : prompt_as<64, __half>(p, map, n, c.device, on.sms, c.stream);
+        CUtensorMap q_map = {};
+        if (by_box) {
+            const cuuint64_t dims[3] = {(cuuint64_t) c.head_dim, (cuuint64_t) n_head, (cuuint64_t) c.n_rows}, strides[2] = {(cuuint64_t) q_head * 2, (cuuint64_t) (c.n_rows > 1 ? q_row : 8) * 2};
+            const cuuint32_t box[3] = {64, (cuuint32_t) a.group, (cuuint32_t) (128 / a.group)};
+            q_map = map_of(bf16, 3, q, dims, strides, box);
+        }
+        const auto as = [&](auto run) { run(p, map, q_map, by_box, n, c.device, on.sms, c.stream); };
+        if (bf16) c.head_dim == 128 ? as(prompt_as<128, __nv_bfloat16>) : as(prompt_as<64, __nv_bfloat16>);
+        else c.head_dim == 128 ? as(prompt_as<128, __half>) : as(prompt_as<64, __half>);
         return;
     }
     const CUtensorMap map = pool_map(c, bf16, 16, 2);

@@ -1,16 +1,22 @@
 // serve_kv16_prompt.cuh — attention of many rows of a sequence over the 16-bit cache (sm_100a, tcgen05): prompts' portions, and the drafts of sequences whose heads share keys.
 //
 // As over the 4-bit cache (serve_prompt.cuh): a unit of work is 256 columns of a sequence (a column is a row and a query head of one KV head) over the tiles of 128 tokens that they see; all units
-// stand in one line that is cut evenly over one block per SM, k_kv16_plan lays it out and k_kv4_prompt_join adds the parts of units that blocks shared. Under a window a unit's tiles are those of
+// stand in one line that is cut evenly over one block per SM, k_kv16_plan lays it out and k_kv16_prompt_join adds the parts of units that blocks shared. Under a window a unit's tiles are those of
 // the first tokens and those of the window.
 //   warps 0-3, 4-7   soft-max of columns 0-127 and 128-255, a thread a column, 64 tokens at a time: its row of S into registers, maximum, exponentials, P back into tensor memory in the
 //                    place of S
-//   warp 8           tiles by TMA, a lane a page: K as rows of tokens, V as it stands too, since the second product takes its B operand with the dims contiguous (MN-major)
-//   warps 9, 10      (of 8-11: registers are shared out by four warps, 168 a thread at launch, then 216, 216 and 72) one thread each issues a half's S = Q K^T (128 x 64 x head_dim) and
-//                    O += P V (P from tensor memory, 128 x head_dim x 64)
+//   warp 8           (of 8-11: registers are shared out by four warps, 168 a thread at launch, then 216, 216 and 72) tiles by TMA, a lane a page: K as rows of tokens, V as it stands too, since
+//                    the second product takes its B operand with the dims contiguous (MN-major)
+//   warps 9, 10      one thread each issues a half's S = Q K^T (128 x 64 x head_dim) and O += P V (P from tensor memory, 128 x head_dim x 64)
+//   warp 11          the next segment's queries, while the last 128 tokens of the one before are worked on, where 128 columns are whole rows of a group: a box. Others the soft-max warps gather
 // Tensor memory: S and P [2 halves][2 turns][64 columns], O [2][head_dim]. Each half has two turns of S, so that the scores of the next 64 tokens are there when those in hand are done with.
-// P is rounded to the type once, with P_LIFT and P_PASS of serve_attn.cuh; the sum of weights is that of the rounded ones, so that a weight's rounding moves a result towards or from that
-// token's value and not its size. O is scaled in tensor memory where the base of P moves.
+// P is rounded to the type once, with P_LIFT and P_PASS of serve_attn.cuh: results are off by 1.2 to 1.35 times (rms) what their own rounding is (bfloat16 2.1e-3 for 1.7e-3, fp16 2.8e-4 for 2.1e-4).
+// In two numbers, as for few rows, the second product would be twice as long; sums of the rounded weights instead of the weights' made 8192 tokens 45 us longer and no result nearer.
+// O is scaled in tensor memory where the base of P moves.
+// Measured with 32 query heads on 8 of 128: 8192 tokens 489 us (1124 TFLOP/s, 68 % of the bf16 rate), 1000 rows behind 5000 positions 109 us, of which 5 the plan and 4 the join. A step of 64
+// tokens takes 1750 clocks: of both halves' products 1280 (those of 64 tokens read 6 KB of shared memory in 48 clocks, for 32 of arithmetic), of exponentials 900, an eighth of them by a
+// polynomial (none 495 us, two eighths 489, three 494). Halves that took turns at exponentials by named barriers 475 to 485 and nothing at 1000 rows. What a warp does between them bounds it: a wait for
+// what is there 130 clocks, 64 scores from tensor memory 60 to 120, the largest 280, P back 120.
 // Every wait on an mbarrier is bounded: where one runs out the block raises *err, waits for nothing more, lets what is under way end and frees its tensor memory; the call's results are worthless.
 #pragma once
 #include "serve_kv16.cuh"
@@ -19,7 +25,8 @@
 namespace b200 {
 namespace srv {
 
-constexpr int P16_THREADS = 384;
+constexpr int P16_THREADS = 384, P16_OVER = 3;      // P16_OVER: what beginning a unit costs, in tiles
+constexpr int P16_EIGHTHS = 1;
 template <typename T> __host__ __device__ constexpr uint32_t p16_idesc(int n, bool b_by_dims) {      // D f32, A and B of T, M = 128
     const uint32_t t = std::is_same<T, __half>::value ? 0u : 1u;
     return (1u << 4) | (t << 7) | (t << 10) | (b_by_dims ? 1u << 16 : 0u) | ((uint32_t) (n >> 3) << 17) | (8u << 24);
@@ -35,6 +42,30 @@ __device__ __forceinline__ void tma_side(uint32_t dst, const CUtensorMap * map, 
     asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
                  :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(dim), "r"(token), "r"(head), "r"(side), "r"(page) : "memory");
 }
+
+// 64 dims of the queries of 128 columns: rows of a head's group one after the other
+__device__ __forceinline__ void tma_queries(uint32_t dst, const CUtensorMap * map, uint32_t bar, int dim, int head, int row) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(dim), "r"(head), "r"(row) : "memory");
+}
+
+// 2^y of two numbers without the special functions' unit: y = n + f with |f| <= 1 / 2, a polynomial of the fourth degree that fits 2^f to 2^-18.5 (least largest relative error, by weighted least
+// squares on Chebyshev's places), times 2^n made from n's bits. 0 from y = -127 down; a NaN stays one
+__device__ __forceinline__ float max_of_nan(float x, float y) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ float2 exp2_pair(float2 y) {
+    constexpr float WHOLE = 12582912.f;                                  // 1.5 x 2^23: added, the last bits are a whole number
+    const uint64_t x = two(max_of_nan(y.x, -127.f), max_of_nan(y.y, -127.f)), t = add2(x, two(WHOLE, WHOLE)), f = fma2(add2(t, two(-WHOLE, -WHOLE)), two(-1.f, -1.f), x);
+    uint64_t p = fma2(f, two(0.009570100344717503f, 0.009570100344717503f), two(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, two(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, two(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, two(0.9999992847442627f, 0.9999992847442627f));
+    const float2 n = split(t);
+    const auto power = [](float n) { return __uint_as_float((__float_as_uint(n) << 23) + 0x3f800000u); };
+    return split(mul2(p, two(power(n.x), power(n.y))));
+}
+// the lowest n bits
+__device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // one block: the line of entries, a thread an entry
 static __global__ void __launch_bounds__(1024) k_kv16_plan(const PromptArgs p, int n_blocks) {
@@ -64,7 +95,7 @@ static __global__ void __launch_bounds__(1024) k_kv16_plan(const PromptArgs p, i
             const int ct = e - entry_of[s], a = ct * PR_COLS / p.a.group, b = min(q.count - 1, (ct * PR_COLS + PR_COLS - 1) / p.a.group);
             const Steps sp = steps_of(c, q, p.a.window, p.a.sinks, a, b, 7);
             p.entries[e] = Entry{q.slot, q.begin, q.count, q.held, ct, sp.lo, sp.n, sp.head};
-            n = (long long) c.n_kv * (sp.n + PR_OVER);
+            n = (long long) c.n_kv * (sp.n + P16_OVER);
         }
         const long long at = total + plan_before(n, some, sums);
         if (e < all) p.a.before[e] = at;
@@ -81,21 +112,21 @@ static __global__ void __launch_bounds__(1024) k_kv16_plan(const PromptArgs p, i
     }
 }
 
-struct Segment16 { Seq q; Steps sp; int ct, head, t0, t1, halves; };
+struct Segment16 { Seq q; Steps sp; int ct, head, t0, t1, halves, n0; };      // n0: the block's tiles in front of it
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs p, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs p, const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap q_map, bool by_box) {
     constexpr int QB = Prompt16Smem<HD>::Q, KVB = Prompt16Smem<HD>::KV, SUB = 128 * 128;      // SUB: 128 rows of 128 bytes
     extern __shared__ uint8_t pr_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_full[2][2];      // [half][turn]
-    __shared__ uint32_t tmem_s;
+    __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_full[2][2];      // [half][turn]
+    __shared__ uint32_t tmem_s, there_s[4];                      // there_s: of a tile, its sixteens of tokens that have a page
     const AttendArgs & a = p.a;
     const Cache & c = a.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t smem = (smem_at(pr_raw) + 1023u) & ~1023u, q_s = smem, k_s = q_s + 2 * QB, v_s = k_s + 2 * KVB;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(smem_at(&q_full[i]), p.queries);
+            mbar_init(smem_at(&q_full[i]), p.queries); mbar_init(smem_at(&q_empty[i]), 5);
             mbar_init(smem_at(&k_full[i]), 1); mbar_init(smem_at(&v_full[i]), 1);
             mbar_init(smem_at(&k_empty[i]), 2); mbar_init(smem_at(&v_empty[i]), 2);
             for (int b = 0; b < 2; b++) { mbar_init(smem_at(&s_full[i][b]), 1); mbar_init(smem_at(&p_full[i][b]), 4); mbar_init(smem_at(&o_full[i][b]), 1); }
@@ -115,12 +146,12 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
     const int per = p.first[0], entries = p.first[1];
     const long long begin = (long long) blockIdx.x * per, end = min(a.before[entries], begin + per);
     // the segments of this block's piece, one after the other and the same for every warp
-    int entry = begin < end ? p.first[2 + blockIdx.x] : 0, head = -1;
+    int entry = begin < end ? p.first[2 + blockIdx.x] : 0, head = -1, tiles_before = 0;
     long long at = begin;
     const auto segment = [&](Segment16 & g) {
         while (at < end) {
             const Entry e = p.entries[entry];
-            const int len = e.n + PR_OVER;
+            const int len = e.n + P16_OVER;
             int from = 0;
             if (head < 0) {                                        // the first one may begin anywhere
                 const long long x = at - a.before[entry];
@@ -131,12 +162,16 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
             g.q = Seq{e.slot, e.begin, e.count, e.held};
             g.sp = Steps{e.head, e.lo, e.n};
             g.ct = e.ct; g.head = head;
-            g.t0 = max(0, from - PR_OVER);
-            g.t1 = to - PR_OVER;
+            g.t0 = max(0, from - P16_OVER);
+            g.t1 = to - P16_OVER;
             g.halves = e.count * a.group - e.ct * PR_COLS > 128 ? 2 : 1;
             at += to - from;
             if (++head == c.n_kv) { head = 0; entry++; }
-            if (g.t1 > 0) return true;
+            if (g.t1 > 0) {
+                g.n0 = tiles_before;
+                tiles_before += g.t1 - g.t0;
+                return true;
+            }
         }
         return false;
     };
@@ -146,19 +181,18 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;          // of the half
         const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, my_s = t_s + lanes + half * 128, my_o = t_o + lanes + half * HD;
         const float factor = fmaxf(fabsf(a.scale_log2), 1.2e-38f);         // (never 0: it meets the -infinity of what is masked)
-        const uint32_t turn_round = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-        int n_s = 0;                                                       // steps of 64 tokens of this half so far
+        const bool turned = a.scale_log2 < 0.f;
+        int n_s = 0, n_q = 0;                                              // steps of 64 tokens and segments of this half so far
         const auto next = [&](Segment16 & g) {                             // the next segment with columns of this half
             do { if (!segment(g)) return false; } while (half >= g.halves);
             return true;
         };
-        // the warp's 32 queries, HD / 8 lanes a row. One with an infinity or a NaN becomes NaN, since its negative scores would look like masked ones
+        // the warp's 32 queries where boxes do not bring them: HD / 8 lanes a row
         const auto queries = [&](const Segment16 & g) {
             const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
-            constexpr int LANES = HD / 8, ROWS = 32 / LANES, X = 8;
+            constexpr int LANES = HD / 8, ROWS = 32 / LANES, X = 4;
             const int64_t mine = i < g.q.count ? (g.q.begin + i) * a.q_row + h * a.q_head : -1;
             const int m = lane % LANES;
-            const unsigned group = (LANES == 16 ? 0xffffu : 0xffu) << (lane / LANES * LANES);
 #pragma unroll 1
             for (int x0 = 0; x0 < 32; x0 += X * ROWS) {
                 uint4 f[X];
@@ -176,10 +210,7 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
 #pragma unroll
                 for (int x = 0; x < X; x++) {
                     const int r = x0 + x * ROWS + lane / LANES;
-                    const bool bad = wild<T>(f[x].x) || wild<T>(f[x].y) || wild<T>(f[x].z) || wild<T>(f[x].w);
-                    if (__ballot_sync(0xffffffffu, bad) & group) f[x] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-                    pr_st_shared(q_s + half * QB + (m >> 3) * SUB + ((warp & 3) * 32 + r) * 128 + (((m & 7) ^ (r & 7)) << 4), f[x].x ^ turn_round, f[x].y ^ turn_round, f[x].z ^ turn_round,
-                                 f[x].w ^ turn_round);
+                    pr_st_shared(q_s + half * QB + (m >> 3) * SUB + ((warp & 3) * 32 + r) * 128 + (((m & 7) ^ (r & 7)) << 4), f[x].x, f[x].y, f[x].z, f[x].w);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -188,40 +219,52 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
         };
         Segment16 g;
         bool more = next(g);
-        if (more) queries(g);
+        if (more && !by_box) queries(g);
         while (more) {
             const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
             const bool in = i < g.q.count;
-            // whether every page of the piece is there; where not, each tile's are looked up again
-            bool whole = g.q.slot >= 0;
-            {
-                const int last = g.q.held + g.q.count - 1, log2 = min(c.page_log2, 7), more_log2 = 7 - log2;       // a page of a tile a lane
-                for (int x = (g.t0 << more_log2) + lane; x < g.t1 << more_log2; x += 32) {
-                    const int pos = step_at(g.sp, x >> more_log2) * PR_KV + ((x & ((1 << more_log2) - 1)) << log2);
-                    if (pos <= last) whole = whole && page_at(c, g.q.slot, pos) >= 0;
-                }
-                whole = __all_sync(0xffffffffu, whole);
-            }
             const int row_lo = g.ct * PR_COLS / a.group, row_hi = min(g.q.count - 1, (g.ct * PR_COLS + PR_COLS - 1) / a.group);
             const int all_see_hi = g.q.held + row_lo, all_see_lo = a.window > 0 ? g.q.held + row_hi - a.window + 1 : 0;
             const int top_pos = in ? g.q.held + i : -1, low_pos = a.window > 0 ? top_pos - a.window : -1;      // sees low_pos < position <= top_pos, and what is below sinks
             float m = -INFINITY, l = 0.f, base = 0.f, limit = -INFINITY;
+            // a query with an infinity or a NaN answers NaN: its negative scores would look like masked ones. A thread looks its own over
+            uint32_t most = 0;
+            pr_wait(smem_at(&q_full[half]), (uint32_t) (n_q & 1), p.polls, dead);
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < HD / 8; x++) {
+                uint4 f;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(f.x), "=r"(f.y), "=r"(f.z), "=r"(f.w) : "r"(q_s + half * QB + (x >> 3) * SUB + row * 128 + (((x & 7) ^ (row & 7)) << 4)) : "memory");
+                most = __vmaxu2(most, __vmaxu2(__vmaxu2(f.x & 0x7fff7fffu, f.y & 0x7fff7fffu), __vmaxu2(f.z & 0x7fff7fffu, f.w & 0x7fff7fffu)));
+            }
+            const bool bad = wild<T>(most);
+            const bool any_bad = __any_sync(0xffffffffu, bad);
+            if (lane == 0) pr_arrive(smem_at(&q_empty[half]));
+            n_q++;
+            const bool odd = any_bad || turned;
             for (int t = 2 * g.t0; t < 2 * g.t1; t++, n_s++) {
                 const int pos = step_at(g.sp, t >> 1) * PR_KV + 64 * (t & 1);
                 const uint32_t at = my_s + 64 * (n_s & 1);
-                const bool edge = !whole || pos + 63 > all_see_hi || (pos < all_see_lo && pos + 63 >= a.sinks);
-                unsigned there = 0xfu;                                     // tiles of 16 tokens that have a page
-                if (!whole) there = __ballot_sync(0xffffffffu, lane < 4 && page_at(c, g.q.slot, pos + 16 * (lane & 3)) >= 0);
                 pr_wait(smem_at(&s_full[half][n_s & 1]), (uint32_t) (n_s >> 1 & 1), p.polls, dead);
                 __syncwarp();
                 pr_fence_after();
+                const unsigned there = there_s[(g.n0 + (t >> 1) - g.t0) & 3] >> (4 * (t & 1)) & 15u;
                 uint32_t r[64];
                 pr_ld64(at, r);
-                if (edge) {                                                // what a column does not see goes to -infinity
-                    const int hi = top_pos - pos, lo = low_pos - pos, sinks = a.sinks - pos;
+                if (odd || there != 15u || pos + 63 > all_see_hi || (pos < all_see_lo && pos + 63 >= a.sinks)) {
+                    if (any_bad) {                                         // every score as good as another: whether it sees anything is told by the sum of weights
 #pragma unroll
-                    for (int x = 0; x < 64; x++)
-                        if (x > hi || (x <= lo && x >= sinks) || !(there >> (x >> 4) & 1)) r[x] = 0xff800000u;
+                        for (int x = 0; x < 64; x++) r[x] = bad ? 0 : r[x];
+                    }
+                    if (turned) {
+#pragma unroll
+                        for (int x = 0; x < 64; x++) r[x] ^= 0x80000000u;
+                    }
+                    // what a column does not see goes to -infinity: a bit a token of what it sees, up to its position, behind the window's beginning or among the first ones, on pages that are there
+                    const uint64_t pages = (there & 1 ? 0xffffull : 0) | (there & 2 ? 0xffffull << 16 : 0) | (there & 4 ? 0xffffull << 32 : 0) | (there & 8 ? 0xffffull << 48 : 0);
+                    const uint64_t seen = first_bits(top_pos - pos + 1) & (~first_bits(low_pos - pos + 1) | first_bits(a.sinks - pos)) & pages;
+#pragma unroll
+                    for (int x = 0; x < 64; x++) r[x] = seen >> x & 1 ? r[x] : 0xff800000u;
                 }
                 float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
@@ -256,9 +299,9 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
 #pragma unroll
                 for (int x = 0; x < 64; x += 2) {
                     const float2 y = split(fma2(two(__uint_as_float(r[x]), __uint_as_float(r[x + 1])), by, less));
-                    w[x / 2] = pair_of<T>(exp2_fast(y.x), exp2_fast(y.y));
-                    const float2 e = floats_of<T>(w[x / 2]);
-                    sum = add2(sum, two(e.x, e.y));
+                    const float2 z = (x >> 1 & 7) < P16_EIGHTHS ? exp2_pair(y) : make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                    sum = add2(sum, two(z.x, z.y));
+                    w[x / 2] = pair_of<T>(z.x, z.y);
                 }
                 pr_st32(at, w);
                 l += split(sum).x + split(sum).y;
@@ -267,10 +310,11 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                 __syncwarp();
                 if (lane == 0) pr_arrive(smem_at(&p_full[half][n_s & 1]));
             }
+            if (bad && l != 0.f) l = NAN;
             // the next segment's queries before this one's results: its first scores are made while these are written
             Segment16 then;
             more = next(then);
-            if (more) queries(then);
+            if (more && !by_box) queries(then);
             pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), p.polls, dead);
             __syncwarp();
             pr_fence_after();
@@ -314,7 +358,7 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                 int page = page_of(g.t0);
                 for (int t = g.t0; t < g.t1; t++, n++) {
                     const int stage = n & 1, then = page_of(t + 1);
-                    const uint32_t round = (uint32_t) (n >> 1);
+                    const uint32_t round = (uint32_t) (n >> 1), found = __ballot_sync(0xffffffffu, page >= 0), there = __ballot_sync(0xffffffffu, lane < 8 && (found >> (lane >> (log2 - 4)) & 1));
                     const int token = (step_at(g.sp, t) * PR_KV + (lane << log2)) & ((1 << c.page_log2) - 1), z = page >= 0 ? page : c.n_pages;
 #pragma unroll
                     for (int side = 0; side < 2; side++) {
@@ -322,7 +366,10 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                         if (n >= 2) pr_wait(smem_at(side ? &v_empty[stage] : &k_empty[stage]), (round - 1) & 1, p.polls, dead);
                         dead = __any_sync(0xffffffffu, dead);
                         if (!dead) {
-                            if (lane == 0) mbar_expect(full, KVB);
+                            if (lane == 0) {
+                                if (side == 0) there_s[n & 3] = there;
+                                mbar_expect(full, KVB);
+                            }
                             __syncwarp();
                             if (lane < pieces)
 #pragma unroll
@@ -336,10 +383,27 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                 pr_wait(smem_at(&k_empty[i & 1]), (uint32_t) (i >> 1 & 1), p.polls, dead);
                 pr_wait(smem_at(&v_empty[i & 1]), (uint32_t) (i >> 1 & 1), p.polls, dead);
             }
+        } else if (warp == 11) {
+            // queries of the next segment as soon as the last scores of the one before are made
+            int n_q[2] = {0, 0};
+            for (Segment16 g; by_box && segment(g);)
+                for (int half = 0; half < g.halves; half++) {
+                    const int use = half ? n_q[1]++ : n_q[0]++;
+                    if (use) pr_wait(smem_at(&q_empty[half]), (uint32_t) ((use - 1) & 1), p.polls, dead);
+                    __syncwarp();
+                    if (pr_elect() && !dead) {
+                        mbar_expect(smem_at(&q_full[half]), QB);
+#pragma unroll
+                        for (int d = 0; d < HD / 64; d++)
+                            tma_queries(q_s + half * QB + d * SUB, &q_map, smem_at(&q_full[half]), 64 * d, g.head * a.group, g.q.begin + (g.ct * PR_COLS + half * 128) / a.group);
+                    }
+                }
+            for (int half = 0; half < 2; half++)                           // as with the last tiles
+                if (n_q[half]) pr_wait(smem_at(&q_empty[half]), (uint32_t) ((n_q[half] - 1) & 1), p.polls, dead);
         } else {
             const int half = warp - 9;
             int n = 0, n_q = 0, n_p = 0;                                   // tiles, segments and steps of this half so far
-            for (Segment16 g; half < 2 && segment(g);) {
+            for (Segment16 g; segment(g);) {
                 const int tiles = g.t1 - g.t0, steps = 2 * tiles;
                 if (pr_elect()) {
                     if (half < g.halves) {
@@ -350,6 +414,7 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                                 pr_mma_ss(t_s + half * 128 + 64 * turn, PR_DESC | (uint64_t) ((q_s + half * QB + (k >> 2) * SUB) >> 4) + 2 * (k & 3),
                                           PR_DESC | (uint64_t) ((k_s + (n + (step >> 1) & 1) * KVB + (k >> 2) * SUB + turn * (SUB / 2)) >> 4) + 2 * (k & 3), p16_idesc<T>(64, false), k > 0);
                             pr_commit(smem_at(&s_full[half][turn]));
+                            if (step == steps - 1) pr_commit(smem_at(&q_empty[half]));
                         };
                         pr_wait(smem_at(&q_full[half]), (uint32_t) (n_q & 1), p.polls, dead);
                         pr_wait(smem_at(&k_full[n & 1]), (uint32_t) (n >> 1 & 1), p.polls, dead);
@@ -361,7 +426,10 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                         }
                         for (int step = 0; step < steps; step++) {
                             const int turn = step & 1, now = n + (step >> 1), stage = now & 1, after = (now + 1) & 1;
-                            if (turn == 0) pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), p.polls, dead);
+                            if (turn == 0) {                               // (a wait for what is there takes 130 clocks: while P is being made)
+                                pr_wait(smem_at(&v_full[stage]), (uint32_t) (now >> 1 & 1), p.polls, dead);
+                                if (step + 2 < steps) pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), p.polls, dead);
+                            }
                             pr_wait(smem_at(&p_full[half][turn]), (uint32_t) ((n_p + step) >> 1 & 1), p.polls, dead);
                             pr_fence_after();
                             if (!dead) {
@@ -373,7 +441,6 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                                 if (turn == 1) pr_commit(smem_at(&v_empty[stage]));
                             }
                             if (step + 2 < steps) {
-                                if (turn == 0) { pr_wait(smem_at(&k_full[after]), (uint32_t) ((now + 1) >> 1 & 1), p.polls, dead); pr_fence_after(); }
                                 if (!dead) {
                                     scores(step + 2);
                                     if (turn == 1) pr_commit(smem_at(&k_empty[after]));
@@ -404,6 +471,67 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
     if (warp == 8) {
         pr_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem));
+    }
+}
+
+// a block 32 columns of a unit that blocks shared: adds its parts, eight on their way at a time. A lane is a column, a warp has every eighth group of 4 dims
+template <int HD, typename T>
+__global__ void __launch_bounds__(256) k_kv16_prompt_join(const PromptArgs p) {
+    constexpr int X = HD / 32, PAD = HD + 4, BATCH = 8;
+    __shared__ __align__(16) float sums[32 * PAD];
+    const AttendArgs & a = p.a;
+    const Cache & c = a.c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x / (PR_COLS / 32), c0 = blockIdx.x % (PR_COLS / 32) * 32, head = blockIdx.y;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (e >= p.first[1]) return;
+    const Entry n = p.entries[e];
+    const int len = n.n + P16_OVER, per = p.first[0], cols = min(PR_COLS, n.count * a.group - n.ct * PR_COLS);
+    if (c0 >= cols) return;
+    const long long u0 = a.before[e] + (long long) head * len;
+    const int w0 = (int) quotient(u0 + P16_OVER, per), w1 = (int) quotient(u0 + len - 1, per);
+    if (w0 == w1) return;
+    const bool in = c0 + lane < cols;                              // (others were not stored)
+    float m = -INFINITY, l = 0.f, o[X][4] = {};
+    for (int w = w0; w <= w1; w += BATCH) {
+        float2 ml[BATCH];
+        float4 v[BATCH][X];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) {
+            const size_t part = 2 * (size_t) (w + i) + (w + i == w0 ? 1 : 0);
+            const bool there = in && w + i <= w1;
+            ml[i] = there ? *reinterpret_cast<const float2 *>(a.ml + (part * PR_COLS + c0 + lane) * 2) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int x = 0; x < X; x++)
+                v[i][x] = there ? reinterpret_cast<const float4 *>(a.part + part * PR_COLS * HD)[(size_t) (warp + 8 * x) * PR_COLS + c0 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) top = fmaxf(top, ml[i].x);
+        const float base = top == -INFINITY ? 0.f : top, old = exp2_fast(m - base);
+        l *= old;
+#pragma unroll
+        for (int x = 0; x < X; x++) { o[x][0] *= old; o[x][1] *= old; o[x][2] *= old; o[x][3] *= old; }
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) {
+            const float by = exp2_fast(ml[i].x - base);
+            l = fmaf(ml[i].y, by, l);
+#pragma unroll
+            for (int x = 0; x < X; x++) {
+                o[x][0] = fmaf(v[i][x].x, by, o[x][0]); o[x][1] = fmaf(v[i][x].y, by, o[x][1]);
+                o[x][2] = fmaf(v[i][x].z, by, o[x][2]); o[x][3] = fmaf(v[i][x].w, by, o[x][3]);
+            }
+        }
+        m = top;
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int x = 0; x < X; x++) *reinterpret_cast<float4 *>(sums + lane * PAD + 4 * (warp + 8 * x)) = make_float4(o[x][0] * inv, o[x][1] * inv, o[x][2] * inv, o[x][3] * inv);
+    __syncthreads();
+    for (int x = warp; x < 32 && c0 + x < cols; x += 8) {
+        const int col = n.ct * PR_COLS + c0 + x, i = col / a.group, h = head * a.group + col - i * a.group;
+        T * y = static_cast<T *>(a.out) + ((size_t) (n.begin + i) * c.n_kv * a.group + h) * HD + X * lane;
+#pragma unroll
+        for (int j = 0; j < X; j++) y[j] = from_f<T>(sums[x * PAD + X * lane + j]);
     }
 }
 

@@ -31,7 +31,7 @@ struct PromptArgs {
     int * first;                         // tiles of a block's piece, entries, the entry that each block's piece begins in
     int * err;
     uint32_t polls;                      // of a wait that is given up
-    int queries;                         // arrivals that tell a half's queries there: 4, one from each warp, or more than come (b200_kv4_drill)
+    int queries;                         // arrivals that tell a half's queries there (4, one from each warp; 1 of a box in serve_kv16_prompt.cuh), or more than come (b200_kv4_drill)
 };
 
 constexpr uint32_t PR_POLLS = 1u << 18;       // a poll that finds nothing takes 7800 clocks: a second
