@@ -49,6 +49,7 @@ template <typename T> void append_to(const b200_kv4 & c, const Cache & d, int dt
     else append_as<__half, T>(c, d, k, kr, kh, v, vr, vh);
 }
 
+int attend_tiles(int group, int max_rows, int nt) { return (int) (((int64_t) group * max_rows + 8 * nt - 1) / (8 * nt)); }
 int attend_nt(int group, int max_rows) { return (int64_t) group * max_rows <= 8 ? 1 : 2; }
 size_t attend_before_bytes(int n_seq) { return ((size_t) (n_seq + 2) * 8 + 255) / 256 * 256; }
 size_t attend_bytes(int n_seq, int head_dim, int nt, int sms) { return attend_before_bytes(n_seq) + 2 * (size_t) sms * A16_WARPS * 8 * nt * (head_dim + 2) * 4; }
@@ -62,9 +63,28 @@ template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, const
     else if (parts > 8) launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, stream, true, 1, a);
     else launch(k_kv4_join<HD, NT, T, 1>, dim3((unsigned) ((items + 7) / 8)), 256, 0, stream, true, 1, a);
 }
-template <typename T> void attend_few(const AttendArgs & a, const CUtensorMap & map, int * err, int head_dim, int nt, int device, int sms, void * stream) {
-    if (head_dim == 128) nt == 1 ? attend_as<128, 1, T>(a, map, err, device, sms, stream) : attend_as<128, 2, T>(a, map, err, device, sms, stream);
-    else nt == 1 ? attend_as<64, 1, T>(a, map, err, device, sms, stream) : attend_as<64, 2, T>(a, map, err, device, sms, stream);
+template <int HD, int NT, typename T> void unit_as(const AttendArgs & a, const CUtensorMap & map, int * err, int n_ct, int cluster, int device, void * stream) {
+    static Limits set;
+    const auto kernel = k_kv16_attend_unit<HD, NT, T>;
+    allow_smem(kernel, device, set);
+    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * n_ct * cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), stream, false, cluster, a, map, err, WAIT_POLLS, n_ct);
+}
+template <typename T> void attend_few(const AttendArgs & a, const CUtensorMap & map, int * err, int head_dim, int nt, int n_ct, int cluster, int device, int sms, void * stream) {
+    const auto as = [&](auto line, auto unit) { cluster ? unit(a, map, err, n_ct, cluster, device, stream) : line(a, map, err, device, sms, stream); };
+    if (head_dim == 128) nt == 1 ? as(attend_as<128, 1, T>, unit_as<128, 1, T>) : as(attend_as<128, 2, T>, unit_as<128, 2, T>);
+    else nt == 1 ? as(attend_as<64, 1, T>, unit_as<64, 1, T>) : as(attend_as<64, 2, T>, unit_as<64, 2, T>);
+}
+// blocks of a cluster a unit where one launch does: all clusters stand on the card at once, and the longest sequence that the table (or the window) allows gives each warp at most UNIT_STEPS steps of
+// 32 tokens. 0: a line of pieces and a join. One launch / two, us with cold memory, 8 KV heads of 128: one sequence of 333 10.3 / 14.3, of 4000 (4 steps a warp) 14.4 / 18.4, of 8000 (8) 16.4 / 20.5, of
+// 20 000 (20) 26.7 / 26.7; 16 of 200 (2) 12.3 / 18.4, of 1000 (8) 20.5 / 24.6; 61 of 1004 (2 heads of 64, 8) 16.4 / 18.5
+constexpr int UNIT_STEPS = 16;
+int unit_cluster(const b200_kv4 & c, int n_ct, int window, int sinks, int sms) {
+    const int64_t units = (int64_t) c.n_seq * c.n_head_kv * n_ct, room = (int64_t) sms * (c.head_dim == 64 ? 2 : 1);
+    int64_t tokens = (int64_t) c.max_pages * c.page_tokens;
+    if (window > 0) tokens = std::min(tokens, (int64_t) window + std::min<int64_t>(sinks, tokens) + 128);
+    int cluster = A16_CLUSTER;
+    while (cluster > 1 && units * cluster > room) cluster /= 2;
+    return units * cluster <= room && (tokens + 31) / 32 <= (int64_t) UNIT_STEPS * A16_WARPS * cluster ? cluster : 0;
 }
 
 template <int HD, typename T> void prompt_as(const PromptArgs & p, const CUtensorMap & map, const CUtensorMap & q_map, bool by_box, int64_t entries, int device, int sms, void * stream) {
@@ -102,7 +122,8 @@ int64_t kv16_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
     check_heads(c, n_head, max_rows);
     On on(c.device);
     if (is_prompt(n_head / c.n_head_kv, max_rows)) return prompt_work(c, n_head / c.n_head_kv, on.sms).bytes;
-    return (int64_t) attend_bytes(c.n_seq, c.head_dim, attend_nt(n_head / c.n_head_kv, max_rows), on.sms);
+    const int nt = attend_nt(n_head / c.n_head_kv, max_rows);
+    return unit_cluster(c, attend_tiles(n_head / c.n_head_kv, max_rows, nt), 0, 0, on.sms) ? 0 : (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms);       // (a window asks for no more)
 }
 
 void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int sinks, int max_rows, void * out, void * work,
@@ -151,11 +172,12 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
     }
     const CUtensorMap map = pool_map(c, bf16, 16, 2);
     const int nt = attend_nt(a.group, max_rows);
-    check_work(work, work_bytes, (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms));
+    const int n_ct = attend_tiles(a.group, max_rows, nt), cluster = unit_cluster(c, n_ct, window, a.sinks, on.sms);
+    if (!cluster) check_work(work, work_bytes, (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms));
     a.before = reinterpret_cast<long long *>(w);
     a.ml = reinterpret_cast<float *>(w + attend_before_bytes(c.n_seq));
     a.part = a.ml + 2 * (size_t) on.sms * A16_WARPS * 8 * nt * 2;
-    bf16 ? attend_few<__nv_bfloat16>(a, map, err, c.head_dim, nt, c.device, on.sms, c.stream) : attend_few<__half>(a, map, err, c.head_dim, nt, c.device, on.sms, c.stream);
+    bf16 ? attend_few<__nv_bfloat16>(a, map, err, c.head_dim, nt, n_ct, cluster, c.device, on.sms, c.stream) : attend_few<__half>(a, map, err, c.head_dim, nt, n_ct, cluster, c.device, on.sms, c.stream);
 }
 
 }  // namespace b200

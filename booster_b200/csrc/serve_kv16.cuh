@@ -16,12 +16,13 @@
 #pragma once
 #include "serve_attn.cuh"
 #include "serve_tma.cuh"
+#include <cooperative_groups.h>
 #include <type_traits>
 
 namespace b200 {
 namespace srv {
 
-constexpr int A16_WARPS = 4, A16_STAGES = 3, A16_STEP = 32;
+constexpr int A16_WARPS = 4, A16_STAGES = 3, A16_STEP = 32, A16_CLUSTER = 8;
 __host__ __device__ constexpr int a16_stage_bytes(int hd) { return A16_STEP * 4 * hd; }
 __host__ __device__ constexpr size_t a16_ring_bytes(int hd) { return (size_t) A16_WARPS * A16_STAGES * a16_stage_bytes(hd); }
 
@@ -61,9 +62,202 @@ template <typename T> __device__ __forceinline__ bool wild(uint32_t p) {
     return (p & M) == M || (p >> 16 & M) == M;
 }
 
+// what a warp holds of a unit: its columns' sums of values, largest scores less P_LIFT and sums of weights. A lane has columns 2 tq, 2 tq + 1 of each eight and the dims 16 k + g, + 8
+template <int HD, int NT> struct Piece16 { float o[NT][HD / 16][4], m[NT][2], l[NT][2]; };
+struct Ring16 { uint32_t at, bars; int n_fill, n_use; };        // a warp's stages, and steps that were asked for and used so far: stage n % A16_STAGES, phase n / A16_STAGES
+
+// steps t0 .. t1 - 1 of the columns ct of a sequence and KV head, by one warp
+template <int HD, int NT, typename T>
+__device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtensorMap & map, const Seq & q, const Steps & sp, int ct, int head, int t0, int t1, Ring16 & ring, uint32_t polls, bool & dead,
+                                             Piece16<HD, NT> & out) {
+    constexpr int COLS = 8 * NT, KS = HD / 16, STAGE = a16_stage_bytes(HD), HALF = 8192;        // HALF: 64 dims of a step; of it 4096 for 16 tokens, keys and values of 2048 each
+    const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+    const Cache & c = a.c;
+    float (&o)[NT][KS][4] = out.o;
+    float (&m)[NT][2] = out.m;
+    float (&l)[NT][2] = out.l;
+    // the columns' queries, B operand of K Q^T: lane (g, tq) holds column g's dims 16 k + 2 tq, + 1 and those 8 further on
+    uint32_t qf[NT][KS][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int col = ct * COLS + 8 * n + g, i = col / a.group, h = head * a.group + col - i * a.group;
+        const T * qp = static_cast<const T *>(a.q) + (q.begin + i) * a.q_row + h * a.q_head + 2 * tq;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                qf[n][k][j] = 0;
+                if (i >= q.count) continue;
+                if (a.q_whole) qf[n][k][j] = *reinterpret_cast<const uint32_t *>(qp + 16 * k + 8 * j);
+                else { const uint16_t * u = reinterpret_cast<const uint16_t *>(qp + 16 * k + 8 * j); qf[n][k][j] = u[0] | (uint32_t) u[1] << 16; }
+            }
+    }
+    // steps on their way: A16_STAGES - 1 ahead of the one in hand. Lanes hold the next 32 pages of the slot
+    int next = t0, pages_from = -64, my_page = -1;
+    uint32_t there = 0;                                        // two bits a step that was asked for: which of its halves have a page. The newest lowest
+    const auto fetch = [&]() {
+        there <<= 2;
+        if (next < t1) {
+            const int pos = step_at(sp, next) << 5, pi = pos >> c.page_log2, pi_b = (pos + 16) >> c.page_log2;
+            if (pi < pages_from || pi_b - pages_from > 31) { pages_from = pi; my_page = page_at(c, q.slot, min(pi + lane, c.max_pages) << c.page_log2); }
+            const int page_a = __shfl_sync(0xffffffffu, my_page, pi - pages_from), page_b = __shfl_sync(0xffffffffu, my_page, pi_b - pages_from);
+            there |= (uint32_t) (page_a >= 0) | (uint32_t) (page_b >= 0) << 1;
+            if (lane == 0) {
+                const int stage = ring.n_fill % A16_STAGES, mask = (1 << c.page_log2) - 1;
+                const uint32_t bar = ring.bars + 8 * stage, dst = ring.at + (uint32_t) (stage * STAGE);
+                mbar_expect(bar, STAGE);
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int h = 0; h < HD / 64; h++)
+                        tma_box(dst + h * HALF + u * 4096, &map, bar, 64 * h, (pos + 16 * u) & mask, head, u ? (page_b >= 0 ? page_b : c.n_pages) : (page_a >= 0 ? page_a : c.n_pages));
+            }
+            ring.n_fill++;
+            next++;
+        }
+    };
+    __syncwarp();                                              // nobody still reads the ring for the piece before
+#pragma unroll
+    for (int i = 0; i < A16_STAGES - 1; i++) fetch();
+    int p_hi[NT][2];                                           // last position that the lane's two columns of S^T see; -1: no column
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        // a query with an infinity has no soft-max that is a number: all NaN, since negative scores would look like masked ones
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < KS; k++) bad = bad || wild<T>(qf[n][k][0]) || wild<T>(qf[n][k][1]);
+        const unsigned any = __ballot_sync(0xffffffffu, bad) >> (4 * g) & 15u;
+#pragma unroll
+        for (int k = 0; k < KS; k++) if (any) qf[n][k][0] = qf[n][k][1] = 0x7fff7fffu;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int cc = ct * COLS + 8 * n + 2 * tq + j;
+            p_hi[n][j] = cc / a.group < q.count ? q.held + cc / a.group : -1;
+        }
+    }
+    const int row_lo = ct * COLS / a.group, row_hi = min(q.count - 1, (ct * COLS + COLS - 1) / a.group);
+    const int all_see_hi = q.held + row_lo, all_see_lo = a.window > 0 ? q.held + row_hi - a.window + 1 : 0;   // positions that every column sees
+    float base[NT][2], limit[NT][2];       // base: what is taken off scores, m or 0; limit: where they move
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) { m[n][j] = limit[n][j] = -INFINITY; l[n][j] = base[n][j] = 0.f; }
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[n][k][j] = 0.f;
+    }
+    const uint32_t k_lane = (uint32_t) ((lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4));
+    const uint32_t v_lane = (uint32_t) (2048 + ((lane & 7) + ((lane >> 4) << 3)) * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4));
+#pragma unroll 1
+    for (int t = t0; t < t1; t++) {
+        const int stage = ring.n_use % A16_STAGES;
+        mbar_wait(ring.bars + 8 * stage, (uint32_t) (ring.n_use / A16_STAGES & 1), polls, dead);
+        ring.n_use++;
+        dead = __any_sync(0xffffffffu, dead);                  // (and all lanes are done with the step before)
+        if (dead) return;
+        fetch();
+        const uint32_t step = ring.at + (uint32_t) (stage * STAGE);
+        const uint32_t both = there >> 2 * (A16_STAGES - 1) & 3;
+        if (both == 0) continue;
+        const int pos = step_at(sp, t) << 5;
+        float st[2][NT][4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) st[u][n][j] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                uint32_t f[4];
+                ldsm4<false>(f, step + (k >> 2) * HALF + u * 4096 + (k_lane ^ (uint32_t) ((k & 3) << 5)));
+#pragma unroll
+                for (int n = 0; n < NT; n++) mma_of<T>(st[u][n], f, qf[n][k][0], qf[n][k][1]);
+            }
+        }
+        bool more = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) { st[0][n][j] *= a.scale_log2; st[1][n][j] *= a.scale_log2; }
+        // rows of S^T: tokens g and g + 8 of each 16
+        if (pos + 31 > all_see_hi || (pos < all_see_lo && pos + 31 >= a.sinks) || both != 3) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int p = pos + g + 16 * u + 8 * (j >> 1), top = p_hi[n][j & 1];
+                        if (p > top || (a.window > 0 && p <= top - a.window && p >= a.sinks) || !(both >> u & 1)) st[u][n][j] = -INFINITY;
+                    }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) more = more || fmaxf(fmaxf(st[0][n][j], st[0][n][j + 2]), fmaxf(st[1][n][j], st[1][n][j + 2])) > limit[n][j];
+        // base moves when a score passes the largest so far by 2^P_PASS
+        if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float x = fmaxf(fmaxf(st[0][n][j], st[0][n][j + 2]), fmaxf(st[1][n][j], st[1][n][j + 2]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float top = fmaxf(m[n][j], x - P_LIFT), down = top > m[n][j] ? exp2_fast(m[n][j] - top) : 1.f;
+                    m[n][j] = top;
+                    base[n][j] = top == -INFINITY ? 0.f : top;
+                    limit[n][j] = top + (P_LIFT + P_PASS);
+                    l[n][j] *= down;
+#pragma unroll
+                    for (int k = 0; k < KS; k++) { o[n][k][j] *= down; o[n][k][j + 2] *= down; }
+                }
+        }
+        uint32_t hi[2][NT][2], lo[2][NT][2];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    st[u][n][j] = exp2_fast(st[u][n][j] - base[n][j & 1]);
+                    l[n][j & 1] += st[u][n][j];
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t p = pair_of<T>(st[u][n][2 * j], st[u][n][2 * j + 1]);
+                    const float2 f = floats_of<T>(p);
+                    hi[u][n][j] = transposed(p);
+                    lo[u][n][j] = transposed(pair_of<T>(st[u][n][2 * j] - f.x, st[u][n][2 * j + 1] - f.y));
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                uint32_t f[4];
+                ldsm4<true>(f, step + (k >> 2) * HALF + u * 4096 + (v_lane ^ (uint32_t) ((k & 3) << 5)));
+#pragma unroll
+                for (int n = 0; n < NT; n++) { mma_of<T>(o[n][k], f, hi[u][n][0], hi[u][n][1]); mma_of<T>(o[n][k], f, lo[u][n][0], lo[u][n][1]); }
+            }
+    }
+    // sums over the tokens, which lie over the lanes' g
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
+            l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
+            l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
+        }
+}
+
 template <int HD, int NT, typename T>
 __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls) {
-    constexpr int COLS = 8 * NT, KS = HD / 16, STAGE = a16_stage_bytes(HD), HALF = 8192;        // HALF: 64 dims of a step; of it 4096 for 16 tokens, keys and values of 2048 each
+    constexpr int COLS = 8 * NT, KS = HD / 16, STAGE = a16_stage_bytes(HD);
     extern __shared__ uint8_t a16_raw[];
     __shared__ long long sums[A16_WARPS];
     __shared__ __align__(8) uint64_t full_s[A16_WARPS][A16_STAGES];
@@ -111,8 +305,7 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
         if (tid == 0) a.before[c.n_seq + 1] = per;
     }
     const int me = warp * (int) gridDim.x + (int) blockIdx.x;      // neighbouring pieces on different SMs
-    const uint32_t ring = smem + (uint32_t) (warp * A16_STAGES * STAGE);
-    int n_fill = 0, n_use = 0;                                     // steps that were asked for and used so far: stage n % A16_STAGES, phase n / A16_STAGES
+    Ring16 ring = {smem + (uint32_t) (warp * A16_STAGES * STAGE), smem_at(&full_s[warp][0]), 0, 0};
     bool dead = false;
     long long at = me * per;
     const long long end = min(total, at + per);
@@ -126,184 +319,9 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
         const int ct = unit / c.n_kv, head = unit - ct * c.n_kv, t0 = max(0, from - AT_OVER), t1 = to - AT_OVER;
         at += to - from;
         if (t1 <= 0) continue;
-        // the columns' queries, B operand of K Q^T: lane (g, tq) holds column g's dims 16 k + 2 tq, + 1 and those 8 further on
-        uint32_t qf[NT][KS][2];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int col = ct * COLS + 8 * n + g, i = col / a.group, h = head * a.group + col - i * a.group;
-            const T * qp = static_cast<const T *>(a.q) + (q.begin + i) * a.q_row + h * a.q_head + 2 * tq;
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    qf[n][k][j] = 0;
-                    if (i >= q.count) continue;
-                    if (a.q_whole) qf[n][k][j] = *reinterpret_cast<const uint32_t *>(qp + 16 * k + 8 * j);
-                    else { const uint16_t * u = reinterpret_cast<const uint16_t *>(qp + 16 * k + 8 * j); qf[n][k][j] = u[0] | (uint32_t) u[1] << 16; }
-                }
-        }
-        // steps on their way: A16_STAGES - 1 ahead of the one in hand. Lanes hold the next 32 pages of the slot
-        int next = t0, pages_from = -64, my_page = -1;
-        uint32_t there = 0;                                        // two bits a step that was asked for: which of its halves have a page. The newest lowest
-        const auto fetch = [&]() {
-            there <<= 2;
-            if (next < t1) {
-                const int pos = step_at(sp, next) << 5, pi = pos >> c.page_log2, pi_b = (pos + 16) >> c.page_log2;
-                if (pi < pages_from || pi_b - pages_from > 31) { pages_from = pi; my_page = page_at(c, q.slot, min(pi + lane, c.max_pages) << c.page_log2); }
-                const int page_a = __shfl_sync(0xffffffffu, my_page, pi - pages_from), page_b = __shfl_sync(0xffffffffu, my_page, pi_b - pages_from);
-                there |= (uint32_t) (page_a >= 0) | (uint32_t) (page_b >= 0) << 1;
-                if (lane == 0) {
-                    const int stage = n_fill % A16_STAGES, mask = (1 << c.page_log2) - 1;
-                    const uint32_t bar = smem_at(&full_s[warp][stage]), dst = ring + (uint32_t) (stage * STAGE);
-                    mbar_expect(bar, STAGE);
-#pragma unroll
-                    for (int u = 0; u < 2; u++)
-#pragma unroll
-                        for (int h = 0; h < HD / 64; h++)
-                            tma_box(dst + h * HALF + u * 4096, &map, bar, 64 * h, (pos + 16 * u) & mask, head, u ? (page_b >= 0 ? page_b : c.n_pages) : (page_a >= 0 ? page_a : c.n_pages));
-                }
-                n_fill++;
-                next++;
-            }
-        };
-        __syncwarp();                                              // nobody still reads the ring for the piece before
-#pragma unroll
-        for (int i = 0; i < A16_STAGES - 1; i++) fetch();
-        int p_hi[NT][2];                                           // last position that the lane's two columns of S^T see; -1: no column
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            // a query with an infinity has no soft-max that is a number: all NaN, since negative scores would look like masked ones
-            bool bad = false;
-#pragma unroll
-            for (int k = 0; k < KS; k++) bad = bad || wild<T>(qf[n][k][0]) || wild<T>(qf[n][k][1]);
-            const unsigned any = __ballot_sync(0xffffffffu, bad) >> (4 * g) & 15u;
-#pragma unroll
-            for (int k = 0; k < KS; k++) if (any) qf[n][k][0] = qf[n][k][1] = 0x7fff7fffu;
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int cc = ct * COLS + 8 * n + 2 * tq + j;
-                p_hi[n][j] = cc / a.group < q.count ? q.held + cc / a.group : -1;
-            }
-        }
-        const int row_lo = ct * COLS / a.group, row_hi = min(q.count - 1, (ct * COLS + COLS - 1) / a.group);
-        const int all_see_hi = q.held + row_lo, all_see_lo = a.window > 0 ? q.held + row_hi - a.window + 1 : 0;   // positions that every column sees
-        float o[NT][KS][4], m[NT][2], l[NT][2], base[NT][2], limit[NT][2];       // m: the largest score less P_LIFT; base: what is taken off scores, m or 0; limit: where they move
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-#pragma unroll
-            for (int j = 0; j < 2; j++) { m[n][j] = limit[n][j] = -INFINITY; l[n][j] = base[n][j] = 0.f; }
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) o[n][k][j] = 0.f;
-        }
-        const uint32_t k_lane = (uint32_t) ((lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4));
-        const uint32_t v_lane = (uint32_t) (2048 + ((lane & 7) + ((lane >> 4) << 3)) * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4));
-#pragma unroll 1
-        for (int t = t0; t < t1; t++) {
-            const int stage = n_use % A16_STAGES;
-            mbar_wait(smem_at(&full_s[warp][stage]), (uint32_t) (n_use / A16_STAGES & 1), polls, dead);
-            n_use++;
-            dead = __any_sync(0xffffffffu, dead);                  // (and all lanes are done with the step before)
-            if (dead) break;
-            fetch();
-            const uint32_t step = ring + (uint32_t) (stage * STAGE);
-            const uint32_t both = there >> 2 * (A16_STAGES - 1) & 3;
-            if (both == 0) continue;
-            const int pos = step_at(sp, t) << 5;
-            float st[2][NT][4];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) st[u][n][j] = 0.f;
-#pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    uint32_t f[4];
-                    ldsm4<false>(f, step + (k >> 2) * HALF + u * 4096 + (k_lane ^ (uint32_t) ((k & 3) << 5)));
-#pragma unroll
-                    for (int n = 0; n < NT; n++) mma_of<T>(st[u][n], f, qf[n][k][0], qf[n][k][1]);
-                }
-            }
-            bool more = false;
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) { st[0][n][j] *= a.scale_log2; st[1][n][j] *= a.scale_log2; }
-            // rows of S^T: tokens g and g + 8 of each 16
-            if (pos + 31 > all_see_hi || (pos < all_see_lo && pos + 31 >= a.sinks) || both != 3) {
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int p = pos + g + 16 * u + 8 * (j >> 1), top = p_hi[n][j & 1];
-                            if (p > top || (a.window > 0 && p <= top - a.window && p >= a.sinks) || !(both >> u & 1)) st[u][n][j] = -INFINITY;
-                        }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) more = more || fmaxf(fmaxf(st[0][n][j], st[0][n][j + 2]), fmaxf(st[1][n][j], st[1][n][j + 2])) > limit[n][j];
-            // base moves when a score passes the largest so far by 2^P_PASS
-            if (__any_sync(0xffffffffu, more)) {
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        float x = fmaxf(fmaxf(st[0][n][j], st[0][n][j + 2]), fmaxf(st[1][n][j], st[1][n][j + 2]));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        const float top = fmaxf(m[n][j], x - P_LIFT), down = top > m[n][j] ? exp2_fast(m[n][j] - top) : 1.f;
-                        m[n][j] = top;
-                        base[n][j] = top == -INFINITY ? 0.f : top;
-                        limit[n][j] = top + (P_LIFT + P_PASS);
-                        l[n][j] *= down;
-#pragma unroll
-                        for (int k = 0; k < KS; k++) { o[n][k][j] *= down; o[n][k][j + 2] *= down; }
-                    }
-            }
-            uint32_t hi[2][NT][2], lo[2][NT][2];
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        st[u][n][j] = exp2_fast(st[u][n][j] - base[n][j & 1]);
-                        l[n][j & 1] += st[u][n][j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint32_t p = pair_of<T>(st[u][n][2 * j], st[u][n][2 * j + 1]);
-                        const float2 f = floats_of<T>(p);
-                        hi[u][n][j] = transposed(p);
-                        lo[u][n][j] = transposed(pair_of<T>(st[u][n][2 * j] - f.x, st[u][n][2 * j + 1] - f.y));
-                    }
-                }
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    uint32_t f[4];
-                    ldsm4<true>(f, step + (k >> 2) * HALF + u * 4096 + (v_lane ^ (uint32_t) ((k & 3) << 5)));
-#pragma unroll
-                    for (int n = 0; n < NT; n++) { mma_of<T>(o[n][k], f, hi[u][n][0], hi[u][n][1]); mma_of<T>(o[n][k], f, lo[u][n][0], lo[u][n][1]); }
-                }
-        }
+        Piece16<HD, NT> w;
+        attend_piece<HD, NT, T>(a, map, q, sp, ct, head, t0, t1, ring, polls, dead, w);
         if (dead) break;
-        // sums over the tokens, which lie over the lanes' g
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
-                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
-                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
-            }
         const bool whole = t0 == 0 && t1 == sp.n;
         const size_t slot = 2 * (size_t) me + (t0 == 0 ? 1 : 0);
 #pragma unroll
@@ -313,19 +331,118 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
                 const int in_tile = 8 * n + 2 * tq + j, col = ct * COLS + in_tile, i = col / a.group, h = head * a.group + col - i * a.group;
                 if (i >= q.count) continue;
                 if (whole) {
-                    const float inv = l[n][j] != 0.f ? 1.f / l[n][j] : 0.f;
+                    const float inv = w.l[n][j] != 0.f ? 1.f / w.l[n][j] : 0.f;
                     T * y = static_cast<T *>(a.out) + ((size_t) (q.begin + i) * c.n_kv * a.group + h) * HD + g;
 #pragma unroll
-                    for (int k = 0; k < KS; k++) { y[16 * k] = from_f<T>(o[n][k][j] * inv); y[16 * k + 8] = from_f<T>(o[n][k][j + 2] * inv); }
+                    for (int k = 0; k < KS; k++) { y[16 * k] = from_f<T>(w.o[n][k][j] * inv); y[16 * k + 8] = from_f<T>(w.o[n][k][j + 2] * inv); }
                 } else {
                     float * y = a.part + (slot * COLS + in_tile) * HD + g;
 #pragma unroll
-                    for (int k = 0; k < KS; k++) { y[16 * k] = o[n][k][j]; y[16 * k + 8] = o[n][k][j + 2]; }
-                    if (g == 0) *reinterpret_cast<float2 *>(a.ml + (slot * COLS + in_tile) * 2) = make_float2(m[n][j], l[n][j]);
+                    for (int k = 0; k < KS; k++) { y[16 * k] = w.o[n][k][j]; y[16 * k + 8] = w.o[n][k][j + 2]; }
+                    if (g == 0) *reinterpret_cast<float2 *>(a.ml + (slot * COLS + in_tile) * 2) = make_float2(w.m[n][j], w.l[n][j]);
                 }
             }
     }
     if (dead) {                                                    // the call's results are worthless; its own copies end before the block gives its memory back
+        if (lane == 0) atomicExch_system(err, 1);
+        for (int j = 0; j < 1000; j++) __nanosleep(1000);
+    }
+}
+
+// Few sequences of bounded length: a cluster of blocks a unit, its warps share the unit's steps evenly and the blocks add what they have through one another's shared memory. One launch, no workspace
+template <int HD, int NT, typename T>
+__global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls, int n_ct) {
+    constexpr int COLS = 8 * NT, KS = HD / 16, STAGE = a16_stage_bytes(HD), PAD = HD + 4;
+    extern __shared__ uint8_t a16_raw[];
+    __shared__ __align__(8) uint64_t full_s[A16_WARPS][A16_STAGES];
+    __shared__ float ml_s[A16_WARPS][COLS][2], ml_b[COLS][2];
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    const uint32_t smem = (smem_at(a16_raw) + 1023u) & ~1023u;
+    float * parts = reinterpret_cast<float *>(a16_raw + (smem - smem_at(a16_raw)));        // [warps][COLS][PAD], then of the block [COLS][PAD], over the ring when it is done with
+    static_assert((A16_WARPS + 1) * COLS * PAD * 4 <= a16_ring_bytes(HD), "parts stand in the ring");
+    float * sums = parts + A16_WARPS * COLS * PAD;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3, rank = (int) cl.block_rank(), blocks = (int) cl.num_blocks();
+    const Cache & c = a.c;
+    if (lane == 0) {
+        for (int i = 0; i < A16_STAGES; i++) mbar_init(smem_at(&full_s[warp][i]), 1);
+        mbar_init_done();
+    }
+    __syncwarp();
+    Ring16 ring = {smem + (uint32_t) (warp * A16_STAGES * STAGE), smem_at(&full_s[warp][0]), 0, 0};
+    const int unit = (int) blockIdx.x / blocks, head = unit % c.n_kv, s = unit / c.n_kv / n_ct;
+    const Seq q = seq_at(c, s);
+    const Steps sp = steps_of(c, q, a.window, a.sinks, 0, q.count - 1, 5);
+    const int all_warps = blocks * A16_WARPS, me = rank * A16_WARPS + warp, per = sp.n / all_warps, more = sp.n % all_warps, t0 = me * per + min(me, more), t1 = t0 + per + (me < more);
+    bool dead = false;
+    for (int ct = unit / c.n_kv % n_ct; ct < col_tiles(q, a.group, COLS); ct += n_ct) {        // (the same for all blocks of the cluster)
+        Piece16<HD, NT> w;
+        attend_piece<HD, NT, T>(a, map, q, sp, ct, head, t0, dead ? t0 : t1, ring, polls, dead, w);
+        __syncthreads();                                           // nobody reads the ring any more
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int col = 8 * n + 2 * tq + j;
+                float * y = parts + (warp * COLS + col) * PAD + g;
+#pragma unroll
+                for (int k = 0; k < KS; k++) { y[16 * k] = w.o[n][k][j]; y[16 * k + 8] = w.o[n][k][j + 2]; }
+                if (g == 0) { ml_s[warp][col][0] = w.m[n][j]; ml_s[warp][col][1] = w.l[n][j]; }
+            }
+        __syncthreads();
+        // the block's sum, four dims a thread
+        for (int i = tid; i < COLS * HD / 4; i += A16_WARPS * 32) {
+            const int col = i / (HD / 4), d = i % (HD / 4) * 4;
+            float top = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int v = 0; v < A16_WARPS; v++) top = fmaxf(top, ml_s[v][col][0]);
+            const float base = top == -INFINITY ? 0.f : top;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int v = 0; v < A16_WARPS; v++) {
+                const float by = exp2_fast(ml_s[v][col][0] - base);
+                const float4 y = *reinterpret_cast<const float4 *>(parts + (v * COLS + col) * PAD + d);
+                l = fmaf(ml_s[v][col][1], by, l);
+                x.x = fmaf(y.x, by, x.x); x.y = fmaf(y.y, by, x.y); x.z = fmaf(y.z, by, x.z); x.w = fmaf(y.w, by, x.w);
+            }
+            *reinterpret_cast<float4 *>(sums + col * PAD + d) = x;
+            if (d == 0) { ml_b[col][0] = top; ml_b[col][1] = l; }
+        }
+        cl.sync();
+        // the blocks', a share of the results each
+        const int first = ct * COLS;
+        for (int i = rank * A16_WARPS * 32 + tid; i < COLS * HD / 4; i += blocks * A16_WARPS * 32) {
+            const int col = i / (HD / 4), d = i % (HD / 4) * 4, r = (first + col) / a.group, h = head * a.group + first + col - r * a.group;
+            if (r >= q.count) continue;
+            float2 ml[A16_CLUSTER];
+            float4 y[A16_CLUSTER];
+#pragma unroll
+            for (int b = 0; b < A16_CLUSTER; b++) {
+                const int o = b < blocks ? b : 0;
+                ml[b] = *reinterpret_cast<const float2 *>(cl.map_shared_rank(&ml_b[col][0], o));
+                y[b] = *reinterpret_cast<const float4 *>(cl.map_shared_rank(sums + col * PAD + d, o));
+            }
+            float top = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int b = 0; b < A16_CLUSTER; b++) top = fmaxf(top, b < blocks ? ml[b].x : -INFINITY);
+            const float base = top == -INFINITY ? 0.f : top;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int b = 0; b < A16_CLUSTER; b++)
+                if (b < blocks) {
+                    const float by = exp2_fast(ml[b].x - base);
+                    l = fmaf(ml[b].y, by, l);
+                    x.x = fmaf(y[b].x, by, x.x); x.y = fmaf(y[b].y, by, x.y); x.z = fmaf(y[b].z, by, x.z); x.w = fmaf(y[b].w, by, x.w);
+                }
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+            Four<T> f;
+            f.v[0] = from_f<T>(x.x * inv); f.v[1] = from_f<T>(x.y * inv); f.v[2] = from_f<T>(x.z * inv); f.v[3] = from_f<T>(x.w * inv);
+            *reinterpret_cast<Four<T> *>(static_cast<T *>(a.out) + ((size_t) (q.begin + r) * c.n_kv * a.group + h) * HD + d) = f;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        cl.sync();                                                 // nobody reads this block's any more: boxes may come into the ring again, or the block ends
+    }
+    if (dead) {
         if (lane == 0) atomicExch_system(err, 1);
         for (int j = 0; j < 1000; j++) __nanosleep(1000);
     }

@@ -44,6 +44,11 @@ class Case:
         self.gen = torch.Generator(device="cuda").manual_seed(seed)
         self.held, self.slots, self.first = ints(at), ints(self.slots_l), ints(self.first_l)
 
+    def widened(self, tokens=100000):
+        """the same under a table that allows sequences of more tokens: what is chosen by the longest possible one is another form"""
+        self.table_l = [row + [-1] * (tokens // self.page) for row in self.table_l]
+        return self
+
     @property
     def table(self):
         return ints(self.table_l)
@@ -164,6 +169,8 @@ def test_attention(dtype, hd, heads, kv, which, page):
     c.fill()
     q = (1.5 * c.randn(c.rows, heads, hd)).to(dtype)
     assert_attends(c, q, serve.kv16_attention(q, *c.args(), slots=c.slots))
+    if max(c.counts) <= 8:
+        assert_attends(c.widened(), q, serve.kv16_attention(q, *c.args(), slots=c.slots))
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 3), (16, 16), (17, 40), (64, 0), (100, 4), (100, 33), (128, 128), (300, 1000), (5000, 9), (2 ** 31 - 1, 2 ** 31 - 1)])
@@ -174,6 +181,7 @@ def test_attention_under_a_window(window, sinks, dtype, hd, heads, kv, which, pa
     c.fill()
     q = (1.5 * c.randn(c.rows, heads, hd)).to(dtype)
     assert_attends(c, q, serve.kv16_attention(q, *c.args(), slots=c.slots, window=window, sinks=sinks), window, sinks)
+    assert_attends(c.widened(), q, serve.kv16_attention(q, *c.args(), slots=c.slots, window=window, sinks=sinks), window, sinks)
 
 
 def test_sinks_count_under_a_window_alone():
@@ -186,7 +194,8 @@ def test_sinks_count_under_a_window_alone():
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("rows", [1, 6, 150])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (40, 5)])
-def test_attention_over_absent_pages_and_slots(dtype, rows, window, sinks):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_over_absent_pages_and_slots(dtype, rows, window, sinks, wide):
     held = [0, 50, 100, 200, 64, 30, 500]
     c = Case(held, [rows] * 7, kv=2, hd=128, seed=rows, dtype=dtype)
     c.fill()
@@ -199,6 +208,8 @@ def test_attention_over_absent_pages_and_slots(dtype, rows, window, sinks):
     slots = list(c.slots_l)
     slots[4] = 1000                                                     # no such slot
     c.table_l[c.slots_l[4]] = [-1] * len(c.table_l[0])                  # (as the oracle sees it)
+    if wide:
+        c.widened()
     out = serve.kv16_attention(q, *c.args(), slots=ints(slots), window=window, sinks=sinks)
     assert_attends(c, q, out, window, sinks)
     assert not out[2 * rows:3 * rows].any() and not out[4 * rows:5 * rows].any()
@@ -217,8 +228,11 @@ def test_rows_beyond_the_table(rows):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("rows", [1, 5, 90])
-def test_tokens_and_queries_that_are_no_numbers(dtype, rows):
+@pytest.mark.parametrize("wide", [False, True])
+def test_tokens_and_queries_that_are_no_numbers(dtype, rows, wide):
     c = Case([40, 200, 10], [rows] * 3, kv=2, hd=64, seed=3, dtype=dtype)
+    if wide:
+        c.widened()
     k, v = (c.randn(250 + 3 * rows, 2, 64) for _ in range(2))
     k[5, 0, 3] = float("nan")                                           # of the first sequence, KV head 0
     v[40 + rows + 100, 1, 3] = float("inf")                             # of the second, KV head 1, position 100
@@ -246,6 +260,7 @@ def test_scales_of_any_sign(rows, scale):
     c.fill()
     q = c.randn(c.rows, 8, 64).bfloat16()
     assert_attends(c, q, serve.kv16_attention(q, *c.args(), slots=c.slots, scale=scale), scale=scale)
+    assert_attends(c.widened(), q, serve.kv16_attention(q, *c.args(), slots=c.slots, scale=scale), scale=scale)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -315,6 +330,7 @@ def test_any_number_of_rows_is_right(counts, max_rows):
     q = c.randn(c.rows, 8, 128).bfloat16()
     assert_attends(c, q, serve.kv16_attention(q, *c.args(), slots=c.slots, max_rows=max_rows))
     assert_attends(c, q, serve.kv16_attention(q, *c.args(), slots=c.slots, max_rows=max_rows, window=33, sinks=5), 33, 5)
+    assert_attends(c.widened(), q, serve.kv16_attention(q, *c.args(), slots=c.slots, max_rows=max_rows))
 
 
 def test_many_sequences():
