@@ -278,20 +278,22 @@ void pages_plan(const b200_pages & p, const int32_t * slots, const int32_t * cou
     heed_waits(p.device);
     static Limits set;
     const bool apart = n_rows > PLAN_ROWS;
-    const size_t smem = words_bytes(p.n_pages) + words_bytes(p.n_slots) + plan_bytes(n);
+    const size_t smem = words_bytes(p.n_slots) + plan_bytes(n), places_smem = 4 * ((size_t) 3 * n + 1);
     allow_smem(k_pages_plan, p.device, set);
     launch(k_pages_plan, dim3(1), PG_THREADS, smem, p.stream, false, 1, d, slots, counts, n, n_rows, first, positions, places, status, !apart);
-    if (apart) launch(k_pages_places, dim3((unsigned) ((n_rows + 1023) / 1024)), 256, 0, p.stream, true, 1, d, slots, first, n, n_rows, positions, places);
+    static Limits places_set;
+    if (apart) allow_smem(k_pages_places, p.device, places_set);
+    if (apart) launch(k_pages_places, dim3((unsigned) ((n_rows + 1023) / 1024)), 256, places_smem, p.stream, true, 1, d, slots, first, n, n_rows, positions, places);
 }
 
 void pages_trim(const b200_pages & p, const int32_t * slots, int n, int window, int sinks) {
     const Pages d = checked(p, false);
-    need(n >= 0 && n <= (1 << 24), "pages_trim: from 0 to 2^24 slots");
+    need(n >= 0 && n <= (1 << 24) && (int64_t) n * ((p.max_pages + 255) / 256) <= 1ll << 33, "pages_trim: from 0 to 2^24 slots, and to 2^41 pages of their tables");
     need(slots || n == 0, "pages_trim: null pointer");
     need(window >= 0 && sinks >= 0, "pages_trim: window is a number of positions, or 0 for all; sinks is a number of positions");
     On on(p.device);
     heed_waits(p.device);
-    if (n) launch(k_pages_trim, dim3((n + 7) / 8), 256, 0, p.stream, false, 1, d, slots, n, window, sinks);
+    if (n) launch(k_pages_trim, dim3((unsigned) (((int64_t) n * ((p.max_pages + 255) / 256) + 7) / 8)), 256, 0, p.stream, false, 1, d, slots, n, window, sinks);
 }
 
 void sample_rows(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature, const int32_t * top_k,

@@ -427,6 +427,36 @@ def test_plan_of_many_rows_and_sequences():
     assert assert_plans(ints([[-1] * 400]), ints([0]), ints([0] * 300), None, [10000], 10000, 32) == 13          # 13 pages are missing
 
 
+@pytest.mark.parametrize("shift", [0, 1])
+def test_plan_in_a_large_pool(shift):
+    """free pages far behind the first 32 768, a few here and there, more than one chunk of them at once; counts off their alignment"""
+    n_pages = 150001
+    r = random.Random(shift)
+    flat = torch.ones(n_pages + shift, dtype=torch.int32, device="cuda")
+    refs = flat[shift:]
+    refs[r.sample(range(70000), 500)] = 0
+    refs[100000:] = 0
+    table, held = ints([[-1] * 3000 for _ in range(4)]), ints([0] * 4)
+    free = torch.nonzero(refs == 0)[:, 0].tolist()
+    for counts, rows in (([16 * 100, 5, 0, 16 * 300], 6500), ([0, 16 * 2500, 16 * 900, 1], 60000)):
+        t, h, f = lists(table, held, refs)
+        want = oracle.plan(t, h, f, [2, 0, 1, 3], counts, rows, 16)
+        assert want[3] == 0
+        got = serve.pages_plan(table, held, refs, ints(counts), 16, rows, ints([2, 0, 1, 3]))
+        for a, b in zip(got, (*want[:3], [0])):
+            assert a.tolist() == b
+        assert table.tolist() == t and refs.tolist() == f
+        held[ints([2, 0, 1, 3]).long()] += ints(counts)
+    assert sorted(p for row in table.tolist() for p in row if p >= 0) == free[:int((table >= 0).sum())]
+    t, h, f = lists(table, held, refs)
+    missing = int((refs == 0).sum()) // 2995 + 1
+    big = ints([[-1] * 3000 for _ in range(missing)])
+    got = serve.pages_plan(big, ints([0] * missing), refs, ints([16 * 3000] * missing), 16, 10)
+    assert got[3].item() == -1                                          # more than 10 rows
+    got = serve.pages_plan(big, ints([0] * missing), refs, ints([16 * 3000] * missing), 16, 16 * 3000 * missing)
+    assert got[3].item() == 3000 * missing - f.count(0) and refs.tolist() == f and (big == -1).all()
+
+
 def test_plans_that_cannot_be():
     base = lambda: (ints([[0, 1, -1, -1], [2, -1, -1, -1], [-1] * 4]), ints([20, 16, 0]), ints([1, 1, 1] + [0] * 9))  # noqa: E731
     for slots, counts, rows in (([0, 0], [1, 1], 4), ([0, 3], [1, 1], 4), ([0, -1], [1, 1], 4), ([0, 1], [1, -1], 4), ([0, 1], [3, 2], 4), ([0], [100], 200), ([0, 1], [2 ** 31 - 1, 2 ** 31 - 1], 7)):
