@@ -49,42 +49,48 @@ template <typename T> void append_to(const b200_kv4 & c, const Cache & d, int dt
     else append_as<__half, T>(c, d, k, kr, kh, v, vr, vh);
 }
 
-int attend_tiles(int group, int max_rows, int nt) { return (int) (((int64_t) group * max_rows + 8 * nt - 1) / (8 * nt)); }
-int attend_nt(int group, int max_rows) { return (int64_t) group * max_rows <= 8 ? 1 : 2; }
+// columns of a unit: 8 or 16 of one warp, in one launch also 32 or 64 of two or four that share what is read
+int attend_cols(int group, int max_rows) { const int64_t n = (int64_t) group * max_rows; return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+int attend_tiles(int group, int max_rows) { const int cols = attend_cols(group, max_rows); return (int) (((int64_t) group * max_rows + cols - 1) / cols); }
 size_t attend_before_bytes(int n_seq) { return ((size_t) (n_seq + 2) * 8 + 255) / 256 * 256; }
-size_t attend_bytes(int n_seq, int head_dim, int nt, int sms) { return attend_before_bytes(n_seq) + 2 * (size_t) sms * A16_WARPS * 8 * nt * (head_dim + 2) * 4; }
-template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, const CUtensorMap & map, int * err, int device, int sms, void * stream) {
+size_t attend_columns(int cols, int sms) { return 2 * (size_t) sms * A16_WARPS * cols; }      // of all pieces' partial results
+size_t attend_bytes(int n_seq, int head_dim, int cols, int sms) { return attend_before_bytes(n_seq) + attend_columns(cols, sms) * (head_dim + 2) * 4; }
+struct Few { CUtensorMap map; int * err; int n_ct, cluster, device, sms; void * stream; };
+template <int HD, int NT, int CW, typename T> void unit_as(const AttendArgs & a, const Few & f) {
+    static Limits set;
+    const auto kernel = k_kv16_attend_unit<HD, NT, CW, T>;
+    allow_smem(kernel, f.device, set);
+    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * f.n_ct * f.cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), f.stream, false, f.cluster, a, f.map, f.err, WAIT_POLLS, f.n_ct);
+}
+template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, const Few & f) {
+    if (f.cluster) return unit_as<HD, NT, 1, T>(a, f);
     static Limits set;
     const auto kernel = k_kv16_attend<HD, NT, T>;
-    allow_smem(kernel, device, set);
-    launch(kernel, dim3(sms), A16_WARPS * 32, 1024 + a16_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8, stream, false, 1, a, map, err, WAIT_POLLS);
-    const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group, parts = (int64_t) sms * A16_WARPS / ((int64_t) a.c.n_seq * a.c.n_kv);
-    if (parts > 32) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, stream, true, 1, a);
-    else if (parts > 8) launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, stream, true, 1, a);
-    else launch(k_kv4_join<HD, NT, T, 1>, dim3((unsigned) ((items + 7) / 8)), 256, 0, stream, true, 1, a);
+    allow_smem(kernel, f.device, set);
+    launch(kernel, dim3(f.sms), A16_WARPS * 32, 1024 + a16_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8, f.stream, false, 1, a, f.map, f.err, WAIT_POLLS);
+    const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group, parts = (int64_t) f.sms * A16_WARPS / ((int64_t) a.c.n_seq * a.c.n_kv);
+    if (parts > 32) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, f.stream, true, 1, a);
+    else if (parts > 8) launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, f.stream, true, 1, a);
+    else launch(k_kv4_join<HD, NT, T, 1>, dim3((unsigned) ((items + 7) / 8)), 256, 0, f.stream, true, 1, a);
 }
-template <int HD, int NT, typename T> void unit_as(const AttendArgs & a, const CUtensorMap & map, int * err, int n_ct, int cluster, int device, void * stream) {
-    static Limits set;
-    const auto kernel = k_kv16_attend_unit<HD, NT, T>;
-    allow_smem(kernel, device, set);
-    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * n_ct * cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), stream, false, cluster, a, map, err, WAIT_POLLS, n_ct);
+template <int HD, typename T> void attend_few(const AttendArgs & a, const Few & f, int cols) {
+    if (cols == 8) attend_as<HD, 1, T>(a, f);
+    else if (cols == 16) attend_as<HD, 2, T>(a, f);
+    else if (cols == 32) unit_as<HD, 2, 2, T>(a, f);
+    else unit_as<HD, 2, 4, T>(a, f);
 }
-template <typename T> void attend_few(const AttendArgs & a, const CUtensorMap & map, int * err, int head_dim, int nt, int n_ct, int cluster, int device, int sms, void * stream) {
-    const auto as = [&](auto line, auto unit) { cluster ? unit(a, map, err, n_ct, cluster, device, stream) : line(a, map, err, device, sms, stream); };
-    if (head_dim == 128) nt == 1 ? as(attend_as<128, 1, T>, unit_as<128, 1, T>) : as(attend_as<128, 2, T>, unit_as<128, 2, T>);
-    else nt == 1 ? as(attend_as<64, 1, T>, unit_as<64, 1, T>) : as(attend_as<64, 2, T>, unit_as<64, 2, T>);
-}
-// blocks of a cluster a unit where one launch does: all clusters stand on the card at once, and the longest sequence that the table (or the window) allows gives each warp at most UNIT_STEPS steps of
-// 32 tokens. 0: a line of pieces and a join. One launch / two, us with cold memory, 8 KV heads of 128: one sequence of 333 10.3 / 14.3, of 4000 (4 steps a warp) 14.4 / 18.4, of 8000 (8) 16.4 / 20.5, of
-// 20 000 (20) 26.7 / 26.7; 16 of 200 (2) 12.3 / 18.4, of 1000 (8) 20.5 / 24.6; 61 of 1004 (2 heads of 64, 8) 16.4 / 18.5
-constexpr int UNIT_STEPS = 16;
-int unit_cluster(const b200_kv4 & c, int n_ct, int window, int sinks, int sms) {
+// blocks of a cluster a unit where one launch does: all clusters stand on the card at once, and the longest sequence that the table (or the window) allows gives each warp (or group of warps) at most
+// so many steps of 32 tokens. 0: a line of pieces and a join, or tcgen05. One launch / two, us with cold memory, 8 KV heads of 128: one sequence of 333 10.3 / 14.3, of 4000 (4 steps a warp) 14.4 / 18.4, of 8000 (8) 16.4 / 20.5, of
+// 20 000 (20) 26.7 / 26.7; 16 of 200 (2) 12.3 / 18.4, of 1000 (8) 20.5 / 24.6; 61 of 1004 (2 heads of 64, 8) 16.4 / 18.5. More columns, one launch / tcgen05: one sequence of 2000, 20 columns (4 steps a group) 14.3 / 22.5, 64 (8) 20.5 / 22.5; of 500, 64 (2) 14.3 / 20.5;
+// 8 of 1000, 32 (8) 20.5 / 26.6, 64 (16) 32.8 / 26.6
+int unit_steps(int cols) { return cols <= 16 ? 16 : 8; }
+int unit_cluster(const b200_kv4 & c, int cols, int n_ct, int window, int sinks, int sms) {
     const int64_t units = (int64_t) c.n_seq * c.n_head_kv * n_ct, room = (int64_t) sms * (c.head_dim == 64 ? 2 : 1);
     int64_t tokens = (int64_t) c.max_pages * c.page_tokens;
     if (window > 0) tokens = std::min(tokens, (int64_t) window + std::min<int64_t>(sinks, tokens) + 128);
     int cluster = A16_CLUSTER;
     while (cluster > 1 && units * cluster > room) cluster /= 2;
-    return units * cluster <= room && (tokens + 31) / 32 <= (int64_t) UNIT_STEPS * A16_WARPS * cluster ? cluster : 0;
+    return cols <= 64 && units * cluster <= room && (tokens + 31) / 32 <= (int64_t) unit_steps(cols) * (cols <= 16 ? A16_WARPS : 64 / cols) * cluster ? cluster : 0;
 }
 
 template <int HD, typename T> void prompt_as(const PromptArgs & p, const CUtensorMap & map, const CUtensorMap & q_map, bool by_box, int64_t entries, int device, int sms, void * stream) {
@@ -95,9 +101,6 @@ template <int HD, typename T> void prompt_as(const PromptArgs & p, const CUtenso
     launch(kernel, dim3(sms), P16_THREADS, Prompt16Smem<HD>::BYTES, stream, true, 1, p, map, q_map, by_box);
     launch(k_kv16_prompt_join<HD, T>, dim3((unsigned) (entries * (PR_COLS / 32)), (unsigned) p.a.c.n_kv), 256, 0, stream, true, 1, p);
 }
-
-// columns of a sequence (rows x query heads of a KV head) from which tcgen05 is worth a plan and a join of its own
-bool is_prompt(int group, int max_rows) { return (int64_t) group * max_rows > 16; }
 
 void check_heads(const b200_kv4 & c, int n_head, int max_rows) {
     need(n_head >= c.n_head_kv && n_head % std::max(1, c.n_head_kv) == 0 && (int64_t) c.n_rows * n_head <= (1 << 30), "n_head is a multiple of n_head_kv, and rows x heads up to 2^30");
@@ -121,9 +124,9 @@ int64_t kv16_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
     checked(c);
     check_heads(c, n_head, max_rows);
     On on(c.device);
-    if (is_prompt(n_head / c.n_head_kv, max_rows)) return prompt_work(c, n_head / c.n_head_kv, on.sms).bytes;
-    const int nt = attend_nt(n_head / c.n_head_kv, max_rows);
-    return unit_cluster(c, attend_tiles(n_head / c.n_head_kv, max_rows, nt), 0, 0, on.sms) ? 0 : (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms);       // (a window asks for no more)
+    const int group = n_head / c.n_head_kv, cols = attend_cols(group, max_rows);
+    if (unit_cluster(c, cols, attend_tiles(group, max_rows), 0, 0, on.sms)) return 0;       // (a window asks for no more)
+    return cols > 16 ? prompt_work(c, group, on.sms).bytes : (int64_t) attend_bytes(c.n_seq, c.head_dim, cols, on.sms);
 }
 
 void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int sinks, int max_rows, void * out, void * work,
@@ -147,7 +150,9 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
     uint8_t * w = static_cast<uint8_t *>(work);
     const bool bf16 = dtype == B200_DTYPE_BF16;
     int * err = wait_word(c.device);
-    if (is_prompt(a.group, max_rows)) {
+    // up to 16 columns of a sequence (rows x query heads of a KV head) are one warp's; more are worth tcgen05's plan and join where one launch does not do
+    const int cols = attend_cols(a.group, max_rows), n_ct = attend_tiles(a.group, max_rows), cluster = unit_cluster(c, cols, n_ct, window, a.sinks, on.sms);
+    if (cols > 16 && !cluster) {
         const PromptWork at = prompt_work(c, a.group, on.sms);
         check_work(work, work_bytes, at.bytes);
         const int drill = drill_polls.load();
@@ -170,14 +175,13 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
         else c.head_dim == 128 ? as(prompt_as<128, __half>) : as(prompt_as<64, __half>);
         return;
     }
-    const CUtensorMap map = pool_map(c, bf16, 16, 2);
-    const int nt = attend_nt(a.group, max_rows);
-    const int n_ct = attend_tiles(a.group, max_rows, nt), cluster = unit_cluster(c, n_ct, window, a.sinks, on.sms);
-    if (!cluster) check_work(work, work_bytes, (int64_t) attend_bytes(c.n_seq, c.head_dim, nt, on.sms));
+    if (!cluster) check_work(work, work_bytes, (int64_t) attend_bytes(c.n_seq, c.head_dim, cols, on.sms));
     a.before = reinterpret_cast<long long *>(w);
     a.ml = reinterpret_cast<float *>(w + attend_before_bytes(c.n_seq));
-    a.part = a.ml + 2 * (size_t) on.sms * A16_WARPS * 8 * nt * 2;
-    bf16 ? attend_few<__nv_bfloat16>(a, map, err, c.head_dim, nt, n_ct, cluster, c.device, on.sms, c.stream) : attend_few<__half>(a, map, err, c.head_dim, nt, n_ct, cluster, c.device, on.sms, c.stream);
+    a.part = a.ml + attend_columns(cols, on.sms) * 2;
+    const Few f = {pool_map(c, bf16, 16, 2), err, n_ct, cluster, c.device, on.sms, c.stream};
+    if (bf16) c.head_dim == 128 ? attend_few<128, __nv_bfloat16>(a, f, cols) : attend_few<64, __nv_bfloat16>(a, f, cols);
+    else c.head_dim == 128 ? attend_few<128, __half>(a, f, cols) : attend_few<64, __half>(a, f, cols);
 }
 
 }  // namespace b200

@@ -22,7 +22,7 @@
 namespace b200 {
 namespace srv {
 
-constexpr int A16_WARPS = 4, A16_STAGES = 3, A16_STEP = 32, A16_CLUSTER = 8;
+constexpr int A16_WARPS = 4, A16_STAGES = 3, A16_STEP = 32, A16_CLUSTER = 8;      // A16_STAGES: a warp
 __host__ __device__ constexpr int a16_stage_bytes(int hd) { return A16_STEP * 4 * hd; }
 __host__ __device__ constexpr size_t a16_ring_bytes(int hd) { return (size_t) A16_WARPS * A16_STAGES * a16_stage_bytes(hd); }
 
@@ -64,12 +64,15 @@ template <typename T> __device__ __forceinline__ bool wild(uint32_t p) {
 
 // what a warp holds of a unit: its columns' sums of values, largest scores less P_LIFT and sums of weights. A lane has columns 2 tq, 2 tq + 1 of each eight and the dims 16 k + g, + 8
 template <int HD, int NT> struct Piece16 { float o[NT][HD / 16][4], m[NT][2], l[NT][2]; };
-struct Ring16 { uint32_t at, bars; int n_fill, n_use; };        // a warp's stages, and steps that were asked for and used so far: stage n % A16_STAGES, phase n / A16_STAGES
+// CW warps go over the same steps with columns of their own: one of them asks for the steps, all tell when they are done with one. Of a ring: where its stages, the barriers that tell a stage full
+// (and, where it is shared, empty) stand, and steps that were asked for and used so far: stage n % (A16_STAGES CW), phase n / (A16_STAGES CW)
+struct Ring16 { uint32_t at, full, empty; int n_fill, n_use; };
 
-// steps t0 .. t1 - 1 of the columns ct of a sequence and KV head, by one warp
-template <int HD, int NT, typename T>
-__device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtensorMap & map, const Seq & q, const Steps & sp, int ct, int head, int t0, int t1, Ring16 & ring, uint32_t polls, bool & dead,
+// steps t0 .. t1 - 1 of the columns ct (a warp's own) of a sequence and KV head
+template <int HD, int NT, int CW, typename T>
+__device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtensorMap & map, const Seq & q, const Steps & sp, int ct, int head, int t0, int t1, Ring16 & ring, bool asks, uint32_t polls, bool & dead,
                                              Piece16<HD, NT> & out) {
+    constexpr int STAGES = A16_STAGES * CW, AHEAD = CW == 1 ? STAGES - 1 : STAGES - 2;         // (of a shared ring a step less, so that the one that asks waits for nobody)
     constexpr int COLS = 8 * NT, KS = HD / 16, STAGE = a16_stage_bytes(HD), HALF = 8192;        // HALF: 64 dims of a step; of it 4096 for 16 tokens, keys and values of 2048 each
     const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
     const Cache & c = a.c;
@@ -93,6 +96,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtenso
             }
     }
     // steps on their way: A16_STAGES - 1 ahead of the one in hand. Lanes hold the next 32 pages of the slot
+    const bool idle = (int64_t) ct * COLS >= (int64_t) q.count * a.group;      // (of a shared ring: a warp without columns)
     int next = t0, pages_from = -64, my_page = -1;
     uint32_t there = 0;                                        // two bits a step that was asked for: which of its halves have a page. The newest lowest
     const auto fetch = [&]() {
@@ -102,9 +106,11 @@ __device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtenso
             if (pi < pages_from || pi_b - pages_from > 31) { pages_from = pi; my_page = page_at(c, q.slot, min(pi + lane, c.max_pages) << c.page_log2); }
             const int page_a = __shfl_sync(0xffffffffu, my_page, pi - pages_from), page_b = __shfl_sync(0xffffffffu, my_page, pi_b - pages_from);
             there |= (uint32_t) (page_a >= 0) | (uint32_t) (page_b >= 0) << 1;
-            if (lane == 0) {
-                const int stage = ring.n_fill % A16_STAGES, mask = (1 << c.page_log2) - 1;
-                const uint32_t bar = ring.bars + 8 * stage, dst = ring.at + (uint32_t) (stage * STAGE);
+            const int stage = ring.n_fill % STAGES;
+            if (CW > 1 && asks && ring.n_fill >= STAGES) mbar_wait(ring.empty + 8 * stage, (uint32_t) ((ring.n_fill / STAGES - 1) & 1), polls, dead);
+            if (asks && lane == 0 && !dead) {
+                const int mask = (1 << c.page_log2) - 1;
+                const uint32_t bar = ring.full + 8 * stage, dst = ring.at + (uint32_t) (stage * STAGE);
                 mbar_expect(bar, STAGE);
 #pragma unroll
                 for (int u = 0; u < 2; u++)
@@ -118,7 +124,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtenso
     };
     __syncwarp();                                              // nobody still reads the ring for the piece before
 #pragma unroll
-    for (int i = 0; i < A16_STAGES - 1; i++) fetch();
+    for (int i = 0; i < AHEAD; i++) fetch();
     int p_hi[NT][2];                                           // last position that the lane's two columns of S^T see; -1: no column
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -151,15 +157,21 @@ __device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtenso
     const uint32_t v_lane = (uint32_t) (2048 + ((lane & 7) + ((lane >> 4) << 3)) * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4));
 #pragma unroll 1
     for (int t = t0; t < t1; t++) {
-        const int stage = ring.n_use % A16_STAGES;
-        mbar_wait(ring.bars + 8 * stage, (uint32_t) (ring.n_use / A16_STAGES & 1), polls, dead);
+        const int stage = ring.n_use % STAGES;
+        mbar_wait(ring.full + 8 * stage, (uint32_t) (ring.n_use / STAGES & 1), polls, dead);
         ring.n_use++;
         dead = __any_sync(0xffffffffu, dead);                  // (and all lanes are done with the step before)
         if (dead) return;
         fetch();
         const uint32_t step = ring.at + (uint32_t) (stage * STAGE);
-        const uint32_t both = there >> 2 * (A16_STAGES - 1) & 3;
-        if (both == 0) continue;
+        const uint32_t both = there >> 2 * AHEAD & 3;
+        const auto leave = [&]() {
+            if (CW > 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ring.empty + 8 * stage);
+            }
+        };
+        if (both == 0 || (CW > 1 && idle)) { leave(); continue; }
         const int pos = step_at(sp, t) << 5;
         float st[2][NT][4];
 #pragma unroll
@@ -243,6 +255,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtenso
 #pragma unroll
                 for (int n = 0; n < NT; n++) { mma_of<T>(o[n][k], f, hi[u][n][0], hi[u][n][1]); mma_of<T>(o[n][k], f, lo[u][n][0], lo[u][n][1]); }
             }
+        leave();
     }
     // sums over the tokens, which lie over the lanes' g
 #pragma unroll
@@ -305,7 +318,7 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
         if (tid == 0) a.before[c.n_seq + 1] = per;
     }
     const int me = warp * (int) gridDim.x + (int) blockIdx.x;      // neighbouring pieces on different SMs
-    Ring16 ring = {smem + (uint32_t) (warp * A16_STAGES * STAGE), smem_at(&full_s[warp][0]), 0, 0};
+    Ring16 ring = {smem + (uint32_t) (warp * A16_STAGES * STAGE), smem_at(&full_s[warp][0]), 0, 0, 0};
     bool dead = false;
     long long at = me * per;
     const long long end = min(total, at + per);
@@ -320,7 +333,7 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
         at += to - from;
         if (t1 <= 0) continue;
         Piece16<HD, NT> w;
-        attend_piece<HD, NT, T>(a, map, q, sp, ct, head, t0, t1, ring, polls, dead, w);
+        attend_piece<HD, NT, 1, T>(a, map, q, sp, ct, head, t0, t1, ring, true, polls, dead, w);
         if (dead) break;
         const bool whole = t0 == 0 && t1 == sp.n;
         const size_t slot = 2 * (size_t) me + (t0 == 0 ? 1 : 0);
@@ -349,59 +362,60 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
     }
 }
 
-// Few sequences of bounded length: a cluster of blocks a unit, its warps share the unit's steps evenly and the blocks add what they have through one another's shared memory. One launch, no workspace
-template <int HD, int NT, typename T>
+// Few sequences of bounded length, up to 64 columns: with more than 16 two or four warps (CW) go over the same steps with 16 columns each, so that keys and values are read once. (In the line of pieces
+// such groups are slower than tcgen05: a step is one chain of 2200 clocks, and a block has one or two of them under way. 48 ragged sequences of 20 columns 121 us and 96, 6 long ones of 40 270 and 100.) A cluster of blocks a unit, its warps share the unit's steps evenly and the blocks add what they have through one another's shared memory. One launch, no workspace
+template <int HD, int NT, int CW, typename T>
 __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls, int n_ct) {
-    constexpr int COLS = 8 * NT, KS = HD / 16, STAGE = a16_stage_bytes(HD), PAD = HD + 4;
+    constexpr int COLS = 8 * NT, ALL = COLS * CW, KS = HD / 16, STAGE = a16_stage_bytes(HD), PAD = HD + 4, GROUPS = A16_WARPS / CW, STAGES = A16_STAGES * CW;
     extern __shared__ uint8_t a16_raw[];
-    __shared__ __align__(8) uint64_t full_s[A16_WARPS][A16_STAGES];
-    __shared__ float ml_s[A16_WARPS][COLS][2], ml_b[COLS][2];
+    __shared__ __align__(8) uint64_t full_s[GROUPS][STAGES], empty_s[GROUPS][STAGES];
+    __shared__ __align__(8) float ml_s[GROUPS][ALL][2], ml_b[ALL][2];
     namespace cg = cooperative_groups;
     cg::cluster_group cl = cg::this_cluster();
     const uint32_t smem = (smem_at(a16_raw) + 1023u) & ~1023u;
-    float * parts = reinterpret_cast<float *>(a16_raw + (smem - smem_at(a16_raw)));        // [warps][COLS][PAD], then of the block [COLS][PAD], over the ring when it is done with
-    static_assert((A16_WARPS + 1) * COLS * PAD * 4 <= a16_ring_bytes(HD), "parts stand in the ring");
-    float * sums = parts + A16_WARPS * COLS * PAD;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3, rank = (int) cl.block_rank(), blocks = (int) cl.num_blocks();
+    float * parts = reinterpret_cast<float *>(a16_raw + (smem - smem_at(a16_raw)));        // [groups][ALL][PAD], then of the block [ALL][PAD], over the ring when it is done with
+    static_assert((GROUPS + 1) * ALL * PAD * 4 <= a16_ring_bytes(HD), "parts stand in the ring");
+    float * sums = parts + GROUPS * ALL * PAD;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cw = warp % CW, group = warp / CW, g = lane >> 2, tq = lane & 3, rank = (int) cl.block_rank(), blocks = (int) cl.num_blocks();
     const Cache & c = a.c;
-    if (lane == 0) {
-        for (int i = 0; i < A16_STAGES; i++) mbar_init(smem_at(&full_s[warp][i]), 1);
+    if (lane == 0 && cw == 0) {
+        for (int i = 0; i < STAGES; i++) { mbar_init(smem_at(&full_s[group][i]), 1); mbar_init(smem_at(&empty_s[group][i]), CW); }
         mbar_init_done();
     }
-    __syncwarp();
-    Ring16 ring = {smem + (uint32_t) (warp * A16_STAGES * STAGE), smem_at(&full_s[warp][0]), 0, 0};
+    if (CW > 1) __syncthreads(); else __syncwarp();
+    Ring16 ring = {smem + (uint32_t) (group * STAGES * STAGE), smem_at(&full_s[group][0]), smem_at(&empty_s[group][0]), 0, 0};
     const int unit = (int) blockIdx.x / blocks, head = unit % c.n_kv, s = unit / c.n_kv / n_ct;
     const Seq q = seq_at(c, s);
     const Steps sp = steps_of(c, q, a.window, a.sinks, 0, q.count - 1, 5);
-    const int all_warps = blocks * A16_WARPS, me = rank * A16_WARPS + warp, per = sp.n / all_warps, more = sp.n % all_warps, t0 = me * per + min(me, more), t1 = t0 + per + (me < more);
+    const int all_groups = blocks * GROUPS, me = rank * GROUPS + group, per = sp.n / all_groups, more = sp.n % all_groups, t0 = me * per + min(me, more), t1 = t0 + per + (me < more);
     bool dead = false;
-    for (int ct = unit / c.n_kv % n_ct; ct < col_tiles(q, a.group, COLS); ct += n_ct) {        // (the same for all blocks of the cluster)
+    for (int ct = unit / c.n_kv % n_ct; ct < col_tiles(q, a.group, ALL); ct += n_ct) {        // (the same for all blocks of the cluster)
         Piece16<HD, NT> w;
-        attend_piece<HD, NT, T>(a, map, q, sp, ct, head, t0, dead ? t0 : t1, ring, polls, dead, w);
+        attend_piece<HD, NT, CW, T>(a, map, q, sp, ct * CW + cw, head, t0, dead ? t0 : t1, ring, cw == 0, polls, dead, w);
         __syncthreads();                                           // nobody reads the ring any more
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const int col = 8 * n + 2 * tq + j;
-                float * y = parts + (warp * COLS + col) * PAD + g;
+                const int col = cw * COLS + 8 * n + 2 * tq + j;
+                float * y = parts + (group * ALL + col) * PAD + g;
 #pragma unroll
                 for (int k = 0; k < KS; k++) { y[16 * k] = w.o[n][k][j]; y[16 * k + 8] = w.o[n][k][j + 2]; }
-                if (g == 0) { ml_s[warp][col][0] = w.m[n][j]; ml_s[warp][col][1] = w.l[n][j]; }
+                if (g == 0) { ml_s[group][col][0] = w.m[n][j]; ml_s[group][col][1] = w.l[n][j]; }
             }
         __syncthreads();
         // the block's sum, four dims a thread
-        for (int i = tid; i < COLS * HD / 4; i += A16_WARPS * 32) {
+        for (int i = tid; i < ALL * HD / 4; i += A16_WARPS * 32) {
             const int col = i / (HD / 4), d = i % (HD / 4) * 4;
             float top = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int v = 0; v < A16_WARPS; v++) top = fmaxf(top, ml_s[v][col][0]);
+            for (int v = 0; v < GROUPS; v++) top = fmaxf(top, ml_s[v][col][0]);
             const float base = top == -INFINITY ? 0.f : top;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int v = 0; v < A16_WARPS; v++) {
+            for (int v = 0; v < GROUPS; v++) {
                 const float by = exp2_fast(ml_s[v][col][0] - base);
-                const float4 y = *reinterpret_cast<const float4 *>(parts + (v * COLS + col) * PAD + d);
+                const float4 y = *reinterpret_cast<const float4 *>(parts + (v * ALL + col) * PAD + d);
                 l = fmaf(ml_s[v][col][1], by, l);
                 x.x = fmaf(y.x, by, x.x); x.y = fmaf(y.y, by, x.y); x.z = fmaf(y.z, by, x.z); x.w = fmaf(y.w, by, x.w);
             }
@@ -410,8 +424,8 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const At
         }
         cl.sync();
         // the blocks', a share of the results each
-        const int first = ct * COLS;
-        for (int i = rank * A16_WARPS * 32 + tid; i < COLS * HD / 4; i += blocks * A16_WARPS * 32) {
+        const int first = ct * ALL;
+        for (int i = rank * A16_WARPS * 32 + tid; i < ALL * HD / 4; i += blocks * A16_WARPS * 32) {
             const int col = i / (HD / 4), d = i % (HD / 4) * 4, r = (first + col) / a.group, h = head * a.group + first + col - r * a.group;
             if (r >= q.count) continue;
             float2 ml[A16_CLUSTER];

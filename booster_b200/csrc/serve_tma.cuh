@@ -12,6 +12,7 @@ constexpr uint32_t WAIT_POLLS = 1u << 18;     // a poll that finds nothing takes
 __device__ __forceinline__ void mbar_init(uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(n) : "memory"); }
 __device__ __forceinline__ void mbar_init_done() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
 // the phase of this parity; where it does not come within `polls` the caller is dead and waits for nothing more
 __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, uint32_t polls, bool & dead) {
     for (uint32_t spins = 0; !dead; spins++) {
