@@ -182,15 +182,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     const int k_all = a.top_k ? a.top_k[row] : 0, k = k_all > 0 && k_all < a.n_vocab ? k_all : 0;
     const bool by_p = top_p < 1.f, cut = temperature > 0.f && (k > 0 || by_p);
     int draft = -1;                                                      // -1: none is checked here
-    if constexpr (VERIFY) {
-        const int s = row_sequence(a.first, a.n_seq, row);
-        if (s < 0) {
-            if (rank == 0 && tid == 0) { a.ids[row] = -1; a.logprobs[row] = 0.f; }
-            return;
-        }
-        if (row + 1 < min(a.first[s + 1], a.n_rows)) { draft = a.step_ids[row + 1]; if ((unsigned) draft >= (unsigned) a.n_vocab) draft = -2; }
-    }
-    const float * q_row = VERIFY && a.probs && draft != -1 ? a.probs + row * a.probs_stride : nullptr;
+    bool homeless = false;                                               // a row of no sequence
+    const float * q_row = nullptr;
+    if (VERIFY) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const auto q_at = [&](int i) { const float q = q_row[i]; return q > 0.f ? (double) q : 0.0; };
     // whether the draft, of weight t, is taken; what is left of a weight for the draw where it is not
     const auto takes = [&](u64 t, u64 total) { return draft >= 0 && (double) a.accept[row] * (q_row ? q_at(draft) : 1.0) * (double) total < (double) t; };
@@ -211,16 +205,30 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     {
         const T * src = static_cast<const T *>(a.logits) + row * a.row_stride + base;
         constexpr int E = 16 / sizeof(T);
-        for (int i = tid; i < SA_BINS; i += SA_THREADS) bins[i] = 0;
-        if (tid < 16) sm.table[tid] = exp2((double) tid / 16.0);
-        if (tid == 0) sm.n_list = 0;
+        const auto meanwhile = [&]() {                                   // what does not depend on the logits, while the first of them are on their way
+            for (int i = tid; i < SA_BINS; i += SA_THREADS) bins[i] = 0;
+            if (tid < 16) sm.table[tid] = exp2((double) tid / 16.0);
+            if (tid == 0) sm.n_list = 0;
+            if constexpr (VERIFY) {
+                const int s = row_sequence(a.first, a.n_seq, row);
+                homeless = s < 0;
+                if (s >= 0 && row + 1 < min(a.first[s + 1], a.n_rows)) {
+                    draft = a.step_ids[row + 1];
+                    if ((unsigned) draft >= (unsigned) a.n_vocab) draft = -2;
+                    if (a.probs) q_row = a.probs + row * a.probs_stride;
+                }
+            }
+        };
         int done = 0;
+        bool first_time = true;
         if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
             done = n / E * E;
-            for (int i0 = tid * E; i0 < done; i0 += 8 * SA_THREADS * E) {
+            for (int i0 = tid * E; __any_sync(0xffffffffu, i0 < done); i0 += 8 * SA_THREADS * E) {
                 uint4 x[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) { const int i = i0 + j * SA_THREADS * E; if (i < done) x[j] = *reinterpret_cast<const uint4 *>(src + i); }
+                if (first_time) meanwhile();
+                first_time = false;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int i = i0 + j * SA_THREADS * E;
@@ -235,7 +243,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                 }
             }
         }
+        if (first_time) meanwhile();
         for (int i = done + tid; i < 4 * groups; i += SA_THREADS) { const T x = i < n ? src[i] : from_f<T>(-INFINITY); vals[i] = x; top = fmaxf(top, to_f(x)); }
+    }
+    if (VERIFY && homeless) {                                            // (the whole cluster)
+        if (rank == 0 && tid == 0) { a.ids[row] = -1; a.logprobs[row] = 0.f; }
+        return;
     }
     top = key_logit(warp_reduce(order_key(top, 0), [](u64 x, u64 y) { return max(x, y); }));
     if (lane == 0) sm.red[warp] = __float_as_uint(top);

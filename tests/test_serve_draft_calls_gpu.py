@@ -1,0 +1,361 @@
+"""Calls of the operators around drafted tokens and the 16-bit cache that a program makes in earnest: captured, on streams, from threads, one behind the other, and all of them together."""
+import ctypes as C
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from booster_b200 import _lib, serve
+from tests import serve_draft_oracle as oracle
+from tests.test_serve_calls_gpu import alone
+from tests.test_serve_draft_gpu import BF16, F16, Case, assert_attends, assert_verifies, ints, step as rows_to_verify
+
+pytestmark = pytest.mark.gpu
+
+# (held, counts, query heads, KV heads, wide table): few rows in one launch, with warps that share what is read, in a line of pieces, and rows for tcgen05
+FORMS = {"unit": ([300, 5, 40], [1, 1, 1], 8, 2, False), "shared": ([300, 5, 40], [5, 2, 7], 8, 2, False), "line": ([3000, 5, 400], [1, 2, 1], 8, 2, True), "rows": ([300, 0, 77], [200, 65, 3], 8, 2, False)}
+
+
+def made(form, hd=64, seed=0, dtype=BF16):
+    held, counts, heads, kv, wide = FORMS[form]
+    c = Case(held, counts, page=16, kv=kv, hd=hd, seed=seed, dtype=dtype)
+    if wide:
+        c.widened()
+    c.fill()
+    return c, c.randn(c.rows, heads, hd).to(dtype)
+
+
+def test_first_calls_inside_a_capture():
+    """every operator for the first time in its process while a graph is captured; the graph then gives what calls give"""
+    alone("""
+import torch
+from booster_b200 import serve
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+gen = torch.Generator(device="cuda").manual_seed(0)
+page = 16
+table, held, refs, counts = torch.full((8, 6), -1, dtype=torch.int32, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda"), torch.zeros(400, dtype=torch.int32, device="cuda"), ints([20, 1, 39])
+wide = torch.full((8, 4000), -1, dtype=torch.int32, device="cuda")
+pool = serve.kv16_pool(400, page, 2, 64, 2)
+k, v, q = (torch.randn(62, h, 64, generator=gen, device="cuda").bfloat16() for h in (2, 2, 8))
+logits, u, accept, ids = torch.randn(62, 5000, generator=gen, device="cuda"), torch.rand(62, generator=gen, device="cuda"), torch.rand(62, generator=gen, device="cuda"), ints(list(range(62)))
+probs, ks, slots = torch.softmax(logits + 1, 1), ints([5] * 30 + [0] * 32), ints([0, 1, 2])
+def step():
+    out = list(serve.pages_plan(table, held, refs, counts, page, 62))
+    first = out[0]
+    for layer in pool:
+        serve.kv16_append(layer, table, held, first, k, v)
+        out += [serve.kv16_attention(q, layer, table, held, first, max_rows=m, window=w, sinks=3) for m in (1, 5, 12, 4096) for w in (0, 9)]
+        wide[:, :6] = table
+        out += [serve.kv16_attention(q, layer, wide, held, first, max_rows=m) for m in (1, 4, 12)]
+    new = serve.verify(logits, ids, first, u, accept, top_k=ks, draft_probs=probs)
+    out += new
+    held[:3] += new[0]
+    serve.pages_trim(table, held, refs, page, slots, 20, 2)
+    return out
+state = (table, held, refs, pool, wide)
+start = [x.clone() for x in state]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = step()
+for x, y in zip(state, start): assert torch.equal(x, y)
+graph.replay()
+torch.cuda.synchronize()
+ends = [x.clone() for x in state]
+for x, y in zip(state, start): x.copy_(y)
+eager = step()
+for x, y in zip(state, ends): assert torch.equal(x, y)
+for x, y in zip(outs, eager): assert torch.equal(x[:60], y[:60])
+assert outs[3].item() == 0 and outs[0].tolist() == [0, 20, 21, 60] and refs.sum().item() > 0
+print("done")
+""")
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_graphs_streams_and_order(form):
+    """captured and replayed with other lengths and queries; two graphs in one pool of memory; another stream; the same call twice gives the same bits"""
+    c, q = made(form)
+    out = torch.zeros_like(q)
+    table, held = c.table, c.held.clone()
+    call = lambda: serve.kv16_attention(q, c.pool[0], table, held, c.first, c.slots, window=100, sinks=7, out=out)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    with torch.cuda.graph(graphs[0]):
+        call()
+    with torch.cuda.graph(graphs[1], pool=graphs[0].pool()):
+        call()
+    for turn in range(4):
+        held.copy_(c.held - turn * (c.held > 10).int())
+        q.copy_(c.randn(*q.shape))
+        c2 = Case.__new__(Case)
+        c2.__dict__.update(c.__dict__)
+        c2.held_l = [held[s].item() for s in c.slots_l]
+        out.zero_()
+        graphs[turn % 2].replay()
+        got = out.clone()
+        assert_attends(c2, q, got, 100, 7)
+        assert torch.equal(call(), got)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = serve.kv16_attention(q, c.pool[0], table, held, c.first, c.slots, window=100, sinks=7)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(again, got)
+
+
+def test_captured_steps_of_tables_and_verification():
+    """a graph of the step's small operators, replayed with other numbers in its inputs"""
+    page, n = 16, 5
+    logits, ids, first, u, accept, filters, probs = rows_to_verify(3, 900, [3, 1, 4, 2, 5], BF16, [dict(temperature=0.7, top_k=40), dict(top_p=0.8), dict()], True)
+    table, held, refs = ints([[-1] * 30] * n), ints([0] * n), ints([0] * 90)
+    counts, slots, ids_t = ints([3, 1, 4, 2, 5]), ints([4, 2, 0, 1, 3]), ints(ids)
+    state = [table, held, refs]
+
+    def step():
+        plan = serve.pages_plan(table, held, refs, counts, page, 15, slots)
+        new = serve.verify(logits, ids_t, plan[0], u, accept, draft_probs=probs)
+        held.index_add_(0, slots.long(), new[0])
+        serve.pages_trim(table, held, refs, page, slots, 33, 5)
+        return [*plan, *new]
+    step()
+    for x, v in zip(state, (-1, 0, 0)):
+        x.fill_(v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    for turn in range(40):
+        counts.copy_(ints([[3, 1, 4, 2, 5], [5, 5, 5, 0, 0], [1, 1, 1, 1, 1]][turn % 3]))
+        u.copy_(torch.rand(15, generator=gen, device="cuda"))
+        accept.copy_(torch.rand(15, generator=gen, device="cuda"))
+        before = [x.clone() for x in state]
+        graph.replay()
+        got, after = [x.clone() for x in outs], [x.clone() for x in state]
+        for x, y in zip(state, before):
+            x.copy_(y)
+        want = step()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(torch.equal(x, y) for x, y in zip(state, after))
+        used = [p for row in table.tolist() for p in row if p >= 0]
+        assert len(used) == len(set(used)) == int(refs.sum()) and got[3].item() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_calls_one_behind_the_other_repeat_themselves(hd, dtype):
+    """blocks of one call begin where those of another have just ended, with barriers and tiles in the same shared memory: every call gives the bits that it gave alone"""
+    calls = []
+    for i, form in enumerate(FORMS):
+        c, q = made(form, hd, i, dtype)
+        calls.append(lambda c=c, q=q, t=c.table: serve.kv16_attention(q, c.pool[0], t, c.held, c.first, c.slots))
+        c4 = serve.kv4_pool(c.pages, 16, 2, hd)
+        calls.append(lambda c=c, q=q, t=c.table, p=c4: serve.kv4_attention(q, p[0], t, c.held, c.first, c.slots))
+    first = []
+    for call in calls:
+        torch.cuda.synchronize()
+        first.append(call())
+        torch.cuda.synchronize()
+    outs = [[call() for call in calls] for _ in range(60)]
+    for out in outs:
+        assert all(torch.equal(x, y) for x, y in zip(out, first))
+
+
+def test_two_streams_at_once():
+    """calls of all forms on two streams, their kernels side by side on the card: nothing is shared but the pools, which are read"""
+    pairs = [made(form, 128, i) for i, form in enumerate(FORMS)]
+    call = lambda c, q, t: serve.kv16_attention(q, c.pool[0], t, c.held, c.first, c.slots)  # noqa: E731
+    tables = [c.table for c, _ in pairs]
+    want = [call(c, q, t) for (c, q), t in zip(pairs, tables)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for turn in range(30):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                k = (turn + i) % len(pairs)
+                got[i].append((k, call(*pairs[k], tables[k])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[k]) for g in got for k, x in g)
+
+
+def test_threads_with_calls_of_different_sizes():
+    """host threads whose calls ask for different forms and sizes at the same time, for the first time in their process"""
+    alone("""
+import threading, torch
+from booster_b200 import serve
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+pool = serve.kv16_pool(40, 16, 2, 64)
+pool.normal_()
+table = torch.arange(40, dtype=torch.int32, device="cuda").reshape(2, 20)
+held = ints([100, 37])
+logits = torch.randn(64, 3000, device="cuda")
+jobs = []
+for rows in (1, 2, 5, 30, 100):
+    q, first = torch.randn(2 * rows, 8, 64, device="cuda").bfloat16(), ints([0, rows, 2 * rows])
+    jobs.append(lambda q=q, first=first, rows=rows: serve.kv16_attention(q, pool[0], table, held, first, max_rows=rows))
+    n = min(64, 2 * rows)
+    jobs.append(lambda n=n: serve.verify(logits[:n], ints(list(range(n))), ints([0, n]), torch.full((n,), 0.3, device="cuda"), torch.full((n,), 0.6, device="cuda"))[1])
+bad, outs = [], [[], []]
+gate = threading.Barrier(2)
+def run(me):
+    try:
+        s = torch.cuda.Stream()
+        gate.wait()
+        with torch.cuda.stream(s):
+            for turn in range(20):
+                for i in range(len(jobs)): outs[me].append((i if not me else len(jobs) - 1 - i, jobs[i if not me else len(jobs) - 1 - i]()))
+        s.synchronize()
+    except Exception as e:
+        bad.append(e)
+torch.cuda.synchronize()
+threads = [threading.Thread(target=run, args=(m,)) for m in (0, 1)]
+[t.start() for t in threads]; [t.join() for t in threads]
+torch.cuda.synchronize()
+assert not bad, bad
+want = [j() for j in jobs]
+assert all(torch.equal(x, want[i]) for o in outs for i, x in o)
+print("done")
+""")
+
+
+def test_a_workspace_is_its_owner_s_again_behind_the_call():
+    """also where the step's rows belong to no sequence; one that is too small or off its alignment is refused, and none is needed where one launch does"""
+    L = _lib.lib()
+    for heads, kv, max_rows, max_pages, n in ((8, 2, 1, 60000, 4096), (64, 2, 1, 60000, 4096), (8, 2, 500, 2, 300), (8, 2, 1, 2, 2)):
+        pool, table, held = serve.kv16_pool(1, 16, kv, 64, dtype=F16)[0], torch.zeros(1, max_pages, dtype=torch.int32, device="cuda").expand(n, -1), ints([0] * n)
+        rows = 5
+        q, out = torch.randn(rows, heads, 64, device="cuda").half(), torch.full((rows, heads, 64), 7.0, dtype=F16, device="cuda")
+        slots, first = ints([0] * n), ints([0] * (n + 1))
+        c = _lib.Kv4(device=0, n_pages=1, page_tokens=16, n_head_kv=kv, head_dim=64, n_slots=1, max_pages=max_pages, n_seq=n, n_rows=rows, stream=torch.cuda.current_stream().cuda_stream,
+                     pool=pool.data_ptr(), page_stride=2 * kv * 16 * 64 * 2, table_stride=max_pages, table=table.data_ptr(), held=held.data_ptr(), slots=slots.data_ptr(), first=first.data_ptr())
+        size = L.b200_kv16_attention_workspace(C.byref(c), heads, max_rows)
+        assert (size == 0) == (n == 2)
+        work = torch.empty(size + 32, dtype=torch.uint8, device="cuda")
+        attend = lambda at, bytes_: L.b200_kv16_attention(C.byref(c), 2, q.data_ptr(), heads * 64, 64, heads, 1.0, 0, 0, max_rows, out.data_ptr(), at, bytes_)  # noqa: E731
+        for _ in range(20):
+            assert attend(work.data_ptr() if size else None, size) == 0, _lib.last_error()
+            work.fill_(0x55)
+            assert (work == 0x55).all()
+        assert (out == 7).all()
+        if size:
+            assert attend(work.data_ptr(), size - 1) and "workspace" in _lib.last_error()
+            assert attend(work.data_ptr() + 8, size) and "16 bytes" in _lib.last_error()
+            assert attend(None, size) and "workspace" in _lib.last_error()
+
+
+@pytest.mark.parametrize("group", [4, 5])
+def test_a_wait_that_runs_out_is_told(group):
+    """queries that never come, as boxes or gathered by warps: the kernel gives up, frees what it holds and says so, whichever call comes next; after it all is as before"""
+    L = _lib.lib()
+    c = Case([300, 5], [64, 1], kv=2, hd=128, dtype=BF16)
+    c.fill()
+    q = c.randn(c.rows, 2 * group, 128).bfloat16()
+    attend = lambda most=64: serve.kv16_attention(q, *c.args(), slots=c.slots, max_rows=most)  # noqa: E731
+    right, few = attend(), attend(1)
+    k = c.randn(c.rows, 2, 128).bfloat16()
+    refs, pool = torch.ones(c.pages, dtype=torch.int32, device="cuda"), c.pool.clone()
+    one = torch.zeros(1, device="cuda")
+    calls = [lambda: serve.kv16_append(*c.args(), k, k, c.slots), attend, lambda: attend(1), lambda: serve.pages_plan(c.table, c.held, refs, ints([1]), 16, 1, c.slots[:1]),
+             lambda: serve.pages_trim(c.table, c.held, refs, 16, c.slots), lambda: serve.verify(torch.zeros(1, 10, device="cuda"), ints([0]), ints([0, 1]), one, one), serve.kv4_status]
+    try:
+        for call in calls:
+            L.b200_kv4_drill(64)
+            attend()
+            L.b200_kv4_drill(0)
+            torch.cuda.synchronize()
+            with pytest.raises(_lib.B200Error, match="ran out"):
+                call()
+            assert torch.equal(c.pool, pool)
+            serve.kv4_status()
+            assert torch.equal(attend(), right) and torch.equal(attend(1), few)
+    finally:
+        L.b200_kv4_drill(0)
+
+
+def test_a_server_that_drafts_ahead():
+    """prompts, then tokens with drafts under a window with sinks, two answers to one prompt, conversations that end, pages moved between: the tokens of greedy requests are those that one token at a
+    time would give, what each slot sees is what its own tokens say, and all pages come back"""
+    heads, kv, hd, page, vocab, slots, window, sinks = 8, 2, 64, 16, 200, 5, 40, 5
+    r = random.Random(7)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    embed = torch.randn(vocab, (heads + 2 * kv) * hd, generator=gen, device="cuda").bfloat16()
+    wq = torch.randn(heads * hd, vocab, generator=gen, device="cuda")
+    pool = serve.kv16_pool(80, page, kv, hd)
+    table, held, refs = ints([[-1] * 40] * slots), ints([0] * slots), ints([0] * 80)
+    said = {s: [] for s in range(slots)}                                # tokens that are certain, the last of them not in the cache yet
+
+    def truth(tokens):
+        """logits behind the last of `tokens`, in 64 bits, and how far off the step's may be"""
+        row = embed[torch.tensor(tokens, device="cuda")].view(len(tokens), -1, hd).double().cpu().numpy()
+        K, V = (row[:, heads + i * kv:heads + (i + 1) * kv].transpose(1, 0, 2) for i in (0, 1))
+        o, e = oracle.attention(row[-1:, :heads], [(K, V, np.ones(len(tokens), bool))], [len(tokens) - 1], [0, 1], window, sinks, hd ** -0.5, 2.0 ** -7)
+        e = e + 2.0 ** -8 * (np.abs(o) + e)
+        w = wq.double().cpu().numpy()
+        return o.reshape(-1) @ w, e.reshape(-1) @ np.abs(w) + 1e-4
+
+    def advance(new):
+        ids, counts = list(new), [len(t) for t in new.values()]
+        on, tokens = ints(ids), torch.tensor(sum(new.values(), []), device="cuda", dtype=torch.int32)
+        first, positions, places, status = serve.pages_plan(table, held, refs, ints(counts), page, len(tokens), on)
+        assert status.item() == 0
+        row = embed[tokens.long()].view(len(tokens), -1, hd)
+        serve.kv16_append(pool[0], table, held, first, row[:, heads:heads + kv], row[:, heads + kv:], on)
+        assert torch.equal(pool[0, places // page, 0, :, places % page], row[:, heads:heads + kv])
+        x = serve.kv16_attention(row[:, :heads], pool[0], table, held, first, on, window=window, sinks=sinks, max_rows=max(counts))
+        return on, tokens, first, x.flatten(1).float() @ wq
+
+    for s, n in ((0, 57), (2, 30), (4, 3)):
+        said[s] = [r.randrange(vocab) for _ in range(n)]
+    on, tokens, first, logits = advance({s: said[s] for s in (0, 2, 4)})
+    held[on.long()] += first.diff()
+    for s, t in zip((0, 2, 4), logits[first[1:].long() - 1].argmax(1).tolist()):
+        said[s].append(t)
+    taken = 0
+    for turn in range(30):
+        live = [s for s in range(slots) if said[s]]
+        new = {}
+        for s in live:                                                  # what the likeliest following tokens are, sometimes another
+            drafts = []
+            for _ in range(r.randrange(0, 5)):
+                best, _ = truth((said[s] + drafts)[-400:] if len(said[s]) < 400 else said[s] + drafts)
+                drafts.append(int(np.argmax(best)) if r.random() < 0.7 else r.randrange(vocab))
+            new[s] = [said[s][-1]] + drafts
+        on, tokens, first, logits = advance(new)
+        zeros = torch.zeros(len(tokens), device="cuda")
+        u = torch.rand(len(tokens), generator=gen, device="cuda")
+        gained, out, _ = serve.verify(logits, tokens, first, u, u, temperature=zeros)
+        for i, s in enumerate(live):
+            a, n = int(first[i]), int(gained[i])
+            got = out[a:a + n].tolist()
+            assert (out[a + n:int(first[i + 1])] == -1).all()
+            for t in got:
+                best, room = truth(said[s])
+                assert best[t] + room[t] >= (best - room).max(), (turn, s)                # the largest, as far as roundings tell
+                said[s].append(t)
+            assert got[:-1] == new[s][1:n]
+            taken += n - 1
+        held.index_add_(0, on.long(), gained)
+        serve.pages_trim(table, held, refs, page, on, window, sinks)
+        assert all(held[s].item() == len(said[s]) - 1 for s in live)
+        for s in live:                                                  # no more pages than the window, the sinks and their edges need
+            assert int((table[s] >= 0).sum()) <= window // page + 2 + 1
+        if turn == 0:                                                   # two answers to one prompt, as long as its first pages are there
+            assert serve.pages_fork(pool, table, held, refs, ints([4]), ints([1])).item() == 0
+            said[1] = list(said[4])
+        if turn in (9, 20):
+            gone = {9: 2, 20: 1}[turn]
+            serve.pages_free(table, held, refs, ints([gone]))
+            said[gone] = []
+            n = serve.pages_compact(pool, table, refs).item()
+            assert n == int((refs > 0).sum()) and not refs[n:].any()
+    assert taken > 30
+    serve.pages_free(table, held, refs, ints(list(range(slots))))
+    assert not refs.any() and (table == -1).all() and not held.any()
+
+
+def test_a_wide_vocabulary_of_drafts():
+    """2^18 logits, as many parts and as long slices as there are, with a drafter's distribution or without"""
+    for drafter in (False, True):
+        for kinds in ([dict()], [dict(top_k=50)], [dict(top_p=0.9)], [dict(top_k=5000, top_p=0.99, temperature=2.0)]):
+            assert_verifies(*rows_to_verify(5, 1 << 18, [3, 2], BF16, kinds, drafter))
