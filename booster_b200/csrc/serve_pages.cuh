@@ -394,11 +394,12 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_fork(const Pages p, const 
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (!refused) {
-        for (int s = warp; s < n; s += PG_THREADS / 32) {          // a child is no parent, a parent's pages are the pool's and held
+        for (int s = warp; s < n; s += PG_THREADS / 32) {          // a child is no parent, a parent's pages are the pool's and held, or absent
             const int a = parents[s], used = (p.held[a] + P - 1) >> p.page_log2;
             if (taken[a >> 5] >> (a & 31) & 1) bad = 1;
             for (int i = lane; i < used; i += 32) {
                 const int page = p.table[(int64_t) a * p.table_stride + i];
+                if (page < 0 && i < p.held[a] >> p.page_log2) continue;      // a full page that k_pages_trim gave back: the child goes without it too
                 if ((unsigned) page >= (unsigned) p.n_pages || p.refs[page] <= 0) bad = 1;
             }
         }
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_fork(const Pages p, const 
         int32_t * mine_row = p.table + (int64_t) c * p.table_stride;
         for (int i = lane; i < p.max_pages; i += 32) {
             int page = -1;
-            if (i < full) { page = row[i]; atomicAdd(&p.refs[page], 1); }
+            if (i < full) { page = row[i]; if (page >= 0) atomicAdd(&p.refs[page], 1); }
             else if (i == full && (p.held[a] & (P - 1))) page = to[before[s]];
             mine_row[i] = page;
         }

@@ -120,13 +120,12 @@ def pages_plan(table: torch.Tensor, held: torch.Tensor, refs: torch.Tensor, coun
 
 
 def pages_trim(table: torch.Tensor, held: torch.Tensor, refs: torch.Tensor, page_tokens: int, slots: torch.Tensor, window: int = 0, sinks: int = 0) -> None:
-    """the slots give back the pages that no row to come sees: those behind their held tokens, and with window > 0 those in front of what the next row sees but for the first `sinks` tokens (a slot
-    without its first pages cannot be forked)"""
+    """the slots give back the pages that no row to come sees: those behind their held tokens, and with window > 0 those in front of what the next row sees but for the first `sinks` tokens"""
     _native().pages_trim(table, held, refs, page_tokens, slots, window, sinks)
 
 
 def pages_fork(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, children: torch.Tensor) -> torch.Tensor:
-    """slot children[i], which is empty, becomes what slot parents[i] is: full pages are shared, a last page that is part full is copied in every layer. Returns the status, see pages_reserve"""
+    """slot children[i], which is empty, becomes what slot parents[i] is: full pages are shared (those that pages_trim gave back neither has), a last page that is part full is copied in every layer. Returns the status, see pages_reserve"""
     return _native().pages_fork(pool, table, held, refs, parents, children)
 
 

@@ -416,9 +416,10 @@ int b200_pages_reserve(const b200_pages * p, const int32_t * slots, const int32_
  * written in any case, first n_rows at most. */
 int b200_pages_plan(const b200_pages * p, const int32_t * slots, const int32_t * counts, int n, int n_rows, int32_t * first, int32_t * positions, int32_t * places, int32_t * status);
 /* pages of the slots that no row to come sees go back: those behind the held tokens (the program has lowered held behind rows that were refused) and, with window > 0, those whose tokens all stand
- * in front of the last window - 1 of the held ones and behind the first sinks. A slot without its first pages cannot be forked */
+ * in front of the last window - 1 of the held ones and behind the first sinks */
 int b200_pages_trim(const b200_pages * p, const int32_t * slots, int n, int window, int sinks);
-/* slot children[i], which is empty, becomes what slot parents[i] is: full pages are shared, the tokens of the last page are copied in every layer when it is part full */
+/* slot children[i], which is empty, becomes what slot parents[i] is: full pages are shared (those that b200_pages_trim gave back neither has), the tokens of the last page are copied in every layer
+ * when it is part full */
 int b200_pages_fork(const b200_pages * p, const int32_t * parents, const int32_t * children, int n, int32_t * status, void * work, int64_t work_bytes);
 /* the slots give their pages back and are empty */
 int b200_pages_free(const b200_pages * p, const int32_t * slots, int n);

@@ -305,7 +305,7 @@ def test_a_server_that_drafts_ahead():
         x = serve.kv16_attention(row[:, :heads], pool[0], table, held, first, on, window=window, sinks=sinks, max_rows=max(counts))
         return on, tokens, first, x.flatten(1).float() @ wq
 
-    for s, n in ((0, 57), (2, 30), (4, 3)):
+    for s, n in ((0, 80), (2, 30), (4, 3)):
         said[s] = [r.randrange(vocab) for _ in range(n)]
     on, tokens, first, logits = advance({s: said[s] for s in (0, 2, 4)})
     held[on.long()] += first.diff()
@@ -340,9 +340,9 @@ def test_a_server_that_drafts_ahead():
         assert all(held[s].item() == len(said[s]) - 1 for s in live)
         for s in live:                                                  # no more pages than the window, the sinks and their edges need
             assert int((table[s] >= 0).sum()) <= window // page + 2 + 1
-        if turn == 0:                                                   # two answers to one prompt, as long as its first pages are there
-            assert serve.pages_fork(pool, table, held, refs, ints([4]), ints([1])).item() == 0
-            said[1] = list(said[4])
+        if turn == 2:                                                   # two answers to one conversation, whose first pages are away
+            assert (table[0, 1:2] == -1).all() and serve.pages_fork(pool, table, held, refs, ints([0]), ints([1])).item() == 0
+            said[1] = list(said[0])
         if turn in (9, 20):
             gone = {9: 2, 20: 1}[turn]
             serve.pages_free(table, held, refs, ints([gone]))

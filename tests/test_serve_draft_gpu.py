@@ -488,6 +488,22 @@ def test_trim(seed, window, sinks):
     assert table.tolist() == t and refs.tolist() == f and held.tolist() == h
 
 
+def test_slots_without_their_first_pages_fork():
+    table, held, refs = ints([[9, -1, -1, 3, 4, -1], [-1] * 6, [-1, 5, -1, -1, -1, -1], [-1] * 6, [7, -1, -1, -1, -1, -1]]), ints([70, 0, 32, 0, 20]), ints([0, 0, 0, 1, 1, 1, 0, 1, 0, 1])
+    pool = serve.kv16_pool(10, 16, 1, 64)
+    pool.copy_(torch.randn(pool.shape, device="cuda"))
+    want = pool.clone()
+    assert serve.pages_fork(pool, table, held, refs, ints([0, 2]), ints([1, 3])).item() == 0
+    want[:, 0] = want[:, 4]                                             # the part-full page's one tile of 16 tokens is a whole page here
+    assert torch.equal(pool, want) and held.tolist() == [70, 70, 32, 32, 20]
+    assert table.tolist() == [[9, -1, -1, 3, 4, -1], [9, -1, -1, 3, 0, -1], [-1, 5, -1, -1, -1, -1], [-1, 5, -1, -1, -1, -1], [7, -1, -1, -1, -1, -1]]
+    assert refs.tolist() == [1, 0, 0, 2, 1, 2, 0, 1, 0, 2]
+    before = [x.clone() for x in (table, held, refs)]
+    serve.pages_free(table, held, refs, ints([1]))
+    assert serve.pages_fork(pool, table, held, refs, ints([4]), ints([1])).item() == -1          # its last page, which is part full, is away
+    assert table[1].tolist() == [-1] * 6 and torch.equal(table[[0, 2, 3, 4]], before[0][[0, 2, 3, 4]]) and torch.equal(pool, want)
+
+
 def test_trim_of_odd_entries():
     table, held, refs = ints([[5, 99, -7, 2], [2, 3, -1, -1]]), ints([-4, 2 ** 31 - 1]), ints([0, 0, 2, 1, 0, 1])
     serve.pages_trim(table, held, refs, 16, ints([0, 1]))
