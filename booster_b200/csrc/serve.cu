@@ -93,7 +93,7 @@ void move_pages(const b200_pages & p, const Pages & d, const int32_t * plan, int
     launch(k_pages_move, dim3(sms * 4), 256, 0, p.stream, true, 1, d, plan, n, parts, moved_to);
 }
 
-template <typename T, bool VERIFY> void sample_as(const SampleArgs & a, int cluster, int device, void * stream) {
+template <typename T, bool VERIFY> void sample_as(const std::conditional_t<VERIFY, VerifyArgs, SampleArgs> & a, int cluster, int device, void * stream) {
     static Limits set;
     const size_t smem = SA_FIXED + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
     const auto kernel = k_sample<T, VERIFY>;
@@ -101,7 +101,7 @@ template <typename T, bool VERIFY> void sample_as(const SampleArgs & a, int clus
     launch(kernel, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, false, cluster, a);
 }
 
-template <bool VERIFY> void sample_all(SampleArgs & a, int dtype, const On & on, void * stream) {
+template <bool VERIFY, typename A> void sample_all(A & a, int dtype, const On & on, void * stream) {
     // slices of 64 KB at most, so that two blocks share an SM; smaller ones while rows leave SMs without a block and a slice has work for its threads. Mixed rows, us: 16 of 128 256 logits
     // by 8 blocks 32, by 4 48; 48 of them 45 and 56; 32 of 32 000 by 4 23, by 2 29; one of 4000 by one block 7.3, by two 7.8
     int cluster = 1;
@@ -323,7 +323,7 @@ void verify_rows(int device, void * stream, int dtype, const void * logits, int6
     need(n_rows == 0 || (logits && ids && u && accept && tokens && logprobs && aligned(logits, size_of(dtype))), "verify: null pointer");
     On on(device);
     heed_waits(device);
-    SampleArgs a = {logits, row_stride, n_rows, n_vocab, 0, u, temperature, top_p, min_p, top_k, tokens, logprobs, ids, first, n_seq, accept, draft_probs, draft_stride, gained};
+    VerifyArgs a = {{logits, row_stride, n_rows, n_vocab, 0, u, temperature, top_p, min_p, top_k, tokens, logprobs}, ids, first, n_seq, accept, draft_probs, draft_stride, gained};
     if (n_rows) sample_all<true>(a, dtype, on, stream);
     if (n_seq) launch(k_verify_ends<128>, dim3((unsigned) ((n_seq + 3) / 4)), 128, 0, stream, true, 1, a);
 }

@@ -17,6 +17,7 @@
 #pragma once
 #include "serve_cache.cuh"
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace b200 {
 namespace srv {
@@ -36,7 +37,8 @@ struct SampleArgs {
     const int32_t * top_k;
     int32_t * ids;
     float * logprobs;
-    // verification of drafted tokens (k_sample<T, true>)
+};
+struct VerifyArgs : SampleArgs {         // of k_sample<T, true>
     const int32_t * step_ids, * first;   // the step's input tokens; sequence i has the rows first[i] .. first[i + 1] - 1
     int n_seq;
     const float * accept, * probs;       // probs: what the drafter drew from, [n_rows] rows probs_stride apart, or NULL: it was sure of its token
@@ -96,12 +98,13 @@ __device__ __forceinline__ u64 warp_sum(u64 x) {
 }
 struct alignas(128) SampleSmem {
     double table[16];
-    u64 red[SA_WARPS], each[SA_MAX_CLUSTER], rest[SA_MAX_CLUSTER], draft[SA_MAX_CLUSTER], turn[2][SA_MAX_CLUSTER], sums[SA_MAX_CLUSTER][2];
+    u64 red[SA_WARPS], each[SA_MAX_CLUSTER], turn[2][SA_MAX_CLUSTER], sums[SA_MAX_CLUSTER][2];
     u64 answer[4];
     u64 parts[SA_SWEEPS][SA_WARPS];
     float top;                           // the block's largest, and its place among the bins
     int place, n_list;
 };
+struct alignas(128) VerifySmem { u64 rest[SA_MAX_CLUSTER], draft[SA_MAX_CLUSTER]; };
 // dynamic shared memory: the list, fine sums, fine counts, bins, the slice
 constexpr int SA_FIXED = 8 * SA_LIST + 12 * SA_FINE + 4 * SA_BINS;
 // a number of every thread of the cluster, joined; all threads get it
@@ -168,9 +171,10 @@ __device__ __forceinline__ float place_from(int p) { return p <= (int) (-SA_FAR 
 // where accept q(x) < p(x); where it is not, a token is drawn from max(p - q, 0) (p, where that is nothing) by u as always. So what comes out has the distribution p whatever the drafter is.
 // p = t / total and r = max(t - rint(q total), 0) are whole multiples of 2^-40 too. ids[row]: the draft that was taken, or -2 - token of one that was drawn, for k_verify_ends.
 template <typename T, bool VERIFY>
-__global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
+__global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional_t<VERIFY, VerifyArgs, SampleArgs> a) {
     extern __shared__ __align__(16) uint8_t sa_raw[];
     __shared__ SampleSmem sm;
+    __shared__ std::conditional_t<VERIFY, VerifySmem, char> vsm;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int) cl.block_rank(), blocks = (int) cl.num_blocks();
     const int row = (int) (blockIdx.x / blocks), base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base)), groups = (n + 3) >> 2;
@@ -182,12 +186,15 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     const int k_all = a.top_k ? a.top_k[row] : 0, k = k_all > 0 && k_all < a.n_vocab ? k_all : 0;
     const bool by_p = top_p < 1.f, cut = temperature > 0.f && (k > 0 || by_p);
     int draft = -1;                                                      // -1: none is checked here
-    bool homeless = false;                                               // a row of no sequence
+    [[maybe_unused]] bool homeless = false;                              // a row of no sequence
+    if constexpr (VERIFY) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const float * q_row = nullptr;
-    if (VERIFY) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const auto q_at = [&](int i) { const float q = q_row[i]; return q > 0.f ? (double) q : 0.0; };
     // whether the draft, of weight t, is taken; what is left of a weight for the draw where it is not
-    const auto takes = [&](u64 t, u64 total) { return draft >= 0 && (double) a.accept[row] * (q_row ? q_at(draft) : 1.0) * (double) total < (double) t; };
+    const auto takes = [&](u64 t, u64 total) {
+        if constexpr (VERIFY) return draft >= 0 && (double) a.accept[row] * (q_row ? q_at(draft) : 1.0) * (double) total < (double) t;
+        else return false;
+    };
     const auto rest_of = [&](u64 t, int i, u64 total) {
         if (t == 0) return t;
         if (!q_row) return i == draft ? 0ull : t;
@@ -205,11 +212,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     {
         const T * src = static_cast<const T *>(a.logits) + row * a.row_stride + base;
         constexpr int E = 16 / sizeof(T);
-        const auto meanwhile = [&]() {                                   // what does not depend on the logits, while the first of them are on their way
-            for (int i = tid; i < SA_BINS; i += SA_THREADS) bins[i] = 0;
-            if (tid < 16) sm.table[tid] = exp2((double) tid / 16.0);
-            if (tid == 0) sm.n_list = 0;
+        for (int i = tid; i < SA_BINS; i += SA_THREADS) bins[i] = 0;
+        if (tid < 16) sm.table[tid] = exp2((double) tid / 16.0);
+        if (tid == 0) sm.n_list = 0;
+        int done = 0;
+        [[maybe_unused]] bool looked = false;
+        [[maybe_unused]] const auto look = [&]() {                       // which draft the row checks: found while the first logits are on their way
             if constexpr (VERIFY) {
+                looked = true;
                 const int s = row_sequence(a.first, a.n_seq, row);
                 homeless = s < 0;
                 if (s >= 0 && row + 1 < min(a.first[s + 1], a.n_rows)) {
@@ -219,16 +229,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                 }
             }
         };
-        int done = 0;
-        bool first_time = true;
         if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
             done = n / E * E;
-            for (int i0 = tid * E; __any_sync(0xffffffffu, i0 < done); i0 += 8 * SA_THREADS * E) {
+            for (int i0 = tid * E; (VERIFY ? i0 - lane * E : i0) < done; i0 += 8 * SA_THREADS * E) {
                 uint4 x[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) { const int i = i0 + j * SA_THREADS * E; if (i < done) x[j] = *reinterpret_cast<const uint4 *>(src + i); }
-                if (first_time) meanwhile();
-                first_time = false;
+                if (VERIFY && !looked) look();
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int i = i0 + j * SA_THREADS * E;
@@ -243,7 +250,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                 }
             }
         }
-        if (first_time) meanwhile();
+        if (VERIFY && !looked) look();
         for (int i = done + tid; i < 4 * groups; i += SA_THREADS) { const T x = i < n ? src[i] : from_f<T>(-INFINITY); vals[i] = x; top = fmaxf(top, to_f(x)); }
     }
     if (VERIFY && homeless) {                                            // (the whole cluster)
@@ -625,9 +632,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     u64 mine = tid < sweeps * SA_WARPS ? sm.parts[tid / SA_WARPS][tid % SA_WARPS] : 0, block_sum;      // (256 parts at most)
     const u64 in_block = block_before64(mine, block_sum, sm.red);
     if (tid < blocks) cl.map_shared_rank(&sm, tid)->each[rank] = block_sum;
-    float v_draft = 0.f;
-    u64 t_draft = 0;
-    const bool draft_here = VERIFY && draft >= base && draft - base < n;
+    [[maybe_unused]] float v_draft = 0.f;
+    [[maybe_unused]] u64 t_draft = 0;
+    [[maybe_unused]] const bool draft_here = VERIFY && draft >= base && draft - base < n;
     if constexpr (VERIFY) {
         if (tid < blocks) {
             if (draft_here) {
@@ -638,7 +645,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) if (((draft - base) & 3) == e) { v_draft = v[e]; t_draft = w[e]; }
             }
-            cl.map_shared_rank(&sm, tid)->draft[rank] = t_draft;
+            cl.map_shared_rank(&vsm, tid)->draft[rank] = t_draft;
         }
     }
     cl.sync();
@@ -649,7 +656,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
     if constexpr (VERIFY) {
         if (draft != -1) {
             u64 t = 0;
-            for (int r = 0; r < blocks; r++) t += sm.draft[r];
+            for (int r = 0; r < blocks; r++) t += vsm.draft[r];
             if (takes(t, whole)) {
                 if (draft_here && tid == 0) finish(draft, log_share(exactly(v_draft), whole), true);
                 return;
@@ -665,10 +672,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
                 __syncthreads();
             }
             const u64 mine_r = tid < sweeps * SA_WARPS ? sm.parts[tid / SA_WARPS][tid % SA_WARPS] : 0, in_block_r = block_before64(mine_r, block_sum, sm.red);
-            if (tid < blocks) cl.map_shared_rank(&sm, tid)->rest[rank] = block_sum;
+            if (tid < blocks) cl.map_shared_rank(&vsm, tid)->rest[rank] = block_sum;
             cl.sync();
             u64 total_r = 0, front_r = in_block_r;
-            for (int r = 0; r < blocks; r++) { if (r < rank) front_r += sm.rest[r]; total_r += sm.rest[r]; }
+            for (int r = 0; r < blocks; r++) { if (r < rank) front_r += vsm.rest[r]; total_r += vsm.rest[r]; }
             if (total_r) { by_rest = true; total = total_r; front = front_r; mine = mine_r; }
         }
     }
@@ -701,7 +708,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const SampleArgs a) {
 
 // a warp a sequence: its rows up to the first whose draft was not taken gain a token each; what stands behind goes to -1 and 0
 template <int THREADS>
-__global__ void __launch_bounds__(THREADS) k_verify_ends(const SampleArgs a) {
+__global__ void __launch_bounds__(THREADS) k_verify_ends(const VerifyArgs a) {
     const int s = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (s >= a.n_seq) return;
