@@ -29,7 +29,7 @@ B200_SYMBOLS = ["b200_last_error", "b200_device_count", "b200_version", "b200_mo
                 "b200_sampler_new", "b200_sampler_set_standard", "b200_sampler_free", "b200_sampler_reset", "b200_sampler_sample",
                 "b200_kv4_append", "b200_kv4_read", "b200_kv4_attention_workspace", "b200_kv4_attention", "b200_kv4_status", "b200_kv4_drill", "b200_pages_workspace", "b200_pages_reserve", "b200_pages_fork",
                 "b200_pages_free", "b200_pages_compact", "b200_pages_copy", "b200_sample",
-                "b200_kv16_append", "b200_kv16_attention_workspace", "b200_kv16_attention", "b200_pages_plan", "b200_pages_trim", "b200_verify"]
+                "b200_kv16_append", "b200_kv16_attention_workspace", "b200_kv16_attention", "b200_pages_plan", "b200_pages_trim", "b200_verify", "b200_verify_workspace"]
 
 
 class Kv4(C.Structure):
@@ -183,7 +183,8 @@ def lib() -> C.CDLL:
     sig("b200_kv16_attention", C.c_int, [kp, C.c_int, vp, C.c_int64, C.c_int64, C.c_int, C.c_float, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int64])
     sig("b200_pages_plan", C.c_int, [pp, vp, vp, C.c_int, C.c_int, vp, vp, vp, vp])
     sig("b200_pages_trim", C.c_int, [pp, vp, C.c_int, C.c_int, C.c_int])
-    sig("b200_verify", C.c_int, [C.c_int, vp, C.c_int, vp, C.c_int64, C.c_int, C.c_int, vp, vp, C.c_int] + [vp] * 7 + [C.c_int64] + [vp] * 3)
+    sig("b200_verify", C.c_int, [C.c_int, vp, C.c_int, vp, C.c_int64, C.c_int, C.c_int, vp, vp, C.c_int] + [vp] * 7 + [C.c_int64] + [vp] * 4 + [C.c_int64])
+    sig("b200_verify_workspace", C.c_int64, [C.c_int])
     sig("b200_sample", C.c_int, [C.c_int, vp, C.c_int, vp, C.c_int64, C.c_int, C.c_int] + [vp] * 7)
     _lib = L
     return L

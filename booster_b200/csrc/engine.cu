@@ -3164,10 +3164,16 @@ extern "C" int b200_pages_trim(const b200_pages * p, const int32_t * slots, int 
 }
 extern "C" int b200_verify(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const int32_t * ids, const int32_t * first, int n_seq,
                            const float * u, const float * accept, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p, const float * draft_probs,
-                           int64_t draft_stride, int32_t * gained, int32_t * tokens, float * logprobs) {
+                           int64_t draft_stride, int32_t * gained, int32_t * tokens, float * logprobs, void * work, int64_t work_bytes) {
     return served("b200_verify", "", [&] {
-        verify_rows(device, stream, dtype, logits, row_stride, n_rows, n_vocab, ids, first, n_seq, u, accept, temperature, top_k, top_p, min_p, draft_probs, draft_stride, gained, tokens, logprobs);
+        verify_rows(device, stream, dtype, logits, row_stride, n_rows, n_vocab, ids, first, n_seq, u, accept, temperature, top_k, top_p, min_p, draft_probs, draft_stride, gained, tokens, logprobs, work,
+                    work_bytes);
     });
+}
+extern "C" int64_t b200_verify_workspace(int n_rows) {
+    int64_t bytes = -1;
+    served("b200_verify_workspace", "", [&] { bytes = verify_workspace(n_rows); });
+    return bytes;
 }
 extern "C" int b200_sample(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature,
                            const int32_t * top_k, const float * top_p, const float * min_p, int32_t * ids, float * logprobs) {

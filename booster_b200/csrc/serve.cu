@@ -98,7 +98,9 @@ template <typename T, bool VERIFY> void sample_as(const std::conditional_t<VERIF
     const size_t smem = SA_FIXED + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
     const auto kernel = k_sample<T, VERIFY>;
     allow_smem(kernel, device, set);
-    launch(kernel, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, false, cluster, a);
+    bool behind = false;
+    if constexpr (VERIFY) behind = a.order;
+    launch(kernel, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, behind, cluster, a);
 }
 
 template <bool VERIFY, typename A> void sample_all(A & a, int dtype, const On & on, void * stream) {
@@ -107,6 +109,10 @@ template <bool VERIFY, typename A> void sample_all(A & a, int dtype, const On & 
     int cluster = 1;
     while (cluster < SA_MAX_CLUSTER && ((int64_t) a.n_vocab * size_of(dtype) > 65536ll * cluster || (a.n_rows * cluster < on.sms && a.n_vocab >= 8192 * cluster))) cluster *= 2;
     a.slice = ((a.n_vocab + cluster - 1) / cluster + 7) / 8 * 8;
+    if constexpr (VERIFY) {
+        if ((int64_t) a.n_rows * cluster <= 2 * on.sms) a.order = a.ended = nullptr;      // all rows are on the card at once
+        else launch(k_verify_order, dim3((unsigned) ((a.n_rows + VO_THREADS - 1) / VO_THREADS)), VO_THREADS, 4 * (2 * (size_t) a.n_seq + 1), stream, false, 1, a);
+    }
     if (dtype == B200_DTYPE_F32) sample_as<float, VERIFY>(a, cluster, on.device, stream);
     else if (dtype == B200_DTYPE_BF16) sample_as<__nv_bfloat16, VERIFY>(a, cluster, on.device, stream);
     else sample_as<__half, VERIFY>(a, cluster, on.device, stream);
@@ -310,9 +316,13 @@ void sample_rows(int device, void * stream, int dtype, const void * logits, int6
     sample_all<false>(a, dtype, on, stream);
 }
 
+int64_t verify_workspace(int n_rows) {
+    need(n_rows >= 0 && n_rows <= (1 << 20), "verify: from 0 to 2^20 rows");
+    return 8 * (int64_t) n_rows;
+}
 void verify_rows(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const int32_t * ids, const int32_t * first, int n_seq, const float * u,
                  const float * accept, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p, const float * draft_probs, int64_t draft_stride,
-                 int32_t * gained, int32_t * tokens, float * logprobs) {
+                 int32_t * gained, int32_t * tokens, float * logprobs, void * work, int64_t work_bytes) {
     check_dtype(dtype, true);
     need(n_vocab >= 1 && n_vocab <= SA_MAX_VOCAB, "verify: from 1 to 2^18 logits a row (got " + std::to_string(n_vocab) + ")");
     need(n_rows >= 0 && n_rows <= (1 << 20), "verify: from 0 to 2^20 rows");
@@ -321,9 +331,11 @@ void verify_rows(int device, void * stream, int dtype, const void * logits, int6
     need(!draft_probs || draft_stride >= n_vocab || n_rows <= 1, "verify: draft_stride is n_vocab at least");
     need(first && (gained || n_seq == 0), "verify: null pointer");
     need(n_rows == 0 || (logits && ids && u && accept && tokens && logprobs && aligned(logits, size_of(dtype))), "verify: null pointer");
+    if (n_rows) check_work(work, work_bytes, verify_workspace(n_rows));
     On on(device);
     heed_waits(device);
-    VerifyArgs a = {{logits, row_stride, n_rows, n_vocab, 0, u, temperature, top_p, min_p, top_k, tokens, logprobs}, ids, first, n_seq, accept, draft_probs, draft_stride, gained};
+    int32_t * order = static_cast<int32_t *>(work);
+    VerifyArgs a = {{logits, row_stride, n_rows, n_vocab, 0, u, temperature, top_p, min_p, top_k, tokens, logprobs}, ids, first, n_seq, accept, draft_probs, draft_stride, gained, order, order + n_rows};
     if (n_rows) sample_all<true>(a, dtype, on, stream);
     if (n_seq) launch(k_verify_ends<128>, dim3((unsigned) ((n_seq + 3) / 4)), 128, 0, stream, true, 1, a);
 }

@@ -28,8 +28,9 @@ void    pages_trim(const b200_pages & p, const int32_t * slots, int n, int windo
 
 void    sample_rows(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature,
                     const int32_t * top_k, const float * top_p, const float * min_p, int32_t * ids, float * logprobs);
+int64_t verify_workspace(int n_rows);
 void    verify_rows(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const int32_t * ids, const int32_t * first, int n_seq, const float * u,
                     const float * accept, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p, const float * draft_probs, int64_t draft_stride,
-                    int32_t * gained, int32_t * tokens, float * logprobs);
+                    int32_t * gained, int32_t * tokens, float * logprobs, void * work, int64_t work_bytes);
 
 }  // namespace b200

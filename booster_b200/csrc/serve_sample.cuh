@@ -44,6 +44,8 @@ struct VerifyArgs : SampleArgs {         // of k_sample<T, true>
     const float * accept, * probs;       // probs: what the drafter drew from, [n_rows] rows probs_stride apart, or NULL: it was sure of its token
     int64_t probs_stride;
     int32_t * gained;
+    // where rows are more than the card holds at once: in which order they are looked at, first rows of all sequences first, and which have ended their sequence. NULL: as they stand
+    int32_t * order, * ended;
 };
 
 // 2^40 exp(d steps ln 2 / 16), d <= 0, to the nearest whole number, or 0: y = d steps = n + f with |f| <= 1 / 2, so a table's 2^(n mod 16 / 16), whose 16 entries are the 32 banks of
@@ -104,7 +106,7 @@ struct alignas(128) SampleSmem {
     float top;                           // the block's largest, and its place among the bins
     int place, n_list;
 };
-struct alignas(128) VerifySmem { u64 rest[SA_MAX_CLUSTER], draft[SA_MAX_CLUSTER]; };
+struct alignas(128) VerifySmem { u64 rest[SA_MAX_CLUSTER], draft[SA_MAX_CLUSTER]; int skip; };
 // dynamic shared memory: the list, fine sums, fine counts, bins, the slice
 constexpr int SA_FIXED = 8 * SA_LIST + 12 * SA_FINE + 4 * SA_BINS;
 // a number of every thread of the cluster, joined; all threads get it
@@ -177,7 +179,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional
     __shared__ std::conditional_t<VERIFY, VerifySmem, char> vsm;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int) cl.block_rank(), blocks = (int) cl.num_blocks();
-    const int row = (int) (blockIdx.x / blocks), base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base)), groups = (n + 3) >> 2;
+    int row = (int) (blockIdx.x / blocks);
+    if constexpr (VERIFY) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        if (a.order) row = a.order[row];
+        if ((unsigned) row >= (unsigned) a.n_rows) return;
+    }
+    const int base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base)), groups = (n + 3) >> 2;
     u64 * list = reinterpret_cast<u64 *>(sa_raw);                        // [SA_LIST]
     u64 * fine = list + SA_LIST;                                         // [SA_FINE] sums
     int * fine_count = reinterpret_cast<int *>(fine + SA_FINE), * bins = fine_count + SA_FINE;
@@ -187,7 +196,6 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional
     const bool by_p = top_p < 1.f, cut = temperature > 0.f && (k > 0 || by_p);
     int draft = -1;                                                      // -1: none is checked here
     [[maybe_unused]] bool homeless = false;                              // a row of no sequence
-    if constexpr (VERIFY) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const float * q_row = nullptr;
     const auto q_at = [&](int i) { const float q = q_row[i]; return q > 0.f ? (double) q : 0.0; };
     // whether the draft, of weight t, is taken; what is left of a weight for the draw where it is not
@@ -222,6 +230,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional
                 looked = true;
                 const int s = row_sequence(a.first, a.n_seq, row);
                 homeless = s < 0;
+                if (a.order) {                                           // (one block looks: the others would look at another time)
+                    if (rank == 0 && warp == 0) {
+                        bool any = false;
+                        if (s >= 0) for (int r = max(a.first[s], 0) + lane; r < row; r += 32) any = any || *reinterpret_cast<const volatile int32_t *>(a.ended + r);
+                        any = __any_sync(0xffffffffu, any);
+                        if (lane == 0) vsm.skip = any;
+                    }
+                }
                 if (s >= 0 && row + 1 < min(a.first[s + 1], a.n_rows)) {
                     draft = a.step_ids[row + 1];
                     if ((unsigned) draft >= (unsigned) a.n_vocab) draft = -2;
@@ -253,10 +269,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional
         if (VERIFY && !looked) look();
         for (int i = done + tid; i < 4 * groups; i += SA_THREADS) { const T x = i < n ? src[i] : from_f<T>(-INFINITY); vals[i] = x; top = fmaxf(top, to_f(x)); }
     }
-    if (VERIFY && homeless) {                                            // (the whole cluster)
-        if (rank == 0 && tid == 0) { a.ids[row] = -1; a.logprobs[row] = 0.f; }
-        return;
-    }
+    if constexpr (VERIFY)
+        if (homeless) {                                                  // (the whole cluster)
+            if (rank == 0 && tid == 0) { a.ids[row] = -1; a.logprobs[row] = 0.f; }
+            return;
+        }
     top = key_logit(warp_reduce(order_key(top, 0), [](u64 x, u64 y) { return max(x, y); }));
     if (lane == 0) sm.red[warp] = __float_as_uint(top);
     __syncthreads();
@@ -269,6 +286,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional
             for (int e = 0; e < 4; e++) atomicAdd(&bins[min(SA_BINS - 1, place - bin_place(v[e]))], 1);
         });
     cl.sync();
+    if constexpr (VERIFY) if (a.order && cl.map_shared_rank(&vsm, 0)->skip) { cl.sync(); return; }        // a row behind the end of its sequence is nobody's (they meet: that block's word has been read)
     int places[SA_MAX_CLUSTER], row_place = (int) (-SA_FAR * SA_PER_NAT);
 #pragma unroll
     for (int r = 0; r < SA_MAX_CLUSTER; r++) {
@@ -277,7 +295,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional
         row_place = max(row_place, places[r]);
         top = fmaxf(top, o->top);
     }
-    const auto finish = [&](int id, float lp, bool taken = false) { a.ids[row] = VERIFY && !taken ? -2 - id : id; if (a.logprobs) a.logprobs[row] = lp; };
+    const auto finish = [&](int id, float lp, bool taken = false) {
+        a.ids[row] = VERIFY && !taken ? -2 - id : id;
+        if (a.logprobs) a.logprobs[row] = lp;
+        if constexpr (VERIFY) if (a.order && !taken) *reinterpret_cast<volatile int32_t *>(a.ended + row) = 1;
+    };
     const auto first_of_largest = [&]() {
         u64 mine = ~0ull;
         each([&](const float (&v)[4], int i) {
@@ -704,6 +726,47 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional
                 if (c > target) { finish(base + 4 * g + e, log_share(exactly(v[e]), whole)); break; }
             }
     }
+}
+
+// The order of rows where they are more than the card holds at once: by their place in their sequence, so that when the later ones' turn comes it is known which sequences have ended and their rows are
+// left. Sequences that top-p cuts off without top-k come before all others: their rows take four times as long, and begun late would be what the call waits for. A thread a row: in front of place d of
+// sequence s stand, of its kind, min(d, length) rows of each sequence and the rows at place d of those before s. Rows of no sequence come last
+constexpr int VO_THREADS = 256;
+static __global__ void __launch_bounds__(VO_THREADS) k_verify_order(const VerifyArgs a) {
+    extern __shared__ int32_t vo_first[];                                // [n_seq + 1], within the rows; then of each sequence whether it takes long
+    int32_t * vo_long = vo_first + a.n_seq + 1;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    bool bad = false;
+    for (int s = threadIdx.x; s <= a.n_seq; s += VO_THREADS) vo_first[s] = min(max(a.first[s], 0), a.n_rows);
+    __syncthreads();
+    for (int s = threadIdx.x; s < a.n_seq; s += VO_THREADS) {
+        const int r = vo_first[s];
+        bad = bad || r > vo_first[s + 1];
+        int is = 0;
+        if (r < vo_first[s + 1] && a.top_p && a.top_p[r] < 1.f && (!a.temperature || a.temperature[r] > 0.f)) { const int k = a.top_k ? a.top_k[r] : 0; is = !(k > 0 && k < a.n_vocab); }
+        vo_long[s] = is;
+    }
+    bad = __syncthreads_or(bad);                                         // (first does not ascend: as they stand)
+    const int r = blockIdx.x * VO_THREADS + threadIdx.x;
+    if (r >= a.n_rows) return;
+    a.ended[r] = 0;
+    int at = r;
+    if (!bad && a.n_seq > 0) {
+        int s = 0;
+        for (int hi = a.n_seq; hi - s > 1;) { const int mid = (s + hi) >> 1; if (vo_first[mid] <= r) s = mid; else hi = mid; }
+        if (r < vo_first[0]) at = vo_first[a.n_seq] - vo_first[0] + r;
+        else if (r < vo_first[s + 1]) {
+            const int d = r - vo_first[s], kind = vo_long[s];
+            at = 0;
+            for (int o = 0; o < a.n_seq; o++) {
+                const int n = vo_first[o + 1] - vo_first[o];
+                if (vo_long[o] == kind) at += min(n, d) + (o < s && n > d);
+                else if (!kind) at += n;
+            }
+        }
+        // (those behind the last sequence stay where they are)
+    }
+    a.order[at] = r;
 }
 
 // a warp a sequence: its rows up to the first whose draft was not taken gain a token each; what stands behind goes to -1 and 0

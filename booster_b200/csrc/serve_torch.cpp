@@ -39,6 +39,7 @@ struct Api {
     decltype(&b200_kv16_attention) kv16_attention;
     decltype(&b200_pages_plan) pages_plan;
     decltype(&b200_pages_trim) pages_trim;
+    decltype(&b200_verify_workspace) verify_workspace;
     decltype(&b200_verify) verify;
 } api;
 PyObject * library_error;
@@ -372,9 +373,9 @@ PyObject * sample(PyObject * const * a) {                                // logi
 
 PyObject * verify(PyObject * const * a) {                                // logits, ids, first, u, accept, temperature, top_k, top_p, min_p, draft_probs
     const at::Tensor & logits = tensor(a[0], "logits");
-    const int index = on(logits), type = type_of(logits);
+    const int type = type_of(logits);
     need(logits.dim() == 2 && type >= 0 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits is a float32, bfloat16 or float16 tensor [rows, n_vocab] of contiguous rows");
-    const int rows = small(logits.size(0), "logits: too many rows"), vocab = small(logits.size(1), "logits: too many a row");
+    const int index = on(logits), rows = small(logits.size(0), "logits: too many rows"), vocab = small(logits.size(1), "logits: too many a row");
     const int64_t n64 = tensor(a[2], "first").numel() - 1;
     need(n64 >= 0, "first has one entry more than there are sequences");
     const int n = small(n64, "first: too many sequences");
@@ -397,8 +398,11 @@ PyObject * verify(PyObject * const * a) {                                // logi
     }
     const at::TensorOptions whole = logits.options().dtype(at::kInt);
     at::Tensor out[3] = {at::empty({n}, whole), at::empty({rows}, whole), at::empty({rows}, logits.options().dtype(at::kFloat))};
+    const int64_t size = api.verify_workspace(rows);
+    done(size >= 0, "verify");
+    const at::Tensor work = at::empty({size}, logits.options().dtype(at::kByte));
     done(api.verify(index, stream_of(index), type, logits.data_ptr(), rows > 1 ? logits.stride(0) : vocab, rows, vocab, ids, first, n, in[0], in[1], temperature, top_k, top_p, min_p, probs,
-                    probs_stride, static_cast<int32_t *>(out[0].data_ptr()), static_cast<int32_t *>(out[1].data_ptr()), static_cast<float *>(out[2].data_ptr())) == 0, "verify");
+                    probs_stride, static_cast<int32_t *>(out[0].data_ptr()), static_cast<int32_t *>(out[1].data_ptr()), static_cast<float *>(out[2].data_ptr()), rows ? work.data_ptr() : nullptr, size) == 0, "verify");
     PyObject * r = PyTuple_New(3);
     for (int i = 0; r && i < 3; i++) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(out[i]));
     return r;

@@ -47,7 +47,7 @@ def _native():
         L = _lib.lib()
         _serve.bind(_lib.B200Error, *(ctypes.cast(getattr(L, "b200_" + name), ctypes.c_void_p).value for name in (
             "last_error", "kv4_append", "kv4_read", "kv4_attention_workspace", "kv4_attention", "pages_workspace", "pages_reserve", "pages_fork", "pages_free", "pages_compact", "pages_copy",
-            "sample", "kv16_append", "kv16_attention_workspace", "kv16_attention", "pages_plan", "pages_trim", "verify")))
+            "sample", "kv16_append", "kv16_attention_workspace", "kv16_attention", "pages_plan", "pages_trim", "verify_workspace", "verify")))
         _module = _serve
     return _module
 

@@ -444,10 +444,12 @@ int b200_sample(int device, void * stream, int dtype, const void * logits, int64
  * taken, with one drawn from p at its last row. So the tokens have the target's distribution, and a sequence of one row gets b200_sample's token. A draft outside 0 .. n_vocab - 1 is never taken and
  * takes nothing off p; entries of q that are negative or NaN count as 0.
  * gained[n_seq]: how many tokens sequence i has gained (drafts taken and one drawn; 0 without rows), which is what its held tokens grow by; tokens[n_rows]: what follows each row up to there, -1
- * behind and for rows of no sequence; logprobs[n_rows]: log p of those (0 at temperature <= 0), 0 where tokens has -1. A row of no finite logit ends its sequence with -1 and -infinity. */
+ * behind and for rows of no sequence; logprobs[n_rows]: log p of those (0 at temperature <= 0), 0 where tokens has -1. A row of no finite logit ends its sequence with -1 and -infinity.
+ * work: b200_verify_workspace() bytes (-1: error) on 16 bytes. */
+int64_t b200_verify_workspace(int n_rows);
 int b200_verify(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const int32_t * ids, const int32_t * first, int n_seq, const float * u,
                 const float * accept, const float * temperature, const int32_t * top_k, const float * top_p, const float * min_p, const float * draft_probs, int64_t draft_stride, int32_t * gained,
-                int32_t * tokens, float * logprobs);
+                int32_t * tokens, float * logprobs, void * work, int64_t work_bytes);
 
 #ifdef __cplusplus
 }

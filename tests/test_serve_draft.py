@@ -61,10 +61,11 @@ def test_descriptions_of_a_16_bit_pool(changes, text):
 
 
 def test_arguments_of_the_verification():
-    good = [0, None, 0, FAKE, 100, 2, 100, FAKE, FAKE, 1, FAKE, FAKE, None, None, None, None, FAKE, 100, FAKE, FAKE, FAKE]
+    good = [0, None, 0, FAKE, 100, 2, 100, FAKE, FAKE, 1, FAKE, FAKE, None, None, None, None, FAKE, 100, FAKE, FAKE, FAKE, FAKE, 16]
+    assert L.b200_verify_workspace(-1) == -1 and L.b200_verify_workspace((1 << 20) + 1) == -1 and L.b200_verify_workspace(2) == 16
     for at, value, text in ((2, 5, "dtype"), (6, 0, "logits a row"), (6, (1 << 18) + 1, "logits a row"), (5, -1, "rows"), (5, (1 << 20) + 1, "rows"), (4, 99, "row_stride"), (17, 99, "draft_stride"),
                             (3, None, "null"), (3, FAKE + 2, "null"), (7, None, "null"), (8, None, "null"), (9, -1, "sequences"), (9, 4097, "sequences"), (10, None, "null"), (11, None, "null"),
-                            (18, None, "null"), (19, None, "null"), (20, None, "null")):
+                            (18, None, "null"), (19, None, "null"), (20, None, "null"), (21, None, "workspace"), (21, FAKE + 4, "workspace"), (22, 15, "workspace has 15")):
         refused(L.b200_verify(*[value if i == at else x for i, x in enumerate(good)]), text)
 
 
@@ -75,7 +76,7 @@ def test_no_cpu_fallback_here_either():
     refused(L.b200_kv16_attention(C.byref(c), 2, FAKE, 256, 64, 4, 1.0, 0, 0, 1, FAKE, FAKE, 1 << 40), "no CUDA device")
     refused(L.b200_pages_plan(C.byref(p), FAKE, FAKE, 1, 4, FAKE, FAKE, FAKE, FAKE), "no CUDA device")
     refused(L.b200_pages_trim(C.byref(p), FAKE, 1, 0, 0), "no CUDA device")
-    refused(L.b200_verify(0, None, 0, FAKE, 100, 2, 100, FAKE, FAKE, 1, FAKE, FAKE, None, None, None, None, None, 0, FAKE, FAKE, FAKE), "no CUDA device")
+    refused(L.b200_verify(0, None, 0, FAKE, 100, 2, 100, FAKE, FAKE, 1, FAKE, FAKE, None, None, None, None, None, 0, FAKE, FAKE, FAKE, FAKE, 16), "no CUDA device")
     ints = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA device"):
         serve.verify(torch.zeros(2, 5), ints, ints, torch.zeros(2), torch.zeros(2))

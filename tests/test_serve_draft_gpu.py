@@ -679,6 +679,30 @@ def test_long_sequences_of_drafts():
 
 
 @pytest.mark.parametrize("drafter", [False, True])
+@pytest.mark.parametrize("vocab,n", [(300, 400), (9000, 130), (70000, 30)])
+def test_more_rows_than_the_card_holds_at_once(vocab, n, drafter):
+    """the later rows of sequences come last, and those behind the end of theirs are left; sequences without rows, of one and of many"""
+    r = random.Random(vocab)
+    counts = [r.choice([0, 1, 1, 2, 3, 5, 8]) for _ in range(n)] + [70, 0]
+    kinds = KINDS if vocab < 70000 else KINDS[:3] + KINDS[4:7]
+    logits, ids, first, u, accept, filters, probs = step(vocab, vocab, counts, F32, kinds, drafter)
+    first_row = first[-1] - 70
+    for i in range(60):                                                 # the long one takes 60 drafts
+        logits[first_row + i, ids[first_row + i + 1]] += 60.0
+    got = assert_verifies(logits, ids, first, u, accept, filters, probs)
+    assert got[0][n] >= 60 and got[0][n + 1] == 0
+    again = verified(logits, ids, first, u, accept, filters, probs)
+    assert [x.tolist() for x in again] == got
+    # rows in front of the first sequence and behind the last one; sequences that do not ascend are bounded by the rows, and others keep their tokens
+    inner = [x + 3 for x in first[:-2]]
+    rows = sum(counts)
+    gained, tokens, logprobs = verified(logits, ids, inner, u, accept, filters, probs)
+    assert (tokens[:3] == -1).all() and not logprobs[:3].any() and (tokens[min(rows, inner[-1]):] == -1).all()
+    gained, tokens, _ = verified(logits, ids, [5, 50, 20, rows + 100, -4, 40], u, accept, filters, probs)
+    assert 0 <= gained.min() and gained.max() <= rows
+
+
+@pytest.mark.parametrize("drafter", [False, True])
 def test_what_comes_out_has_the_target_s_distribution(drafter):
     """the first token of 2 x 10^5 sequences whose drafts come from another distribution: counts within five standard deviations of the target's"""
     vocab, n, rounds = 6, 4000, 50
