@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
         // the warp's 32 queries where boxes do not bring them: HD / 8 lanes a row
         const auto queries = [&](const Segment16 & g) {
             const int col = g.ct * PR_COLS + half * 128 + row, i = col / a.group, h = g.head * a.group + col - i * a.group;
-            constexpr int LANES = HD / 8, ROWS = 32 / LANES, X = 4;
+            constexpr int LANES = HD / 8, ROWS = 32 / LANES, X = HD == 128 ? 4 : 8;
             const int64_t mine = i < g.q.count ? (g.q.begin + i) * a.q_row + h * a.q_head : -1;
             const int m = lane % LANES;
 #pragma unroll 1
@@ -474,10 +474,11 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
     }
 }
 
-// a block 32 columns of a unit that blocks shared: adds its parts, eight on their way at a time. A lane is a column, a warp has every eighth group of 4 dims
+// a block 32 columns of a unit that blocks shared: adds its parts, four on their way at a time and four blocks an SM (eight and two: 1000 rows behind 5000
+// positions, whose parts are 38 MB, 15 us for 10). A lane is a column, a warp has every eighth group of 4 dims
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) k_kv16_prompt_join(const PromptArgs p) {
-    constexpr int X = HD / 32, PAD = HD + 4, BATCH = 8;
+__global__ void __launch_bounds__(256, 4) k_kv16_prompt_join(const PromptArgs p) {
+    constexpr int X = HD / 32, PAD = HD + 4, BATCH = 4;
     __shared__ __align__(16) float sums[32 * PAD];
     const AttendArgs & a = p.a;
     const Cache & c = a.c;
