@@ -13,7 +13,7 @@
 // P is rounded to the type once, with P_LIFT and P_PASS of serve_attn.cuh: results are off by 1.2 to 1.35 times (rms) what their own rounding is (bfloat16 2.1e-3 for 1.7e-3, fp16 2.8e-4 for 2.1e-4).
 // In two numbers, as for few rows, the second product would be twice as long; sums of the rounded weights instead of the weights' made 8192 tokens 45 us longer and no result nearer.
 // O is scaled in tensor memory where the base of P moves.
-// Measured with 32 query heads on 8 of 128: 8192 tokens 489 us (1124 TFLOP/s, 68 % of the bf16 rate), 1000 rows behind 5000 positions 109 us, of which 5 the plan and 4 the join. A step of 64
+// Measured with 32 query heads on 8 of 128: 8192 tokens 473 us (1162 TFLOP/s, 71 % of the bf16 rate), 1000 rows behind 5000 positions 100 us, of which 5 the plan and 10 the join. A step of 64
 // tokens takes 1750 clocks: of both halves' products 1280 (those of 64 tokens read 6 KB of shared memory in 48 clocks, for 32 of arithmetic), of exponentials 900, an eighth of them by a
 // polynomial (none 495 us, two eighths 489, three 494). Halves that took turns at exponentials by named barriers 475 to 485 and nothing at 1000 rows. What a warp does between them bounds it: a wait for
 // what is there 130 clocks, 64 scores from tensor memory 60 to 120, the largest 280, P back 120.

@@ -5,7 +5,8 @@
 // where pages are copied a second kernel that moves them in every layer at the memory's rate.
 // Measured: 48 pages reserved in a pool of 4096 8.6 us, of 65 536 13 us (a block reads 256 KB of counts); 24 slots forked 9 us and their part-full pages copied 7 (8 layers, 15 MB read and written); 12 slots freed
 // 2.5 us; 255 MB compacted 8 us for the plan and 43 for the moves (6.0 TB/s, 93 % of the copy rate); 600 pages of 32 layers copied 461 us (6.1 TB/s). One block plans because every page that
-// is taken depends on all that were taken before; latency bounds it.
+// is taken depends on all that were taken before; latency bounds it. Tables of a step: 48 sequences in 4096 pages 9.6 us for the plan and 2.4 for what is trimmed, 300 (three with 900 rows) in 60 000
+// pages 12.3 and 2.5.
 #pragma once
 #include "serve_cache.cuh"
 
