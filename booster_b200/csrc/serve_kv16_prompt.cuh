@@ -483,14 +483,19 @@ __global__ void __launch_bounds__(256, 4) k_kv16_prompt_join(const PromptArgs p)
     const AttendArgs & a = p.a;
     const Cache & c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x / (PR_COLS / 32), c0 = blockIdx.x % (PR_COLS / 32) * 32, head = blockIdx.y;
+    // the plan is done with: the kernel in front waited for it before it let this one begin. Its own results are behind the wait, for which blocks without work stay too
+    Entry n = {};
+    int cols = 0, w0 = 0, w1 = 0;
+    if (e < p.first[1]) {
+        n = p.entries[e];
+        const int len = n.n + P16_OVER, per = p.first[0];
+        cols = min(PR_COLS, n.count * a.group - n.ct * PR_COLS);
+        const long long u0 = a.before[e] + (long long) head * len;
+        w0 = (int) quotient(u0 + P16_OVER, per);
+        w1 = (int) quotient(u0 + len - 1, per);
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (e >= p.first[1]) return;
-    const Entry n = p.entries[e];
-    const int len = n.n + P16_OVER, per = p.first[0], cols = min(PR_COLS, n.count * a.group - n.ct * PR_COLS);
-    if (c0 >= cols) return;
-    const long long u0 = a.before[e] + (long long) head * len;
-    const int w0 = (int) quotient(u0 + P16_OVER, per), w1 = (int) quotient(u0 + len - 1, per);
-    if (w0 == w1) return;
+    if (c0 >= cols || w0 == w1) return;
     const bool in = c0 + lane < cols;                              // (others were not stored)
     float m = -INFINITY, l = 0.f, o[X][4] = {};
     for (int w = w0; w <= w1; w += BATCH) {

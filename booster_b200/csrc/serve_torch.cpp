@@ -242,8 +242,9 @@ PyObject * kv16_attention(PyObject * const * a) {                        // q, p
     }
     const int64_t size = api.kv16_attention_workspace(&c, heads, most);
     done(size >= 0, "kv16_attention");
-    const at::Tensor work = at::empty({size}, pool.options().dtype(at::kByte));
-    done(api.kv16_attention(&c, type_of(q), q.data_ptr(), r.row, r.head, heads, (float) scale, window, sinks, most, out.data_ptr(), work.data_ptr(), size) == 0, "kv16_attention");
+    at::Tensor work;
+    if (size) work = at::empty({size}, pool.options().dtype(at::kByte));
+    done(api.kv16_attention(&c, type_of(q), q.data_ptr(), r.row, r.head, heads, (float) scale, window, sinks, most, out.data_ptr(), size ? work.data_ptr() : nullptr, size) == 0, "kv16_attention");
     return THPVariable_Wrap(out);
 }
 
