@@ -98,9 +98,7 @@ template <typename T, bool VERIFY> void sample_as(const std::conditional_t<VERIF
     const size_t smem = SA_FIXED + ((size_t) a.slice * sizeof(T) + 15) / 16 * 16;
     const auto kernel = k_sample<T, VERIFY>;
     allow_smem(kernel, device, set);
-    bool behind = false;
-    if constexpr (VERIFY) behind = a.order;
-    launch(kernel, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, behind, cluster, a);
+    launch(kernel, dim3((unsigned) (a.n_rows * cluster)), SA_THREADS, smem, stream, VERIFY, cluster, a);
 }
 
 template <bool VERIFY, typename A> void sample_all(A & a, int dtype, const On & on, void * stream) {
@@ -111,7 +109,7 @@ template <bool VERIFY, typename A> void sample_all(A & a, int dtype, const On & 
     a.slice = ((a.n_vocab + cluster - 1) / cluster + 7) / 8 * 8;
     if constexpr (VERIFY) {
         if ((int64_t) a.n_rows * cluster <= 2 * on.sms) a.order = a.ended = nullptr;      // all rows are on the card at once
-        else launch(k_verify_order, dim3((unsigned) ((a.n_rows + VO_THREADS - 1) / VO_THREADS)), VO_THREADS, 4 * (2 * (size_t) a.n_seq + 1), stream, false, 1, a);
+        else launch(k_verify_order, dim3((unsigned) ((a.n_rows + VO_THREADS - 1) / VO_THREADS)), VO_THREADS, 4 * (2 * (size_t) a.n_seq + 1), stream, true, 1, a);
     }
     if (dtype == B200_DTYPE_F32) sample_as<float, VERIFY>(a, cluster, on.device, stream);
     else if (dtype == B200_DTYPE_BF16) sample_as<__nv_bfloat16, VERIFY>(a, cluster, on.device, stream);
@@ -286,7 +284,7 @@ void pages_plan(const b200_pages & p, const int32_t * slots, const int32_t * cou
     const bool apart = n_rows > PLAN_ROWS;
     const size_t smem = words_bytes(p.n_slots) + plan_bytes(n), places_smem = 4 * ((size_t) 3 * n + 1);
     allow_smem(k_pages_plan, p.device, set);
-    launch(k_pages_plan, dim3(1), PG_THREADS, smem, p.stream, false, 1, d, slots, counts, n, n_rows, first, positions, places, status, !apart);
+    launch(k_pages_plan, dim3(1), PG_THREADS, smem, p.stream, true, 1, d, slots, counts, n, n_rows, first, positions, places, status, !apart);
     static Limits places_set;
     if (apart) allow_smem(k_pages_places, p.device, places_set);
     if (apart) launch(k_pages_places, dim3((unsigned) ((n_rows + 1023) / 1024)), 256, places_smem, p.stream, true, 1, d, slots, first, n, n_rows, positions, places);
@@ -299,7 +297,7 @@ void pages_trim(const b200_pages & p, const int32_t * slots, int n, int window, 
     need(window >= 0 && sinks >= 0, "pages_trim: window is a number of positions, or 0 for all; sinks is a number of positions");
     On on(p.device);
     heed_waits(p.device);
-    if (n) launch(k_pages_trim, dim3((unsigned) (((int64_t) n * ((p.max_pages + 255) / 256) + 7) / 8)), 256, 0, p.stream, false, 1, d, slots, n, window, sinks);
+    if (n) launch(k_pages_trim, dim3((unsigned) (((int64_t) n * ((p.max_pages + 255) / 256) + 7) / 8)), 256, 0, p.stream, true, 1, d, slots, n, window, sinks);
 }
 
 void sample_rows(int device, void * stream, int dtype, const void * logits, int64_t row_stride, int n_rows, int n_vocab, const float * u, const float * temperature, const int32_t * top_k,

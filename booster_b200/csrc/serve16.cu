@@ -39,7 +39,7 @@ int row_passes(const b200_kv4 & c) { return (int64_t) c.n_rows * c.n_head_kv > 1
 template <typename S, typename T> void append_as(const b200_kv4 & c, const Cache & d, const void * k, int64_t kr, int64_t kh, const void * v, int64_t vr, int64_t vh) {
     const Row16Src<S> src = {static_cast<const S *>(k), kr, kh, static_cast<const S *>(v), vr, vh, aligned(k, 16) && aligned(v, 16) && !((kr | kh | vr | vh) & (16 / (int64_t) sizeof(S) - 1))};
     const int per = row_passes(c) * (256 / c.head_dim), parts = (c.n_head_kv + per - 1) / per;
-    const auto rows = [&](auto kernel) { launch(kernel, dim3((unsigned) (((int64_t) c.n_rows * parts + 7) / 8)), 256, 0, c.stream, false, 1, d, src, parts); };
+    const auto rows = [&](auto kernel) { launch(kernel, dim3((unsigned) (((int64_t) c.n_rows * parts + 7) / 8)), 256, 0, c.stream, true, 1, d, src, parts); };
     if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv16_append<S, T, 128, 1>) : rows(k_kv16_append<S, T, 64, 1>);
     else c.head_dim == 128 ? rows(k_kv16_append<S, T, 128, 4>) : rows(k_kv16_append<S, T, 64, 4>);
 }
@@ -60,14 +60,14 @@ template <int HD, int NT, int CW, typename T> void unit_as(const AttendArgs & a,
     static Limits set;
     const auto kernel = k_kv16_attend_unit<HD, NT, CW, T>;
     allow_smem(kernel, f.device, set);
-    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * f.n_ct * f.cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), f.stream, false, f.cluster, a, f.map, f.err, WAIT_POLLS, f.n_ct);
+    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * f.n_ct * f.cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), f.stream, true, f.cluster, a, f.map, f.err, WAIT_POLLS, f.n_ct);
 }
 template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, const Few & f) {
     if (f.cluster) return unit_as<HD, NT, 1, T>(a, f);
     static Limits set;
     const auto kernel = k_kv16_attend<HD, NT, T>;
     allow_smem(kernel, f.device, set);
-    launch(kernel, dim3(f.sms), A16_WARPS * 32, 1024 + a16_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8, f.stream, false, 1, a, f.map, f.err, WAIT_POLLS);
+    launch(kernel, dim3(f.sms), A16_WARPS * 32, 1024 + a16_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8, f.stream, true, 1, a, f.map, f.err, WAIT_POLLS);
     const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group, parts = (int64_t) f.sms * A16_WARPS / ((int64_t) a.c.n_seq * a.c.n_kv);
     if (parts > 32) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, f.stream, true, 1, a);
     else if (parts > 8) launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, f.stream, true, 1, a);
@@ -97,7 +97,7 @@ template <int HD, typename T> void prompt_as(const PromptArgs & p, const CUtenso
     static Limits set;
     const auto kernel = k_kv16_prompt<HD, T>;
     allow_smem(kernel, device, set);
-    launch(k_kv16_plan, dim3(1), 1024, (size_t) (p.a.c.n_seq + 1) * 4, stream, false, 1, p, sms);
+    launch(k_kv16_plan, dim3(1), 1024, (size_t) (p.a.c.n_seq + 1) * 4, stream, true, 1, p, sms);
     launch(kernel, dim3(sms), P16_THREADS, Prompt16Smem<HD>::BYTES, stream, true, 1, p, map, q_map, by_box);
     launch(k_kv16_prompt_join<HD, T>, dim3((unsigned) (entries * (PR_COLS / 32)), (unsigned) p.a.c.n_kv), 256, 0, stream, true, 1, p);
 }

@@ -24,6 +24,8 @@
 namespace b200 {
 namespace srv {
 
+// The first kernel of a call stands ready behind the work in front of it (programmatic launch), waits for that before it touches any memory of the call, and only then lets the kernel behind it
+// begin, which may read ahead of its own wait what the call was given. Rows of 4 sequences written and attended to, calls one after another: 12.3 us without, 7.7 so.
 constexpr int A16_WARPS = 4, A16_STAGES = 3, A16_STEP = 32, A16_CLUSTER = 8;      // A16_STAGES: a warp
 __host__ __device__ constexpr int a16_stage_bytes(int hd) { return A16_STEP * 4 * hd; }
 __host__ __device__ constexpr size_t a16_ring_bytes(int hd) { return (size_t) A16_WARPS * A16_STAGES * a16_stage_bytes(hd); }
@@ -280,11 +282,12 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
     long long * before = reinterpret_cast<long long *>(a16_raw + (smem - smem_at(a16_raw)) + a16_ring_bytes(HD));       // [n_seq + 1]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
     const Cache & c = a.c;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (lane == 0) {
         for (int i = 0; i < A16_STAGES; i++) mbar_init(smem_at(&full_s[warp][i]), 1);
         mbar_init_done();
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // steps in front of each sequence
     {
         constexpr int THREADS = A16_WARPS * 32, BATCH = 4;
@@ -386,6 +389,7 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const At
     }
     if (CW > 1) __syncthreads(); else __syncwarp();
     Ring16 ring = {smem + (uint32_t) (group * STAGES * STAGE), smem_at(&full_s[group][0]), smem_at(&empty_s[group][0]), 0, 0};
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int unit = (int) blockIdx.x / blocks, head = unit % c.n_kv, s = unit / c.n_kv / n_ct;
     const Seq q = seq_at(c, s);
     const Steps sp = steps_of(c, q, a.window, a.sinks, 0, q.count - 1, 5);
@@ -491,6 +495,7 @@ __global__ void __launch_bounds__(256) k_kv16_append(const Cache c, const Row16S
     constexpr int LANES = HD / 8, PER = 32 / LANES;
     const int64_t item = ((int64_t) blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31, li = lane % LANES, row = (int) (item / parts), h0 = (int) (item % parts) * PASSES * PER + lane / LANES;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= c.n_rows) return;
     uint32_t k[PASSES][4] = {}, v[PASSES][4] = {};
 #pragma unroll

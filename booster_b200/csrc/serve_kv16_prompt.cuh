@@ -73,6 +73,7 @@ static __global__ void __launch_bounds__(1024) k_kv16_plan(const PromptArgs p, i
     __shared__ long long sums[32];
     const Cache & c = p.a.c;
     const int tid = threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int all = 0;
     for (int s0 = 0; s0 < c.n_seq; s0 += 1024) {

@@ -211,6 +211,7 @@ static __global__ void __launch_bounds__(PG_THREADS) k_pages_plan(const Pages p,
     uint32_t * seen = pg_smem;
     int32_t * first = reinterpret_cast<int32_t *>(seen + slot_words), * from = first + n + 1, * before = from + n, * slot_of = before + n + 1, * held_of = slot_of + n, * long_of = held_of + n,
             * chunk = long_of + n;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const bool whole = (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0;
     int4 v[8];
@@ -353,6 +354,7 @@ static __global__ void __launch_bounds__(256) k_pages_places(const Pages p, cons
 static __global__ void __launch_bounds__(256) k_pages_trim(const Pages p, const int32_t * slots, int n, int window, int sinks) {
     const int64_t item = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, parts = (p.max_pages + 255) >> 8, s = (int) (item / parts), i0 = (int) (item % parts) * 256 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (s >= n) return;
     const int slot = slots[s];
     if ((unsigned) slot >= (unsigned) p.n_slots) return;

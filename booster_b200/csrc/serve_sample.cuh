@@ -735,6 +735,7 @@ constexpr int VO_THREADS = 256;
 static __global__ void __launch_bounds__(VO_THREADS) k_verify_order(const VerifyArgs a) {
     extern __shared__ int32_t vo_first[];                                // [n_seq + 1], within the rows; then of each sequence whether it takes long
     int32_t * vo_long = vo_first + a.n_seq + 1;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     bool bad = false;
     for (int s = threadIdx.x; s <= a.n_seq; s += VO_THREADS) vo_first[s] = min(max(a.first[s], 0), a.n_rows);

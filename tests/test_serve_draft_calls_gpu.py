@@ -104,6 +104,104 @@ def test_graphs_streams_and_order(form):
         assert torch.equal(again, got)
 
 
+def test_calls_see_what_the_call_in_front_wrote():
+    """a step's calls stand ready behind one another and behind other kernels, some of which let the next one begin early: with nothing waited for between them they give what they give one by one"""
+    page, kv, hd, slots = 16, 2, 64, 6
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    logits = 3 * torch.randn(40, 4000, generator=gen, device="cuda")
+    wide = 2 * torch.randn(60, 70000, generator=gen, device="cuda")
+
+    def state():
+        return [ints([[-1] * 60] * slots), ints([0] * slots), ints([0] * 400), torch.zeros(1, 400, 2, kv, page, hd, dtype=BF16, device="cuda"), torch.zeros(400 * page, dtype=torch.int32, device="cuda")]
+
+    def steps(sync):
+        table, held, refs, pool, marks = state()
+        r, g, seen = random.Random(1), torch.Generator(device="cuda").manual_seed(3), []
+        done = torch.cuda.synchronize if sync else lambda: None
+        for turn in range(25):
+            counts = [r.choice([0, 1, 4, 6]) for _ in range(slots)] if turn % 5 else [r.choice([1, 30]) for _ in range(slots)]
+            rows = sum(counts)
+            n, ids = ints(counts), torch.randint(0, 4000, (rows,), generator=g, device="cuda", dtype=torch.int32)
+            done()
+            first, positions, places, status = serve.pages_plan(table, held, refs, n, page, rows)
+            done()
+            marks[places.long()] = ids
+            k, v, q = (torch.randn(rows, h, hd, generator=g, device="cuda").bfloat16() for h in (kv, kv, 8))
+            serve.kv16_append(pool[0], table, held, first, k, v)
+            done()
+            outs = [serve.kv16_attention(q, pool[0], table, held, first, max_rows=max(counts + [1]), window=200, sinks=3)]
+            done()
+            outs.append(serve.kv16_attention(q, pool[0], torch.cat([table, torch.full((slots, 5000), -1, dtype=torch.int32, device="cuda")], 1), held, first, max_rows=2))
+            done()
+            outs.append(serve.kv16_attention(q, pool[0], table, held, first, max_rows=100))
+            done()
+            u = torch.rand(max(rows, 60), generator=g, device="cuda")
+            new = serve.verify(logits[:min(rows, 40)], ids[:40], first.clamp(max=min(rows, 40)), u[:min(rows, 40)], u[:min(rows, 40)])
+            done()
+            many = serve.verify(wide, ids.repeat(60)[:60] if rows else ints([0] * 60), torch.arange(0, 61, 2, device="cuda").int(), u[:60], u[:60])
+            done()
+            held += torch.maximum(new[0], torch.minimum(n, torch.full_like(n, 2)))
+            held.copy_(torch.minimum(held, torch.full_like(held, 700)))
+            serve.pages_trim(table, held, refs, page, torch.arange(slots, device="cuda").int(), 200, 3)
+            done()
+            seen += [first, positions, places, status, *outs, *new, *many, table.clone(), refs.clone()]
+        return [x.clone() for x in seen] + [pool, marks]
+    want = steps(True)
+    for _ in range(3):
+        got = steps(False)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_captured_behind_what_is_no_kernel():
+    """first in a graph, behind a memset, behind a copy, and where two streams meet"""
+    c, q = made("unit")
+    line, q_line = made("line")
+    rows, q_rows = made("rows")
+    table, out = c.table, torch.zeros_like(q)
+    t_line, t_rows = line.table, rows.table
+    k = torch.randn(3, 2, 64, device="cuda").bfloat16()
+    src = c.held.clone()
+    held, other = c.held.clone(), torch.zeros(1 << 20, device="cuda")
+    refs = torch.ones(c.pages, dtype=torch.int32, device="cuda")
+    logits, u = torch.randn(3, 500, device="cuda"), torch.full((3,), 0.5, device="cuda")
+    side = torch.cuda.Stream()
+
+    def work():
+        a = [serve.kv16_attention(q, c.pool[0], table, held, c.first, c.slots)]
+        held.zero_()
+        serve.kv16_append(c.pool[0], table, held, c.first, k, k, c.slots)
+        held.copy_(src, non_blocking=True)
+        a.append(serve.kv16_attention(q, c.pool[0], table, held, c.first, c.slots))
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                other.add_(1.0)
+            held.copy_(src)
+        a.append(serve.kv16_attention(q_line, line.pool[0], t_line, line.held, line.first, line.slots))
+        torch.cuda.current_stream().wait_stream(side)
+        a.append(serve.kv16_attention(q_rows, rows.pool[0], t_rows, rows.held, rows.first, rows.slots))
+        torch.cuda.current_stream().wait_stream(side)
+        a += serve.verify(logits, ints_kept, c.first, u, u)
+        other.zero_()
+        serve.pages_trim(table, held, refs, 16, c.slots)
+        a += serve.pages_plan(table, held, refs, counts, 16, 9, c.slots)
+        return a
+    ints_kept, counts = ints([1, 2, 3]), ints([1, 1, 1])
+    pool = c.pool.clone()
+    kept = table.clone()
+    want = [x.clone() for x in work()]
+    torch.cuda.synchronize()
+    c.pool.copy_(pool); table.copy_(kept); held.copy_(src); refs.fill_(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for _ in range(3):
+        c.pool.copy_(pool); table.copy_(kept); held.copy_(src); refs.fill_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_captured_steps_of_tables_and_verification():
     """a graph of the step's small operators, replayed with other numbers in its inputs"""
     page, n = 16, 5
