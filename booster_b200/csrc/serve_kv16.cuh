@@ -488,8 +488,8 @@ template <typename S, typename T> __device__ __forceinline__ void eight_as(const
         for (int i = 0; i < 4; i++) w[i] = pair_of<T>(to_f(p[2 * i]), to_f(p[2 * i + 1]));
     }
 }
-// A warp a row and PASSES passes of its heads (two heads at head_dim 128, four at 64), 16 bytes a lane; latency bounds few rows (row -> sequence -> slot -> page: 48 of 8 heads 2.8 us), the memory many
-// (5200 rows from fp32, 62 MB, 9.1 us)
+// A warp a row and PASSES passes of its heads (two heads at head_dim 128, four at 64), 16 bytes a lane; latency bounds few rows (row -> sequence -> slot -> page: 48 of 8 heads 2.2 us), the memory many
+// (5200 rows from fp32, 62 MB, 8.6 us)
 template <typename S, typename T, int HD, int PASSES>
 __global__ void __launch_bounds__(256) k_kv16_append(const Cache c, const Row16Src<S> src, int parts) {
     constexpr int LANES = HD / 8, PER = 32 / LANES;
