@@ -96,7 +96,7 @@ def kv16_append(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, fir
 def kv16_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first: torch.Tensor, slots: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                    window: int = 0, sinks: int = 0, max_rows: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """attention of the step's rows q [rows, n_head, head_dim] (of the pool's type, any strides over rows and heads) over the positions up to their own, kv16_append having put those into the pool;
-    window > 0: over the last `window` of them and the sequence's first `sinks`. scale, max_rows and out as in kv4_attention"""
+    window > 0: over the last `window` of them and the sequence's first `sinks`. scale, max_rows and out as in kv4_attention; out may be q itself"""
     return _native().kv16_attention(q, pool, table, held, first, slots, scale, window, sinks, max_rows, out)
 
 

@@ -152,6 +152,74 @@ def test_calls_see_what_the_call_in_front_wrote():
         assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+def test_results_in_the_queries_place(form, hd):
+    """a query is read by those who work on its result alone, and before that is written"""
+    c, q = made(form, hd)
+    want = serve.kv16_attention(q, *c.args(), slots=c.slots)
+    for _ in range(20):
+        x = q.clone()
+        assert serve.kv16_attention(x, *c.args(), slots=c.slots, out=x).data_ptr() == x.data_ptr()
+        assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_behind_the_operators_of_the_4_bit_cache(captured):
+    """calls of both kinds of cache one behind the other, on tables that the call in front wrote"""
+    page, kv, hd, slots, rows = 16, 2, 64, 5, 60
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    k, v, q = (torch.randn(rows, h, hd, generator=gen, device="cuda").bfloat16() for h in (kv, kv, 8))
+    logits, u = torch.randn(rows, 3000, generator=gen, device="cuda"), torch.rand(rows, generator=gen, device="cuda")
+    table, held, refs = ints([[-1] * 40] * slots), ints([0] * slots), ints([0] * 250)
+    four, wide = serve.kv4_pool(250, page, kv, hd), torch.zeros(1, 250, 2, kv, page, hd, dtype=BF16, device="cuda")
+    counts, some = ints([12, 1, 30, 0, 17]), ints([3, 0, 4])
+    own, far = torch.arange(slots, device="cuda").int(), ints([[-1] * 5000] * slots)
+
+    def work(done=lambda: None):
+        out = []
+        for turn in range(6):
+            first = torch.cat([ints_0, counts.cumsum(0).int()])
+            for call in (lambda: serve.pages_reserve(table, held, refs, first, page), lambda: serve.kv4_append(four[0], table, held, first, k, v), lambda: serve.kv16_append(wide[0], table, held, first, k, v),
+                         lambda: serve.kv4_attention(q, four[0], table, held, first), lambda: serve.kv16_attention(q, wide[0], table, held, first),
+                         lambda: serve.kv4_attention(q, four[0], table, held, first, max_rows=1), lambda: serve.kv16_attention(q, wide[0], torch.cat([table, far], 1), held, first, max_rows=1),
+                         lambda: serve.sample(logits, u)[0], lambda: serve.verify(logits, counts.repeat(12), first, u, u)[0]):
+                out.append(call())
+                done()
+            held.add_(torch.maximum(out[-1], torch.minimum(counts, ones)))
+            serve.pages_trim(table, held, refs, page, own)
+            done()
+            serve.pages_free(table, held, refs, some)
+            done()
+            out += serve.pages_plan(table, held, refs, counts, page, rows)
+            done()
+            serve.pages_compact(four, table, refs) if turn == 2 else serve.pages_trim(table, held, refs, page, own, 20, 3)
+            done()
+            out += [table.clone(), refs.clone(), held.clone()]
+        return [x for x in out if x is not None]
+
+    def fresh():
+        table.fill_(-1); held.zero_(); refs.zero_(); wide.zero_(); four.zero_()
+    ints_0, ones = ints([0]), ints([4] * slots)
+    want = [x.clone() for x in work(torch.cuda.synchronize)]
+    fresh()
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = work()
+        for _ in range(3):
+            fresh()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+    else:
+        for _ in range(3):
+            got = work()
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+            fresh()
+
+
 def test_captured_behind_what_is_no_kernel():
     """first in a graph, behind a memset, behind a copy, and where two streams meet"""
     c, q = made("unit")

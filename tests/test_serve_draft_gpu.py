@@ -333,12 +333,13 @@ def test_any_number_of_rows_is_right(counts, max_rows):
     assert_attends(c.widened(), q, serve.kv16_attention(q, *c.args(), slots=c.slots, max_rows=max_rows))
 
 
-def test_many_sequences():
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_sequences(hd):
     n = 4096
     r = random.Random(5)
-    c = Case([r.randrange(0, 40) for _ in range(n)], [1] * n, kv=1, hd=64, dtype=BF16)
+    c = Case([r.randrange(0, 40) for _ in range(n)], [1] * n, kv=1, hd=hd, dtype=BF16)
     c.fill()
-    q = c.randn(n, 2, 64).bfloat16()
+    q = c.randn(n, 2, hd).bfloat16()
     assert_attends(c, q, serve.kv16_attention(q, *c.args(), slots=c.slots))
     assert_attends(c, q, serve.kv16_attention(q, *c.args(), slots=c.slots, max_rows=200, window=9, sinks=2), 9, 2)
 
