@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <array>
 #include <climits>
 #include <cmath>
 #include <stdexcept>
@@ -328,6 +329,20 @@ PyObject * pages_copy(PyObject * const * a) {                            // pool
     done(api.pages_copy(&p, src, dst, n, static_cast<int32_t *>(status.data_ptr()), work.data_ptr(), work.numel()) == 0, "pages_copy");
     return THPVariable_Wrap(status);
 }
+// tensors of so many entries in one piece of memory, each from 16 bytes on (a plan of 48 sequences takes the host 4.8 us, 6.4 with a request of its own for each of the four)
+template <size_t N> std::array<at::Tensor, N> beside(const at::TensorOptions & like, const int64_t (&sizes)[N]) {
+    int64_t all = 0;
+    for (const int64_t n : sizes) all += (n + 3) / 4 * 4;
+    const at::Tensor whole = at::empty({all}, like);
+    std::array<at::Tensor, N> out;
+    int64_t at = 0;
+    for (size_t i = 0; i < N; at += (sizes[i] + 3) / 4 * 4, i++) {
+        out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+        out[i].unsafeGetTensorImpl()->set_storage_offset(at);
+        out[i].unsafeGetTensorImpl()->set_sizes_contiguous({sizes[i]});
+    }
+    return out;
+}
 PyObject * pages_plan(PyObject * const * a) {                            // table, held, refs, counts, page_tokens, rows, slots
     const int64_t n64 = tensor(a[3], "counts").numel();
     const int n = small(n64, "counts: too many sequences"), rows = number(a[5], "rows");
@@ -335,8 +350,7 @@ PyObject * pages_plan(PyObject * const * a) {                            // tabl
     const b200_pages p = pages_of(a[0], a[1], a[2], number(a[4], "page_tokens"), nullptr);
     need(a[6] != Py_None || n <= p.n_slots, "without slots, sequence i is slot i: more sequences than slots");
     const int32_t * slots = a[6] != Py_None ? ints("slots", a[6], p.device, n) : nullptr, * counts = ints("counts", a[3], p.device);
-    const at::TensorOptions like = THPVariable_Unpack(a[2]).options();
-    at::Tensor out[4] = {at::empty({n + 1}, like), at::empty({rows}, like), at::empty({rows}, like), at::empty({1}, like)};
+    const std::array<at::Tensor, 4> out = beside(THPVariable_Unpack(a[2]).options(), {n + 1, rows, rows, 1});
     done(api.pages_plan(&p, slots, counts, n, rows, static_cast<int32_t *>(out[0].data_ptr()), static_cast<int32_t *>(out[1].data_ptr()), static_cast<int32_t *>(out[2].data_ptr()),
                         static_cast<int32_t *>(out[3].data_ptr())) == 0, "pages_plan");
     PyObject * r = PyTuple_New(4);
