@@ -152,6 +152,71 @@ def test_calls_see_what_the_call_in_front_wrote():
         assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("call", [*FORMS, "append", "plan", "trim", "verify", "verify many"])
+def test_what_another_stream_wrote(call, captured):
+    """a call that stands ready behind a kernel of its own stream waits for another stream's event too: what that one wrote late is what the call sees"""
+    c, q = made(call if call in FORMS else "unit")
+    front, q_front = made("unit", seed=3)
+    table, big = c.table, torch.zeros(1 << 24, device="cuda")
+    refs = torch.zeros(c.pages, dtype=torch.int32, device="cuda")
+    k = torch.randn(c.rows, 2, 64, device="cuda").bfloat16()
+    logits = torch.randn(60, 70000 if call == "verify many" else 500, device="cuda")
+    ids, u, ends = torch.arange(60, device="cuda").int(), torch.full((60,), 0.4, device="cuda"), torch.arange(0, 61, 4, device="cuda").int()
+    counts = ints([1, 2, 3])
+    late = {"append": (c.held,), "plan": (c.held, counts, refs), "trim": (c.held, table), "verify": (logits, ends), "verify many": (logits, ends)}.get(call, (c.held, c.first, q))
+    right, side = [x.clone() for x in late], torch.cuda.Stream()
+    t_front, pool = front.table, c.pool.clone()
+    tables, counted = table.clone(), refs.clone()
+
+    def run():
+        if call == "append":
+            serve.kv16_append(c.pool[0], table, c.held, c.first, k, k, c.slots)
+            return [c.pool]
+        if call == "plan":
+            return [*serve.pages_plan(table, c.held, refs, counts, 16, 9, c.slots), table, refs]
+        if call == "trim":
+            serve.pages_trim(table, c.held, refs, 16, c.slots, 20, 3)
+            return [table, refs]
+        if call.startswith("verify"):
+            return list(serve.verify(logits, ids, ends, u, u))
+        return [serve.kv16_attention(q, c.pool[0], table, c.held, c.first, c.slots)]
+
+    def reset(wrong):
+        c.pool.copy_(pool), table.copy_(tables), refs.copy_(counted)
+        for x, y in zip(late, right):
+            x.zero_() if wrong else x.copy_(y)
+
+    def work():
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                big.add_(1.0)
+            for x, y in zip(late, right):
+                x.copy_(y)
+        serve.kv16_attention(q_front, front.pool[0], t_front, front.held, front.first, front.slots)
+        torch.cuda.current_stream().wait_stream(side)
+        return run()
+    reset(False)
+    torch.cuda.synchronize()
+    want = [x.clone() for x in run()]
+    reset(True)
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            got = work()
+    for _ in range(5):
+        reset(True)
+        torch.cuda.synchronize()
+        if captured:
+            graph.replay()
+        else:
+            got = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("form", FORMS)
 def test_results_in_the_queries_place(form, hd):
