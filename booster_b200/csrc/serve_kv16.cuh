@@ -12,7 +12,7 @@
 // A step (K and V of 32 tokens, 128 head_dim bytes) comes by one TMA box for each 16 tokens and 64 dims, with the 128-byte swizzle that ldmatrix reads without bank conflicts; a page that is
 // absent is a box outside the pool, which reads 0. Every warp has a ring of its own, two steps ahead.
 // P = hi + lo in two numbers of the type: 16 and 22 bits of a weight, so that results are as good as their own rounding (one number of 8 bits would be another rounding of the result's size;
-// the second product hides behind the loads). P_LIFT and P_PASS as in serve_attn.cuh; sums are fp32.
+// the second product hides behind the loads). Sums are fp32; of fp16 P_LIFT and P_PASS as in serve_attn.cuh, of bfloat16 see p16_lift.
 // Measured with 32 query heads on 8 of 128: HBM bounds long contexts (48 sequences of 90 to 4090 tokens, 410 MB, 72 us: 92 % of the copy rate while it streams; one of 20 000 27 us); one launch of clusters 5.8 us at
 // one sequence of 333 tokens, 8.4 at 61 under a window of 1000 with 4 sinks (8 heads on 2 of 64), of which 5 are the launch and the way slot -> length -> page -> box -> products -> the cluster's meetings.
 #pragma once
@@ -29,6 +29,11 @@ namespace srv {
 constexpr int A16_WARPS = 4, A16_STAGES = 3, A16_STEP = 32, A16_CLUSTER = 8;      // A16_STAGES: a warp
 __host__ __device__ constexpr int a16_stage_bytes(int hd) { return A16_STEP * 4 * hd; }
 __host__ __device__ constexpr size_t a16_ring_bytes(int hd) { return (size_t) A16_WARPS * A16_STAGES * a16_stage_bytes(hd); }
+
+// what the base of a weight 2^(score - base) is below the largest score (serve_attn.cuh). bfloat16 keeps its 8 bits at any size, so it needs no lift; but its values go up to fp32's largest, and so
+// would sums of values with weights above 1. With weights of 2^-38 at the largest score, 2^-30 until the base moves, those of the 2^30 tokens that a slot can have sum up to less than 1, and no sum of
+// values passes the largest value. At the other end, what of a result is below 2^-88 may be lost.
+template <typename T> constexpr float p16_lift = std::is_same<T, __half>::value ? P_LIFT : -30.f - P_PASS;
 
 // steps of 2^log2 tokens that the rows a .. b of a sequence see: `head` of them from position 0, the others from step lo on
 struct Steps { int head, lo, n; };
@@ -66,7 +71,7 @@ template <typename T> __device__ __forceinline__ bool wild(uint32_t p) {
     return (p & M) == M || (p >> 16 & M) == M;
 }
 
-// what a warp holds of a unit: its columns' sums of values, largest scores less P_LIFT and sums of weights. A lane has columns 2 tq, 2 tq + 1 of each eight and the dims 16 k + g, + 8
+// what a warp holds of a unit: its columns' sums of values, largest scores less the lift and sums of weights. A lane has columns 2 tq, 2 tq + 1 of each eight and the dims 16 k + g, + 8
 template <int HD, int NT> struct Piece16 { float o[NT][HD / 16][4], m[NT][2], l[NT][2]; };
 // CW warps go over the same steps with columns of their own: one of them asks for the steps, all tell when they are done with one. Of a ring: where its stages, the barriers that tell a stage full
 // (and, where it is shared, empty) stand, and steps that were asked for and used so far: stage n % (A16_STAGES CW), phase n / (A16_STAGES CW)
@@ -223,10 +228,10 @@ __device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtenso
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    const float top = fmaxf(m[n][j], x - P_LIFT), down = top > m[n][j] ? exp2_fast(m[n][j] - top) : 1.f;
+                    const float top = fmaxf(m[n][j], x - p16_lift<T>), down = top > m[n][j] ? exp2_fast(m[n][j] - top) : 1.f;
                     m[n][j] = top;
                     base[n][j] = top == -INFINITY ? 0.f : top;
-                    limit[n][j] = top + (P_LIFT + P_PASS);
+                    limit[n][j] = top + (p16_lift<T> + P_PASS);
                     l[n][j] *= down;
 #pragma unroll
                     for (int k = 0; k < KS; k++) { o[n][k][j] *= down; o[n][k][j + 2] *= down; }

@@ -10,7 +10,7 @@
 //   warps 9, 10      one thread each issues a half's S = Q K^T (128 x 64 x head_dim) and O += P V (P from tensor memory, 128 x head_dim x 64)
 //   warp 11          the next segment's queries, while the last 128 tokens of the one before are worked on, where 128 columns are whole rows of a group: a box. Others the soft-max warps gather
 // Tensor memory: S and P [2 halves][2 turns][64 columns], O [2][head_dim]. Each half has two turns of S, so that the scores of the next 64 tokens are there when those in hand are done with.
-// P is rounded to the type once, with P_LIFT and P_PASS of serve_attn.cuh: results are off by 1.2 to 1.35 times (rms) what their own rounding is (bfloat16 2.1e-3 for 1.7e-3, fp16 2.8e-4 for 2.1e-4).
+// P is rounded to the type once, with p16_lift of serve_kv16.cuh: results are off by 1.2 to 1.35 times (rms) what their own rounding is (bfloat16 2.1e-3 for 1.7e-3, fp16 2.8e-4 for 2.1e-4).
 // In two numbers, as for few rows, the second product would be twice as long; sums of the rounded weights instead of the weights' made 8192 tokens 45 us longer and no result nearer.
 // O is scaled in tensor memory where the base of P moves.
 // Measured with 32 query heads on 8 of 128: 8192 tokens 473 us (1162 TFLOP/s, 71 % of the bf16 rate), 1000 rows behind 5000 positions 100 us, of which 5 the plan and 10 the join. A step of 64
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                 }
                 const float high = fmaxf(x0, x1), score = high == -INFINITY ? high : high * factor;
                 if (__any_sync(0xffffffffu, score > limit)) {
-                    const float top = fmaxf(m, score - P_LIFT), down = top > m ? exp2_fast(m - top) : 1.f;
+                    const float top = fmaxf(m, score - p16_lift<T>), down = top > m ? exp2_fast(m - top) : 1.f;
                     if (t > 2 * g.t0 && __any_sync(0xffffffffu, down != 1.f)) {
                         pr_wait(smem_at(&o_full[half][(n_s - 1) & 1]), (uint32_t) ((n_s - 1) >> 1 & 1), p.polls, dead);
                         __syncwarp();
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                     }
                     m = top;
                     base = top == -INFINITY ? 0.f : top;
-                    limit = top + (P_LIFT + P_PASS);
+                    limit = top + (p16_lift<T> + P_PASS);
                     l *= down;
                 }
                 const uint64_t by = two(factor, factor), less = two(-base, -base);
