@@ -1,10 +1,12 @@
-"""Attention over the 16-bit cache on the GPU, each of its forms by itself (tests/serve_draft_bounds.py): values up to the ends of the type's range."""
+"""Attention over the 16-bit cache on the GPU, each of its forms by itself (tests/serve_draft_bounds.py): the bits that a form keeps, the edges of windows and first tokens at long contexts, values up
+to the ends of the type's range."""
+import numpy as np
 import pytest
 import torch
 
 from booster_b200 import serve
 from tests import serve_draft_bounds as bounds
-from tests.test_serve_draft_gpu import BF16, Case
+from tests.test_serve_draft_gpu import BF16, F16, Case
 
 pytestmark = pytest.mark.gpu
 
@@ -20,6 +22,40 @@ def made(form, held, kv=2, hd=64, page=32, dtype=BF16, seed=0):
 
 def attend(c, q, **more):
     return serve.kv16_attention(q, *c.args(), slots=c.slots, max_rows=max(c.counts), **more)
+
+
+@pytest.mark.parametrize("form", bounds.FORMS)
+@pytest.mark.parametrize("dtype,hd,window,sinks", [(BF16, 128, 0, 0), (BF16, 64, 50, 3), (F16, 64, 0, 0), (F16, 128, 50, 3)])
+def test_bits_of_each_form(form, dtype, hd, window, sinks):
+    c, group, once = made(form, [30, 190, 0], hd=hd, dtype=dtype, seed=hd)
+    c.fill()
+    q = (1.5 * c.randn(c.rows, 2 * group, hd)).to(dtype)
+    out = attend(c, q, window=window, sinks=sinks).double().cpu().numpy()
+    want, room = bounds.attention(q.double().cpu().numpy(), c.seen(), c.held_l, c.first_l, window, sinks, hd ** -0.5, dtype == BF16, once)
+    over = np.abs(out - want) / room
+    assert over.max() <= 1.0, f"off by {over.max():.3g} of what the form's roundings allow"
+
+
+@pytest.mark.parametrize("form", bounds.FORMS)
+@pytest.mark.parametrize("hd,page,window,sinks", [(64, 32, 1500, 4), (64, 16, 70, 33), (128, 256, 1203, 129), (128, 64, 0, 0), (64, 128, 1, 0), (64, 64, 33, 5000), (128, 16, 517, 31)])
+def test_edges_of_windows_and_first_tokens(form, hd, page, window, sinks):
+    """keys of 0 and values that are 1 at one dim each: results count, for each dim, the positions that are seen. What nobody may see is 100"""
+    c, group, _ = made(form, [1903, 777, 5], hd=hd, page=page, dtype=BF16)
+    c.pool[0, :, 0], c.pool[0, :, 1] = 0.0, 100.0
+    eye = torch.eye(hd, dtype=BF16, device="cuda")
+    for s, h, n in zip(c.slots_l, c.held_l, c.counts):
+        for i in range(-(-(h + n) // page)):
+            some = min(page, h + n - i * page)
+            c.pool[0, c.table_l[s][i], 1, :, :some] = eye[torch.arange(i * page, i * page + some, device="cuda") % hd]
+    q = c.randn(c.rows, 2 * group, hd).to(BF16)
+    out = attend(c, q, window=window, sinks=sinks).double().cpu().numpy()
+    for s, (h, n) in enumerate(zip(c.held_l, c.counts)):
+        for r in range(n):
+            j = bounds.seen(h + r, np.ones(h + n, bool), window, sinks)
+            count = np.bincount(j % hd, minlength=hd)
+            got = out[c.first_l[s] + r] * j.size
+            assert (np.rint(got) == count).all()
+            assert (np.abs(got - count) <= count * (2.0 ** -8 + 2.0 ** -12)).all()      # (weights are all the same: one rounding of the result)
 
 
 @pytest.mark.parametrize("form", bounds.FORMS)
