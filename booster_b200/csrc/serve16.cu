@@ -55,19 +55,19 @@ int attend_tiles(int group, int max_rows) { const int cols = attend_cols(group, 
 size_t attend_before_bytes(int n_seq) { return ((size_t) (n_seq + 2) * 8 + 255) / 256 * 256; }
 size_t attend_columns(int cols, int sms) { return 2 * (size_t) sms * A16_WARPS * cols; }      // of all pieces' partial results
 size_t attend_bytes(int n_seq, int head_dim, int cols, int sms) { return attend_before_bytes(n_seq) + attend_columns(cols, sms) * (head_dim + 2) * 4; }
-struct Few { CUtensorMap map; int * err; int n_ct, cluster, device, sms; void * stream; };
+struct Few { CUtensorMap map; int * err; uint32_t polls; int boxes, n_ct, cluster, device, sms; void * stream; };
 template <int HD, int NT, int CW, typename T> void unit_as(const AttendArgs & a, const Few & f) {
     static Limits set;
     const auto kernel = k_kv16_attend_unit<HD, NT, CW, T>;
     allow_smem(kernel, f.device, set);
-    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * f.n_ct * f.cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), f.stream, true, f.cluster, a, f.map, f.err, WAIT_POLLS, f.n_ct);
+    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * f.n_ct * f.cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), f.stream, true, f.cluster, a, f.map, f.err, f.polls, f.boxes, f.n_ct);
 }
 template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, const Few & f) {
     if (f.cluster) return unit_as<HD, NT, 1, T>(a, f);
     static Limits set;
     const auto kernel = k_kv16_attend<HD, NT, T>;
     allow_smem(kernel, f.device, set);
-    launch(kernel, dim3(f.sms), A16_WARPS * 32, 1024 + a16_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8, f.stream, true, 1, a, f.map, f.err, WAIT_POLLS);
+    launch(kernel, dim3(f.sms), A16_WARPS * 32, 1024 + a16_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8, f.stream, true, 1, a, f.map, f.err, f.polls, f.boxes);
     const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group, parts = (int64_t) f.sms * A16_WARPS / ((int64_t) a.c.n_seq * a.c.n_kv);
     if (parts > 32) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, f.stream, true, 1, a);
     else if (parts > 8) launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, f.stream, true, 1, a);
@@ -150,16 +150,17 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
     uint8_t * w = static_cast<uint8_t *>(work);
     const bool bf16 = dtype == B200_DTYPE_BF16;
     int * err = wait_word(c.device);
+    const int drill = drill_polls.load(), never = 1 << 19;       // (more arrivals than come)
+    const uint32_t polls = drill ? (uint32_t) drill : WAIT_POLLS;
     // up to 16 columns of a sequence (rows x query heads of a KV head) are one warp's; more are worth tcgen05's plan and join where one launch does not do
     const int cols = attend_cols(a.group, max_rows), n_ct = attend_tiles(a.group, max_rows), cluster = unit_cluster(c, cols, n_ct, window, a.sinks, on.sms);
     if (cols > 16 && !cluster) {
         const PromptWork at = prompt_work(c, a.group, on.sms);
         check_work(work, work_bytes, at.bytes);
-        const int drill = drill_polls.load();
         const int64_t n = prompt_entries(c, a.group);
         // 128 columns as one box: whole rows of a group, rows and heads at distances that a tensor map can have
         const bool by_box = a.q_whole && 128 % a.group == 0 && q_head > 0 && (q_row > 0 || c.n_rows == 1) && q_row < (1ll << 38) && q_head < (1ll << 38);
-        PromptArgs p = {a, (int) n, reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.first), err, drill ? (uint32_t) drill : WAIT_POLLS, drill ? 1 << 19 : by_box ? 1 : 4};
+        PromptArgs p = {a, (int) n, reinterpret_cast<Entry *>(w + at.entries), reinterpret_cast<int *>(w + at.first), err, polls, drill ? never : by_box ? 1 : 4};
         p.a.before = reinterpret_cast<long long *>(w);
         p.a.ml = reinterpret_cast<float *>(w + at.ml);
         p.a.part = reinterpret_cast<float *>(w + at.part);
@@ -179,7 +180,7 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
     a.before = reinterpret_cast<long long *>(w);
     a.ml = reinterpret_cast<float *>(w + attend_before_bytes(c.n_seq));
     a.part = a.ml + attend_columns(cols, on.sms) * 2;
-    const Few f = {pool_map(c, bf16, 16, 2), err, n_ct, cluster, c.device, on.sms, c.stream};
+    const Few f = {pool_map(c, bf16, 16, 2), err, polls, drill ? never : 1, n_ct, cluster, c.device, on.sms, c.stream};
     if (bf16) c.head_dim == 128 ? attend_few<128, __nv_bfloat16>(a, f, cols) : attend_few<64, __nv_bfloat16>(a, f, cols);
     else c.head_dim == 128 ? attend_few<128, __half>(a, f, cols) : attend_few<64, __half>(a, f, cols);
 }

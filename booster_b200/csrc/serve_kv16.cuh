@@ -277,8 +277,9 @@ __device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtenso
         }
 }
 
+// boxes: arrivals that tell a step there, 1, or more than come (b200_kv4_drill)
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls) {
+__global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls, int boxes) {
     constexpr int COLS = 8 * NT, KS = HD / 16, STAGE = a16_stage_bytes(HD);
     extern __shared__ uint8_t a16_raw[];
     __shared__ long long sums[A16_WARPS];
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
     const Cache & c = a.c;
     if (lane == 0) {
-        for (int i = 0; i < A16_STAGES; i++) mbar_init(smem_at(&full_s[warp][i]), 1);
+        for (int i = 0; i < A16_STAGES; i++) mbar_init(smem_at(&full_s[warp][i]), boxes);
         mbar_init_done();
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
 // Few sequences of bounded length, up to 64 columns: with more than 16 two or four warps (CW) go over the same steps with 16 columns each, so that keys and values are read once. (In the line of pieces
 // such groups are slower than tcgen05: a step is one chain of 2200 clocks, and a block has one or two of them under way. 48 ragged sequences of 20 columns 121 us and 96, 6 long ones of 40 270 and 100.) A cluster of blocks a unit, its warps share the unit's steps evenly and the blocks add what they have through one another's shared memory. One launch, no workspace
 template <int HD, int NT, int CW, typename T>
-__global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls, int n_ct) {
+__global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls, int boxes, int n_ct) {
     constexpr int COLS = 8 * NT, ALL = COLS * CW, KS = HD / 16, STAGE = a16_stage_bytes(HD), PAD = HD + 4, GROUPS = A16_WARPS / CW, STAGES = A16_STAGES * CW;
     extern __shared__ uint8_t a16_raw[];
     __shared__ __align__(8) uint64_t full_s[GROUPS][STAGES], empty_s[GROUPS][STAGES];
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const At
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cw = warp % CW, group = warp / CW, g = lane >> 2, tq = lane & 3, rank = (int) cl.block_rank(), blocks = (int) cl.num_blocks();
     const Cache & c = a.c;
     if (lane == 0 && cw == 0) {
-        for (int i = 0; i < STAGES; i++) { mbar_init(smem_at(&full_s[group][i]), 1); mbar_init(smem_at(&empty_s[group][i]), CW); }
+        for (int i = 0; i < STAGES; i++) { mbar_init(smem_at(&full_s[group][i]), boxes); mbar_init(smem_at(&empty_s[group][i]), CW); }
         mbar_init_done();
     }
     if (CW > 1) __syncthreads(); else __syncwarp();

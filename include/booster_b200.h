@@ -393,8 +393,8 @@ int b200_kv16_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q
  * out fails with a message that says so, has done nothing itself and may be repeated. b200_kv4_status asks without doing anything else: 0, or non-zero where a wait ran out that no call has told
  * of yet. Work that is still on its way is not waited for, so a program that replays graphs asks behind a synchronisation. */
 int b200_kv4_status(int device);
-/* polls > 0: from now on b200_kv4_attention's kernels of many rows wait for queries that never come, that many polls (of 4 us) long, and give up; 0: as always. Process-wide; exists so that
- * tests cover waits that run out. */
+/* polls > 0: from now on the kernels of many rows of b200_kv4_attention and b200_kv16_attention wait for queries that never come, and b200_kv16_attention's of few rows for keys, that many polls
+ * (of 4 us) long, and give up; 0: as always. Process-wide; exists so that tests cover waits that run out. */
 void b200_kv4_drill(int polls);
 
 /* The pages' life. refs[n_pages] counts the slots that hold a page (0: free); table and held as above, here [n_slots] of all slots. pool: n_layer layers, layer_stride

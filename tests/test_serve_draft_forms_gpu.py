@@ -1,10 +1,10 @@
 """Attention over the 16-bit cache on the GPU, each of its forms by itself (tests/serve_draft_bounds.py): the bits that a form keeps, the edges of windows and first tokens at long contexts, values up
-to the ends of the type's range."""
+to the ends of the type's range, and waits that run out."""
 import numpy as np
 import pytest
 import torch
 
-from booster_b200 import serve
+from booster_b200 import _lib, serve
 from tests import serve_draft_bounds as bounds
 from tests.test_serve_draft_gpu import BF16, F16, Case
 
@@ -94,3 +94,26 @@ def test_the_largest_number_as_it_stands(form):
     assert torch.isfinite(attend(c, q)).all()
     c.pool[0, :, 0], c.pool[0, :, 1] = 0.0, most
     assert torch.equal(attend(c, q), torch.full_like(q, most))
+
+
+@pytest.mark.parametrize("form", bounds.FORMS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_waits_that_run_out_in_each_form(form, hd):
+    """what a wait is for never comes: the kernel gives up and ends, the next call says so and does nothing, and after it all is as before"""
+    c, group, _ = made(form, [1000, 333, 0], hd=hd, page=16)
+    c.fill()
+    q = c.randn(c.rows, 2 * group, hd).to(BF16)
+    right = attend(c, q)
+    pool = c.pool.clone()
+    serve.kv4_status()
+    try:
+        _lib.lib().b200_kv4_drill(64)
+        attend(c, q)
+        _lib.lib().b200_kv4_drill(0)
+        torch.cuda.synchronize()
+        with pytest.raises(_lib.B200Error, match="ran out"):
+            attend(c, q)
+        serve.kv4_status()
+        assert torch.equal(c.pool, pool) and torch.equal(attend(c, q), right)
+    finally:
+        _lib.lib().b200_kv4_drill(0)
