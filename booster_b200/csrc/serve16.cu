@@ -51,16 +51,15 @@ template <typename T> void append_to(const b200_kv4 & c, const Cache & d, int dt
 
 // columns of a unit: 8 or 16 of one warp, in one launch also 32 or 64 of two or four that share what is read
 int attend_cols(int group, int max_rows) { const int64_t n = (int64_t) group * max_rows; return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128; }
-int attend_tiles(int group, int max_rows) { const int cols = attend_cols(group, max_rows); return (int) (((int64_t) group * max_rows + cols - 1) / cols); }
 size_t attend_before_bytes(int n_seq) { return ((size_t) (n_seq + 2) * 8 + 255) / 256 * 256; }
 size_t attend_columns(int cols, int sms) { return 2 * (size_t) sms * A16_WARPS * cols; }      // of all pieces' partial results
 size_t attend_bytes(int n_seq, int head_dim, int cols, int sms) { return attend_before_bytes(n_seq) + attend_columns(cols, sms) * (head_dim + 2) * 4; }
-struct Few { CUtensorMap map; int * err; uint32_t polls; int boxes, n_ct, cluster, device, sms; void * stream; };
+struct Few { CUtensorMap map; int * err; uint32_t polls; int boxes, cluster, device, sms; void * stream; };
 template <int HD, int NT, int CW, typename T> void unit_as(const AttendArgs & a, const Few & f) {
     static Limits set;
     const auto kernel = k_kv16_attend_unit<HD, NT, CW, T>;
     allow_smem(kernel, f.device, set);
-    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * f.n_ct * f.cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), f.stream, true, f.cluster, a, f.map, f.err, f.polls, f.boxes, f.n_ct);
+    launch(kernel, dim3((unsigned) (a.c.n_seq * a.c.n_kv * f.cluster)), A16_WARPS * 32, 1024 + a16_ring_bytes(HD), f.stream, true, f.cluster, a, f.map, f.err, f.polls, f.boxes);
 }
 template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, const Few & f) {
     if (f.cluster) return unit_as<HD, NT, 1, T>(a, f);
@@ -84,8 +83,8 @@ template <int HD, typename T> void attend_few(const AttendArgs & a, const Few & 
 // 20 000 (20) 26.7 / 26.7; 16 of 200 (2) 12.3 / 18.4, of 1000 (8) 20.5 / 24.6; 61 of 1004 (2 heads of 64, 8) 16.4 / 18.5. More columns, one launch / tcgen05: one sequence of 2000, 20 columns (4 steps a group) 14.3 / 22.5, 64 (8) 20.5 / 22.5; of 500, 64 (2) 14.3 / 20.5;
 // 8 of 1000, 32 (8) 20.5 / 26.6, 64 (16) 32.8 / 26.6
 int unit_steps(int cols) { return cols <= 16 ? 16 : 8; }
-int unit_cluster(const b200_kv4 & c, int cols, int n_ct, int window, int sinks, int sms) {
-    const int64_t units = (int64_t) c.n_seq * c.n_head_kv * n_ct, room = (int64_t) sms * (c.head_dim == 64 ? 2 : 1);
+int unit_cluster(const b200_kv4 & c, int cols, int window, int sinks, int sms) {
+    const int64_t units = (int64_t) c.n_seq * c.n_head_kv, room = (int64_t) sms * (c.head_dim == 64 ? 2 : 1);
     int64_t tokens = (int64_t) c.max_pages * c.page_tokens;
     if (window > 0) tokens = std::min(tokens, (int64_t) window + std::min<int64_t>(sinks, tokens) + 128);
     int cluster = A16_CLUSTER;
@@ -125,7 +124,7 @@ int64_t kv16_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
     check_heads(c, n_head, max_rows);
     On on(c.device);
     const int group = n_head / c.n_head_kv, cols = attend_cols(group, max_rows);
-    if (unit_cluster(c, cols, attend_tiles(group, max_rows), 0, 0, on.sms)) return 0;       // (a window asks for no more)
+    if (unit_cluster(c, cols, 0, 0, on.sms)) return 0;       // (a window asks for no more)
     return cols > 16 ? prompt_work(c, group, on.sms).bytes : (int64_t) attend_bytes(c.n_seq, c.head_dim, cols, on.sms);
 }
 
@@ -153,7 +152,7 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
     const int drill = drill_polls.load(), never = 1 << 19;       // (more arrivals than come)
     const uint32_t polls = drill ? (uint32_t) drill : WAIT_POLLS;
     // up to 16 columns of a sequence (rows x query heads of a KV head) are one warp's; more are worth tcgen05's plan and join where one launch does not do
-    const int cols = attend_cols(a.group, max_rows), n_ct = attend_tiles(a.group, max_rows), cluster = unit_cluster(c, cols, n_ct, window, a.sinks, on.sms);
+    const int cols = attend_cols(a.group, max_rows), cluster = unit_cluster(c, cols, window, a.sinks, on.sms);
     if (cols > 16 && !cluster) {
         const PromptWork at = prompt_work(c, a.group, on.sms);
         check_work(work, work_bytes, at.bytes);
@@ -180,7 +179,7 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
     a.before = reinterpret_cast<long long *>(w);
     a.ml = reinterpret_cast<float *>(w + attend_before_bytes(c.n_seq));
     a.part = a.ml + attend_columns(cols, on.sms) * 2;
-    const Few f = {pool_map(c, bf16, 16, 2), err, polls, drill ? never : 1, n_ct, cluster, c.device, on.sms, c.stream};
+    const Few f = {pool_map(c, bf16, 16, 2), err, polls, drill ? never : 1, cluster, c.device, on.sms, c.stream};
     if (bf16) c.head_dim == 128 ? attend_few<128, __nv_bfloat16>(a, f, cols) : attend_few<64, __nv_bfloat16>(a, f, cols);
     else c.head_dim == 128 ? attend_few<128, __half>(a, f, cols) : attend_few<64, __half>(a, f, cols);
 }

@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend(const AttendA
 // Few sequences of bounded length, up to 64 columns: with more than 16 two or four warps (CW) go over the same steps with 16 columns each, so that keys and values are read once. (In the line of pieces
 // such groups are slower than tcgen05: a step is one chain of 2200 clocks, and a block has one or two of them under way. 48 ragged sequences of 20 columns 121 us and 96, 6 long ones of 40 270 and 100.) A cluster of blocks a unit, its warps share the unit's steps evenly and the blocks add what they have through one another's shared memory. One launch, no workspace
 template <int HD, int NT, int CW, typename T>
-__global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls, int boxes, int n_ct) {
+__global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const AttendArgs a, const __grid_constant__ CUtensorMap map, int * err, uint32_t polls, int boxes) {
     constexpr int COLS = 8 * NT, ALL = COLS * CW, KS = HD / 16, STAGE = a16_stage_bytes(HD), PAD = HD + 4, GROUPS = A16_WARPS / CW, STAGES = A16_STAGES * CW;
     extern __shared__ uint8_t a16_raw[];
     __shared__ __align__(8) uint64_t full_s[GROUPS][STAGES], empty_s[GROUPS][STAGES];
@@ -396,12 +396,12 @@ __global__ void __launch_bounds__(A16_WARPS * 32, 1) k_kv16_attend_unit(const At
     if (CW > 1) __syncthreads(); else __syncwarp();
     Ring16 ring = {smem + (uint32_t) (group * STAGES * STAGE), smem_at(&full_s[group][0]), smem_at(&empty_s[group][0]), 0, 0};
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int unit = (int) blockIdx.x / blocks, head = unit % c.n_kv, s = unit / c.n_kv / n_ct;
+    const int unit = (int) blockIdx.x / blocks, head = unit % c.n_kv, s = unit / c.n_kv;
     const Seq q = seq_at(c, s);
     const Steps sp = steps_of(c, q, a.window, a.sinks, 0, q.count - 1, 5);
     const int all_groups = blocks * GROUPS, me = rank * GROUPS + group, per = sp.n / all_groups, more = sp.n % all_groups, t0 = me * per + min(me, more), t1 = t0 + per + (me < more);
     bool dead = false;
-    for (int ct = unit / c.n_kv % n_ct; ct < col_tiles(q, a.group, ALL); ct += n_ct) {        // (the same for all blocks of the cluster)
+    for (int ct = 0; ct < col_tiles(q, a.group, ALL); ct++) {       // (more than one where a sequence has more rows than max_rows says. The same for all blocks of the cluster)
         Piece16<HD, NT> w;
         attend_piece<HD, NT, CW, T>(a, map, q, sp, ct * CW + cw, head, t0, dead ? t0 : t1, ring, cw == 0, polls, dead, w);
         __syncthreads();                                           // nobody reads the ring any more
