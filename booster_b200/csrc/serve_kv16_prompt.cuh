@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(f.x), "=r"(f.y), "=r"(f.z), "=r"(f.w) : "r"(q_s + half * QB + (x >> 3) * SUB + row * 128 + (((x & 7) ^ (row & 7)) << 4)) : "memory");
                 most = __vmaxu2(most, __vmaxu2(__vmaxu2(f.x & 0x7fff7fffu, f.y & 0x7fff7fffu), __vmaxu2(f.z & 0x7fff7fffu, f.w & 0x7fff7fffu)));
             }
-            const bool bad = wild<T>(most);
+            const bool bad = in && wild<T>(most);
             const bool any_bad = __any_sync(0xffffffffu, bad);
             if (lane == 0) pr_arrive(smem_at(&q_empty[half]));
             n_q++;
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(P16_THREADS, 1) k_kv16_prompt(const PromptArgs
                     x0 = fmaxf(x0, fmaxf(__uint_as_float(r[x]), __uint_as_float(r[x + 1])));
                     x1 = fmaxf(x1, fmaxf(__uint_as_float(r[x + 2]), __uint_as_float(r[x + 3])));
                 }
-                const float high = fmaxf(x0, x1), score = high == -INFINITY ? high : high * factor;
+                const float high = in ? fmaxf(x0, x1) : -INFINITY, score = high == -INFINITY ? high : high * factor;      // (a box's columns behind the sequence's rows, which others write, move no base)
                 if (__any_sync(0xffffffffu, score > limit)) {
                     const float top = fmaxf(m, score - p16_lift<T>), down = top > m ? exp2_fast(m - top) : 1.f;
                     if (t > 2 * g.t0 && __any_sync(0xffffffffu, down != 1.f)) {

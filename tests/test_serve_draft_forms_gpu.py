@@ -117,3 +117,25 @@ def test_waits_that_run_out_in_each_form(form, hd):
         assert torch.equal(c.pool, pool) and torch.equal(attend(c, q), right)
     finally:
         _lib.lib().b200_kv4_drill(0)
+
+
+@pytest.mark.parametrize("rows,group,wide", [(1, 4, False), (3, 5, False), (5, 4, False), (9, 7, False), (2, 4, True), (3, 5, True), (5, 4, True), (37, 4, True), (9, 2, True), (40, 16, True), (7, 5, True)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_other_sequences_queries_change_nothing(rows, group, wide, dtype):
+    """bit by bit: what stands beside a sequence's rows, behind its last one, or is written there by the same call (out is q) is nothing to them"""
+    c = Case([300, 700, 20, 1000, 64, 411], [rows] * 6, page=16, dtype=dtype, seed=5)
+    if wide:
+        c.widened()
+    c.fill()
+    q = (2.0 * c.randn(c.rows, 2 * group, 64)).to(dtype)
+    right = attend(c, q)
+    mine = torch.zeros(c.rows, dtype=torch.bool, device="cuda")
+    for s in (0, 2, 4):
+        mine[c.first_l[s]:c.first_l[s + 1]] = True
+    for other in (30.0, 0.0, float("nan"), float("inf")):
+        p = q.clone()
+        p[~mine] = p[~mine] * other if other < 100 else other
+        assert torch.equal(attend(c, p)[mine], right[mine])
+    for _ in range(20):
+        p = q.clone()
+        assert torch.equal(attend(c, p, out=p), right)
