@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const std::conditional
     };
     if (top == -INFINITY || !(temperature > 0.f)) {                      // (behind the join nobody reads here any more)
         const int i = first_of_largest();
-        if (rank == 0 && tid == 0) finish(top == -INFINITY ? -1 : i, top == -INFINITY ? -INFINITY : 0.f, VERIFY && draft >= 0 && draft == i && top != -INFINITY);
+        if (rank == 0 && tid == 0) finish(top == -INFINITY ? -1 : i, top == -INFINITY ? -INFINITY : 0.f, draft == i && top != -INFINITY && takes(1, 1));       // (p is 1 there)
         return;
     }
     const auto exactly = [&](float v) { return v == top ? 0.0 : (double) top - (double) v; };   // how far a logit is from the largest

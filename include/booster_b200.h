@@ -441,8 +441,8 @@ int b200_sample(int device, void * stream, int dtype, const void * logits, int64
  * then its drafts, and logits[row] are the target's for what follows the row. With p the distribution that b200_sample draws from (temperature, top_k, top_p, min_p by row; temperature <= 0:
  * all on the first of the largest) and q = draft_probs[row * draft_stride + i] (F32) what the drafter drew the row's draft ids[row + 1] from (NULL: it was sure, 1 at the draft), the draft is taken if
  * accept[row] q(draft) < p(draft). Where it is not, the sequence ends with a token drawn by u[row] as b200_sample draws, from max(p - q, 0) instead of p (p where that is nothing); where all are
- * taken, with one drawn from p at its last row. So the tokens have the target's distribution, and a sequence of one row gets b200_sample's token. A draft outside 0 .. n_vocab - 1 is never taken and
- * takes nothing off p; entries of q that are negative or NaN count as 0.
+ * taken, with one drawn from p at its last row. So the tokens have the target's distribution, and a sequence of one row gets b200_sample's token. A draft outside 0 .. n_vocab - 1 is never taken; without
+ * draft_probs it takes nothing off p, with them its row's q comes off as always. Entries of q that are negative or NaN count as 0.
  * gained[n_seq]: how many tokens sequence i has gained (drafts taken and one drawn; 0 without rows), which is what its held tokens grow by; tokens[n_rows]: what follows each row up to there, -1
  * behind and for rows of no sequence; logprobs[n_rows]: log p of those (0 at temperature <= 0), 0 where tokens has -1. A row of no finite logit ends its sequence with -1 and -infinity.
  * work: b200_verify_workspace() bytes (-1: error) on 16 bytes. */
