@@ -78,18 +78,40 @@ template <int HD, typename T> void attend_few(const AttendArgs & a, const Few & 
     else if (cols == 32) unit_as<HD, 2, 2, T>(a, f);
     else unit_as<HD, 2, 4, T>(a, f);
 }
-// blocks of a cluster a unit where one launch does: all clusters stand on the card at once, and the longest sequence that the table (or the window) allows gives each warp (or group of warps) at most
-// so many steps of 32 tokens. 0: a line of pieces and a join, or tcgen05. One launch / two, us with cold memory, 8 KV heads of 128: one sequence of 333 10.3 / 14.3, of 4000 (4 steps a warp) 14.4 / 18.4, of 8000 (8) 16.4 / 20.5, of
-// 20 000 (20) 26.7 / 26.7; 16 of 200 (2) 12.3 / 18.4, of 1000 (8) 20.5 / 24.6; 61 of 1004 (2 heads of 64, 8) 16.4 / 18.5. More columns, one launch / tcgen05: one sequence of 2000, 20 columns (4 steps a group) 14.3 / 22.5, 64 (8) 20.5 / 22.5; of 500, 64 (2) 14.3 / 20.5;
-// 8 of 1000, 32 (8) 20.5 / 26.6, 64 (16) 32.8 / 26.6
-int unit_steps(int cols) { return cols <= 16 ? 16 : 8; }
-int unit_cluster(const b200_kv4 & c, int cols, int window, int sinks, int sms) {
-    const int64_t units = (int64_t) c.n_seq * c.n_head_kv, room = (int64_t) sms * (c.head_dim == 64 ? 2 : 1);
+// clusters of so many blocks (2, 4 or 8) that the card holds at once: a cluster stands within one group of SMs, and those are not all of a size that 8 goes into (two blocks an SM with heads of 64). All
+// of k_kv16_attend_unit's forms for a head_dim have the same of it
+int clusters_at_once(int head_dim, int cluster, int device) {
+    static std::atomic<int> known[2][A16_CLUSTER + 1][MAX_DEVICES];       // one more than there are
+    static Limits set[2];
+    const bool wide = head_dim == 128;
+    std::atomic<int> & n = known[wide][cluster][device];
+    if (const int have = n.load()) return have - 1;
+    const auto kernel = wide ? k_kv16_attend_unit<128, 1, 1, __nv_bfloat16> : k_kv16_attend_unit<64, 1, 1, __nv_bfloat16>;
+    allow_smem(kernel, device, set[wide]);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = cluster; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(cluster); cfg.blockDim = dim3(A16_WARPS * 32); cfg.dynamicSmemBytes = 1024 + a16_ring_bytes(head_dim); cfg.attrs = &at; cfg.numAttrs = 1;
+    int got = 0;
+    cu(cudaOccupancyMaxActiveClusters(&got, kernel, &cfg), "cudaOccupancyMaxActiveClusters");
+    n.store(got + 1);
+    return got;
+}
+// blocks of a cluster a unit where one launch does: all clusters stand on the card at once (in two waves two sequences of 2000 take 13.7 us for 9.0 by half as large ones), and the longest sequence that
+// the table (or the window) allows gives each warp (or group of warps) at most so many steps of 32 tokens. 0: a line of pieces and a join, or tcgen05. It goes by the table's width because the host does not
+// know the lengths: under a table for long contexts short sequences take the other form. One launch / two, us a call among others, 8 KV heads of 128: one sequence of 333 (1 step) 5.6 / 8.5, of 8000 (8)
+// 12.2 / 14.2, of 16 000 (16) 18.7 / 18.9; 2 of 2000 (4) 9.0 / 12.1, of 8000 (16) 18.5 / 19.2; 16 of 200 (2) 7.2 / 11.4, of 1000 (8) 14.9 / 18.8; 61 of 1000 (2 heads of 64, 8) 10.1 / 13.7. More columns,
+// one launch / tcgen05: 20 columns, one of 1000 (2) 8.9 / 14.7, of 3900 (8) 15.0 / 19.9, 2 of 1900 (8) 15.6 / 17.2, 8 of 1000 (8) 16.5 / 20.2; 64 columns, one of 1000 (4) 12.5 / 14.7, of 1900 (8) 17.0 / 17.9, 4 of 500 (5) 16.2 / 16.4, but 2 of
+// 1000 (8, by 4 blocks) 19.5 / 16.1
+int unit_steps(int cols, int cluster) { return cols <= 16 ? 16 : cols <= 32 || cluster == A16_CLUSTER ? 8 : 4; }
+int unit_cluster(const b200_kv4 & c, int cols, int window, int sinks, const On & on) {
+    const int64_t units = (int64_t) c.n_seq * c.n_head_kv, room = (int64_t) on.sms * (c.head_dim == 64 ? 2 : 1);
+    if (cols > 64 || units > room) return 0;
     int64_t tokens = (int64_t) c.max_pages * c.page_tokens;
     if (window > 0) tokens = std::min(tokens, (int64_t) window + std::min<int64_t>(sinks, tokens) + 128);
     int cluster = A16_CLUSTER;
-    while (cluster > 1 && units * cluster > room) cluster /= 2;
-    return cols <= 64 && units * cluster <= room && (tokens + 31) / 32 <= (int64_t) unit_steps(cols) * (cols <= 16 ? A16_WARPS : 64 / cols) * cluster ? cluster : 0;
+    while (cluster > 1 && units > clusters_at_once(c.head_dim, cluster, on.device)) cluster /= 2;
+    return (tokens + 31) / 32 <= (int64_t) unit_steps(cols, cluster) * (cols <= 16 ? A16_WARPS : 64 / cols) * cluster ? cluster : 0;
 }
 
 template <int HD, typename T> void prompt_as(const PromptArgs & p, const CUtensorMap & map, const CUtensorMap & q_map, bool by_box, int64_t entries, int device, int sms, void * stream) {
@@ -124,7 +146,7 @@ int64_t kv16_attention_workspace(const b200_kv4 & c, int n_head, int max_rows) {
     check_heads(c, n_head, max_rows);
     On on(c.device);
     const int group = n_head / c.n_head_kv, cols = attend_cols(group, max_rows);
-    if (unit_cluster(c, cols, 0, 0, on.sms)) return 0;       // (a window asks for no more)
+    if (unit_cluster(c, cols, 0, 0, on)) return 0;       // (a window asks for no more)
     return cols > 16 ? prompt_work(c, group, on.sms).bytes : (int64_t) attend_bytes(c.n_seq, c.head_dim, cols, on.sms);
 }
 
@@ -152,7 +174,7 @@ void kv16_attention(const b200_kv4 & c, int dtype, const void * q, int64_t q_row
     const int drill = drill_polls.load(), never = 1 << 19;       // (more arrivals than come)
     const uint32_t polls = drill ? (uint32_t) drill : WAIT_POLLS;
     // up to 16 columns of a sequence (rows x query heads of a KV head) are one warp's; more are worth tcgen05's plan and join where one launch does not do
-    const int cols = attend_cols(a.group, max_rows), cluster = unit_cluster(c, cols, window, a.sinks, on.sms);
+    const int cols = attend_cols(a.group, max_rows), cluster = unit_cluster(c, cols, window, a.sinks, on);
     if (cols > 16 && !cluster) {
         const PromptWork at = prompt_work(c, a.group, on.sms);
         check_work(work, work_bytes, at.bytes);

@@ -139,3 +139,15 @@ def test_other_sequences_queries_change_nothing(rows, group, wide, dtype):
     for _ in range(20):
         p = q.clone()
         assert torch.equal(attend(c, p, out=p), right)
+
+
+@pytest.mark.parametrize("hd,units", [(128, [1, 14, 15, 16, 18, 32, 33, 34, 37, 73, 74, 75, 147, 148, 149]), (64, [32, 33, 34, 37, 70, 71, 72, 74, 148, 149, 295, 296, 297])])
+def test_as_many_units_as_the_card_just_holds(hd, units):
+    """clusters of 8, 4 and 2 blocks a unit, up to and beyond what stands on the card at once"""
+    for n in units:
+        c = Case([(37 * i) % 90 for i in range(n)], [1 + i % 2 for i in range(n)], kv=1, hd=hd, page=16, dtype=BF16, seed=n)
+        c.fill()
+        q = (1.5 * c.randn(c.rows, 4, hd)).to(BF16)
+        out = attend(c, q).double().cpu().numpy()
+        want, room = bounds.attention(q.double().cpu().numpy(), c.seen(), c.held_l, c.first_l, 0, 0, hd ** -0.5, True, False)
+        assert (np.abs(out - want) <= room).all(), n
