@@ -34,14 +34,11 @@ CUtensorMap pool_map(const b200_kv4 & c, bool bf16, int tokens, int sides) {
     return map_of(bf16, 5, c.pool, dims, strides, box);
 }
 
-// heads of a row one after the other in a warp only where there are rows enough to fill the card without
-int row_passes(const b200_kv4 & c) { return (int64_t) c.n_rows * c.n_head_kv > 16384 ? 4 : 1; }
 template <typename S, typename T> void append_as(const b200_kv4 & c, const Cache & d, const void * k, int64_t kr, int64_t kh, const void * v, int64_t vr, int64_t vh) {
     const Row16Src<S> src = {static_cast<const S *>(k), kr, kh, static_cast<const S *>(v), vr, vh, aligned(k, 16) && aligned(v, 16) && !((kr | kh | vr | vh) & (16 / (int64_t) sizeof(S) - 1))};
-    const int per = row_passes(c) * (256 / c.head_dim), parts = (c.n_head_kv + per - 1) / per;
+    const int per = 256 / c.head_dim, parts = (c.n_head_kv + per - 1) / per;
     const auto rows = [&](auto kernel) { launch(kernel, dim3((unsigned) (((int64_t) c.n_rows * parts + 7) / 8)), 256, 0, c.stream, true, 1, d, src, parts); };
-    if (row_passes(c) == 1) c.head_dim == 128 ? rows(k_kv16_append<S, T, 128, 1>) : rows(k_kv16_append<S, T, 64, 1>);
-    else c.head_dim == 128 ? rows(k_kv16_append<S, T, 128, 4>) : rows(k_kv16_append<S, T, 64, 4>);
+    c.head_dim == 128 ? rows(k_kv16_append<S, T, 128>) : rows(k_kv16_append<S, T, 64>);
 }
 template <typename T> void append_to(const b200_kv4 & c, const Cache & d, int dtype, const void * k, int64_t kr, int64_t kh, const void * v, int64_t vr, int64_t vh) {
     if (dtype == B200_DTYPE_F32) append_as<float, T>(c, d, k, kr, kh, v, vr, vh);

@@ -494,45 +494,36 @@ template <typename S, typename T> __device__ __forceinline__ void eight_as(const
         for (int i = 0; i < 4; i++) w[i] = pair_of<T>(to_f(p[2 * i]), to_f(p[2 * i + 1]));
     }
 }
-// A warp a row and PASSES passes of its heads (two heads at head_dim 128, four at 64), 16 bytes a lane; latency bounds few rows (row -> sequence -> slot -> page: 48 of 8 heads 2.2 us), the memory many
-// (5200 rows from fp32, 62 MB, 8.6 us)
-template <typename S, typename T, int HD, int PASSES>
+// A warp a row and two of its heads (four of 64 dims), 16 bytes a lane; latency bounds few rows (row -> sequence -> slot -> page: 48 of 8 heads 2.2 us), the memory many. Several heads one after the other in a
+// warp were slower at all sizes but one: 500 rows of 8 heads of 128 3.4 us for 2.9, 3000 6.2 for 6.4, 8192 13.4 for 12.8, 5200 from fp32 14.9 for 13.7 (62 MB, 4.5 TB/s), 8192 of 2 heads of 64 6.9 for 3.8
+template <typename S, typename T, int HD>
 __global__ void __launch_bounds__(256) k_kv16_append(const Cache c, const Row16Src<S> src, int parts) {
     constexpr int LANES = HD / 8, PER = 32 / LANES;
     const int64_t item = ((int64_t) blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31, li = lane % LANES, row = (int) (item / parts), h0 = (int) (item % parts) * PASSES * PER + lane / LANES;
+    const int lane = threadIdx.x & 31, li = lane % LANES, row = (int) (item / parts), head = (int) (item % parts) * PER + lane / LANES;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= c.n_rows) return;
-    uint32_t k[PASSES][4] = {}, v[PASSES][4] = {};
-#pragma unroll
-    for (int i = 0; i < PASSES; i++) {
-        const int head = h0 + i * PER;
-        if (head < c.n_kv) {
-            eight_as<S, T>(src.k + row * src.k_row + head * src.k_head + 8 * li, src.whole8, k[i]);
-            eight_as<S, T>(src.v + row * src.v_row + head * src.v_head + 8 * li, src.whole8, v[i]);
-        }
+    uint32_t k[4] = {}, v[4] = {};
+    if (head < c.n_kv) {
+        eight_as<S, T>(src.k + row * src.k_row + head * src.k_head + 8 * li, src.whole8, k);
+        eight_as<S, T>(src.v + row * src.v_row + head * src.v_head + 8 * li, src.whole8, v);
     }
     const int s = seq_of_row_warp(c, row);
     if (s < 0) return;
     const Seq q = seq_at(c, s);
     const int pos = q.held + row - q.begin, page = page_at(c, q.slot, pos);
     if (page < 0) return;
-    const int64_t to = (int64_t) page * c.page_stride;
     const unsigned mine = (LANES == 16 ? 0xffffu : 0xffu) << (lane / LANES * LANES);
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < PASSES; i++) {
-        bool bad = false;
+    for (int j = 0; j < 4; j++) bad = bad || wild<T>(k[j]) || wild<T>(v[j]);
+    if (__ballot_sync(0xffffffffu, bad) & mine)
 #pragma unroll
-        for (int j = 0; j < 4; j++) bad = bad || wild<T>(k[i][j]) || wild<T>(v[i][j]);
-        if (__ballot_sync(0xffffffffu, bad) & mine)
-#pragma unroll
-            for (int j = 0; j < 4; j++) { k[i][j] = 0x7fff7fffu; v[i][j] = 0; }
-        const int head = h0 + i * PER;
-        if (head < c.n_kv) {
-            const int64_t rest = (((int64_t) head << c.page_log2) + (pos & ((1 << c.page_log2) - 1))) * (2 * HD) + 16 * li, side = ((int64_t) c.n_kv << c.page_log2) * (2 * HD);
-            *reinterpret_cast<uint4 *>(c.pool + to + rest) = make_uint4(k[i][0], k[i][1], k[i][2], k[i][3]);
-            *reinterpret_cast<uint4 *>(c.pool + to + side + rest) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
-        }
+        for (int j = 0; j < 4; j++) { k[j] = 0x7fff7fffu; v[j] = 0; }
+    if (head < c.n_kv) {
+        uint8_t * to = c.pool + (int64_t) page * c.page_stride + (((int64_t) head << c.page_log2) + (pos & ((1 << c.page_log2) - 1))) * (2 * HD) + 16 * li;
+        *reinterpret_cast<uint4 *>(to) = make_uint4(k[0], k[1], k[2], k[3]);
+        *reinterpret_cast<uint4 *>(to + ((int64_t) c.n_kv << c.page_log2) * (2 * HD)) = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
 
