@@ -15,7 +15,8 @@ def row(q, k, v, scale, bf16, once):
     A weight is 2^y, y = s - b in log2 units, with b the same for all. Off by: the score's sum, hd exact products added by hd / 16 instructions, each off by 2^-22 of the largest sum at most; its
     scaling, 2^-22; y's rounding, 2^-24 of |y|, which is the distance from the largest score and up to 46 (bfloat16: weights from 2^-38 to 2^-30) or 15 (fp16: 2^7 to 2^15); 2^y, 2^-22 (of many rows
     2^-18.5, the polynomial's). These are the same above and below the line of the quotient. What is multiplied with values is rounded to the type once (half a step) or in two numbers (half a step of
-    half a step), of fp16 below 2^-14 by half a step of 2^-24, the largest weight being 2^7 at least. Sums of values take n / 8 instructions at most, sums of weights as many."""
+    half a step), of fp16 below 2^-14 by half a step of 2^-24, the largest weight being 2^7 at least. Sums of values take n / 8 instructions at most, sums of weights as many.
+    The result is rounded to the type: of fp16 below 2^-14, whose steps are 2^-24 there, by 2^-25."""
     n, hd = k.shape
     s = scale * (k @ q)
     p = np.exp(s - s.max())
@@ -27,7 +28,7 @@ def row(q, k, v, scale, bf16, once):
     part = eps / 2 if once else (eps / 2) ** 2
     size = np.abs(v)
     room = (p * (weight + part)) @ size + np.abs(r) * (p @ weight) + (p @ size + np.abs(r)) * (n / 8 + 16) * 2.0 ** -22 + 2.0 ** -32 * size.sum(0)
-    return p, r, room + eps / 2 * (np.abs(r) + room) + 2.0 ** -25 * eps
+    return p, r, room + eps / 2 * (np.abs(r) + room) + (0.0 if bf16 else 2.0 ** -25)
 
 
 def seen(p, there, window, sinks):
