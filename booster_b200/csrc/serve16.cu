@@ -64,6 +64,9 @@ template <int HD, int NT, typename T> void attend_as(const AttendArgs & a, const
     const auto kernel = k_kv16_attend<HD, NT, T>;
     allow_smem(kernel, f.device, set);
     launch(kernel, dim3(f.sms), A16_WARPS * 32, 1024 + a16_ring_bytes(HD) + (size_t) (a.c.n_seq + 1) * 8, f.stream, true, 1, a, f.map, f.err, f.polls, f.boxes);
+    // warps that add a unit's parts, where it has so many on average, 16 / 4 / 1, us a call: one of 20 000 (74) 21.9 / 25.0 / 29.9, 2 of 30 000 (37) 47.6 / 49.8 / 52.6, 4 of 12 000 (18) 39.9 / 40.1 / 42.0, 16 of 20 000 (2 heads of 64,
+    // 18) 34.7 / 34.3 / 35.9, 12 of 3000 (6) 33.8 / 32.7 / 32.0, 48 ragged (1.5) 83.8 / 75.9 / 74.4, 200 of 500 112 / 83 / 77. What beginning a unit costs (AT_OVER, in pairs of 4-bit tiles 3) is 3 steps here too: 48 ragged 79, 77, 74,
+    // 75, 74, 74 with 0, 1, 2, 3, 4, 6, four rows each 102, 89, 84, 81, 81, 80
     const int64_t items = (int64_t) a.c.n_rows * a.c.n_kv * a.group, parts = (int64_t) f.sms * A16_WARPS / ((int64_t) a.c.n_seq * a.c.n_kv);
     if (parts > 32) launch(k_kv4_join<HD, NT, T, 16>, dim3((unsigned) items), 512, 0, f.stream, true, 1, a);
     else if (parts > 8) launch(k_kv4_join<HD, NT, T, 4>, dim3((unsigned) items), 128, 0, f.stream, true, 1, a);

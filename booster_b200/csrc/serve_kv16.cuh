@@ -13,8 +13,9 @@
 // absent is a box outside the pool, which reads 0. Every warp has a ring of its own, two steps ahead.
 // P = hi + lo in two numbers of the type: 16 and 22 bits of a weight, so that results are as good as their own rounding (one number of 8 bits would be another rounding of the result's size;
 // the second product hides behind the loads). Sums are fp32; of fp16 P_LIFT and P_PASS as in serve_attn.cuh, of bfloat16 see p16_lift.
-// Measured with 32 query heads on 8 of 128: HBM bounds long contexts (48 sequences of 90 to 4090 tokens, 410 MB, 72 us: 92 % of the copy rate while it streams; one of 20 000 27 us); one launch of clusters 5.8 us at
-// one sequence of 333 tokens, 8.4 at 61 under a window of 1000 with 4 sinks (8 heads on 2 of 64), of which 5 are the launch and the way slot -> length -> page -> box -> products -> the cluster's meetings.
+// Measured with 32 query heads on 8 of 128, calls one after another on inputs that change: HBM bounds long contexts (48 sequences of 90 to 4090 tokens, 410 MB, 74 us, 86 % of the copy rate over the whole call;
+// one of 20 000, 82 MB, 23 us); one launch of clusters 5.8 us at one sequence of 333 tokens, 9.1 at 61 under a window of 1000 with 4 sinks (8 heads on 2 of 64), of which 5 are the launch and the way
+// slot -> length -> page -> box -> products -> the cluster's meetings.
 #pragma once
 #include "serve_attn.cuh"
 #include "serve_tma.cuh"
@@ -104,7 +105,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs & a, const CUtenso
                 else { const uint16_t * u = reinterpret_cast<const uint16_t *>(qp + 16 * k + 8 * j); qf[n][k][j] = u[0] | (uint32_t) u[1] << 16; }
             }
     }
-    // steps on their way: A16_STAGES - 1 ahead of the one in hand. Lanes hold the next 32 pages of the slot
+    // steps on their way: AHEAD of the one in hand. Lanes hold the next 32 pages of the slot
     const bool idle = (int64_t) ct * COLS >= (int64_t) q.count * a.group;      // (of a shared ring: a warp without columns)
     int next = t0, pages_from = -64, my_page = -1;
     uint32_t there = 0;                                        // two bits a step that was asked for: which of its halves have a page. The newest lowest

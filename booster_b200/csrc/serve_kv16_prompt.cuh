@@ -13,7 +13,8 @@
 // P is rounded to the type once, with p16_lift of serve_kv16.cuh: results are off by 1.2 to 1.35 times (rms) what their own rounding is (bfloat16 2.1e-3 for 1.7e-3, fp16 2.8e-4 for 2.1e-4).
 // In two numbers, as for few rows, the second product would be twice as long; sums of the rounded weights instead of the weights' made 8192 tokens 45 us longer and no result nearer.
 // O is scaled in tensor memory where the base of P moves.
-// Measured with 32 query heads on 8 of 128: 8192 tokens 473 us (1162 TFLOP/s, 71 % of the bf16 rate), 1000 rows behind 5000 positions 100 us, of which 5 the plan and 10 the join. A step of 64
+// Measured with 32 query heads on 8 of 128: 8192 tokens 467 us (1177 TFLOP/s, 71 % of the bf16 rate; 522 in calls one after another, which the card's power bounds), 1000 rows behind 5000 positions 100 us by
+// itself behind other work, 107 in calls from Python on inputs that change, of which 5 the plan and 10 the join. A step of 64
 // tokens takes 1750 clocks: of both halves' products 1280 (those of 64 tokens read 6 KB of shared memory in 48 clocks, for 32 of arithmetic), of exponentials 900, an eighth of them by a
 // polynomial (none 495 us, two eighths 489, three 494). Halves that took turns at exponentials by named barriers 475 to 485 and nothing at 1000 rows. What a warp does between them bounds it: a wait for
 // what is there 130 clocks, 64 scores from tensor memory 60 to 120, the largest 280, P back 120.
@@ -25,7 +26,8 @@
 namespace b200 {
 namespace srv {
 
-constexpr int P16_THREADS = 384, P16_OVER = 3;      // P16_OVER: what beginning a unit costs, in tiles
+// P16_OVER: what beginning a unit costs, in tiles. With 1, 2, 3, 4, 6, us: 2000 tokens 65, 57, 56, 57, 59; ragged portions 107, 99, 98, 100, 103; 1000 rows behind 5000 90, 90, 90, 91, 93; 48 sequences of 8 rows 88, 89, 90, 92, 95
+constexpr int P16_THREADS = 384, P16_OVER = 3;
 constexpr int P16_EIGHTHS = 1;
 template <typename T> __host__ __device__ constexpr uint32_t p16_idesc(int n, bool b_by_dims) {      // D f32, A and B of T, M = 128
     const uint32_t t = std::is_same<T, __half>::value ? 0u : 1u;

@@ -169,7 +169,7 @@ __device__ __forceinline__ int bin_place(float v) { return __float_as_int(__fmaf
 // the smallest float whose place is p or more
 __device__ __forceinline__ float place_from(int p) { return p <= (int) (-SA_FAR * SA_PER_NAT) ? -INFINITY : (float) p * (1.f / SA_PER_NAT); }
 
-// VERIFY (5 rows of 128 256 logits 13.8 us with the launches beside it, a draw from them 9.6; 168 mixed rows with drafters' distributions 83 and 69): the row's draft is the next row's input token, unless the row is its sequence's last. With p the distribution that the draw is from and q the drafter's, the draft x is taken
+// VERIFY (5 rows of 128 256 logits 13.0 us a call, a draw from them 9.6; 168 mixed rows with drafters' distributions 94 to 107 by how many drafts stand, on the same inputs again and again 83, a draw from them 69): the row's draft is the next row's input token, unless the row is its sequence's last. With p the distribution that the draw is from and q the drafter's, the draft x is taken
 // where accept q(x) < p(x); where it is not, a token is drawn from max(p - q, 0) (p, where that is nothing) by u as always. So what comes out has the distribution p whatever the drafter is.
 // p = t / total and r = max(t - rint(q total), 0) are whole multiples of 2^-40 too. ids[row]: the draft that was taken, or -2 - token of one that was drawn, for k_verify_ends.
 template <typename T, bool VERIFY>

@@ -96,7 +96,9 @@ def kv16_append(pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, fir
 def kv16_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, held: torch.Tensor, first: torch.Tensor, slots: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                    window: int = 0, sinks: int = 0, max_rows: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """attention of the step's rows q [rows, n_head, head_dim] (of the pool's type, any strides over rows and heads) over the positions up to their own, kv16_append having put those into the pool;
-    window > 0: over the last `window` of them and the sequence's first `sinks`. scale, max_rows and out as in kv4_attention; out may be q itself"""
+    window > 0: over the last `window` of them and the sequence's first `sinks`. scale, max_rows and out as in kv4_attention; out may be q itself. Few sequences of up to 16
+    query heads x rows a KV head take one launch where the table is narrow enough (of 8 KV heads of 128: 16 384 positions at one sequence, 8192 at two to four, 4096 at five to nine, 2048 at ten to
+    eighteen; or a window as short): 5.6 us for 8.5 at one of 333. A view of the table's first pages, table[:, :n], does where the program knows that nobody is longer"""
     return _native().kv16_attention(q, pool, table, held, first, slots, scale, window, sinks, max_rows, out)
 
 

@@ -151,3 +151,14 @@ def test_as_many_units_as_the_card_just_holds(hd, units):
         out = attend(c, q).double().cpu().numpy()
         want, room = bounds.attention(q.double().cpu().numpy(), c.seen(), c.held_l, c.first_l, 0, 0, hd ** -0.5, True, False)
         assert (np.abs(out - want) <= room).all(), n
+
+
+def test_a_view_of_a_wide_table_is_a_narrow_one():
+    c = Case([333, 90, 12], [1, 1, 1], kv=8, hd=128, page=16, dtype=BF16)
+    c.fill()
+    q = c.randn(3, 32, 128).to(BF16)
+    narrow = attend(c, q)
+    width = len(c.table_l[0])
+    c.widened()
+    out = serve.kv16_attention(q, c.pool[0], c.table[:, :width], c.held, c.first, c.slots, max_rows=1)
+    assert torch.equal(out, narrow)
