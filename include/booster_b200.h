@@ -384,7 +384,7 @@ int b200_kv4_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_
 int b200_kv16_append(const b200_kv4 * c, int pool_dtype, int dtype, const void * k, int64_t k_row, int64_t k_head, const void * v, int64_t v_row, int64_t v_head);
 /* attention as b200_kv4_attention has it, q and out of the pool's dtype. With window > 0 a row at position p sees, of the positions j <= p that have a page, those with j > p - window or
  * j < sinks (the first ones stay visible); window 0: all, whatever sinks is. A row that sees nothing answers 0, one whose query holds an infinity or a NaN and that sees something NaN; scores beyond
- * fp32's range are infinities. Values may be as large as the type has them; with bfloat16, what of a result is below 2^-88 may be lost. work: b200_kv16_attention_workspace() bytes (0: none; -1: error) on 16 bytes. */
+ * fp32's range are infinities, of which a negative one counts as not seen. Values may be as large as the type has them; with bfloat16, what of a result is below 2^-88 may be lost. work: b200_kv16_attention_workspace() bytes (0: none; -1: error) on 16 bytes. */
 int64_t b200_kv16_attention_workspace(const b200_kv4 * c, int n_head, int max_rows);
 int b200_kv16_attention(const b200_kv4 * c, int dtype, const void * q, int64_t q_row, int64_t q_head, int n_head, float scale, int window, int sinks, int max_rows, void * out, void * work,
                         int64_t work_bytes);
